@@ -234,6 +234,128 @@ int thff_fill_uniform(int precision, void* d_out, long long count, unsigned long
  * HIP call; bytes = 0 is a no-op.  Asynchronous on `stream`. */
 int thff_copy_nt(void* d_dst, const void* d_src, long long bytes, void* stream);
 
+/* ---- Sequence operators beside the long convolutions (no reference counterpart) ----
+ *
+ * The gated linear recurrence, the other mixer of a sequence model next to the
+ * long convolution, and the layer norm before either.  They need no
+ * thff_initialize.  precision: THFF_FLOAT, THFF_HALF or THFF_BFLOAT16, the
+ * type of the values (here real ones: float, half, bfloat16); states, weights,
+ * biases and their gradients are fp32 for all three.  Sums, states and
+ * statistics are held in fp32 and every output is rounded once, to nearest
+ * even.  The same call gives the same bits each time.  Nothing is kept between
+ * calls: scratch memory is the caller's, so calls on any streams and captured
+ * calls do not meet.  THFF_EINVAL for bad arguments before any HIP call,
+ * THFF_EIO for HIP failures; every synchronous call has an _async twin that
+ * returns once the work is enqueued on `stream`. */
+#define THFF_BFLOAT16 2
+
+/* Layouts of a scan's values: channels last is [batch][n][channels], one row of
+ * `channels` values a step; channels first is [batch][channels][n], the
+ * convolutions' layout, one row of n values a channel. */
+#define THFF_CHANNELS_LAST 0
+#define THFF_CHANNELS_FIRST 1
+
+/* What a scan's calls work on.  Strides are elements between the starts of
+ * consecutive rows, at least a row's length, or 0 for rows without a gap: with
+ * channels last and x_stride = gate_stride = 2 * channels, x and gate are the
+ * halves of one projection's rows.  x_stride and gate_stride hold for the
+ * gradients of x and the gate too, y_stride for y and its gradient.  batch, n
+ * and channels may be 0, and are at most 2^30, batch * channels at most
+ * 2^31 - 1.  states: rows of the state pool that slots index (unused without
+ * slots). */
+typedef struct thff_scan_shape {
+    int precision, layout;
+    int batch, n, channels, states;
+    long long x_stride, gate_stride, y_stride;
+} thff_scan_shape;
+
+/* Bytes of d_saved (what the forward pass keeps for the backward pass) and of
+ * d_workspace (scratch of one call) for a shape; THFF_EINVAL for a bad shape.
+ * 0: the pointer may be null. */
+long long thff_gated_scan_saved_bytes(const thff_scan_shape* shape);
+long long thff_gated_scan_workspace_bytes(const thff_scan_shape* shape);
+
+/* Gated linear recurrence, for every sequence b and channel c, with
+ * f[t] = 1 / (1 + exp(-gate[t])):
+ *   h[t] = f[t] * h[t-1] + (1 - f[t]) * x[t],   y[t] = h[t],   t < lengths[b].
+ * h before the first step is the state d_state_in, and the state after the last
+ * one goes to d_state_out; both are fp32 rows of `channels` values, row b for
+ * sequence b, or row slots[b] of a pool of shape->states rows.  A slot outside
+ * the pool (-1, say) is an empty place: it starts from zero and stores no state.
+ * Two places with the same slot race.  d_state_out may be d_state_in (one
+ * token after another in place: n = 1); the two must not overlap otherwise.
+ * lengths[b] is taken into [0, n]; y is 0 from there on, and x and the gate are
+ * not used there, whatever they hold.  Null d_state_in: zeros; null
+ * d_state_out, d_saved: not stored; null d_slots: row b; null d_lengths: n each.
+ * An infinity or NaN in x or the gate makes later outputs of its sequence and
+ * channel infinite or NaN, and no others.
+ * x, gate and y start on a boundary of their element, states, slots and lengths
+ * on 4 bytes, d_saved and d_workspace on 16.  y may alias neither x nor gate
+ * (disjoint rows interleaved in one buffer are fine).  Empty batches and
+ * channels are no-ops; n = 0 copies the states. */
+int thff_gated_scan(const thff_scan_shape* shape, const void* d_x, const void* d_gate, void* d_y,
+                    const void* d_state_in, void* d_state_out, const void* d_slots,
+                    const void* d_lengths, void* d_saved, void* d_workspace, void* stream);
+int thff_gated_scan_async(const thff_scan_shape* shape, const void* d_x, const void* d_gate,
+                          void* d_y, const void* d_state_in, void* d_state_out,
+                          const void* d_slots, const void* d_lengths, void* d_saved,
+                          void* d_workspace, void* stream);
+
+/* Gradients of thff_gated_scan, from dy and the gradient of the final states
+ * (d_dstate_out, null: zeros): lam[t] = dy[t] + f[t+1] * lam[t+1], at the last
+ * step lam = dy + dstate_out,
+ *   dx[t] = (1 - f[t]) * lam[t],   dgate[t] = lam[t] * (h[t-1] - x[t]) * f[t] * (1 - f[t]),
+ * both 0 from lengths[b] on, and d_dstate_in = f[0] * lam[0] (null: not stored),
+ * dstate_out where the length is 0.  The dstates are [batch][channels], row b
+ * for sequence b.  d_saved is what the forward call of the same shape, x, gate
+ * and lengths wrote.  dx and dgate may alias no input.  Alignment as above;
+ * n = 0 copies dstate_out. */
+int thff_gated_scan_backward(const thff_scan_shape* shape, const void* d_dy, const void* d_x,
+                             const void* d_gate, const void* d_saved, const void* d_dstate_out,
+                             const void* d_lengths, void* d_dx, void* d_dgate, void* d_dstate_in,
+                             void* d_workspace, void* stream);
+int thff_gated_scan_backward_async(const thff_scan_shape* shape, const void* d_dy,
+                                   const void* d_x, const void* d_gate, const void* d_saved,
+                                   const void* d_dstate_out, const void* d_lengths, void* d_dx,
+                                   void* d_dgate, void* d_dstate_in, void* d_workspace,
+                                   void* stream);
+
+/* Layer norm of `rows` rows of `cols` values, `*_stride` elements between the
+ * starts of consecutive rows (at least cols, or 0 for cols):
+ *   y = (x - mean) * rstd * weight + bias,   rstd = 1 / sqrt(var + eps),
+ * mean and var (divided by cols) of the row.  weight and bias are fp32 [cols]
+ * (null: ones, zeros); d_mean and d_rstd, fp32 [rows], keep the statistics for
+ * the backward pass (null: not stored).  cols >= 1, eps >= 0; rows = 0 is a
+ * no-op.  x and y start on a boundary of their element, the fp32 arrays on 4
+ * bytes; y may not alias x. */
+int thff_layer_norm(int precision, const void* d_x, long long x_stride, const void* d_weight,
+                    const void* d_bias, float eps, void* d_y, long long y_stride, void* d_mean,
+                    void* d_rstd, long long rows, int cols, void* stream);
+int thff_layer_norm_async(int precision, const void* d_x, long long x_stride,
+                          const void* d_weight, const void* d_bias, float eps, void* d_y,
+                          long long y_stride, void* d_mean, void* d_rstd, long long rows, int cols,
+                          void* stream);
+
+/* Bytes of thff_layer_norm_backward's d_workspace (0: may be null). */
+long long thff_layer_norm_workspace_bytes(long long rows, int cols);
+
+/* Gradients of thff_layer_norm from dy, x and the statistics: with
+ * xh = (x - mean) * rstd and g = dy * weight,
+ *   dx = rstd * (g - mean(g) - xh * mean(g * xh)),
+ *   dweight = sum over the rows of dy * xh,   dbias = sum over the rows of dy,
+ * fp32 [cols], not accumulated (null: not computed; zeros where rows = 0).
+ * dx may alias neither dy nor x.  Alignment as above, d_workspace on 16 bytes. */
+int thff_layer_norm_backward(int precision, const void* d_dy, long long dy_stride,
+                             const void* d_x, long long x_stride, const void* d_mean,
+                             const void* d_rstd, const void* d_weight, void* d_dx,
+                             long long dx_stride, void* d_dweight, void* d_dbias,
+                             void* d_workspace, long long rows, int cols, void* stream);
+int thff_layer_norm_backward_async(int precision, const void* d_dy, long long dy_stride,
+                                   const void* d_x, long long x_stride, const void* d_mean,
+                                   const void* d_rstd, const void* d_weight, void* d_dx,
+                                   long long dx_stride, void* d_dweight, void* d_dbias,
+                                   void* d_workspace, long long rows, int cols, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

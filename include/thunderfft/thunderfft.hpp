@@ -13,6 +13,7 @@
 // hold N throws std::runtime_error instead of running without it.
 #pragma once
 
+#include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -163,6 +164,99 @@ inline void ThunderFFT_conv2d(const vec2_t<T>* d_x, const vec2_t<T>* d_h, vec2_t
                   "ThunderFFT_conv2d supports 64 x 64, 128 x 128 and 1024 x 1024 images");
     detail::check(thff_conv2d(detail::precision_code<T>(), Rows, Cols, d_x, d_h, d_y, batch,
                               static_cast<void*>(stream)));
+}
+
+// ---- Sequence operators beside the long convolutions (no reference counterpart; the
+// contracts are stated at the C ABI's entry points).  T is float, half or __hip_bfloat16. ----
+
+namespace detail {
+
+template <class T>
+constexpr int value_code() {
+    static_assert(std::is_same_v<T, float> || std::is_same_v<T, half> ||
+                      std::is_same_v<T, __hip_bfloat16>,
+                  "the sequence operators support float, half and __hip_bfloat16 only");
+    return std::is_same_v<T, float> ? THFF_FLOAT : std::is_same_v<T, half> ? THFF_HALF
+                                                                          : THFF_BFLOAT16;
+}
+
+inline size_t check_bytes(long long bytes) {
+    if (bytes < 0) check(static_cast<int>(bytes));
+    return static_cast<size_t>(bytes);
+}
+
+}  // namespace detail
+
+// Shape of [batch][n][channels] values (channels last) or [batch][channels][n] ones, rows
+// without gaps; set the strides and the pool's rows (states) in it where they differ.
+template <typename T>
+inline thff_scan_shape ThunderFFT_scan_shape(int batch, int n, int channels,
+                                             bool channels_first = false) {
+    return {detail::value_code<T>(), channels_first ? THFF_CHANNELS_FIRST : THFF_CHANNELS_LAST,
+            batch, n, channels, batch, 0, 0, 0};
+}
+
+inline size_t ThunderFFT_gated_scan_saved_bytes(const thff_scan_shape& shape) {
+    return detail::check_bytes(thff_gated_scan_saved_bytes(&shape));
+}
+
+inline size_t ThunderFFT_gated_scan_workspace_bytes(const thff_scan_shape& shape) {
+    return detail::check_bytes(thff_gated_scan_workspace_bytes(&shape));
+}
+
+// Gated linear recurrence h[t] = f[t] h[t-1] + (1 - f[t]) x[t], f = sigmoid(gate), y = h.
+// Synchronises `stream` before returning, as the other calls here.
+template <typename T>
+inline void ThunderFFT_gated_scan(const thff_scan_shape& shape, const T* d_x, const T* d_gate,
+                                  T* d_y, const float* d_state_in, float* d_state_out,
+                                  const int* d_slots, const int* d_lengths, void* d_saved,
+                                  void* d_workspace, hipStream_t stream = 0) {
+    if (shape.precision != detail::value_code<T>())
+        throw std::invalid_argument("ThunderFFT_gated_scan: the shape is of another type");
+    detail::check(thff_gated_scan(&shape, d_x, d_gate, d_y, d_state_in, d_state_out, d_slots,
+                                  d_lengths, d_saved, d_workspace, static_cast<void*>(stream)));
+}
+
+template <typename T>
+inline void ThunderFFT_gated_scan_backward(const thff_scan_shape& shape, const T* d_dy,
+                                           const T* d_x, const T* d_gate, const void* d_saved,
+                                           const float* d_dstate_out, const int* d_lengths,
+                                           T* d_dx, T* d_dgate, float* d_dstate_in,
+                                           void* d_workspace, hipStream_t stream = 0) {
+    if (shape.precision != detail::value_code<T>())
+        throw std::invalid_argument("ThunderFFT_gated_scan_backward: the shape is of another type");
+    detail::check(thff_gated_scan_backward(&shape, d_dy, d_x, d_gate, d_saved, d_dstate_out,
+                                           d_lengths, d_dx, d_dgate, d_dstate_in, d_workspace,
+                                           static_cast<void*>(stream)));
+}
+
+// Layer norm of `rows` rows of `cols` values; strides of 0: rows without gaps.
+template <typename T>
+inline void ThunderFFT_layer_norm(const T* d_x, const float* d_weight, const float* d_bias,
+                                  float eps, T* d_y, long long rows, int cols,
+                                  float* d_mean = nullptr, float* d_rstd = nullptr,
+                                  long long x_stride = 0, long long y_stride = 0,
+                                  hipStream_t stream = 0) {
+    detail::check(thff_layer_norm(detail::value_code<T>(), d_x, x_stride, d_weight, d_bias, eps,
+                                  d_y, y_stride, d_mean, d_rstd, rows, cols,
+                                  static_cast<void*>(stream)));
+}
+
+inline size_t ThunderFFT_layer_norm_workspace_bytes(long long rows, int cols) {
+    return detail::check_bytes(thff_layer_norm_workspace_bytes(rows, cols));
+}
+
+template <typename T>
+inline void ThunderFFT_layer_norm_backward(const T* d_dy, const T* d_x, const float* d_mean,
+                                           const float* d_rstd, const float* d_weight, T* d_dx,
+                                           float* d_dweight, float* d_dbias, void* d_workspace,
+                                           long long rows, int cols, long long dy_stride = 0,
+                                           long long x_stride = 0, long long dx_stride = 0,
+                                           hipStream_t stream = 0) {
+    detail::check(thff_layer_norm_backward(detail::value_code<T>(), d_dy, dy_stride, d_x, x_stride,
+                                           d_mean, d_rstd, d_weight, d_dx, dx_stride, d_dweight,
+                                           d_dbias, d_workspace, rows, cols,
+                                           static_cast<void*>(stream)));
 }
 
 }  // namespace thunderfft

@@ -26,10 +26,17 @@ __all__ = [
     "ThunderFFT_global", "ThunderFFT_global_async", "twiddle_info", "fill_uniform",
     "fft", "transforms_per_block", "LIB_PATH", "ThunderFFT_conv1d", "ThunderFFT_conv1d_async",
     "ThunderFFT_conv2d", "ThunderFFT_conv2d_async", "ThunderFFT_conv2d_noalloc", "copy_nt",
+    "VALUE_TYPES", "ScanShape", "ThunderFFT_gated_scan", "ThunderFFT_gated_scan_async",
+    "ThunderFFT_gated_scan_backward", "ThunderFFT_gated_scan_backward_async",
+    "ThunderFFT_layer_norm", "ThunderFFT_layer_norm_async", "ThunderFFT_layer_norm_backward",
+    "ThunderFFT_layer_norm_backward_async", "layer_norm_workspace_bytes", "gated_scan",
+    "layer_norm",
 ]
 
 SUPPORTED_N = (64, 128, 256, 512, 1024, 2048, 4096)
 PRECISIONS = {"float": 0, "half": 1}
+# Types of the sequence operators' values.
+VALUE_TYPES = {"float": 0, "half": 1, "bfloat16": 2}
 THFF_OK, THFF_EINVAL, THFF_EIO = 0, -22, -5
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libthunderfft_amd.so")
@@ -82,6 +89,20 @@ def lib() -> ctypes.CDLL:
         L.thff_fill_uniform.argtypes = [ctypes.c_int, vp, ctypes.c_longlong, ctypes.c_ulonglong,
                                         ctypes.c_longlong, vp]
         L.thff_copy_nt.argtypes = [vp, vp, ctypes.c_longlong, vp]
+        i32, i64, f32 = ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+        sp = ctypes.POINTER(ScanShape)
+        for name in ("saved", "workspace"):
+            fn = getattr(L, f"thff_gated_scan_{name}_bytes")
+            fn.argtypes, fn.restype = [sp], i64
+        L.thff_layer_norm_workspace_bytes.argtypes = [i64, i32]
+        L.thff_layer_norm_workspace_bytes.restype = i64
+        for twin in ("", "_async"):
+            getattr(L, "thff_gated_scan" + twin).argtypes = [sp] + [vp] * 10
+            getattr(L, "thff_gated_scan_backward" + twin).argtypes = [sp] + [vp] * 11
+            getattr(L, "thff_layer_norm" + twin).argtypes = [
+                i32, vp, i64, vp, vp, f32, vp, i64, vp, vp, i64, i32, vp]
+            getattr(L, "thff_layer_norm_backward" + twin).argtypes = [
+                i32, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i32, vp]
         _lib = L
     return _lib
 
@@ -230,6 +251,189 @@ def ThunderFFT_conv2d_noalloc(T, rows: int, cols: int, d_x, d_h, d_y, batch: int
     that overlap on one GPU race)."""
     _raise(lib().thff_conv2d_noalloc(_precision(T), int(rows), int(cols), _ptr(d_x), _ptr(d_h),
                                      _ptr(d_y), int(batch), _stream(stream)))
+
+
+def _value_type(T) -> int:
+    if isinstance(T, str) and T in VALUE_TYPES:
+        return VALUE_TYPES[T]
+    name = str(T).rpartition(".")[2]
+    for key, code in (("float32", 0), ("float16", 1), ("bfloat16", 2)):
+        if name == key:
+            return code
+    raise ValueError(f"the sequence operators support float, half and bfloat16 only (got {T!r})")
+
+
+class ScanShape(ctypes.Structure):
+    """What a gated scan works on; kept by the caller from call to call.
+
+    T: "float", "half" or "bfloat16" (or the torch dtype).  layout: "channels_last",
+    values [batch][n][channels], or "channels_first", values [batch][channels][n] as the
+    convolutions have them.  Strides: elements between the starts of consecutive rows (a
+    step's channels, or a channel's steps), None for rows without a gap; x_stride and
+    gate_stride hold for the gradients of x and the gate too.  states: rows of the state
+    pool that slots index (None: batch).
+    """
+
+    _fields_ = [("precision", ctypes.c_int), ("layout", ctypes.c_int), ("batch", ctypes.c_int),
+                ("n", ctypes.c_int), ("channels", ctypes.c_int), ("states", ctypes.c_int),
+                ("x_stride", ctypes.c_longlong), ("gate_stride", ctypes.c_longlong),
+                ("y_stride", ctypes.c_longlong)]
+    LAYOUTS = {"channels_last": 0, "channels_first": 1}
+
+    def __init__(self, T, batch, n, channels, layout="channels_last", x_stride=None,
+                 gate_stride=None, y_stride=None, states=None):
+        if layout not in self.LAYOUTS:
+            raise ValueError(f"layout must be one of {sorted(self.LAYOUTS)} (got {layout!r})")
+        states = batch if states is None else states
+        for v, what in ((batch, "batch"), (n, "n"), (channels, "channels"), (states, "states")):
+            if not -2**31 <= int(v) < 2**31:
+                raise ValueError(f"{what} is out of range")
+        super().__init__(_value_type(T), self.LAYOUTS[layout], int(batch), int(n), int(channels),
+                         int(states), int(x_stride or 0), int(gate_stride or 0),
+                         int(y_stride or 0))
+
+    def saved_bytes(self) -> int:
+        """Bytes that the forward call keeps for the backward call (d_saved)."""
+        return _bytes(lib().thff_gated_scan_saved_bytes(ctypes.byref(self)))
+
+    def workspace_bytes(self) -> int:
+        """Bytes of a call's scratch memory (d_workspace)."""
+        return _bytes(lib().thff_gated_scan_workspace_bytes(ctypes.byref(self)))
+
+
+def _bytes(rc: int) -> int:
+    if rc < 0:
+        _raise(int(rc))
+    return int(rc)
+
+
+def _gated_scan(call, shape, d_x, d_gate, d_y, d_state_in, d_state_out, d_slots, d_lengths,
+                d_saved, d_workspace, stream):
+    _raise(call(shape, _ptr(d_x), _ptr(d_gate), _ptr(d_y), _ptr(d_state_in), _ptr(d_state_out),
+                _ptr(d_slots), _ptr(d_lengths), _ptr(d_saved), _ptr(d_workspace), _stream(stream)))
+
+
+def ThunderFFT_gated_scan(shape, d_x, d_gate, d_y, d_state_in=None, d_state_out=None, d_slots=None,
+                          d_lengths=None, d_saved=None, d_workspace=None, stream=0) -> None:
+    """Gated linear recurrence h[t] = f[t] h[t-1] + (1 - f[t]) x[t], f = sigmoid(gate), y = h,
+    on values of ``shape`` (a ScanShape).  The states before the first step (d_state_in) and
+    after the last (d_state_out, the same buffer if wanted) are float32 rows of `channels`,
+    row b for sequence b or row d_slots[b] (int32) of a pool; d_lengths (int32) ends each
+    sequence early.  d_saved (shape.saved_bytes()) is kept for the backward call, d_workspace
+    (shape.workspace_bytes()) is scratch.  Synchronous."""
+    _gated_scan(lib().thff_gated_scan, shape, d_x, d_gate, d_y, d_state_in, d_state_out, d_slots,
+                d_lengths, d_saved, d_workspace, stream)
+
+
+def ThunderFFT_gated_scan_async(shape, d_x, d_gate, d_y, d_state_in=None, d_state_out=None,
+                                d_slots=None, d_lengths=None, d_saved=None, d_workspace=None,
+                                stream=0) -> None:
+    """As ThunderFFT_gated_scan, but returns once the work is enqueued on ``stream``."""
+    _gated_scan(lib().thff_gated_scan_async, shape, d_x, d_gate, d_y, d_state_in, d_state_out,
+                d_slots, d_lengths, d_saved, d_workspace, stream)
+
+
+def _gated_scan_backward(call, shape, d_dy, d_x, d_gate, d_saved, d_dx, d_dgate, d_dstate_out,
+                         d_dstate_in, d_lengths, d_workspace, stream):
+    _raise(call(shape, _ptr(d_dy), _ptr(d_x), _ptr(d_gate), _ptr(d_saved), _ptr(d_dstate_out),
+                _ptr(d_lengths), _ptr(d_dx), _ptr(d_dgate), _ptr(d_dstate_in), _ptr(d_workspace),
+                _stream(stream)))
+
+
+def ThunderFFT_gated_scan_backward(shape, d_dy, d_x, d_gate, d_saved, d_dx, d_dgate,
+                                   d_dstate_out=None, d_dstate_in=None, d_lengths=None,
+                                   d_workspace=None, stream=0) -> None:
+    """Gradients of ThunderFFT_gated_scan by x, the gate and the first state (d_dstate_in,
+    float32 [batch][channels]) from those by y (d_dy) and by the last states (d_dstate_out,
+    None: zero); d_saved is what the forward call of the same shape, x, gate and lengths
+    wrote.  Synchronous."""
+    _gated_scan_backward(lib().thff_gated_scan_backward, shape, d_dy, d_x, d_gate, d_saved, d_dx,
+                         d_dgate, d_dstate_out, d_dstate_in, d_lengths, d_workspace, stream)
+
+
+def ThunderFFT_gated_scan_backward_async(shape, d_dy, d_x, d_gate, d_saved, d_dx, d_dgate,
+                                         d_dstate_out=None, d_dstate_in=None, d_lengths=None,
+                                         d_workspace=None, stream=0) -> None:
+    """As ThunderFFT_gated_scan_backward, but returns once the work is enqueued."""
+    _gated_scan_backward(lib().thff_gated_scan_backward_async, shape, d_dy, d_x, d_gate, d_saved,
+                         d_dx, d_dgate, d_dstate_out, d_dstate_in, d_lengths, d_workspace, stream)
+
+
+def _layer_norm(call, T, d_x, d_weight, d_bias, eps, d_y, rows, cols, d_mean, d_rstd, x_stride,
+                y_stride, stream):
+    _raise(call(_value_type(T), _ptr(d_x), x_stride or 0, _ptr(d_weight), _ptr(d_bias), eps,
+                _ptr(d_y), y_stride or 0, _ptr(d_mean), _ptr(d_rstd), rows, _int(cols),
+                _stream(stream)))
+
+
+def _int(v) -> int:
+    # ctypes would wrap a larger number round.
+    if not -2**31 <= v < 2**31:
+        raise ValueError(f"{v} is out of range")
+    return v
+
+
+def ThunderFFT_layer_norm(T, d_x, d_weight, d_bias, eps, d_y, rows, cols, d_mean=None, d_rstd=None,
+                          x_stride=None, y_stride=None, stream=0) -> None:
+    """Layer norm y = (x - mean) rstd weight + bias of `rows` rows of `cols` values of type T;
+    weight and bias float32 (None: ones, zeros); d_mean and d_rstd (float32, one a row) keep
+    the statistics for the backward call.  Synchronous."""
+    _layer_norm(lib().thff_layer_norm, T, d_x, d_weight, d_bias, eps, d_y, rows, cols, d_mean,
+                d_rstd, x_stride, y_stride, stream)
+
+
+def ThunderFFT_layer_norm_async(T, d_x, d_weight, d_bias, eps, d_y, rows, cols, d_mean=None,
+                                d_rstd=None, x_stride=None, y_stride=None, stream=0) -> None:
+    """As ThunderFFT_layer_norm, but returns once the launch is enqueued on ``stream``."""
+    _layer_norm(lib().thff_layer_norm_async, T, d_x, d_weight, d_bias, eps, d_y, rows, cols, d_mean,
+                d_rstd, x_stride, y_stride, stream)
+
+
+def layer_norm_workspace_bytes(rows: int, cols: int) -> int:
+    """Bytes of ThunderFFT_layer_norm_backward's d_workspace."""
+    return _bytes(lib().thff_layer_norm_workspace_bytes(int(rows), _int(int(cols))))
+
+
+def _layer_norm_backward(call, T, d_dy, d_x, d_mean, d_rstd, d_weight, d_dx, d_dweight, d_dbias,
+                         d_workspace, rows, cols, dy_stride, x_stride, dx_stride, stream):
+    _raise(call(_value_type(T), _ptr(d_dy), dy_stride or 0, _ptr(d_x), x_stride or 0, _ptr(d_mean),
+                _ptr(d_rstd), _ptr(d_weight), _ptr(d_dx), dx_stride or 0, _ptr(d_dweight),
+                _ptr(d_dbias), _ptr(d_workspace), rows, _int(cols), _stream(stream)))
+
+
+def ThunderFFT_layer_norm_backward(T, d_dy, d_x, d_mean, d_rstd, d_weight, d_dx, d_dweight, d_dbias,
+                                   d_workspace, rows, cols, dy_stride=None, x_stride=None,
+                                   dx_stride=None, stream=0) -> None:
+    """Gradients of ThunderFFT_layer_norm by x and, in float32, by the weight and the bias
+    (None: not computed), from that by y, x and the forward call's statistics.  Synchronous."""
+    _layer_norm_backward(lib().thff_layer_norm_backward, T, d_dy, d_x, d_mean, d_rstd, d_weight,
+                         d_dx, d_dweight, d_dbias, d_workspace, rows, cols, dy_stride, x_stride,
+                         dx_stride, stream)
+
+
+def ThunderFFT_layer_norm_backward_async(T, d_dy, d_x, d_mean, d_rstd, d_weight, d_dx, d_dweight,
+                                         d_dbias, d_workspace, rows, cols, dy_stride=None,
+                                         x_stride=None, dx_stride=None, stream=0) -> None:
+    """As ThunderFFT_layer_norm_backward, but returns once the work is enqueued."""
+    _layer_norm_backward(lib().thff_layer_norm_backward_async, T, d_dy, d_x, d_mean, d_rstd,
+                         d_weight, d_dx, d_dweight, d_dbias, d_workspace, rows, cols, dy_stride,
+                         x_stride, dx_stride, stream)
+
+
+def gated_scan(x, gate, state=None, lengths=None, layout="channels_last"):
+    """(y, last states) of the gated linear recurrence on CUDA tensors, differentiable by x,
+    gate and state: see thunderfft_amd.sequence.gated_scan."""
+    from . import sequence
+
+    return sequence.gated_scan(x, gate, state, lengths, layout)
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
+    """Layer norm of a CUDA tensor's last axis, differentiable by x, weight and bias: see
+    thunderfft_amd.sequence.layer_norm."""
+    from . import sequence
+
+    return sequence.layer_norm(x, weight, bias, eps)
 
 
 def twiddle_info(T) -> tuple[int, int]:

@@ -50,8 +50,11 @@ def units() -> list[tuple[str, str, list[str]]]:
     for n in LENGTHS:
         out.append((os.path.join(CSRC, "c2c_instance.hip"), os.path.join(BUILD, f"c2c_n{n}.o"),
                     [f"-DTHFF_N={n}"]))
-    out.append((os.path.join(CSRC, "fill.hip"), os.path.join(BUILD, "fill.o"), []))
-    out.append((os.path.join(CSRC, "capi.cpp"), os.path.join(BUILD, "capi.o"), ["-x", "hip"]))
+    for name in ("fill", "scan", "norm"):
+        out.append((os.path.join(CSRC, name + ".hip"), os.path.join(BUILD, name + ".o"), []))
+    for name in ("capi", "capi_sequence"):
+        out.append((os.path.join(CSRC, name + ".cpp"), os.path.join(BUILD, name + ".o"),
+                    ["-x", "hip"]))
     return out
 
 

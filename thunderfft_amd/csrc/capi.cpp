@@ -16,10 +16,11 @@
 #include <string>
 #include <vector>
 
+#include "errors.hpp"
 #include "launch.hpp"
 #include "thunderfft/thunderfft.h"
 
-namespace {
+namespace thff {
 
 thread_local std::string g_last_error;
 
@@ -31,6 +32,14 @@ int fail(int code, const std::string& message) {
 int fail_hip(hipError_t err, const char* context) {
     return fail(THFF_EIO, std::string("[ThunderFFT] ") + context + ": " + hipGetErrorString(err));
 }
+
+}  // namespace thff
+
+namespace {
+
+using thff::fail;
+using thff::fail_hip;
+using thff::g_last_error;
 
 bool supported_length(int n) {
     return n == 64 || n == 128 || n == 256 || n == 512 || n == 1024 || n == 2048 || n == 4096;
