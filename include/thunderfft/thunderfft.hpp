@@ -13,7 +13,6 @@
 // hold N throws std::runtime_error instead of running without it.
 #pragma once
 
-#include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -22,6 +21,9 @@
 #include <type_traits>
 
 #include "thunderfft/thunderfft.h"
+
+// Only pointers to it appear here; <hip/hip_bf16.h>, which g++ does not take, defines it.
+struct __hip_bfloat16;
 
 template <class T>
 using vec2_t = typename std::conditional_t<std::is_same_v<std::remove_cv_t<T>, float>, float2,
