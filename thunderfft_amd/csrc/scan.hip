@@ -3,28 +3,19 @@
 // and its gradients: lam[t] = dy[t] + f[t+1] lam[t+1],
 //   dx[t] = (1 - f[t]) lam[t],  dgate[t] = lam[t] (h[t-1] - x[t]) f[t] (1 - f[t]).
 // Values of steps at or past a sequence's length reach no result.
+#include <algorithm>
+#include <atomic>
+
+#include "scan_last.hpp"
 #include "sequence.hpp"
 #include "sequence_io.hpp"
 
 namespace thff {
 namespace {
 
-// Steps between the states that the forward pass saves for the backward pass.
-constexpr int kSavedSteps = 16;
+// Steps between the saved states of the channels-first kernels.
+constexpr int kChunk = 16;
 constexpr int kLanes = 256;
-
-struct Gate {
-    float keep;   // sigmoid(g)
-    float enter;  // 1 - sigmoid(g) = sigmoid(-g)
-};
-
-// Both from e = exp(-|g|) <= 1, so that neither overflows nor cancels.
-__device__ __forceinline__ Gate gate_of(float g) {
-    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
-    const float r = __builtin_amdgcn_rcpf(1.0f + e);
-    const float s = e * r;
-    return g >= 0.0f ? Gate{r, s} : Gate{s, r};
-}
 
 struct Element {
     long long x, gate, y;  // offsets of step t
@@ -41,17 +32,6 @@ __device__ __forceinline__ Element first_element(const ScanShape& s, int b, int 
             s.x_stride, s.gate_stride, s.y_stride};
 }
 
-__device__ __forceinline__ int length_of(const int* lengths, int b, int n) {
-    return lengths ? min(max(lengths[b], 0), n) : n;
-}
-
-// Row of the state pool for sequence b, or -1 (none).
-__device__ __forceinline__ int state_row(const ScanShape& s, const int* slots, int b) {
-    if (!slots) return b;
-    const int row = slots[b];
-    return row >= 0 && row < s.states ? row : -1;
-}
-
 template <class T>
 __global__ __launch_bounds__(kLanes) void scan_forward(ScanShape s, ScanForward a) {
     const long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x;
@@ -59,12 +39,12 @@ __global__ __launch_bounds__(kLanes) void scan_forward(ScanShape s, ScanForward 
     const int b = static_cast<int>(i / s.channels), c = static_cast<int>(i % s.channels);
     const int len = length_of(a.lengths, b, s.n), row = state_row(s, a.slots, b);
     const long long state = static_cast<long long>(row) * s.channels + c;
-    const int chunks = (s.n + kSavedSteps - 1) / kSavedSteps;
+    const int chunks = (s.n + kChunk - 1) / kChunk;
     Element e = first_element(s, b, c);
     float h = a.state_in && row >= 0 ? a.state_in[state] : 0.0f;
     for (int t = 0; t < s.n; ++t) {
-        if (a.saved && t % kSavedSteps == 0)
-            a.saved[(static_cast<long long>(b) * chunks + t / kSavedSteps) * s.channels + c] = h;
+        if (a.saved && t % kChunk == 0)
+            a.saved[(static_cast<long long>(b) * chunks + t / kChunk) * s.channels + c] = h;
         float out = 0.0f;
         if (t < len) {
             const Gate g = gate_of(to_float(static_cast<const T*>(a.gate)[e.gate]));
@@ -83,7 +63,7 @@ __global__ __launch_bounds__(kLanes) void scan_backward(ScanShape s, ScanBackwar
     if (i >= static_cast<long long>(s.batch) * s.channels) return;
     const int b = static_cast<int>(i / s.channels), c = static_cast<int>(i % s.channels);
     const int len = length_of(a.lengths, b, s.n);
-    const int chunks = (s.n + kSavedSteps - 1) / kSavedSteps;
+    const int chunks = (s.n + kChunk - 1) / kChunk;
     const Element e = first_element(s, b, c);
     const T* x = static_cast<const T*>(a.x) + e.x;
     const T* gate = static_cast<const T*>(a.gate) + e.gate;
@@ -92,17 +72,17 @@ __global__ __launch_bounds__(kLanes) void scan_backward(ScanShape s, ScanBackwar
     T* dgate = static_cast<T*>(a.dgate) + e.gate;
     float carried = a.dstate_out ? a.dstate_out[i] : 0.0f;
     for (int chunk = chunks - 1; chunk >= 0; --chunk) {
-        const int t0 = chunk * kSavedSteps;
-        float before[kSavedSteps];
+        const int t0 = chunk * kChunk;
+        float before[kChunk];
         float h = a.saved[(static_cast<long long>(b) * chunks + chunk) * s.channels + c];
-        for (int k = 0; k < kSavedSteps; ++k) {
+        for (int k = 0; k < kChunk; ++k) {
             before[k] = h;
             if (t0 + k < len) {
                 const Gate g = gate_of(to_float(gate[(t0 + k) * e.gate_step]));
                 h = fmaf(g.keep, h, g.enter * to_float(x[(t0 + k) * e.x_step]));
             }
         }
-        for (int k = kSavedSteps - 1; k >= 0; --k) {
+        for (int k = kChunk - 1; k >= 0; --k) {
             const int t = t0 + k;
             if (t >= s.n) continue;
             float gx = 0.0f, gg = 0.0f;
@@ -125,40 +105,157 @@ unsigned blocks_of(const ScanShape& s) {
                                  kLanes);
 }
 
+// Compute units of the current device.
+hipError_t compute_units(int* out) {
+    constexpr int kMost = 64;
+    static std::atomic<int> known[kMost] = {};
+    int device = 0;
+    hipError_t err = hipGetDevice(&device);
+    if (err != hipSuccess) return err;
+    const bool kept = device >= 0 && device < kMost;
+    int cus = kept ? known[device].load(std::memory_order_relaxed) : 0;
+    if (cus == 0) {
+        err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+        if (err != hipSuccess) return err;
+        if (kept) known[device].store(cus, std::memory_order_relaxed);
+    }
+    *out = cus;
+    return hipSuccess;
+}
+
+// Empties the chain's words and sets its counter to zero.  (A kernel: a captured memset is
+// not replayed reliably.)
+__global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long count) {
+    const long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x;
+    if (i >= count) return;
+    const unsigned v = i < kChainHead / 16 ? 0u : ~0u;
+    to[i] = make_uint4(v, v, v, v);
+}
+
+// Lanes along the channels: all 64 of a wave, or 16 where that leaves far fewer of them idle.
+bool narrow(const ScanShape& s) {
+    const long long wide = (s.channels + 127LL) / 128 * 128, thin = (s.channels + 31LL) / 32 * 32;
+    return 4 * wide > 5 * thin;
+}
+
+// Calls f with the tile type of a shape's forward or backward pass.
+template <class T, bool Backward, class F>
+auto with_tile(const ScanShape& s, F f) {
+    constexpr int S = !Backward && sizeof(T) == 2 ? 16 : 8;
+    return narrow(s) ? f(Tile<2, 16, S, 8>{}) : f(Tile<2, 64, S, 8>{});
+}
+
+// Calls f with a value of the shape's type.
+template <class F>
+auto with_type(const ScanShape& s, F f) {
+    if (s.precision == THFF_FLOAT) return f(float{});
+    if (s.precision == THFF_HALF) return f(half_t{});
+    return f(bfloat_t{});
+}
+
+template <class L>
+Chain chain_of(const ScanShape& s, void* workspace) {
+    Chain chain;
+    chain.drawn = static_cast<unsigned*>(workspace);
+    chain.words = reinterpret_cast<Word*>(static_cast<char*>(workspace) + kChainHead);
+    chain.slabs = (s.channels + L::kChannels - 1) / L::kChannels;
+    chain.tiles = s.n > 0 ? (s.n + L::kSteps - 1) / L::kSteps : 1;
+    chain.total = static_cast<unsigned>(s.batch) * chain.slabs * chain.tiles;
+    return chain;
+}
+
+template <class L>
+long long chain_bytes(const ScanShape& s) {
+    const Chain chain = chain_of<L>(s, nullptr);
+    if (chain.tiles <= 1) return 0;
+    return kChainHead + 8LL * s.batch * chain.slabs * L::kChannels * chain.tiles;
+}
+
+template <class L>
+bool chain_fits(const ScanShape& s) {
+    const Chain chain = chain_of<L>(s, nullptr);
+    return static_cast<__int128>(s.batch) * chain.slabs * chain.tiles <= 0x7fffffff;
+}
+
+template <class T, class L, class Args>
+hipError_t launch_last(void (*kernel)(ScanShape, Args, Chain), const ScanShape& s, const Args& a,
+                       hipStream_t stream) {
+    int cus = 0;
+    hipError_t err = compute_units(&cus);
+    if (err != hipSuccess) return err;
+    const Chain chain = chain_of<L>(s, a.workspace);
+    const long long bytes = chain_bytes<L>(s);
+    if (bytes) {
+        const long long count = bytes / 16;
+        clear_chain<<<static_cast<unsigned>((count + kLanes - 1) / kLanes), kLanes, 0, stream>>>(
+            static_cast<uint4*>(a.workspace), count);
+        err = hipGetLastError();
+        if (err != hipSuccess) return err;
+    }
+    // Two workgroups of 8 waves a compute unit, each tile after tile.
+    const unsigned blocks = std::min(chain.total, static_cast<unsigned>(2 * cus));
+    kernel<<<blocks, L::kLanes, 0, stream>>>(s, a, chain);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 long long scan_saved_bytes(const ScanShape& s) {
-    const long long chunks = (static_cast<long long>(s.n) + kSavedSteps - 1) / kSavedSteps;
+    const int steps = s.channels_first ? kChunk : kSavedSteps;
+    const long long chunks = (static_cast<long long>(s.n) + steps - 1) / steps;
     return 4 * chunks * s.batch * s.channels;
 }
 
-long long scan_workspace_bytes(const ScanShape&) { return 0; }
+long long scan_workspace_bytes(const ScanShape& s) {
+    if (s.channels_first) return 0;
+    const auto bytes = [&](auto tile) { return chain_bytes<decltype(tile)>(s); };
+    return with_type(s, [&](auto v) {
+        using T = decltype(v);
+        return std::max(with_tile<T, false>(s, bytes), with_tile<T, true>(s, bytes));
+    });
+}
 
 bool scan_fits(const ScanShape& s) {
-    return static_cast<long long>(s.batch) * s.channels <= 0x7fffffffLL;
+    if (static_cast<long long>(s.batch) * s.channels > 0x7fffffffLL) return false;
+    if (s.channels_first) return true;
+    const auto fits = [&](auto tile) { return chain_fits<decltype(tile)>(s); };
+    return with_type(s, [&](auto v) {
+        using T = decltype(v);
+        return with_tile<T, false>(s, fits) && with_tile<T, true>(s, fits);
+    });
+}
+
+template <class T>
+hipError_t forward_of(const ScanShape& s, const ScanForward& a, hipStream_t stream) {
+    if (s.channels_first) {
+        scan_forward<T><<<blocks_of(s), kLanes, 0, stream>>>(s, a);
+        return hipGetLastError();
+    }
+    return with_tile<T, false>(s, [&](auto tile) {
+        using L = decltype(tile);
+        return launch_last<T, L>(scan_last_forward<T, L>, s, a, stream);
+    });
+}
+
+template <class T>
+hipError_t backward_of(const ScanShape& s, const ScanBackward& a, hipStream_t stream) {
+    if (s.channels_first) {
+        scan_backward<T><<<blocks_of(s), kLanes, 0, stream>>>(s, a);
+        return hipGetLastError();
+    }
+    return with_tile<T, true>(s, [&](auto tile) {
+        using L = decltype(tile);
+        return launch_last<T, L>(scan_last_backward<T, L>, s, a, stream);
+    });
 }
 
 hipError_t launch_gated_scan(const ScanShape& s, const ScanForward& a, hipStream_t stream) {
-    const unsigned blocks = blocks_of(s);
-    if (s.precision == THFF_FLOAT)
-        scan_forward<float><<<blocks, kLanes, 0, stream>>>(s, a);
-    else if (s.precision == THFF_HALF)
-        scan_forward<half_t><<<blocks, kLanes, 0, stream>>>(s, a);
-    else
-        scan_forward<bfloat_t><<<blocks, kLanes, 0, stream>>>(s, a);
-    return hipGetLastError();
+    return with_type(s, [&](auto v) { return forward_of<decltype(v)>(s, a, stream); });
 }
 
 hipError_t launch_gated_scan_backward(const ScanShape& s, const ScanBackward& a,
                                       hipStream_t stream) {
-    const unsigned blocks = blocks_of(s);
-    if (s.precision == THFF_FLOAT)
-        scan_backward<float><<<blocks, kLanes, 0, stream>>>(s, a);
-    else if (s.precision == THFF_HALF)
-        scan_backward<half_t><<<blocks, kLanes, 0, stream>>>(s, a);
-    else
-        scan_backward<bfloat_t><<<blocks, kLanes, 0, stream>>>(s, a);
-    return hipGetLastError();
+    return with_type(s, [&](auto v) { return backward_of<decltype(v)>(s, a, stream); });
 }
 
 }  // namespace thff

@@ -19,4 +19,41 @@ __device__ __forceinline__ T from_float(float v) {
     return static_cast<T>(v);
 }
 
+// V values in one access that needs no more than the element's alignment (the hardware takes
+// unaligned vectors; rows of an odd length start on any element).
+template <class T, int V>
+using pack = T __attribute__((ext_vector_type(V), aligned(alignof(T))));
+
+template <class T, int V>
+__device__ __forceinline__ pack<T, V> load_pack(const T* p) {
+    return *reinterpret_cast<const pack<T, V>*>(p);
+}
+
+template <class T, int V>
+__device__ __forceinline__ void store_pack(T* p, pack<T, V> v) {
+    *reinterpret_cast<pack<T, V>*>(p) = v;
+}
+
+// The first `count` of V values; zeros for the others.
+template <class T, int V>
+__device__ __forceinline__ pack<T, V> load_some(const T* p, int count) {
+    if (count >= V) return load_pack<T, V>(p);
+    pack<T, V> v = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < count) v[i] = p[i];
+    return v;
+}
+
+template <class T, int V>
+__device__ __forceinline__ void store_some(T* p, pack<T, V> v, int count) {
+    if (count >= V) {
+        store_pack<T, V>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < count) p[i] = v[i];
+}
+
 }  // namespace thff
