@@ -4,7 +4,6 @@
 //   dx[t] = (1 - f[t]) lam[t],  dgate[t] = lam[t] (h[t-1] - x[t]) f[t] (1 - f[t]).
 // Values of steps at or past a sequence's length reach no result.
 #include <algorithm>
-#include <atomic>
 
 #include "scan_last.hpp"
 #include "sequence.hpp"
@@ -105,44 +104,28 @@ unsigned blocks_of(const ScanShape& s) {
                                  kLanes);
 }
 
-// Compute units of the current device.
-hipError_t compute_units(int* out) {
-    constexpr int kMost = 64;
-    static std::atomic<int> known[kMost] = {};
-    int device = 0;
-    hipError_t err = hipGetDevice(&device);
-    if (err != hipSuccess) return err;
-    const bool kept = device >= 0 && device < kMost;
-    int cus = kept ? known[device].load(std::memory_order_relaxed) : 0;
-    if (cus == 0) {
-        err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
-        if (err != hipSuccess) return err;
-        if (kept) known[device].store(cus, std::memory_order_relaxed);
-    }
-    *out = cus;
-    return hipSuccess;
-}
-
-// Empties the chain's words and sets its counter to zero.  (A kernel: a captured memset is
-// not replayed reliably.)
-__global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long count) {
+// Sets the counters of a chain to zero and empties its words.  (A kernel: a captured memset
+// is not replayed reliably.)
+__global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long counters,
+                                                      long long count) {
     const long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x;
     if (i >= count) return;
-    const unsigned v = i < kChainHead / 16 ? 0u : ~0u;
+    const unsigned v = i < counters ? 0u : ~0u;
     to[i] = make_uint4(v, v, v, v);
 }
 
-// Lanes along the channels: all 64 of a wave, or 16 where that leaves far fewer of them idle.
-bool narrow(const ScanShape& s) {
-    const long long wide = (s.channels + 127LL) / 128 * 128, thin = (s.channels + 31LL) / 32 * 32;
-    return 4 * wide > 5 * thin;
-}
-
-// Calls f with the tile type of a shape's forward or backward pass.
+// Calls f with the tile type of a shape's forward or backward pass: 4 bytes a lane and row;
+// lanes along the channels all 64 of a wave, or 16 where that leaves far fewer of them idle.
 template <class T, bool Backward, class F>
 auto with_tile(const ScanShape& s, F f) {
-    constexpr int S = !Backward && sizeof(T) == 2 ? 16 : 8;
-    return narrow(s) ? f(Tile<2, 16, S, 8>{}) : f(Tile<2, 64, S, 8>{});
+    constexpr int VEC = 4 / sizeof(T);
+    using Wide = std::conditional_t<Backward, Tile<VEC, 64, 8, 14, 2, 4>, Tile<VEC, 64, 8, 14, 2, 8>>;
+    using Thin = std::conditional_t<Backward, Tile<VEC, 16, 8, 14, 2, 4>, Tile<VEC, 16, 8, 14, 2, 8>>;
+    const auto taken = [&](long long channels) {
+        return (s.channels + channels - 1) / channels * channels;
+    };
+    const bool thin = 4 * taken(Wide::kChannels) > 5 * taken(Thin::kChannels);
+    return thin ? f(Thin{}) : f(Wide{});
 }
 
 // Calls f with a value of the shape's type.
@@ -156,11 +139,12 @@ auto with_type(const ScanShape& s, F f) {
 template <class L>
 Chain chain_of(const ScanShape& s, void* workspace) {
     Chain chain;
-    chain.drawn = static_cast<unsigned*>(workspace);
-    chain.words = reinterpret_cast<Word*>(static_cast<char*>(workspace) + kChainHead);
     chain.slabs = (s.channels + L::kChannels - 1) / L::kChannels;
     chain.tiles = s.n > 0 ? (s.n + L::kSteps - 1) / L::kSteps : 1;
-    chain.total = static_cast<unsigned>(s.batch) * chain.slabs * chain.tiles;
+    chain.columns = static_cast<unsigned>(s.batch) * chain.slabs;
+    chain.drawn = static_cast<unsigned*>(workspace);
+    chain.words = reinterpret_cast<Word*>(static_cast<char*>(workspace) +
+                                          static_cast<long long>(chain.columns) * kCounterBytes);
     return chain;
 }
 
@@ -168,7 +152,7 @@ template <class L>
 long long chain_bytes(const ScanShape& s) {
     const Chain chain = chain_of<L>(s, nullptr);
     if (chain.tiles <= 1) return 0;
-    return kChainHead + 8LL * s.batch * chain.slabs * L::kChannels * chain.tiles;
+    return chain.columns * (kCounterBytes + 8LL * L::kChannels * chain.tiles);
 }
 
 template <class L>
@@ -180,28 +164,23 @@ bool chain_fits(const ScanShape& s) {
 template <class T, class L, class Args>
 hipError_t launch_last(void (*kernel)(ScanShape, Args, Chain), const ScanShape& s, const Args& a,
                        hipStream_t stream) {
-    int cus = 0;
-    hipError_t err = compute_units(&cus);
-    if (err != hipSuccess) return err;
     const Chain chain = chain_of<L>(s, a.workspace);
     const long long bytes = chain_bytes<L>(s);
     if (bytes) {
         const long long count = bytes / 16;
         clear_chain<<<static_cast<unsigned>((count + kLanes - 1) / kLanes), kLanes, 0, stream>>>(
-            static_cast<uint4*>(a.workspace), count);
-        err = hipGetLastError();
+            static_cast<uint4*>(a.workspace), chain.columns * (kCounterBytes / 16LL), count);
+        const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
-    // Two workgroups of 8 waves a compute unit, each tile after tile.
-    const unsigned blocks = std::min(chain.total, static_cast<unsigned>(2 * cus));
-    kernel<<<blocks, L::kLanes, 0, stream>>>(s, a, chain);
+    kernel<<<chain.columns * chain.tiles, L::kLanes, 0, stream>>>(s, a, chain);
     return hipGetLastError();
 }
 
 }  // namespace
 
 long long scan_saved_bytes(const ScanShape& s) {
-    const int steps = s.channels_first ? kChunk : kSavedSteps;
+    const int steps = s.channels_first ? kChunk : kSaved;
     const long long chunks = (static_cast<long long>(s.n) + steps - 1) / steps;
     return 4 * chunks * s.batch * s.channels;
 }

@@ -4,16 +4,21 @@
 // A step is h -> f h + u with u = (1 - f) x.  Steps compose: (A, B) then (f, u) is
 // (f A, f B + u).  A lane takes VEC neighbouring channels of S steps and composes them; the
 // lanes and waves of a workgroup join theirs through LDS, and a tile's (A, B) is published
-// for the tiles behind it.  Every kGroup-th tile, the first one among them, publishes the
-// state after it instead; a tile starts from the last such state before it, led through the
-// (A, B) of the tiles in between, always in this order, so that the result does not depend
-// on timing.  The backward pass goes the same way from the last step to the first, with
-// c -> f (dy + c), c the gradient that reaches a step from the steps behind it.
+// for the tiles behind it.  Counted from the first, every 64th tile publishes the state
+// after it instead, and every 8th the span of the 8 tiles up to it: a tile starts from the
+// last such state before it, led through at most 7 spans of 8 tiles and 7 of single ones,
+// always in this order, so that the result does not depend on timing.  Only every 64th tile
+// waits for another's wait.  The backward pass goes the same way from the last step to the
+// first, with c -> f (dy + c), c the gradient that reaches a step from the steps behind it.
 //
 // Published words are 64 bits, (A, B) or (0, state), and empty ones all ones: each is
-// valid as soon as it is seen, without fences.  Workgroups draw tiles from a counter,
-// first steps first, and publish before they wait, and wait only for tiles drawn earlier,
-// which running workgroups hold: every wait ends.
+// valid as soon as it is seen, without fences.  A workgroup draws its tile from a counter
+// of its column, first steps first, publishes before it waits, and waits only for tiles
+// drawn earlier, which running workgroups hold: every wait ends.  (One counter for all
+// columns takes 11.6 ns a draw, 48 us for 4096 workgroups; one for each takes nothing.)
+//
+// A workgroup takes one tile and ends: one that goes on to the next waits, with the first
+// load it needs, for its last tile's stores, which the same counter counts.
 #pragma once
 
 #include <type_traits>
@@ -28,12 +33,12 @@ struct Gate {
     float enter;  // 1 - sigmoid(g) = sigmoid(-g)
 };
 
-// Both from e = exp(-|g|) <= 1, so that neither overflows nor cancels.
+// Both from e = exp(-g), so that neither cancels; e is held at 2^126, where f is 2^-126 and
+// 1 - f is 1, so that it does not overflow.  A NaN stays one (the minimum that keeps it).
 __device__ __forceinline__ Gate gate_of(float g) {
-    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
-    const float r = __builtin_amdgcn_rcpf(1.0f + e);
-    const float s = e * r;
-    return g >= 0.0f ? Gate{r, s} : Gate{s, r};
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(-1.44269504f * g, 126.0f));
+    const float f = __builtin_amdgcn_rcpf(1.0f + e);
+    return {f, e * f};
 }
 
 __device__ __forceinline__ int length_of(const int* lengths, int b, int n) {
@@ -47,9 +52,7 @@ __device__ __forceinline__ int state_row(const ScanShape& s, const int* slots, i
     return row >= 0 && row < s.states ? row : -1;
 }
 
-// Steps between the states that the forward pass saves for the backward pass.
-constexpr int kSavedSteps = 64;
-constexpr int kGroup = 16;
+constexpr int kGroup = 8, kSuper = 64;
 
 // (A, B) of some steps: h -> A h + B.
 struct Span {
@@ -81,25 +84,29 @@ __device__ __forceinline__ Span span_of(Word w) {
     return {__uint_as_float(static_cast<unsigned>(w)), __uint_as_float(static_cast<unsigned>(w >> 32))};
 }
 
-// The workspace: a counter, then a word for every channel of every tile.
+// The workspace: a counter for every column of tiles, far enough apart, then a word for every
+// channel of every tile.
 struct Chain {
     unsigned* drawn;
     Word* words;
     int slabs, tiles;  // tiles along the channels, along the steps
-    unsigned total;    // batch * slabs * tiles
+    unsigned columns;  // batch * slabs
 };
-constexpr long long kChainHead = 128;
+constexpr int kCounterBytes = 64;
 
 // VEC channels and S steps a lane; CL lanes side by side along the channels, the other
-// lanes of a wave and the W waves one behind the other along the steps.
-template <int VEC_, int CL_, int S_, int W_>
+// lanes of a wave and the W waves one behind the other along the steps.  C more waves draw
+// tiles and wait for the chain, a lane for each channel or two.  Occupancy: waves that a
+// SIMD is to hold.
+template <int VEC_, int CL_, int S_, int W_, int C_, int Occupancy_>
 struct Tile {
-    static constexpr int VEC = VEC_, CL = CL_, S = S_, W = W_;
+    static constexpr int VEC = VEC_, CL = CL_, S = S_, W = W_, C = C_;
+    static constexpr int kOccupancy = Occupancy_, kLanes = 64 * (W + C);
     static constexpr int kChannels = VEC * CL;
-    static constexpr int kSubs = W * (64 / CL);
-    static constexpr int kSteps = kSubs * S;
-    static constexpr int kLanes = 64 * W;
+    static constexpr int kSteps = W * (64 / CL) * S;
 };
+// Steps between the states that the forward pass saves for the backward pass.
+constexpr int kSaved = 56;
 
 // Joins the lanes' spans of a wave along the steps (lanes CL apart): `mine` becomes the span
 // of everything up to and with this lane, the result is that of everything before it.
@@ -122,50 +129,86 @@ __device__ __forceinline__ Span join_lanes(Span& mine) {
     return before;
 }
 
-// What the r-th tile of a column's chain starts from, put into `items` for the whole
-// workgroup: for r = 0 the state given (`first`, `some` values, or null for zeros), else
-// the last published state before the tile and the spans of the tiles in between, an item
-// for each lane along the steps to wait for.  words: the chain's first tile; step: words
-// from a tile to the next.
-template <class L>
-__device__ __forceinline__ void gather(const float* first, int some, const Word* words,
-                                       long long step, int r, Span (*items)[L::kChannels]) {
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int sub = wave * (64 / L::CL) + lane / L::CL, c = lane % L::CL * L::VEC;
-    if (r == 0) {
-        // Through LDS, so that it has been read before anyone stores a last state there.
-        if (sub == 0) {
-#pragma unroll
-            for (int v = 0; v < L::VEC; ++v)
-                items[0][c + v] = {0.0f, first && v < some ? first[v] : 0.0f};
-        }
-        return;
-    }
-    const int base = (r - 1) / kGroup * kGroup;
-    for (int item = sub; item < r - base; item += L::kSubs) {
-        const Word* at = words + (base + item) * step + c;
-        Word w[L::VEC];
-        bool all;
-        do {
-            all = true;
-#pragma unroll
-            for (int v = 0; v < L::VEC; ++v) w[v] = look(at + v);
-#pragma unroll
-            for (int v = 0; v < L::VEC; ++v) all = all && static_cast<unsigned>(w[v]) != ~0u;
-        } while (!all);
-#pragma unroll
-        for (int v = 0; v < L::VEC; ++v) items[item][c + v] = span_of(w[v]);
-    }
+// What a tile publishes for a channel.
+__device__ __forceinline__ Span seen(Word& w, const Word* at) {
+    while (static_cast<unsigned>(w) == ~0u) w = look(at);
+    return span_of(w);
 }
 
-// The state at the start of the r-th tile of the chain, for the channel at `c`.
-template <class L>
-__device__ __forceinline__ float start_of(int r, int c, const Span (*items)[L::kChannels]) {
-    float h = items[0][c].b;
-    const int count = r == 0 ? 1 : r - (r - 1) / kGroup * kGroup;
-    for (int i = 1; i < count; ++i) h = after(items[i][c], h);
-    return h;
-}
+// N channels of the r-th tile of a chain.  words: theirs of the chain's first tile; step:
+// words from a tile to the next.
+template <int N>
+struct Link {
+    Word* words;
+    long long step;
+    int r;
+    Word one[kGroup - 1][N], group[kGroup - 1][N], state[N];
+
+    __device__ __forceinline__ int base() const { return (r - 1) / kSuper * kSuper; }
+    __device__ __forceinline__ int groups() const { return (r - 1 - base()) / kGroup; }
+    __device__ __forceinline__ int single() const { return (r - 1 - base()) % kGroup; }
+    __device__ __forceinline__ const Word* at_one(int i) const {
+        return words + (base() + groups() * kGroup + 1 + i) * step;
+    }
+    __device__ __forceinline__ const Word* at_group(int i) const {
+        return words + (base() + (i + 1) * kGroup) * step;
+    }
+
+    // Asks for what the tile needs of those before it, without waiting.
+    __device__ __forceinline__ void ask() {
+        if (r == 0) return;
+#pragma unroll
+        for (int i = 0; i < kGroup - 1; ++i)
+#pragma unroll
+            for (int v = 0; v < N; ++v) {
+                if (i < single()) one[i][v] = look(at_one(i) + v);
+                if (i < groups()) group[i][v] = look(at_group(i) + v);
+            }
+#pragma unroll
+        for (int v = 0; v < N; ++v) state[v] = look(words + base() * step + v);
+    }
+
+    // Publishes what the tiles behind it need (if `later`) of the tile, whose span is `own`,
+    // waits for the answers, and returns the state that the tile starts from, which for
+    // r = 0 is the one given.
+    __device__ __forceinline__ void join(float (&h)[N], const Span (&own)[N], bool later,
+                                         const float (&given)[N]) {
+        Word* here = words + r * step;
+        if (later && r % kGroup != 0) {
+#pragma unroll
+            for (int v = 0; v < N; ++v) publish(here + v, own[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < N; ++v) h[v] = given[v];
+        if (r > 0) {
+            Span near[N];
+#pragma unroll
+            for (int v = 0; v < N; ++v) near[v] = {1.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kGroup - 1; ++i)
+#pragma unroll
+                for (int v = 0; v < N; ++v)
+                    if (i < single()) near[v] = then(near[v], seen(one[i][v], at_one(i) + v));
+            if (later && r % kGroup == 0 && r % kSuper != 0) {
+#pragma unroll
+                for (int v = 0; v < N; ++v) publish(here + v, then(near[v], own[v]));
+            }
+#pragma unroll
+            for (int v = 0; v < N; ++v) h[v] = seen(state[v], words + base() * step + v).b;
+#pragma unroll
+            for (int i = 0; i < kGroup - 1; ++i)
+#pragma unroll
+                for (int v = 0; v < N; ++v)
+                    if (i < groups()) h[v] = after(seen(group[i][v], at_group(i) + v), h[v]);
+#pragma unroll
+            for (int v = 0; v < N; ++v) h[v] = after(near[v], h[v]);
+        }
+        if (later && r % kSuper == 0) {
+#pragma unroll
+            for (int v = 0; v < N; ++v) publish(here + v, {0.0f, after(own[v], h[v])});
+        }
+    }
+};
 
 template <class T>
 __device__ __forceinline__ T open_gate() {
@@ -184,289 +227,364 @@ __device__ __forceinline__ LaneOffset<L::CL> lane_offset(long long stride) {
     return lane / L::CL * L::S * stride + lane % L::CL * L::VEC;
 }
 
-// `inside` of the rows, and `some` values of each; `none` in the place of the others.
+// A stride that the compiler sees anew each time: it would keep a multiple of it for every
+// row, and has not so many registers.
+__device__ __forceinline__ long long anew(long long stride) {
+    asm volatile("" : "+s"(stride));
+    return stride;
+}
+
+// A lane's rows: `inside` are steps of the sequence, the next ones up to `rows` lie in the
+// tensor, and `some` of VEC channels.  full: all of the wave's are inside.
+struct Inside {
+    bool full;
+    int inside, rows, some;
+};
+
+// `none` in the place of what is not inside.  Where not all is, a lane reads its last row
+// instead of those past the tensor, and the last VEC channels instead of some of them and some
+// that are not there, so that no load waits for another or for a branch.
 template <class T, class L, class Offset>
 __device__ __forceinline__ void load_steps(pack<T, L::VEC> (&to)[L::S], const T* at, Offset lane,
-                                           long long stride, bool full, int inside, int some,
-                                           T none) {
-    if (full) {
+                                           long long stride, Inside in, int channels, T none) {
+    constexpr int VEC = L::VEC, S = L::S;
+    static_assert(VEC <= 4, "vectors are shifted by up to 3");
+    stride = anew(stride);
+    if (in.full) {
 #pragma unroll
-        for (int k = 0; k < L::S; ++k) to[k] = load_pack<T, L::VEC>(at + k * stride + lane);
+        for (int k = 0; k < S; ++k, at += stride) to[k] = load_pack<T, VEC>(at + lane);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < S; ++k) to[k] = none;
+    if (in.rows <= 0 || in.some <= 0) return;
+    const int shift = VEC - in.some;
+    const T* p = at + lane;
+    pack<T, VEC> v[S];
+    if (channels < VEC) {
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+            v[k] = none;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (i >= shift) v[k][i] = p[i - shift];
+            if (k < in.rows - 1) p += stride;
+        }
     } else {
+        p -= shift;
 #pragma unroll
-        for (int k = 0; k < L::S; ++k) {
-            to[k] = none;
-            if (k < inside && some > 0) to[k] = load_some<T, L::VEC>(at + k * stride + lane, some);
+        for (int k = 0; k < S; ++k) {
+            v[k] = load_pack<T, VEC>(p);
+            if (k < in.rows - 1) p += stride;
         }
     }
-}
-
-// Stores S rows, `rows` of them in the tensor, zeros from `inside` on.
-template <class T, class L, class Offset>
-__device__ __forceinline__ void store_steps(T* at, Offset lane, long long stride,
-                                            const pack<T, L::VEC> (&from)[L::S], bool full,
-                                            int inside, int rows, int some) {
-    if (full) {
 #pragma unroll
-        for (int k = 0; k < L::S; ++k) store_pack<T, L::VEC>(at + k * stride + lane, from[k]);
-    } else {
+    for (int k = 0; k < S; ++k) {
 #pragma unroll
-        for (int k = 0; k < L::S; ++k)
-            if (k < rows && some > 0)
-                store_some<T, L::VEC>(at + k * stride + lane,
-                                      k < inside ? from[k] : pack<T, L::VEC>{}, some);
+        for (int by = 1; by < VEC; by *= 2)
+            if (shift & by) {
+#pragma unroll
+                for (int i = 0; i + by < VEC; ++i) v[k][i] = v[k][i + by];
+            }
+        if (k < in.inside) to[k] = v[k];
     }
 }
 
-// Draws a tile.
-__device__ __forceinline__ unsigned draw(const Chain& chain) {
-    return __hip_atomic_fetch_add(chain.drawn, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Stores row k of a lane's S; zeros past the sequence's end.
+template <class T, int VEC>
+__device__ __forceinline__ void store_step(T* at, pack<T, VEC> v, int k, Inside in) {
+    if (in.full)
+        store_pack<T, VEC>(at, v);
+    else if (k < in.rows && in.some > 0)
+        store_some<T, VEC>(at, k < in.inside ? v : pack<T, VEC>{}, in.some);
+}
+
+// Where a tile lies: the same on every lane.
+template <class L, bool Backward>
+struct Place {
+    int tile, b, c0, len, column;
+
+    // The workgroup's, the `drawn`-th of its column.
+    __device__ __forceinline__ Place(int drawn, const ScanShape& s, const int* lengths,
+                                     const Chain& chain) {
+        tile = Backward ? chain.tiles - 1 - drawn : drawn;
+        column = blockIdx.x % chain.columns;
+        b = column / chain.slabs;
+        c0 = column % chain.slabs * L::kChannels;
+        len = length_of(lengths, b, s.n);
+    }
+    __device__ __forceinline__ int t0() const { return tile * L::kSteps; }
+    // A tile that lies past the sequence's end has zeros to write and no part in the chain.
+    __device__ __forceinline__ bool part() const { return t0() < len || tile == 0; }
+    // The lane's, whose first step is `sub` from the tile's.
+    __device__ __forceinline__ Inside inside(const ScanShape& s, int wave, int sub) const {
+        const int t = t0() + sub;
+        return {t0() + (wave + 1) * (64 / L::CL) * L::S <= len && c0 + L::kChannels <= s.channels,
+                max(0, min(L::S, len - t)), max(0, min(L::S, s.n - t)),
+                max(0, min(L::VEC,
+                           s.channels - c0 - static_cast<int>(threadIdx.x) % L::CL * L::VEC))};
+    }
+    // The first of the wave's rows.
+    __device__ __forceinline__ long long row(const ScanShape& s, int wave) const {
+        return static_cast<long long>(b) * s.n + t0() + wave * (64 / L::CL) * L::S;
+    }
+};
+
+__device__ __forceinline__ long long saved_at(const ScanShape& s, int b, int t, int steps) {
+    return (static_cast<long long>(b) * ((s.n + steps - 1) / steps) + t / steps) * s.channels;
+}
+
+// The waves that publish and wait for other tiles: spans of a tile's waves in
+// `waves`, in the order of the chain, and the state that the tile starts from in `start`.
+// state(p): where that of the chain's first tile is given for channel p.c0, or null.
+template <class L, bool Backward, class State>
+__device__ __forceinline__ void run_chain(const ScanShape& s, const int* lengths, const Chain& chain,
+                                          const Span (*waves)[L::kChannels], float* start,
+                                          int ticket, State state) {
+    constexpr int N = L::kChannels > 64 * L::C ? L::kChannels / (64 * L::C) : 1;
+    const int lane = threadIdx.x - 64 * L::W, c = lane * N;
+    const Place<L, Backward> p(ticket, s, lengths, chain);
+    const bool part = p.part() && c < L::kChannels;
+    Link<N> link;
+    link.words = chain.words + static_cast<long long>(p.column) * L::kChannels + c;
+    link.step = static_cast<long long>(chain.columns) * L::kChannels;
+    link.r = Backward ? max(p.len - 1, 0) / L::kSteps - p.tile : p.tile;
+    float given[N] = {};
+    if (part) {
+        link.ask();
+        const float* from = state(p);
+#pragma unroll
+        for (int v = 0; v < N; ++v)
+            if (link.r == 0 && from && p.c0 + c + v < s.channels) given[v] = from[c + v];
+    }
+    __syncthreads();
+    if (part) {
+        // Whether a tile waits for this one.
+        const bool later = Backward ? p.tile > 0 : p.t0() + L::kSteps < p.len;
+        Span all[N];
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            all[v] = waves[0][c + v];
+#pragma unroll
+            for (int w = 1; w < L::W; ++w) all[v] = then(all[v], waves[w][c + v]);
+        }
+        float h[N];
+        link.join(h, all, later, given);
+#pragma unroll
+        for (int v = 0; v < N; ++v) start[c + v] = h[v];
+    }
+    __syncthreads();
+}
+
+// Draws the workgroup's tile of its column, where tiles wait for each other.
+__device__ __forceinline__ int draw_tile(const Chain& chain, int* drawn) {
+    if (chain.tiles <= 1) return 0;
+    if (threadIdx.x == 0) {
+        unsigned* counter = chain.drawn + blockIdx.x % chain.columns * (kCounterBytes / 4);
+        *drawn = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(*drawn);
 }
 
 template <class T, class L>
-__global__ __launch_bounds__(L::kLanes, 4) void scan_last_forward(ScanShape s, ScanForward a,
+__global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(ScanShape s, ScanForward a,
                                                                   Chain chain) {
     constexpr int VEC = L::VEC, S = L::S, TL = 64 / L::CL;
+    using Where = Place<L, false>;
     __shared__ Span waves[L::W][L::kChannels];
-    __shared__ Span items[kGroup][L::kChannels];
-    __shared__ unsigned drawn;
+    __shared__ float start[L::kChannels];
+    __shared__ int drawn;
+    const int ticket = draw_tile(chain, &drawn);
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int sub = wave * TL + lane / L::CL, cl = lane % L::CL * VEC;
+    const int cl = lane % L::CL * VEC, sub = (wave * TL + lane / L::CL) * S;
+    if (wave >= L::W) {
+        run_chain<L, false>(s, a.lengths, chain, waves, start, ticket, [&](const Where& p) {
+            const int row = state_row(s, a.slots, p.b);
+            return a.state_in && row >= 0
+                       ? a.state_in + static_cast<long long>(row) * s.channels + p.c0
+                       : nullptr;
+        });
+        return;
+    }
     const auto at_x = lane_offset<L>(s.x_stride), at_gate = lane_offset<L>(s.gate_stride),
                at_y = lane_offset<L>(s.y_stride);
-    const bool chained = chain.tiles > 1;
-    const int columns = s.batch * chain.slabs;
-
-    unsigned ticket = blockIdx.x;
-    if (chained) {
-        if (threadIdx.x == 0) drawn = draw(chain);
-        __syncthreads();
-        ticket = __builtin_amdgcn_readfirstlane(drawn);
-        __syncthreads();
+    const Where p(ticket, s, a.lengths, chain);
+    const long long first = p.row(s, wave);
+    const Inside in = p.inside(s, wave, sub);
+    pack<T, VEC> x[S], g[S];
+    load_steps<T, L>(g, static_cast<const T*>(a.gate) + first * s.gate_stride + p.c0, at_gate,
+                     s.gate_stride, in, s.channels, open_gate<T>());
+    load_steps<T, L>(x, static_cast<const T*>(a.x) + first * s.x_stride + p.c0, at_x, s.x_stride, in,
+                     s.channels, static_cast<T>(0.0f));
+    float f[S][VEC], u[S][VEC];
+    Span before[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) before[v] = {1.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const Gate q = gate_of(to_float<T>(g[k][v]));
+            f[k][v] = q.keep;
+            u[k][v] = q.enter * to_float<T>(x[k][v]);
+            before[v] = then(before[v], {f[k][v], u[k][v]});
+        }
     }
-    while (ticket < chain.total) {
-        unsigned next = 0;
-        if (chained && threadIdx.x == 0) next = draw(chain);
-        const int tile = ticket / columns, column = ticket % columns;
-        const int b = column / chain.slabs, c0 = column % chain.slabs * L::kChannels, c = c0 + cl;
-        const int some = max(0, min(VEC, s.channels - c));
-        const int len = length_of(a.lengths, b, s.n);
-        const int t0 = tile * L::kSteps, t = t0 + sub * S;
-        const int rows = max(0, min(S, s.n - t)), inside = max(0, min(S, len - t));
-        const long long row = static_cast<long long>(b) * s.n + t0 + wave * TL * S;  // the wave's first
-        T* y = static_cast<T*>(a.y) + row * s.y_stride + c0;
-        const bool full = t0 + L::kSteps <= len && c0 + L::kChannels <= s.channels;
-        // A tile that lies past the sequence's end has zeros to write and no part in the chain.
-        const bool part = t0 < len || tile == 0;
-        pack<T, VEC> x[S], g[S];
-        float f[S][VEC], u[S][VEC];
-        Span mine[VEC], before[VEC];
-        if (part) {
-            load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + c0, at_gate, s.gate_stride,
-                             full, inside, some, open_gate<T>());
-            load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + c0, at_x, s.x_stride,
-                             full, inside, some, static_cast<T>(0.0f));
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                mine[v] = {1.0f, 0.0f};
+    for (int v = 0; v < VEC; ++v) {
+        Span mine = before[v];
+        before[v] = join_lanes<L::CL, false>(mine);
+        if (lane / L::CL == TL - 1) waves[wave][cl + v] = mine;
+    }
+    __syncthreads();
 #pragma unroll
-                for (int k = 0; k < S; ++k) {
-                    const Gate q = gate_of(to_float<T>(g[k][v]));
-                    f[k][v] = q.keep;
-                    u[k][v] = q.enter * to_float<T>(x[k][v]);
-                    mine[v] = then(mine[v], {f[k][v], u[k][v]});
-                }
-                before[v] = join_lanes<L::CL, false>(mine[v]);
-                if (lane / L::CL == TL - 1) waves[wave][cl + v] = mine[v];
-            }
+    for (int v = 0; v < VEC; ++v) {
+        Span ahead = {1.0f, 0.0f};
+        for (int w = 0; w < wave; ++w) ahead = then(ahead, waves[w][cl + v]);
+        before[v] = then(ahead, before[v]);
+    }
+    __syncthreads();
+    const int t = p.t0() + sub, row = state_row(s, a.slots, p.b);
+    float h[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[v] = after(before[v], start[cl + v]);
+    T* y = static_cast<T*>(a.y) + first * s.y_stride + p.c0;
+    const long long stride = anew(s.y_stride);
+#pragma unroll
+    for (int k = 0; k < S; ++k, y += stride) {
+        if (k % 8 == 0 && a.saved && (t + k) % kSaved == 0 && t + k < s.n) {
+            float* saved = a.saved + saved_at(s, p.b, t + k, kSaved) + p.c0 + cl;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                if (v < in.some) saved[v] = h[v];
         }
-        if (chained && threadIdx.x == 0) drawn = next;
-        __syncthreads();
-        if (chained) next = __builtin_amdgcn_readfirstlane(drawn);
-        Word* words = chain.words + static_cast<long long>(column) * L::kChannels;
-        const long long step = static_cast<long long>(columns) * L::kChannels;
-        const bool gives_state = tile % kGroup == 0;
-        const bool later = chained && t0 + L::kSteps < len;  // a tile waits for this one
-        const int srow = state_row(s, a.slots, b);
-        const long long state = static_cast<long long>(srow) * s.channels + c;
-        Span ahead[VEC];  // of the waves before this one
-        if (part) {
+        pack<T, VEC> out;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                ahead[v] = {1.0f, 0.0f};
-                for (int w = 0; w < wave; ++w) ahead[v] = then(ahead[v], waves[w][cl + v]);
-            }
-            if (later && !gives_state && sub == L::kSubs - 1) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    publish(words + tile * step + cl + v, then(ahead[v], mine[v]));
-            }
-            gather<L>(a.state_in && srow >= 0 ? a.state_in + state : nullptr, some, words, step,
-                      tile, items);
+        for (int v = 0; v < VEC; ++v) {
+            h[v] = fmaf(f[k][v], h[v], u[k][v]);
+            out[v] = from_float<T>(h[v]);
         }
-        __syncthreads();
-        if (part) {
-            pack<T, VEC> out[S];
+        store_step<T, VEC>(y + at_y, out, k, in);
+    }
+    if (a.state_out && row >= 0 && (p.len > 0 ? t < p.len && p.len <= t + S : t == 0)) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float h = after(ahead[v], start_of<L>(tile, cl + v, items));
-                if (later && gives_state && sub == L::kSubs - 1)
-                    publish(words + tile * step + cl + v, {0.0f, after(mine[v], h)});
-                h = after(before[v], h);
-                if (a.saved && t % kSavedSteps == 0 && t < s.n && v < some)
-                    a.saved[(static_cast<long long>(b) * ((s.n + kSavedSteps - 1) / kSavedSteps) +
-                             t / kSavedSteps) * s.channels + c + v] = h;
-#pragma unroll
-                for (int k = 0; k < S; ++k) {
-                    h = fmaf(f[k][v], h, u[k][v]);
-                    out[k][v] = from_float<T>(h);
-                }
-                if (a.state_out && srow >= 0 && v < some &&
-                    (len > 0 ? t < len && len <= t + S : sub == 0 && tile == 0))
-                    a.state_out[state + v] = h;
-            }
-            store_steps<T, L>(y, at_y, s.y_stride, out, full, inside, rows, some);
-        } else {
-            const pack<T, VEC> out[S] = {};
-            store_steps<T, L>(y, at_y, s.y_stride, out, false, 0, rows, some);
-        }
-        ticket = chained ? next : ticket + gridDim.x;
+        for (int v = 0; v < VEC; ++v)
+            if (v < in.some)
+                a.state_out[static_cast<long long>(row) * s.channels + p.c0 + cl + v] = h[v];
     }
 }
 
 template <class T, class L>
-__global__ __launch_bounds__(L::kLanes, 4) void scan_last_backward(ScanShape s, ScanBackward a,
+__global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(ScanShape s, ScanBackward a,
                                                                    Chain chain) {
-    constexpr int VEC = L::VEC, S = L::S, TL = 64 / L::CL;
-    static_assert(L::kSteps % kSavedSteps == 0, "a tile starts from a saved state");
-    __shared__ Span waves[L::W][L::kChannels], back[L::W][L::kChannels];
-    __shared__ Span items[kGroup][L::kChannels];
-    __shared__ unsigned drawn;
+    constexpr int VEC = L::VEC, S = L::S, W = L::W, TL = 64 / L::CL;
+    static_assert(L::kSteps % kSaved == 0, "a tile starts from a saved state");
+    using Where = Place<L, true>;
+    // Spans of h, and of the gradient that goes back (the last wave's first).
+    __shared__ Span waves[W][L::kChannels], back[W][L::kChannels];
+    __shared__ float start[L::kChannels];
+    __shared__ int drawn;
+    const int ticket = draw_tile(chain, &drawn);
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int sub = wave * TL + lane / L::CL, cl = lane % L::CL * VEC;
+    const int cl = lane % L::CL * VEC, sub = (wave * TL + lane / L::CL) * S;
+    if (wave >= W) {
+        run_chain<L, true>(s, a.lengths, chain, back, start, ticket, [&](const Where& p) {
+            return a.dstate_out
+                       ? a.dstate_out + static_cast<long long>(p.b) * s.channels + p.c0
+                       : nullptr;
+        });
+        return;
+    }
     const auto at_x = lane_offset<L>(s.x_stride), at_gate = lane_offset<L>(s.gate_stride),
                at_y = lane_offset<L>(s.y_stride);
-    const bool chained = chain.tiles > 1;
-    const int columns = s.batch * chain.slabs;
-
-    unsigned ticket = blockIdx.x;
-    if (chained) {
-        if (threadIdx.x == 0) drawn = draw(chain);
-        __syncthreads();
-        ticket = __builtin_amdgcn_readfirstlane(drawn);
-        __syncthreads();
+    const Where p(ticket, s, a.lengths, chain);
+    const long long row = p.row(s, wave);
+    const Inside in = p.inside(s, wave, sub);
+    pack<T, VEC> x[S], g[S], dy[S];
+    float h[VEC];
+    load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + p.c0, at_gate,
+                     s.gate_stride, in, s.channels, open_gate<T>());
+    load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + p.c0, at_x, s.x_stride, in,
+                     s.channels, static_cast<T>(0.0f));
+    load_steps<T, L>(dy, static_cast<const T*>(a.dy) + row * s.y_stride + p.c0, at_y, s.y_stride, in,
+                     s.channels, static_cast<T>(0.0f));
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+        h[v] = p.t0() < p.len && v < in.some  // the state before the tile
+                   ? a.saved[saved_at(s, p.b, p.t0(), kSaved) + p.c0 + cl + v]
+                   : 0.0f;
+    float f[S][VEC], enter[S][VEC], q[S][VEC];
+    Span before[VEC], past[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) before[v] = past[v] = {1.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const Gate r = gate_of(to_float<T>(g[k][v]));
+            f[k][v] = r.keep;
+            enter[k][v] = r.enter;
+            q[k][v] = to_float<T>(x[k][v]);
+            before[v] = then(before[v], {r.keep, r.enter * q[k][v]});
+        }
     }
-    while (ticket < chain.total) {
-        unsigned next = 0;
-        if (chained && threadIdx.x == 0) next = draw(chain);
-        const int tile = chain.tiles - 1 - static_cast<int>(ticket / columns);
-        const int column = ticket % columns;
-        const int b = column / chain.slabs, c0 = column % chain.slabs * L::kChannels, c = c0 + cl;
-        const int some = max(0, min(VEC, s.channels - c));
-        const int len = length_of(a.lengths, b, s.n);
-        const int t0 = tile * L::kSteps, t = t0 + sub * S;
-        const int rows = max(0, min(S, s.n - t)), inside = max(0, min(S, len - t));
-        const long long row = static_cast<long long>(b) * s.n + t0 + wave * TL * S;  // the wave's first
-        T* dx = static_cast<T*>(a.dx) + row * s.x_stride + c0;
-        T* dgate = static_cast<T*>(a.dgate) + row * s.gate_stride + c0;
-        const bool full = t0 + L::kSteps <= len && c0 + L::kChannels <= s.channels;
-        const bool part = t0 < len || tile == 0;
-        pack<T, VEC> x[S], g[S], dy[S];
-        float f[S][VEC], enter[S][VEC], q[S][VEC];
-        Span mine[VEC], before[VEC], behind[VEC], past[VEC];
-        if (part) {
-            load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + c0, at_gate, s.gate_stride,
-                             full, inside, some, open_gate<T>());
-            load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + c0, at_x, s.x_stride,
-                             full, inside, some, static_cast<T>(0.0f));
-            load_steps<T, L>(dy, static_cast<const T*>(a.dy) + row * s.y_stride + c0, at_y, s.y_stride,
-                             full, inside, some, static_cast<T>(0.0f));
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                mine[v] = {1.0f, 0.0f};
-                behind[v] = {1.0f, 0.0f};
+    for (int k = S - 1; k >= 0; --k)
 #pragma unroll
-                for (int k = 0; k < S; ++k) {
-                    const Gate p = gate_of(to_float<T>(g[k][v]));
-                    f[k][v] = p.keep;
-                    enter[k][v] = p.enter;
-                    mine[v] = then(mine[v], {p.keep, p.enter * to_float<T>(x[k][v])});
-                }
+        for (int v = 0; v < VEC; ++v)
+            past[v] = then(past[v], {f[k][v], f[k][v] * to_float<T>(dy[k][v])});
 #pragma unroll
-                for (int k = S - 1; k >= 0; --k)
-                    behind[v] = then(behind[v], {f[k][v], f[k][v] * to_float<T>(dy[k][v])});
-                before[v] = join_lanes<L::CL, false>(mine[v]);
-                past[v] = join_lanes<L::CL, true>(behind[v]);
-                if (lane / L::CL == TL - 1) waves[wave][cl + v] = mine[v];
-                if (lane / L::CL == 0) back[wave][cl + v] = behind[v];
-            }
+    for (int v = 0; v < VEC; ++v) {
+        Span mine = before[v], behind = past[v];
+        before[v] = join_lanes<L::CL, false>(mine);
+        past[v] = join_lanes<L::CL, true>(behind);
+        if (lane / L::CL == TL - 1) waves[wave][cl + v] = mine;
+        if (lane / L::CL == 0) back[W - 1 - wave][cl + v] = behind;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        Span ahead = {1.0f, 0.0f}, rest = {1.0f, 0.0f};
+        for (int w = 0; w < wave; ++w) ahead = then(ahead, waves[w][cl + v]);
+        for (int w = 0; w < W - 1 - wave; ++w) rest = then(rest, back[w][cl + v]);
+        past[v] = then(rest, past[v]);
+        h[v] = after(before[v], after(ahead, h[v]));
+    }
+    // q becomes what lam is multiplied with for the gate's gradient.
+#pragma unroll
+    for (int k = 0; k < S; ++k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float in = q[k][v];
+            q[k][v] = (h[v] - in) * (f[k][v] * enter[k][v]);
+            h[v] = fmaf(f[k][v], h[v], enter[k][v] * in);
         }
-        if (chained && threadIdx.x == 0) drawn = next;
-        __syncthreads();
-        if (chained) next = __builtin_amdgcn_readfirstlane(drawn);
-        const int last = max(len - 1, 0) / L::kSteps, r = last - tile;
-        Word* words = chain.words + static_cast<long long>(column) * L::kChannels;
-        const long long step = static_cast<long long>(columns) * L::kChannels;
-        const bool gives_state = r % kGroup == 0;
-        const bool later = chained && tile > 0;
-        const long long state = static_cast<long long>(b) * s.channels + c;
-        Span ahead[VEC], rest[VEC];  // of the waves before this one, and of those behind it
-        if (part) {
+    __syncthreads();
+    const long long stride_x = anew(s.x_stride), stride_gate = anew(s.gate_stride);
+    T* dx = static_cast<T*>(a.dx) + (row + S - 1) * s.x_stride + p.c0;
+    T* dgate = static_cast<T*>(a.dgate) + (row + S - 1) * s.gate_stride + p.c0;
+    float grad[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                ahead[v] = {1.0f, 0.0f};
-                rest[v] = {1.0f, 0.0f};
-                for (int w = L::W - 1; w > wave; --w) rest[v] = then(rest[v], back[w][cl + v]);
-            }
-            if (later && !gives_state && sub == 0) {
+    for (int v = 0; v < VEC; ++v) grad[v] = after(past[v], start[cl + v]);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    publish(words + r * step + cl + v, then(rest[v], behind[v]));
-            }
-            gather<L>(a.dstate_out ? a.dstate_out + state : nullptr, some, words, step, r, items);
+    for (int k = S - 1; k >= 0; --k, dx -= stride_x, dgate -= stride_gate) {
+        pack<T, VEC> outx, outg;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                for (int w = 0; w < wave; ++w) ahead[v] = then(ahead[v], waves[w][cl + v]);
-                float h = 0.0f;
-                if (t0 < s.n && v < some)
-                    h = a.saved[(static_cast<long long>(b) * ((s.n + kSavedSteps - 1) / kSavedSteps) +
-                                 t0 / kSavedSteps) * s.channels + c + v];
-                h = after(before[v], after(ahead[v], h));
-#pragma unroll
-                for (int k = 0; k < S; ++k) {
-                    const float in = to_float<T>(x[k][v]);
-                    q[k][v] = (h - in) * (f[k][v] * enter[k][v]);
-                    h = fmaf(f[k][v], h, enter[k][v] * in);
-                }
-            }
+        for (int v = 0; v < VEC; ++v) {
+            const float lam = to_float<T>(dy[k][v]) + grad[v];
+            outx[v] = from_float<T>(enter[k][v] * lam);
+            outg[v] = from_float<T>(q[k][v] * lam);
+            grad[v] = f[k][v] * lam;
         }
-        __syncthreads();
-        if (part) {
-            pack<T, VEC> outx[S], outg[S];
+        store_step<T, VEC>(dx + at_x, outx, k, in);
+        store_step<T, VEC>(dgate + at_gate, outg, k, in);
+    }
+    if (a.dstate_in && p.tile == 0 && sub == 0) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                // What reaches this wave's last step from behind it.
-                float grad = after(rest[v], start_of<L>(r, cl + v, items));
-                if (later && gives_state && sub == 0)
-                    publish(words + r * step + cl + v, {0.0f, after(behind[v], grad)});
-                grad = after(past[v], grad);
-#pragma unroll
-                for (int k = S - 1; k >= 0; --k) {
-                    const float lam = to_float<T>(dy[k][v]) + grad;
-                    outx[k][v] = from_float<T>(enter[k][v] * lam);
-                    outg[k][v] = from_float<T>(q[k][v] * lam);
-                    grad = f[k][v] * lam;
-                }
-                if (a.dstate_in && tile == 0 && sub == 0 && v < some) a.dstate_in[state + v] = grad;
-            }
-            store_steps<T, L>(dx, at_x, s.x_stride, outx, full, inside, rows, some);
-            store_steps<T, L>(dgate, at_gate, s.gate_stride, outg, full, inside, rows, some);
-        } else {
-            const pack<T, VEC> out[S] = {};
-            store_steps<T, L>(dx, at_x, s.x_stride, out, false, 0, rows, some);
-            store_steps<T, L>(dgate, at_gate, s.gate_stride, out, false, 0, rows, some);
-        }
-        ticket = chained ? next : ticket + gridDim.x;
+        for (int v = 0; v < VEC; ++v)
+            if (v < in.some)
+                a.dstate_in[static_cast<long long>(p.b) * s.channels + p.c0 + cl + v] = grad[v];
     }
 }
 

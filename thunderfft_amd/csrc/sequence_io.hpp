@@ -34,17 +34,7 @@ __device__ __forceinline__ void store_pack(T* p, pack<T, V> v) {
     *reinterpret_cast<pack<T, V>*>(p) = v;
 }
 
-// The first `count` of V values; zeros for the others.
-template <class T, int V>
-__device__ __forceinline__ pack<T, V> load_some(const T* p, int count) {
-    if (count >= V) return load_pack<T, V>(p);
-    pack<T, V> v = {};
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (i < count) v[i] = p[i];
-    return v;
-}
-
+// Stores the first `count` of V values.
 template <class T, int V>
 __device__ __forceinline__ void store_some(T* p, pack<T, V> v, int count) {
     if (count >= V) {
