@@ -29,9 +29,13 @@ __device__ __forceinline__ pack<T, V> load_pack(const T* p) {
     return *reinterpret_cast<const pack<T, V>*>(p);
 }
 
+// Past the caches: the next kernel's workgroups read from other L2s than the ones that wrote,
+// and the lines would be written back first.  Layer norm 32768 x 2048 bfloat16 forward 57 -> 54
+// us, backward 95 -> 92 us; 60000 x 256 half 14.2 -> 11.7 and 30.7 -> 25.8 us; the recurrence
+// 8 x 4096 x 2048 95 -> 90 us; single rows the same.
 template <class T, int V>
 __device__ __forceinline__ void store_pack(T* p, pack<T, V> v) {
-    *reinterpret_cast<pack<T, V>*>(p) = v;
+    __builtin_nontemporal_store(v, reinterpret_cast<pack<T, V>*>(p));
 }
 
 // Stores the first `count` of V values.
