@@ -261,8 +261,8 @@ int thff_copy_nt(void* d_dst, const void* d_src, long long bytes, void* stream);
  * halves of one projection's rows.  x_stride and gate_stride hold for the
  * gradients of x and the gate too, y_stride for y and its gradient.  batch, n
  * and channels may be 0, and are at most 2^30, batch * channels at most
- * 2^31 - 1.  states: rows of the state pool that slots index (unused without
- * slots). */
+ * 2^31 - 256 (THFF_EINVAL too where one launch does not take the shape).
+ * states: rows of the state pool that slots index (unused without slots). */
 typedef struct thff_scan_shape {
     int precision, layout;
     int batch, n, channels, states;

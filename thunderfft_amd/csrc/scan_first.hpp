@@ -1,0 +1,295 @@
+// scan_first.hpp -- the gated recurrence on [batch][channels][n] values (the convolutions'
+// layout): one pass over the data.  A lane takes 8 neighbouring steps and composes them; the
+// lanes of a row join theirs in registers, its waves through LDS, and where a row takes several
+// workgroups, they join through the chain.  Short rows lie side by side in a wave.
+#pragma once
+
+#include "scan_chain.hpp"
+
+namespace thff {
+
+// LPR lanes of each of WPR waves a row; a row's tile is kSteps steps.
+template <int LPR_, int WPR_>
+struct Line {
+    static constexpr int V = 8, W = 8, LPR = LPR_, WPR = WPR_, kLanes = 64 * W;
+    static constexpr int kSteps = LPR * WPR * V, kRows = W / WPR * (64 / LPR);
+    static constexpr bool kChained = WPR == W;  // a workgroup has one row
+};
+
+// `v` of the lane that Control moves here, `none` where there is none.
+template <int Control, int Rows>
+__device__ __forceinline__ float moved(float v, float none) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), Control,
+                                                      Rows, 0xf, false));
+}
+
+template <int Control, int Rows = 0xf>
+__device__ __forceinline__ Span moved(Span s) {
+    return {moved<Control, Rows>(s.a, 1.0f), moved<Control, Rows>(s.b, 0.0f)};
+}
+
+// Joins the spans of groups of LPR lanes: `mine` becomes that of all up to and with this lane,
+// the result is that of all before it.
+template <int LPR>
+__device__ __forceinline__ Span join_line(Span& mine) {
+    constexpr Span kNone = {1.0f, 0.0f};
+    const int lane = threadIdx.x % LPR;
+    static_assert(LPR == 4 || LPR == 16 || LPR == 64, "groups that the moves below keep apart");
+    if constexpr (LPR == 4) {
+        const Span one = moved<0x111>(mine);  // from the lane before
+        mine = then(lane >= 1 ? one : kNone, mine);
+        const Span two = moved<0x112>(mine);
+        mine = then(lane >= 2 ? two : kNone, mine);
+    } else {
+        mine = then(moved<0x111>(mine), mine);
+        mine = then(moved<0x112>(mine), mine);
+        mine = then(moved<0x114>(mine), mine);
+        mine = then(moved<0x118>(mine), mine);
+        if constexpr (LPR == 64) {
+            mine = then(moved<0x142, 0xa>(mine), mine);  // a row of 16's last to the next one
+            mine = then(moved<0x143, 0xc>(mine), mine);  // lane 31 to the upper half
+        }
+    }
+    const Span before = moved<0x138>(mine);  // from the lane before, across rows of 16 too
+    return lane == 0 ? kNone : before;
+}
+
+// The same from the last lane to the first.
+template <int LPR>
+__device__ __forceinline__ Span join_line_back(Span& mine) {
+    const auto mirrored = [](Span s) -> Span { return {__shfl_xor(s.a, LPR - 1), __shfl_xor(s.b, LPR - 1)}; };
+    Span m = mirrored(mine);
+    const Span before = mirrored(join_line<LPR>(m));
+    mine = mirrored(m);
+    return before;
+}
+
+// A lane's 8 steps: those of its own that are `in` the sequence; the first `skip` of the vector
+// it reads are another lane's (the row ends inside its own), the others up to `own` are in the
+// tensor.
+template <class L>
+struct Stretch {
+    int row, b, c, tile, len, first, at, skip;
+    bool active;
+
+    __device__ __forceinline__ Stretch(const ScanShape& s, const int* lengths, int tile_) : tile(tile_) {
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+        const int rows = s.batch * s.channels;
+        const int mine = L::kChained ? blockIdx.x % static_cast<unsigned>(rows)
+                                     : blockIdx.x * L::kRows + wave / L::WPR * (64 / L::LPR) + lane / L::LPR;
+        active = mine < rows;
+        row = min(mine, rows - 1);
+        b = row / s.channels;
+        c = row - b * s.channels;
+        len = length_of(lengths, b, s.n);
+        first = tile * L::kSteps + (wave % L::WPR * L::LPR + lane % L::LPR) * L::V;
+        at = max(0, min(first, s.n - L::V));
+        skip = min(first - at, L::V);
+    }
+    // Whether step i of the vector is the lane's and in the sequence.
+    __device__ __forceinline__ bool in(int i) const { return i >= skip && at + i < len; }
+    // Whether all of the wave's are.
+    __device__ __forceinline__ bool full() const {
+        return __ballot(skip == 0 && first + L::V <= len) == ~0ull;
+    }
+};
+
+template <class T, class L>
+__device__ __forceinline__ pack<T, L::V> load_line(const T* row, const Stretch<L>& p, int n) {
+    if (n >= L::V) return load_pack<T, L::V>(row + p.at);
+    pack<T, L::V> v = {};
+#pragma unroll
+    for (int i = 0; i < L::V; ++i)
+        if (i < n) v[i] = row[i];
+    return v;
+}
+
+// Stores the lane's steps, zeros past the sequence's end.
+template <class T, class L>
+__device__ __forceinline__ void store_line(T* row, pack<T, L::V> v, const Stretch<L>& p, int n, bool full) {
+    if (!full) {
+#pragma unroll
+        for (int i = 0; i < L::V; ++i)
+            if (!p.in(i)) v[i] = static_cast<T>(0.0f);
+    }
+    if (!p.active) return;
+    if (p.skip == 0 && n >= L::V) {
+        store_pack<T, L::V>(row + p.at, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < L::V; ++i)
+            if (i >= p.skip && i < n) row[p.at + i] = v[i];
+    }
+}
+
+// Joins a workgroup's waves, whose spans are in `waves` in the order of the chain, and the
+// tiles; returns the state before the wave's first step in that order.  `given`: the row's
+// first state, on every lane.  own: the wave's place in its row.
+template <class L>
+__device__ __forceinline__ float join_tile(const Chain& chain, const Span* waves, float* start, int own,
+                                           int r, bool part, bool later, float given) {
+    const int wave = threadIdx.x / 64;
+    if constexpr (L::WPR == 1) return given;
+    if constexpr (L::kChained) {
+        if (chain.tiles > 1) {
+            const unsigned row = blockIdx.x % chain.columns;
+            Link<1> link;
+            link.words = chain.words + row;
+            link.step = chain.columns;
+            link.r = r;
+            if (threadIdx.x == 0 && part) link.ask();
+            __syncthreads();
+            if (threadIdx.x == 0 && part) {
+                Span all = waves[0];
+#pragma unroll
+                for (int w = 1; w < L::W; ++w) all = then(all, waves[w]);
+                const Span own_span[1] = {all};
+                const float first[1] = {given};
+                float h[1];
+                link.join(h, own_span, later, first);
+                start[0] = h[0];
+            }
+            __syncthreads();
+            given = start[0];
+        } else {
+            __syncthreads();
+            given = start[0];
+        }
+    } else {
+        __syncthreads();
+        given = start[wave / L::WPR];
+    }
+    const Span* before = waves + wave / L::WPR * L::WPR;
+    for (int w = 0; w < own; ++w) given = after(before[w], given);
+    return given;
+}
+
+template <class T, class L>
+__global__ __launch_bounds__(L::kLanes) void scan_first_forward(ScanShape s, ScanForward a, Chain chain) {
+    constexpr int V = L::V;
+    __shared__ Span waves[L::W];
+    __shared__ float start[L::W];
+    __shared__ int drawn;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const Stretch<L> p(s, a.lengths, draw_tile(chain, &drawn));
+    const int srow = state_row(s, a.slots, p.b);
+    const long long state = static_cast<long long>(srow) * s.channels + p.c;
+    // A tile that lies past the sequence's end has zeros to write and no part in the chain.
+    const bool part = p.tile * L::kSteps < p.len || p.tile == 0;
+    pack<T, V> g = {}, x = {};
+    if (s.n > 0) {
+        g = load_line<T, L>(static_cast<const T*>(a.gate) + p.row * s.gate_stride, p, s.n);
+        x = load_line<T, L>(static_cast<const T*>(a.x) + p.row * s.x_stride, p, s.n);
+    }
+    float given = p.tile == 0 && a.state_in && srow >= 0 ? a.state_in[state] : 0.0f;
+    const bool full = p.full();
+    float f[V], u[V];
+    Span mine = {1.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const Gate q = gate_of(to_float<T>(g[i]));
+        f[i] = q.keep;
+        u[i] = q.enter * to_float<T>(x[i]);
+    }
+    if (!full) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (!p.in(i)) f[i] = 1.0f, u[i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) mine = then(mine, {f[i], u[i]});
+    const Span before = join_line<L::LPR>(mine);
+    if (L::WPR > 1) {
+        if (lane == 63) waves[wave] = mine;
+        // Through LDS, so that it has been read before anyone stores a last state there.
+        if (lane == 0 && wave % L::WPR == 0) start[wave / L::WPR] = given;
+    }
+    float h = join_tile<L>(chain, waves, start, wave % L::WPR, p.tile, part,
+                           (p.tile + 1) * static_cast<long long>(L::kSteps) < p.len, given);
+    if (a.saved && p.active && p.first == p.tile * L::kSteps)
+        a.saved[static_cast<long long>(p.row) * chain.tiles + p.tile] = h;
+    h = after(before, h);
+    pack<T, V> out;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        h = fmaf(f[i], h, u[i]);
+        out[i] = from_float<T>(h);
+    }
+    store_line<T, L>(static_cast<T*>(a.y) + p.row * s.y_stride, out, p, s.n, full);
+    // The lane that has the last step, or none to do.
+    if (a.state_out && p.active && srow >= 0 &&
+        (p.len > 0 ? p.first < p.len && p.len <= p.first + V : p.first == 0))
+        a.state_out[state] = h;
+}
+
+template <class T, class L>
+__global__ __launch_bounds__(L::kLanes) void scan_first_backward(ScanShape s, ScanBackward a, Chain chain) {
+    constexpr int V = L::V;
+    // Spans of h, and of the gradient that goes back (the last wave's first).
+    __shared__ Span waves[L::W], back[L::W];
+    __shared__ float start[L::W];
+    __shared__ int drawn;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const Stretch<L> p(s, a.lengths, chain.tiles - 1 - draw_tile(chain, &drawn));
+    const bool part = p.tile * L::kSteps < p.len || p.tile == 0;
+    const int r = max(p.len - 1, 0) / L::kSteps - p.tile;
+    pack<T, V> g = {}, x = {}, dy = {};
+    if (s.n > 0) {
+        g = load_line<T, L>(static_cast<const T*>(a.gate) + p.row * s.gate_stride, p, s.n);
+        x = load_line<T, L>(static_cast<const T*>(a.x) + p.row * s.x_stride, p, s.n);
+        dy = load_line<T, L>(static_cast<const T*>(a.dy) + p.row * s.y_stride, p, s.n);
+    }
+    float given = r == 0 && a.dstate_out ? a.dstate_out[p.row] : 0.0f;
+    float h = part && s.n > 0 ? a.saved[static_cast<long long>(p.row) * chain.tiles + p.tile] : 0.0f;
+    const bool full = p.full();
+    float f[V], enter[V], q[V], d[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const Gate e = gate_of(to_float<T>(g[i]));
+        f[i] = e.keep;
+        enter[i] = e.enter;
+        q[i] = to_float<T>(x[i]);
+        d[i] = to_float<T>(dy[i]);
+    }
+    if (!full) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (!p.in(i)) f[i] = 1.0f, enter[i] = 0.0f, q[i] = 0.0f, d[i] = 0.0f;
+    }
+    Span mine = {1.0f, 0.0f}, behind = {1.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < V; ++i) mine = then(mine, {f[i], enter[i] * q[i]});
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i) behind = then(behind, {f[i], f[i] * d[i]});
+    const Span before = join_line<L::LPR>(mine);
+    const Span past = join_line_back<L::LPR>(behind);
+    const int own = wave % L::WPR;
+    if (L::WPR > 1) {
+        if (lane == 63) waves[wave] = mine;
+        if (lane == 0) back[wave - own + L::WPR - 1 - own] = behind;
+        if (lane == 0 && own == 0) start[wave / L::WPR] = given;
+    }
+    float grad = join_tile<L>(chain, back, start, L::WPR - 1 - own, r, part, p.tile > 0, given);
+    for (int w = 0; w < own; ++w) h = after(waves[wave - own + w], h);
+    h = after(before, h);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float in = q[i];
+        q[i] = (h - in) * (f[i] * enter[i]);
+        h = fmaf(f[i], h, enter[i] * in);
+    }
+    grad = after(past, grad);
+    pack<T, V> outx, outg;
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i) {
+        const float lam = d[i] + grad;
+        outx[i] = from_float<T>(enter[i] * lam);
+        outg[i] = from_float<T>(q[i] * lam);
+        grad = f[i] * lam;
+    }
+    store_line<T, L>(static_cast<T*>(a.dx) + p.row * s.x_stride, outx, p, s.n, full);
+    store_line<T, L>(static_cast<T*>(a.dgate) + p.row * s.gate_stride, outg, p, s.n, full);
+    if (a.dstate_in && p.active && p.first == 0) a.dstate_in[p.row] = grad;
+}
+
+}  // namespace thff
