@@ -123,8 +123,10 @@ def _ptr(x) -> int:
         return 0
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return int(x.data_ptr())
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     raise TypeError(f"expected a device pointer or tensor, got {type(x).__name__}")
 
 
@@ -254,8 +256,9 @@ def ThunderFFT_conv2d_noalloc(T, rows: int, cols: int, d_x, d_h, d_y, batch: int
 
 
 def _value_type(T) -> int:
-    if isinstance(T, str) and T in VALUE_TYPES:
-        return VALUE_TYPES[T]
+    code = VALUE_TYPES.get(T) if isinstance(T, str) else None
+    if code is not None:
+        return code
     name = str(T).rpartition(".")[2]
     for key, code in (("float32", 0), ("float16", 1), ("bfloat16", 2)):
         if name == key:

@@ -7,6 +7,7 @@
 
 #include "scan_first.hpp"
 #include "scan_last.hpp"
+#include "scan_step.hpp"
 
 namespace thff {
 namespace {
@@ -23,8 +24,9 @@ __global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long count
     to[i] = make_uint4(v, v, v, v);
 }
 
-// Channels last: calls f with the tile type of a shape's forward or backward pass: 4 bytes a lane and row;
-// lanes along the channels all 64 of a wave, or 16 where that leaves far fewer of them idle.
+// Channels last: calls f with the tile type of a shape's forward or backward pass: 4 bytes a
+// lane and row; lanes along the channels all 64 of a wave, or 16 where that leaves far fewer of
+// them idle.
 template <class T, bool Backward, class F>
 auto with_tile(const ScanShape& s, F f) {
     constexpr int VEC = 4 / sizeof(T);
@@ -120,8 +122,25 @@ hipError_t launch_first(void (*kernel)(ScanShape, Args, Chain), const ScanShape&
     return hipGetLastError();
 }
 
+// One step: 16 bytes of states a lane where the channels lie side by side.
+template <class T>
+hipError_t launch_step(const ScanShape& s, const ScanForward& a, hipStream_t stream) {
+    const auto channel = [&](long long stride) { return s.channels_first ? stride : 1LL; };
+    const auto row = [&](long long stride) { return s.channels_first ? s.channels * stride : stride; };
+    const StepStrides d{channel(s.x_stride), channel(s.gate_stride), channel(s.y_stride),
+                        row(s.x_stride),     row(s.gate_stride),     row(s.y_stride)};
+    const auto launch = [&](void (*kernel)(ScanShape, ScanForward, StepStrides), int channels) {
+        const long long lanes = static_cast<long long>(s.batch) * ((s.channels + channels - 1) / channels);
+        kernel<<<static_cast<unsigned>((lanes + kStepLanes - 1) / kStepLanes), kStepLanes, 0, stream>>>(s, a, d);
+        return hipGetLastError();
+    };
+    if (d.x == 1 && d.gate == 1 && d.y == 1) return launch(scan_step<T, 4>, 4);
+    return launch(scan_step<T, 1>, 1);
+}
+
 template <class T>
 hipError_t forward_of(const ScanShape& s, const ScanForward& a, hipStream_t stream) {
+    if (s.n == 1) return launch_step<T>(s, a, stream);
     if (s.channels_first)
         return with_line(s, [&](auto line) {
             using L = decltype(line);
