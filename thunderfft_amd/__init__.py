@@ -121,12 +121,12 @@ def _precision(T) -> int:
 def _ptr(x) -> int:
     if x is None:
         return 0
-    if isinstance(x, int):
-        return x
     try:
         return x.data_ptr()
     except AttributeError:
         pass
+    if isinstance(x, int):
+        return x
     raise TypeError(f"expected a device pointer or tensor, got {type(x).__name__}")
 
 

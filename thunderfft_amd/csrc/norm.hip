@@ -215,14 +215,15 @@ __global__ __launch_bounds__(R::kLanes) void norm_backward(NormBackward a, int p
     const long long steps = (a.rows + every - 1) / every;
     if constexpr (R::W < 16) {
         // The next row's loads are under way while a row is worked on, and go before its stores: a
-        // wait for them is none for those.  Nothing in the loop branches, so that the compiler can
-        // tell which is which.
+        // wait for them is none for those.  Nothing in the loop branches around a load or a store,
+        // so that the compiler can tell which is which.
         Row one, two;
         load(one, row0);
         for (long long n = 0; n < steps; n += 2) {
             const long long row = row0 + n * every;
             load(two, row + every);
             take(one, row, n);
+            if (n + 1 == steps) break;
             load(one, row + 2 * every);
             take(two, row + every, n + 1);
         }
