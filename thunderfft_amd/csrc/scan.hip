@@ -65,6 +65,9 @@ Chain chain_of(const ScanShape& s, int channels, int steps, void* workspace) {
     chain.slabs = channels ? (s.channels + channels - 1) / channels : s.channels;
     chain.tiles = s.n > 0 ? (s.n + steps - 1) / steps : 1;
     chain.columns = static_cast<unsigned>(s.batch) * chain.slabs;
+    // (An empty shape has no columns, and launches nothing.)
+    chain.by_columns = Divider(std::max(chain.columns, 1u));
+    chain.by_slabs = Divider(std::max(chain.slabs, 1));
     chain.drawn = static_cast<unsigned*>(workspace);
     chain.words = reinterpret_cast<Word*>(static_cast<char*>(workspace) +
                                           static_cast<long long>(chain.columns) * kCounterBytes);

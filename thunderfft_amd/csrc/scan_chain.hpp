@@ -81,6 +81,23 @@ __device__ __forceinline__ Span span_of(Word w) {
     return {__uint_as_float(static_cast<unsigned>(w)), __uint_as_float(static_cast<unsigned>(w >> 32))};
 }
 
+// Division by a number that the host knows: n / d = n m >> shift for n < 2^31, with
+// 2^(s-1) < d <= 2^s, shift = 31 + s and m = ceil(2^shift / d), which is off by less than d
+// units of 2^-shift a unit of n: too little to reach the next whole number.
+struct Divider {
+    unsigned d, m;
+    int shift;
+
+    Divider() = default;
+    explicit Divider(unsigned by) : d(by), shift(31) {
+        while ((1ull << (shift - 31)) < by) ++shift;
+        m = static_cast<unsigned>(((1ull << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ int quotient(unsigned n) const {
+        return static_cast<int>(static_cast<unsigned long long>(n) * m >> shift);
+    }
+};
+
 // The workspace: a counter for every column of tiles, far enough apart, then a word for every
 // channel of every tile.
 struct Chain {
@@ -88,6 +105,11 @@ struct Chain {
     Word* words;
     int slabs, tiles;  // tiles along the channels, along the steps
     unsigned columns;  // batch * slabs
+    Divider by_columns, by_slabs;
+
+    // The column of a workgroup, and the tile of it that it expects to draw.
+    __device__ __forceinline__ int expected() const { return by_columns.quotient(blockIdx.x); }
+    __device__ __forceinline__ int column() const { return blockIdx.x - expected() * columns; }
 };
 constexpr int kCounterBytes = 64;
 
@@ -177,11 +199,10 @@ __device__ __forceinline__ T open_gate() {
     return static_cast<T>(__builtin_inff());
 }
 
-// Draws the workgroup's tile of its column, where tiles wait for each other.
-__device__ __forceinline__ int draw_tile(const Chain& chain, int* drawn) {
-    if (chain.tiles <= 1) return 0;
-    if (threadIdx.x == 0) {
-        unsigned* counter = chain.drawn + blockIdx.x % chain.columns * (kCounterBytes / 4);
+// Draws the workgroup's tile of its column, by the first lane of wave `drawer`.
+__device__ __forceinline__ int draw_tile(const Chain& chain, int* drawn, int drawer) {
+    if (static_cast<int>(threadIdx.x) == 64 * drawer) {
+        unsigned* counter = chain.drawn + chain.column() * (kCounterBytes / 4);
         *drawn = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();

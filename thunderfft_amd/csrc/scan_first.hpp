@@ -72,14 +72,15 @@ struct Stretch {
     int row, b, c, tile, len, first, at, skip;
     bool active;
 
-    __device__ __forceinline__ Stretch(const ScanShape& s, const int* lengths, int tile_) : tile(tile_) {
+    __device__ __forceinline__ Stretch(const ScanShape& s, const int* lengths, const Chain& chain, int tile_)
+        : tile(tile_) {
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         const int rows = s.batch * s.channels;
-        const int mine = L::kChained ? blockIdx.x % static_cast<unsigned>(rows)
+        const int mine = L::kChained ? chain.column()
                                      : blockIdx.x * L::kRows + wave / L::WPR * (64 / L::LPR) + lane / L::LPR;
         active = mine < rows;
         row = min(mine, rows - 1);
-        b = row / s.channels;
+        b = chain.by_slabs.quotient(row);
         c = row - b * s.channels;
         len = length_of(lengths, b, s.n);
         first = tile * L::kSteps + (wave % L::WPR * L::LPR + lane % L::LPR) * L::V;
@@ -132,9 +133,8 @@ __device__ __forceinline__ float join_tile(const Chain& chain, const Span* waves
     if constexpr (L::WPR == 1) return given;
     if constexpr (L::kChained) {
         if (chain.tiles > 1) {
-            const unsigned row = blockIdx.x % chain.columns;
             Link<1> link;
-            link.words = chain.words + row;
+            link.words = chain.words + chain.column();
             link.step = chain.columns;
             link.r = r;
             if (threadIdx.x == 0 && part) link.ask();
@@ -171,7 +171,8 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_forward(ScanShape s, Sca
     __shared__ float start[L::W];
     __shared__ int drawn;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const Stretch<L> p(s, a.lengths, draw_tile(chain, &drawn));
+    const bool chained = L::kChained && chain.tiles > 1;
+    const Stretch<L> p(s, a.lengths, chain, chained ? draw_tile(chain, &drawn, 0) : 0);
     const int srow = state_row(s, a.slots, p.b);
     const long long state = static_cast<long long>(srow) * s.channels + p.c;
     // A tile that lies past the sequence's end has zeros to write and no part in the chain.
@@ -230,7 +231,8 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_backward(ScanShape s, Sc
     __shared__ float start[L::W];
     __shared__ int drawn;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const Stretch<L> p(s, a.lengths, chain.tiles - 1 - draw_tile(chain, &drawn));
+    const bool chained = L::kChained && chain.tiles > 1;
+    const Stretch<L> p(s, a.lengths, chain, chained ? chain.tiles - 1 - draw_tile(chain, &drawn, 0) : 0);
     const bool part = p.tile * L::kSteps < p.len || p.tile == 0;
     const int r = max(p.len - 1, 0) / L::kSteps - p.tile;
     pack<T, V> g = {}, x = {}, dy = {};

@@ -133,13 +133,13 @@ template <class L, bool Backward>
 struct Place {
     int tile, b, c0, len, column;
 
-    // The workgroup's, the `drawn`-th of its column.
+    // The workgroup's, the `drawn`-th of its column in the order of the chain.
     __device__ __forceinline__ Place(int drawn, const ScanShape& s, const int* lengths,
                                      const Chain& chain) {
         tile = Backward ? chain.tiles - 1 - drawn : drawn;
-        column = blockIdx.x % chain.columns;
-        b = column / chain.slabs;
-        c0 = column % chain.slabs * L::kChannels;
+        column = chain.column();
+        b = chain.by_slabs.quotient(column);
+        c0 = (column - b * chain.slabs) * L::kChannels;
         len = length_of(lengths, b, s.n);
     }
     __device__ __forceinline__ int t0() const { return tile * L::kSteps; }
@@ -213,10 +213,11 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(Sc
     __shared__ Span waves[L::W][L::kChannels];
     __shared__ float start[L::kChannels];
     __shared__ int drawn;
-    const int ticket = draw_tile(chain, &drawn);
+    const bool chained = chain.tiles > 1;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int cl = lane % L::CL * VEC, sub = (wave * TL + lane / L::CL) * S;
     if (wave >= L::W) {
+        const int ticket = chained ? draw_tile(chain, &drawn, L::W) : 0;
         run_chain<L, false>(s, a.lengths, chain, waves, start, ticket, [&](const Where& p) {
             const int row = state_row(s, a.slots, p.b);
             return a.state_in && row >= 0
@@ -227,14 +228,28 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(Sc
     }
     const auto at_x = lane_offset<L>(s.x_stride), at_gate = lane_offset<L>(s.gate_stride),
                at_y = lane_offset<L>(s.y_stride);
-    const Where p(ticket, s, a.lengths, chain);
+    // The loads of the tile that it expects to draw go before the draw; they are done again if
+    // it draws another.
+    Where p(chained ? chain.expected() : 0, s, a.lengths, chain);
+    pack<T, VEC> x[S], g[S];
+    const auto load = [&] {
+        const long long row = p.row(s, wave);
+        const Inside in = p.inside(s, wave, sub);
+        load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + p.c0, at_gate,
+                         s.gate_stride, in, s.channels, open_gate<T>());
+        load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + p.c0, at_x, s.x_stride,
+                         in, s.channels, static_cast<T>(0.0f));
+    };
+    load();
+    if (chained) {
+        const int ticket = draw_tile(chain, &drawn, L::W);
+        if (ticket != chain.expected()) {
+            p = Where(ticket, s, a.lengths, chain);
+            load();
+        }
+    }
     const long long first = p.row(s, wave);
     const Inside in = p.inside(s, wave, sub);
-    pack<T, VEC> x[S], g[S];
-    load_steps<T, L>(g, static_cast<const T*>(a.gate) + first * s.gate_stride + p.c0, at_gate,
-                     s.gate_stride, in, s.channels, open_gate<T>());
-    load_steps<T, L>(x, static_cast<const T*>(a.x) + first * s.x_stride + p.c0, at_x, s.x_stride, in,
-                     s.channels, static_cast<T>(0.0f));
     float f[S][VEC], u[S][VEC];
     Span before[VEC];
 #pragma unroll
@@ -303,10 +318,11 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
     __shared__ Span waves[W][L::kChannels], back[W][L::kChannels];
     __shared__ float start[L::kChannels];
     __shared__ int drawn;
-    const int ticket = draw_tile(chain, &drawn);
+    const bool chained = chain.tiles > 1;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int cl = lane % L::CL * VEC, sub = (wave * TL + lane / L::CL) * S;
     if (wave >= W) {
+        const int ticket = chained ? draw_tile(chain, &drawn, W) : 0;
         run_chain<L, true>(s, a.lengths, chain, back, start, ticket, [&](const Where& p) {
             return a.dstate_out
                        ? a.dstate_out + static_cast<long long>(p.b) * s.channels + p.c0
@@ -316,22 +332,34 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
     }
     const auto at_x = lane_offset<L>(s.x_stride), at_gate = lane_offset<L>(s.gate_stride),
                at_y = lane_offset<L>(s.y_stride);
-    const Where p(ticket, s, a.lengths, chain);
+    Where p(chained ? chain.expected() : 0, s, a.lengths, chain);
+    pack<T, VEC> x[S], g[S], dy[S];
+    float h[VEC];  // the state before the tile
+    const auto load = [&] {
+        const long long row = p.row(s, wave);
+        const Inside in = p.inside(s, wave, sub);
+        load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + p.c0, at_gate,
+                         s.gate_stride, in, s.channels, open_gate<T>());
+        load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + p.c0, at_x, s.x_stride,
+                         in, s.channels, static_cast<T>(0.0f));
+        load_steps<T, L>(dy, static_cast<const T*>(a.dy) + row * s.y_stride + p.c0, at_y, s.y_stride,
+                         in, s.channels, static_cast<T>(0.0f));
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+            h[v] = p.t0() < p.len && v < in.some
+                       ? a.saved[saved_at(s, p.b, p.t0(), kSaved) + p.c0 + cl + v]
+                       : 0.0f;
+    };
+    load();
+    if (chained) {
+        const int ticket = draw_tile(chain, &drawn, W);
+        if (ticket != chain.expected()) {
+            p = Where(ticket, s, a.lengths, chain);
+            load();
+        }
+    }
     const long long row = p.row(s, wave);
     const Inside in = p.inside(s, wave, sub);
-    pack<T, VEC> x[S], g[S], dy[S];
-    float h[VEC];
-    load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + p.c0, at_gate,
-                     s.gate_stride, in, s.channels, open_gate<T>());
-    load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + p.c0, at_x, s.x_stride, in,
-                     s.channels, static_cast<T>(0.0f));
-    load_steps<T, L>(dy, static_cast<const T*>(a.dy) + row * s.y_stride + p.c0, at_y, s.y_stride, in,
-                     s.channels, static_cast<T>(0.0f));
-#pragma unroll
-    for (int v = 0; v < VEC; ++v)
-        h[v] = p.t0() < p.len && v < in.some  // the state before the tile
-                   ? a.saved[saved_at(s, p.b, p.t0(), kSaved) + p.c0 + cl + v]
-                   : 0.0f;
     float f[S][VEC], enter[S][VEC], q[S][VEC];
     Span before[VEC], past[VEC];
 #pragma unroll
