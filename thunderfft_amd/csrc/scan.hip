@@ -30,8 +30,8 @@ __global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long count
 template <class T, bool Backward, class F>
 auto with_tile(const ScanShape& s, F f) {
     constexpr int VEC = 4 / sizeof(T);
-    using Wide = std::conditional_t<Backward, Tile<VEC, 64, 8, 14, 2, 4>, Tile<VEC, 64, 8, 14, 2, 8>>;
-    using Thin = std::conditional_t<Backward, Tile<VEC, 16, 8, 14, 2, 4>, Tile<VEC, 16, 8, 14, 2, 8>>;
+    using Wide = std::conditional_t<Backward, Tile<VEC, 64, 4, 14, 2, 8>, Tile<VEC, 64, 8, 14, 2, 8>>;
+    using Thin = std::conditional_t<Backward, Tile<VEC, 16, 4, 14, 2, 8>, Tile<VEC, 16, 8, 14, 2, 8>>;
     const auto taken = [&](long long channels) {
         return (s.channels + channels - 1) / channels * channels;
     };

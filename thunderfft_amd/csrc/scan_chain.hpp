@@ -126,7 +126,7 @@ struct Link {
     Word* words;
     long long step;
     int r;
-    Word one[kGroup - 1][N], group[kGroup - 1][N], state[N];
+    Word one[kGroup - 1][N], group[kSuper / kGroup - 1][N], state[N];
 
     __device__ __forceinline__ int base() const { return (r - 1) / kSuper * kSuper; }
     __device__ __forceinline__ int groups() const { return (r - 1 - base()) / kGroup; }
@@ -144,10 +144,13 @@ struct Link {
 #pragma unroll
         for (int i = 0; i < kGroup - 1; ++i)
 #pragma unroll
-            for (int v = 0; v < N; ++v) {
+            for (int v = 0; v < N; ++v)
                 if (i < single()) one[i][v] = look(at_one(i) + v);
+#pragma unroll
+        for (int i = 0; i < kSuper / kGroup - 1; ++i)
+#pragma unroll
+            for (int v = 0; v < N; ++v)
                 if (i < groups()) group[i][v] = look(at_group(i) + v);
-            }
 #pragma unroll
         for (int v = 0; v < N; ++v) state[v] = look(words + base() * step + v);
     }
@@ -180,7 +183,7 @@ struct Link {
 #pragma unroll
             for (int v = 0; v < N; ++v) h[v] = seen(state[v], words + base() * step + v).b;
 #pragma unroll
-            for (int i = 0; i < kGroup - 1; ++i)
+            for (int i = 0; i < kSuper / kGroup - 1; ++i)
 #pragma unroll
                 for (int v = 0; v < N; ++v)
                     if (i < groups()) h[v] = after(seen(group[i][v], at_group(i) + v), h[v]);

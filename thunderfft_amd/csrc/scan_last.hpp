@@ -164,11 +164,12 @@ __device__ __forceinline__ long long saved_at(const ScanShape& s, int b, int t, 
 }
 
 // The waves that publish and wait for other tiles: spans of a tile's waves in
-// `waves`, in the order of the chain, and the state that the tile starts from in `start`.
+// `waves`, in the order of the chain, which become those of all waves before each, and the state
+// that the tile starts from in `start`.
 // state(p): where that of the chain's first tile is given for channel p.c0, or null.
 template <class L, bool Backward, class State>
 __device__ __forceinline__ void run_chain(const ScanShape& s, const int* lengths, const Chain& chain,
-                                          const Span (*waves)[L::kChannels], float* start,
+                                          Span (*waves)[L::kChannels], float* start,
                                           int ticket, State state) {
     constexpr int N = L::kChannels > 64 * L::C ? L::kChannels / (64 * L::C) : 1;
     const int lane = threadIdx.x - 64 * L::W, c = lane * N;
@@ -193,9 +194,22 @@ __device__ __forceinline__ void run_chain(const ScanShape& s, const int* lengths
         Span all[N];
 #pragma unroll
         for (int v = 0; v < N; ++v) {
-            all[v] = waves[0][c + v];
+            // A wave's own span makes room for that of the waves before it; some at a time, for
+            // want of registers.
+            constexpr int kSome = L::W / 2;
+            static_assert(L::W % 2 == 0, "two halves");
+            all[v] = {1.0f, 0.0f};
 #pragma unroll
-            for (int w = 1; w < L::W; ++w) all[v] = then(all[v], waves[w][c + v]);
+            for (int w0 = 0; w0 < L::W; w0 += kSome) {
+                Span each[kSome];
+#pragma unroll
+                for (int w = 0; w < kSome; ++w) each[w] = waves[w0 + w][c + v];
+#pragma unroll
+                for (int w = 0; w < kSome; ++w) {
+                    waves[w0 + w][c + v] = all[v];
+                    all[v] = then(all[v], each[w]);
+                }
+            }
         }
         float h[N];
         link.join(h, all, later, given);
@@ -271,17 +285,12 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(Sc
         if (lane / L::CL == TL - 1) waves[wave][cl + v] = mine;
     }
     __syncthreads();
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        Span ahead = {1.0f, 0.0f};
-        for (int w = 0; w < wave; ++w) ahead = then(ahead, waves[w][cl + v]);
-        before[v] = then(ahead, before[v]);
-    }
     __syncthreads();
     const int t = p.t0() + sub, row = state_row(s, a.slots, p.b);
     float h[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = after(before[v], start[cl + v]);
+    for (int v = 0; v < VEC; ++v)
+        h[v] = after(before[v], after(waves[wave][cl + v], start[cl + v]));
     T* y = static_cast<T*>(a.y) + first * s.y_stride + p.c0;
     const long long stride = anew(s.y_stride);
 #pragma unroll
@@ -391,10 +400,8 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        Span ahead = {1.0f, 0.0f}, rest = {1.0f, 0.0f};
+        Span ahead = {1.0f, 0.0f};
         for (int w = 0; w < wave; ++w) ahead = then(ahead, waves[w][cl + v]);
-        for (int w = 0; w < W - 1 - wave; ++w) rest = then(rest, back[w][cl + v]);
-        past[v] = then(rest, past[v]);
         h[v] = after(before[v], after(ahead, h[v]));
     }
     // q becomes what lam is multiplied with for the gate's gradient.
@@ -412,7 +419,8 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
     T* dgate = static_cast<T*>(a.dgate) + (row + S - 1) * s.gate_stride + p.c0;
     float grad[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) grad[v] = after(past[v], start[cl + v]);
+    for (int v = 0; v < VEC; ++v)
+        grad[v] = after(past[v], after(back[W - 1 - wave][cl + v], start[cl + v]));
 #pragma unroll
     for (int k = S - 1; k >= 0; --k, dx -= stride_x, dgate -= stride_gate) {
         pack<T, VEC> outx, outg;
