@@ -47,16 +47,27 @@ auto with_type(const ScanShape& s, F f) {
     return f(bfloat_t{});
 }
 
-// Channels first: calls f with the kind of row for n steps: as many lanes as have some, 8 waves
-// at most.
-template <class F>
+// Rows of more than one tile, both ways; shorter rows have one tile of whatever kind.
+using LongLine = Line<8, 64, 8, true>;
+
+// Channels first: calls f with the kind of row for n steps of T: as many lanes as have some, 8
+// waves at most.  8 steps a lane; long rows of 2-byte values forward 16 (half 256 x 64 x 4096: 72
+// against 79 us; backward, which has more to keep, 123 against 117, and float 117 against 71 at
+// 64 x 512 x 1024: its lanes' 64 bytes are four loads that each touch every line).
+template <class T, bool Backward, class F>
 auto with_line(const ScanShape& s, F f) {
-    if (s.n <= Line<4, 1>::kSteps) return f(Line<4, 1>{});
-    if (s.n <= Line<16, 1>::kSteps) return f(Line<16, 1>{});
-    if (s.n <= Line<64, 1>::kSteps) return f(Line<64, 1>{});
-    if (s.n <= Line<64, 2>::kSteps) return f(Line<64, 2>{});
-    if (s.n <= Line<64, 4>::kSteps) return f(Line<64, 4>{});
-    return f(Line<64, 8>{});
+    constexpr int V = !Backward && sizeof(T) == 2 ? 16 : 8;
+    const auto within = [&](auto line) { return s.n <= decltype(line)::kSteps; };
+    if (within(Line<8, 4, 1>{})) return f(Line<8, 4, 1>{});
+    if (within(Line<8, 8, 1>{})) return f(Line<8, 8, 1>{});
+    if (within(Line<8, 16, 1>{})) return f(Line<8, 16, 1>{});
+    if (within(Line<8, 32, 1>{})) return f(Line<8, 32, 1>{});
+    if (within(Line<8, 64, 1>{})) return f(Line<8, 64, 1>{});
+    if (within(Line<V, 64, 1>{})) return f(Line<V, 64, 1>{});
+    if (within(Line<V, 64, 2>{})) return f(Line<V, 64, 2>{});
+    if (within(Line<V, 64, 4>{})) return f(Line<V, 64, 4>{});
+    if (within(Line<8, 64, 8>{})) return f(Line<8, 64, 8>{});
+    return f(LongLine{});
 }
 
 // The chain of a shape whose tiles are kSteps long and kChannels wide (0: one channel, a row).
@@ -145,7 +156,7 @@ template <class T>
 hipError_t forward_of(const ScanShape& s, const ScanForward& a, hipStream_t stream) {
     if (s.n == 1) return launch_step<T>(s, a, stream);
     if (s.channels_first)
-        return with_line(s, [&](auto line) {
+        return with_line<T, false>(s, [&](auto line) {
             using L = decltype(line);
             return launch_first<L>(scan_first_forward<T, L>, s, a, stream);
         });
@@ -158,7 +169,7 @@ hipError_t forward_of(const ScanShape& s, const ScanForward& a, hipStream_t stre
 template <class T>
 hipError_t backward_of(const ScanShape& s, const ScanBackward& a, hipStream_t stream) {
     if (s.channels_first)
-        return with_line(s, [&](auto line) {
+        return with_line<T, true>(s, [&](auto line) {
             using L = decltype(line);
             return launch_first<L>(scan_first_backward<T, L>, s, a, stream);
         });
@@ -173,18 +184,12 @@ hipError_t backward_of(const ScanShape& s, const ScanBackward& a, hipStream_t st
 long long scan_saved_bytes(const ScanShape& s) {
     if (s.n == 0) return 0;
     const long long rows = static_cast<long long>(s.batch) * s.channels;
-    if (s.channels_first)
-        return with_line(s, [&](auto line) {
-            return 4 * rows * first_chain<decltype(line)>(s, nullptr).tiles;
-        });
+    if (s.channels_first) return 4 * rows * first_chain<LongLine>(s, nullptr).tiles;
     return 4 * rows * ((static_cast<long long>(s.n) + kSaved - 1) / kSaved);
 }
 
 long long scan_workspace_bytes(const ScanShape& s) {
-    if (s.channels_first)
-        return with_line(s, [&](auto line) {
-            return chain_bytes(first_chain<decltype(line)>(s, nullptr), 0);
-        });
+    if (s.channels_first) return chain_bytes(first_chain<LongLine>(s, nullptr), 0);
     const auto bytes = [&](auto tile) {
         using L = decltype(tile);
         return chain_bytes(last_chain<L>(s, nullptr), L::kChannels);
@@ -197,10 +202,7 @@ long long scan_workspace_bytes(const ScanShape& s) {
 
 bool scan_fits(const ScanShape& s) {
     if (static_cast<long long>(s.batch) * s.channels > 0x7fffff00LL) return false;
-    if (s.channels_first)
-        return with_line(s, [&](auto line) {
-            return chain_fits(first_chain<decltype(line)>(s, nullptr));
-        });
+    if (s.channels_first) return chain_fits(first_chain<LongLine>(s, nullptr));
     const auto fits = [&](auto tile) { return chain_fits(last_chain<decltype(tile)>(s, nullptr)); };
     return with_type(s, [&](auto v) {
         using T = decltype(v);

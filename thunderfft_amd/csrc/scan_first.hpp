@@ -1,5 +1,5 @@
 // scan_first.hpp -- the gated recurrence on [batch][channels][n] values (the convolutions'
-// layout): one pass over the data.  A lane takes 8 neighbouring steps and composes them; the
+// layout): one pass over the data.  A lane takes 8 or 16 neighbouring steps and composes them; the
 // lanes of a row join theirs in registers, its waves through LDS, and where a row takes several
 // workgroups, they join through the chain.  Short rows lie side by side in a wave.
 #pragma once
@@ -8,12 +8,15 @@
 
 namespace thff {
 
-// LPR lanes of each of WPR waves a row; a row's tile is kSteps steps.
-template <int LPR_, int WPR_>
+// V steps a lane, LPR lanes of each of WPR waves a row; a row's tile is kSteps steps.  Chained:
+// rows of several tiles, each a workgroup's.  (A kernel for rows of one tile has no code for
+// more, which costs registers.)
+template <int V_, int LPR_, int WPR_, bool Chained_ = false>
 struct Line {
-    static constexpr int V = 8, W = 8, LPR = LPR_, WPR = WPR_, kLanes = 64 * W;
+    static constexpr int V = V_, LPR = LPR_, WPR = WPR_, W = WPR_ > 4 ? 8 : 4, kLanes = 64 * W;
     static constexpr int kSteps = LPR * WPR * V, kRows = W / WPR * (64 / LPR);
-    static constexpr bool kChained = WPR == W;  // a workgroup has one row
+    static constexpr bool kChained = Chained_;
+    static_assert(!kChained || WPR == W, "a workgroup of a chain has one row");
 };
 
 // `v` of the lane that Control moves here, `none` where there is none.
@@ -34,21 +37,25 @@ template <int LPR>
 __device__ __forceinline__ Span join_line(Span& mine) {
     constexpr Span kNone = {1.0f, 0.0f};
     const int lane = threadIdx.x % LPR;
-    static_assert(LPR == 4 || LPR == 16 || LPR == 64, "groups that the moves below keep apart");
-    if constexpr (LPR == 4) {
+    static_assert(LPR >= 4 && LPR <= 64 && (LPR & (LPR - 1)) == 0, "a power of two");
+    if constexpr (LPR < 16) {
+        // Groups that a row of 16 lanes has several of.
         const Span one = moved<0x111>(mine);  // from the lane before
         mine = then(lane >= 1 ? one : kNone, mine);
         const Span two = moved<0x112>(mine);
         mine = then(lane >= 2 ? two : kNone, mine);
+        if constexpr (LPR == 8) {
+            const Span four = moved<0x114>(mine);
+            mine = then(lane >= 4 ? four : kNone, mine);
+        }
     } else {
         mine = then(moved<0x111>(mine), mine);
         mine = then(moved<0x112>(mine), mine);
         mine = then(moved<0x114>(mine), mine);
         mine = then(moved<0x118>(mine), mine);
-        if constexpr (LPR == 64) {
-            mine = then(moved<0x142, 0xa>(mine), mine);  // a row of 16's last to the next one
-            mine = then(moved<0x143, 0xc>(mine), mine);  // lane 31 to the upper half
-        }
+        // A row of 16's last lane to the next row; lane 31 to the upper half.
+        if constexpr (LPR >= 32) mine = then(moved<0x142, 0xa>(mine), mine);
+        if constexpr (LPR == 64) mine = then(moved<0x143, 0xc>(mine), mine);
     }
     const Span before = moved<0x138>(mine);  // from the lane before, across rows of 16 too
     return lane == 0 ? kNone : before;
@@ -64,7 +71,7 @@ __device__ __forceinline__ Span join_line_back(Span& mine) {
     return before;
 }
 
-// A lane's 8 steps: those of its own that are `in` the sequence; the first `skip` of the vector
+// A lane's V steps: those of its own that are `in` the sequence; the first `skip` of the vector
 // it reads are another lane's (the row ends inside its own), the others up to `own` are in the
 // tensor.
 template <class L>
@@ -123,38 +130,73 @@ __device__ __forceinline__ void store_line(T* row, pack<T, L::V> v, const Stretc
     }
 }
 
+// The chain's link of a row's r-th tile, by the 16 first lanes of a wave, a word each: the
+// published state on lane 0, spans of 8 tiles on the next, single ones from lane 8 on.
+struct RowLink {
+    Word* words;
+    long long step;
+    int r;
+    const Word* at;
+    Word word;
+    bool has;
+
+    // Asks without waiting.
+    __device__ __forceinline__ RowLink(Word* words_, long long step_, int r_) : words(words_), step(step_), r(r_) {
+        const int lane = threadIdx.x % 64;
+        const int base = (r - 1) / kSuper * kSuper, groups = (r - 1 - base) / kGroup;
+        const int single = (r - 1 - base) % kGroup;
+        static_assert(kGroup == 8 && kSuper == 64, "at most 7 words of either kind");
+        const int tile = lane < 8 ? base + lane * kGroup : base + groups * kGroup + 1 + lane - 8;
+        has = r > 0 && (lane < 8 ? lane <= groups : lane - 8 < single);
+        at = words + tile * step;
+        if (has) word = look(at);
+    }
+
+    // Publishes what the tiles behind it need (if `later`) of the tile, whose span is `own`,
+    // waits for the answers, and returns the state that the tile starts from, which for r = 0
+    // is the one given; all on every lane.
+    __device__ __forceinline__ float join(Span own, bool later, float given) {
+        constexpr Span kNone = {1.0f, 0.0f};
+        const int lane = threadIdx.x % 64;
+        const bool publisher = later && lane == 0;
+        if (publisher && r % kGroup != 0) publish(words + r * step, own);
+        Span mine = kNone;
+        if (has) mine = seen(word, at);
+        if (r == 0 && lane == 0) mine = {0.0f, given};
+        Span near = lane >= 8 ? mine : kNone;
+        join_line<16>(near);
+        near = {__shfl(near.a, 15), __shfl(near.b, 15)};
+        if (publisher && r % kGroup == 0 && r % kSuper != 0) publish(words + r * step, then(near, own));
+        join_line<16>(mine);
+        const float h = __shfl(mine.b, 15);
+        if (publisher && r % kSuper == 0) publish(words + r * step, {0.0f, after(own, h)});
+        return h;
+    }
+};
+
 // Joins a workgroup's waves, whose spans are in `waves` in the order of the chain, and the
 // tiles; returns the state before the wave's first step in that order.  `given`: the row's
 // first state, on every lane.  own: the wave's place in its row.
 template <class L>
 __device__ __forceinline__ float join_tile(const Chain& chain, const Span* waves, float* start, int own,
                                            int r, bool part, bool later, float given) {
-    const int wave = threadIdx.x / 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     if constexpr (L::WPR == 1) return given;
     if constexpr (L::kChained) {
-        if (chain.tiles > 1) {
-            Link<1> link;
-            link.words = chain.words + chain.column();
-            link.step = chain.columns;
-            link.r = r;
-            if (threadIdx.x == 0 && part) link.ask();
+        if (wave == 0) {
+            RowLink link(chain.words + chain.column(), chain.columns, part ? r : 0);
             __syncthreads();
-            if (threadIdx.x == 0 && part) {
-                Span all = waves[0];
+            Span all = waves[0];
 #pragma unroll
-                for (int w = 1; w < L::W; ++w) all = then(all, waves[w]);
-                const Span own_span[1] = {all};
-                const float first[1] = {given};
-                float h[1];
-                link.join(h, own_span, later, first);
-                start[0] = h[0];
-            }
+            for (int w = 1; w < L::W; ++w) all = then(all, waves[w]);
+            const float h = link.join(all, part && later, given);
+            if (threadIdx.x == 0) start[0] = h;
             __syncthreads();
-            given = start[0];
         } else {
             __syncthreads();
-            given = start[0];
+            __syncthreads();
         }
+        given = start[0];
     } else {
         __syncthreads();
         given = start[wave / L::WPR];
@@ -170,9 +212,8 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_forward(ScanShape s, Sca
     __shared__ Span waves[L::W];
     __shared__ float start[L::W];
     __shared__ int drawn;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const bool chained = L::kChained && chain.tiles > 1;
-    const Stretch<L> p(s, a.lengths, chain, chained ? draw_tile(chain, &drawn, 0) : 0);
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const Stretch<L> p(s, a.lengths, chain, L::kChained ? draw_tile(chain, &drawn, 0) : 0);
     const int srow = state_row(s, a.slots, p.b);
     const long long state = static_cast<long long>(srow) * s.channels + p.c;
     // A tile that lies past the sequence's end has zeros to write and no part in the chain.
@@ -230,9 +271,8 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_backward(ScanShape s, Sc
     __shared__ Span waves[L::W], back[L::W];
     __shared__ float start[L::W];
     __shared__ int drawn;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const bool chained = L::kChained && chain.tiles > 1;
-    const Stretch<L> p(s, a.lengths, chain, chained ? chain.tiles - 1 - draw_tile(chain, &drawn, 0) : 0);
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const Stretch<L> p(s, a.lengths, chain, L::kChained ? chain.tiles - 1 - draw_tile(chain, &drawn, 0) : 0);
     const bool part = p.tile * L::kSteps < p.len || p.tile == 0;
     const int r = max(p.len - 1, 0) / L::kSteps - p.tile;
     pack<T, V> g = {}, x = {}, dy = {};
