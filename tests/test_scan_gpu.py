@@ -459,6 +459,14 @@ def test_drawn(seed):
             gap=gap, offset=offset)
 
 
+@pytest.mark.parametrize("T", ["float", "bfloat16"])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("size", [(1, 7400, 64), (2, 9000, 65), (1, 33000, 5)], ids=str)
+def test_few_channels_and_many_steps(T, layout, size):
+    """Chains of tens to hundreds of tiles, one or a few side by side."""
+    compare(T, layout, *values(sum(size), T, layout, *size))
+
+
 def test_long_sequences():
     """More steps than any workgroup keeps, few channels: the state is carried a long way
     (nearly closed gates), against the definition."""

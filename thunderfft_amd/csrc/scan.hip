@@ -25,18 +25,25 @@ __global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long count
 }
 
 // Channels last: calls f with the tile type of a shape's forward or backward pass: 4 bytes a
-// lane and row; lanes along the channels all 64 of a wave, or 16 where that leaves far fewer of
-// them idle.
+// lane and row.  Lanes along the channels are all 64 of a wave, or 16
+//  - where that leaves far fewer of them idle (half 128 x 1000 x 64: 18.7 against 23.5 us forward,
+//    37 against 42 backward; 64 x 1000 x 200, which takes 256 or 224: 39 against 26 and 78
+//    against 44), and
+//  - where one or two columns of tiles are so long that they wait for each other's ends: tiles
+//    of four times the steps have a quarter of those (float 1 x 46504 x 64: 21 against 35 and 33
+//    against 50 us; half 1 x 65536 x 512, four columns: 83 against 66 and 177 against 117).
 template <class T, bool Backward, class F>
 auto with_tile(const ScanShape& s, F f) {
-    constexpr int VEC = 4 / sizeof(T);
-    using Wide = std::conditional_t<Backward, Tile<VEC, 64, 4, 14, 2, 8>, Tile<VEC, 64, 8, 14, 2, 8>>;
-    using Thin = std::conditional_t<Backward, Tile<VEC, 16, 4, 14, 2, 8>, Tile<VEC, 16, 8, 14, 2, 8>>;
+    constexpr int VEC = 4 / sizeof(T), S = Backward ? 4 : 8;
+    using Wide = Tile<VEC, 64, S, 14, 2, 8>;
+    using Thin = Tile<VEC, 16, S, 14, 2, 8>;
     const auto taken = [&](long long channels) {
         return (s.channels + channels - 1) / channels * channels;
     };
-    const bool thin = 4 * taken(Wide::kChannels) > 5 * taken(Thin::kChannels);
-    return thin ? f(Thin{}) : f(Wide{});
+    const bool idle = 4 * taken(Wide::kChannels) > 5 * taken(Thin::kChannels);
+    const bool long_few = s.batch * taken(Wide::kChannels) <= 2 * Wide::kChannels &&
+                          s.n / Wide::kSteps >= kSuper;
+    return idle || long_few ? f(Thin{}) : f(Wide{});
 }
 
 // Calls f with a value of the shape's type.

@@ -70,14 +70,13 @@ struct Inside {
     int inside, rows, some;
 };
 
-// `none` in the place of what is not inside.  Where not all is, a lane reads its last row
-// instead of those past the tensor, and the last VEC channels instead of some of them and some
-// that are not there, so that no load waits for another or for a branch.
+// Where not all is inside, a lane reads its last row instead of those past the tensor, and the
+// last VEC channels instead of some of them and some that are not there, so that no load waits
+// for another or for a branch; keep_inside() puts that right when all loads are under way.
 template <class T, class L, class Offset>
 __device__ __forceinline__ void load_steps(pack<T, L::VEC> (&to)[L::S], const T* at, Offset lane,
-                                           long long stride, Inside in, int channels, T none) {
+                                           long long stride, Inside in, int channels) {
     constexpr int VEC = L::VEC, S = L::S;
-    static_assert(VEC <= 4, "vectors are shifted by up to 3");
     stride = anew(stride);
     if (in.full) {
 #pragma unroll
@@ -85,37 +84,38 @@ __device__ __forceinline__ void load_steps(pack<T, L::VEC> (&to)[L::S], const T*
         return;
     }
 #pragma unroll
-    for (int k = 0; k < S; ++k) to[k] = none;
+    for (int k = 0; k < S; ++k) to[k] = pack<T, VEC>{};
     if (in.rows <= 0 || in.some <= 0) return;
     const int shift = VEC - in.some;
     const T* p = at + lane;
-    pack<T, VEC> v[S];
     if (channels < VEC) {
 #pragma unroll
         for (int k = 0; k < S; ++k) {
-            v[k] = none;
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                if (i >= shift) v[k][i] = p[i - shift];
+                if (i >= shift) to[k][i] = p[i - shift];
             if (k < in.rows - 1) p += stride;
         }
     } else {
         p -= shift;
 #pragma unroll
         for (int k = 0; k < S; ++k) {
-            v[k] = load_pack<T, VEC>(p);
+            to[k] = load_pack<T, VEC>(p);
             if (k < in.rows - 1) p += stride;
         }
     }
+}
+
+// Moves the channels of a vector that was read further back to its start, and puts `none` in the
+// place of steps that are not inside.
+template <class T, class L>
+__device__ __forceinline__ void keep_inside(pack<T, L::VEC> (&v)[L::S], Inside in, T none) {
+    static_assert(L::VEC <= 2, "a vector is cut after its first channel");
+    if (in.full) return;
 #pragma unroll
-    for (int k = 0; k < S; ++k) {
-#pragma unroll
-        for (int by = 1; by < VEC; by *= 2)
-            if (shift & by) {
-#pragma unroll
-                for (int i = 0; i + by < VEC; ++i) v[k][i] = v[k][i + by];
-            }
-        if (k < in.inside) to[k] = v[k];
+    for (int k = 0; k < L::S; ++k) {
+        if (in.some < L::VEC) v[k][0] = v[k][L::VEC - 1];
+        if (k >= in.inside) v[k] = none;
     }
 }
 
@@ -250,9 +250,9 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(Sc
         const long long row = p.row(s, wave);
         const Inside in = p.inside(s, wave, sub);
         load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + p.c0, at_gate,
-                         s.gate_stride, in, s.channels, open_gate<T>());
+                         s.gate_stride, in, s.channels);
         load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + p.c0, at_x, s.x_stride,
-                         in, s.channels, static_cast<T>(0.0f));
+                         in, s.channels);
     };
     load();
     if (chained) {
@@ -264,6 +264,8 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(Sc
     }
     const long long first = p.row(s, wave);
     const Inside in = p.inside(s, wave, sub);
+    keep_inside<T, L>(g, in, open_gate<T>());
+    keep_inside<T, L>(x, in, static_cast<T>(0.0f));
     float f[S][VEC], u[S][VEC];
     Span before[VEC];
 #pragma unroll
@@ -348,11 +350,11 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
         const long long row = p.row(s, wave);
         const Inside in = p.inside(s, wave, sub);
         load_steps<T, L>(g, static_cast<const T*>(a.gate) + row * s.gate_stride + p.c0, at_gate,
-                         s.gate_stride, in, s.channels, open_gate<T>());
+                         s.gate_stride, in, s.channels);
         load_steps<T, L>(x, static_cast<const T*>(a.x) + row * s.x_stride + p.c0, at_x, s.x_stride,
-                         in, s.channels, static_cast<T>(0.0f));
+                         in, s.channels);
         load_steps<T, L>(dy, static_cast<const T*>(a.dy) + row * s.y_stride + p.c0, at_y, s.y_stride,
-                         in, s.channels, static_cast<T>(0.0f));
+                         in, s.channels);
 #pragma unroll
         for (int v = 0; v < VEC; ++v)
             h[v] = p.t0() < p.len && v < in.some
@@ -369,6 +371,9 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
     }
     const long long row = p.row(s, wave);
     const Inside in = p.inside(s, wave, sub);
+    keep_inside<T, L>(g, in, open_gate<T>());
+    keep_inside<T, L>(x, in, static_cast<T>(0.0f));
+    keep_inside<T, L>(dy, in, static_cast<T>(0.0f));
     float f[S][VEC], enter[S][VEC], q[S][VEC];
     Span before[VEC], past[VEC];
 #pragma unroll
