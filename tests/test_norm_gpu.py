@@ -219,6 +219,17 @@ def test_offsets_past_32_bits():
         oracle.check(name, v, want[name])
 
 
+def test_more_rows_than_one_launch_has_lanes():
+    """2^30 rows of one value take several launches: each is its mean, so y is the bias."""
+    rows = (1 << 30) + 5
+    x = torch.ones(rows, 1, dtype=torch.float16, device="cuda")
+    y = torch.full_like(x, float("nan"))
+    mean, rstd = torch.full((rows,), GUARD, device="cuda"), torch.full((rows,), GUARD, device="cuda")
+    bias = torch.full((1,), 0.75, device="cuda")
+    thff.ThunderFFT_layer_norm("half", x, None, bias, 1.0, y, rows, 1, d_mean=mean, d_rstd=rstd)
+    assert bool((y == 0.75).all()) and bool((mean == 1).all()) and bool((rstd == 1).all())
+
+
 def test_gradients_against_differences():
     """As the recurrence's: a central difference of the float forward pass, off by its
     roundings and by the truncation that the same quotient in 64 bits has."""

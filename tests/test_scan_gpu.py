@@ -154,6 +154,15 @@ def test_lengths(T, layout):
         assert torch.equal(within[name], outside[name]), name
 
 
+@pytest.mark.parametrize("T", ["float", "half"])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_short_lengths_of_long_rows(T, layout):
+    """Most of the steps are padding: states and gradients pass over it unchanged."""
+    lengths = torch.tensor([0, 1, 130, 9000, 4700], dtype=torch.int32, device="cuda")
+    x, gate, dy, state, dstate = values(15, T, layout, len(lengths), 9000, 18)
+    compare(T, layout, x, gate, dy, state, dstate, lengths)
+
+
 @pytest.mark.parametrize("layout", LAYOUTS)
 def test_no_steps(layout):
     """n = 0 hands the states through, also by slots."""

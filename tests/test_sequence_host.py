@@ -47,6 +47,16 @@ def test_shapes_refused():
     assert L.thff_gated_scan_saved_bytes(None) == thff.THFF_EINVAL
 
 
+def test_launch_limits():
+    """Shapes whose workgroups one launch does not have are refused; the largest ones are not."""
+    for layout in ("channels_last", "channels_first"):
+        with pytest.raises(ValueError, match="exceeds one launch"):
+            shape(batch=1 << 20, n=1 << 28, channels=64, layout=layout).saved_bytes()
+        assert shape(batch=1 << 30, n=2, channels=1, layout=layout).saved_bytes() > 0
+        assert shape(batch=1 << 20, n=3, channels=64, layout=layout).saved_bytes() > 0
+        assert shape(batch=1, n=1 << 30, channels=128, layout=layout).workspace_bytes() > 0
+
+
 def test_sizes():
     """Sizes are counted, not negative, and grow with what has to be kept."""
     for layout in ("channels_last", "channels_first"):

@@ -367,24 +367,28 @@ __global__ __launch_bounds__(kLongLanes) void long_backward(NormBackward a) {
 template <class T>
 __global__ __launch_bounds__(1024) void long_weights(NormBackward a) {
     __shared__ float lds[2][32][33];
-    const int lane = threadIdx.x % 32, group = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
-    float w = 0.0f, b = 0.0f;
-    if (c < a.cols)
-        for (long long row = group; row < a.rows; row += 32) {
-            const float dy = to_float<T>(static_cast<const T*>(a.dy)[row * a.dy_stride + c]);
-            const float x = to_float<T>(static_cast<const T*>(a.x)[row * a.x_stride + c]);
-            w = fmaf(dy, (x - a.mean[row]) * a.rstd[row], w);
-            b += dy;
+    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+    for (long long c0 = 32LL * blockIdx.x; c0 < a.cols; c0 += 32LL * gridDim.x) {
+        const long long c = c0 + lane;
+        float w = 0.0f, b = 0.0f;
+        if (c < a.cols)
+            for (long long row = group; row < a.rows; row += 32) {
+                const float dy = to_float<T>(static_cast<const T*>(a.dy)[row * a.dy_stride + c]);
+                const float x = to_float<T>(static_cast<const T*>(a.x)[row * a.x_stride + c]);
+                w = fmaf(dy, (x - a.mean[row]) * a.rstd[row], w);
+                b += dy;
+            }
+        __syncthreads();
+        lds[0][group][lane] = w;
+        lds[1][group][lane] = b;
+        __syncthreads();
+        w = lane_sum<32>(lds[0][lane][group]);
+        b = lane_sum<32>(lds[1][lane][group]);
+        const long long to = c0 + group;
+        if (lane == 0 && to < a.cols) {
+            if (a.dweight) a.dweight[to] = w;
+            if (a.dbias) a.dbias[to] = b;
         }
-    lds[0][group][lane] = w;
-    lds[1][group][lane] = b;
-    __syncthreads();
-    w = lane_sum<32>(lds[0][lane][group]);
-    b = lane_sum<32>(lds[1][lane][group]);
-    const int to = blockIdx.x * 32 + group;
-    if (lane == 0 && to < a.cols) {
-        if (a.dweight) a.dweight[to] = w;
-        if (a.dbias) a.dbias[to] = b;
     }
 }
 
@@ -419,8 +423,10 @@ auto with_type(int precision, F f) {
     return f(bfloat_t{});
 }
 
-unsigned long_blocks(long long rows) {
-    return static_cast<unsigned>(std::min<long long>(rows, 1 << 30));
+// Workgroups of 1024 lanes, each for every so-many-th row or group of columns: a launch has less
+// than 2^32 lanes.
+unsigned long_blocks(long long count) {
+    return static_cast<unsigned>(std::min<long long>(count, 1 << 20));
 }
 
 // Forward: 32 values a lane, which are all that it keeps.  Backward: 16, next to the weights,
@@ -446,8 +452,8 @@ hipError_t forward_of(const NormForward& a, hipStream_t stream) {
     hipError_t err = hipSuccess;
     const bool held = with_forward_rows<T>(a.cols, [&](auto type) {
         using R = decltype(type);
-        // At most 2^30 workgroups a launch.
-        constexpr long long kMost = static_cast<long long>(R::kRows) << 30;
+        // A launch has less than 2^32 lanes.
+        constexpr long long kMost = (1LL << 31) / R::kLanes * R::kRows;
         NormForward part = a;
         for (long long done = 0; done < a.rows && err == hipSuccess; done += kMost) {
             part.rows = std::min(kMost, a.rows - done);
@@ -478,7 +484,7 @@ hipError_t backward_of(const NormBackward& a, hipStream_t stream) {
     });
     if (!held) {
         if (a.rows > 0) long_backward<T><<<long_blocks(a.rows), kLongLanes, 0, stream>>>(a);
-        if (weights) long_weights<T><<<(a.cols + 31) / 32, 1024, 0, stream>>>(a);
+        if (weights) long_weights<T><<<long_blocks((a.cols + 31LL) / 32), 1024, 0, stream>>>(a);
     }
     return hipGetLastError();
 }

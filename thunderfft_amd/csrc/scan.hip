@@ -18,10 +18,11 @@ constexpr int kLanes = 256;
 // is not replayed reliably.)
 __global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long counters,
                                                       long long count) {
-    const long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x;
-    if (i >= count) return;
-    const unsigned v = i < counters ? 0u : ~0u;
-    to[i] = make_uint4(v, v, v, v);
+    for (long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x; i < count;
+         i += static_cast<long long>(gridDim.x) * kLanes) {
+        const unsigned v = i < counters ? 0u : ~0u;
+        to[i] = make_uint4(v, v, v, v);
+    }
 }
 
 // Channels last: calls f with the tile type of a shape's forward or backward pass: 4 bytes a
@@ -77,7 +78,7 @@ auto with_line(const ScanShape& s, F f) {
     return f(LongLine{});
 }
 
-// The chain of a shape whose tiles are kSteps long and kChannels wide (0: one channel, a row).
+// The chain of a shape whose tiles are `steps` long and `channels` wide (0: one channel, a row).
 Chain chain_of(const ScanShape& s, int channels, int steps, void* workspace) {
     Chain chain;
     chain.slabs = channels ? (s.channels + channels - 1) / channels : s.channels;
@@ -94,12 +95,22 @@ Chain chain_of(const ScanShape& s, int channels, int steps, void* workspace) {
 
 template <class L>
 Chain last_chain(const ScanShape& s, void* workspace) {
-    return chain_of(s, L::kChannels, L::kSteps, workspace);
+    Chain chain = chain_of(s, L::kChannels, L::kSteps, workspace);
+    chain.blocks = chain.columns * chain.tiles;
+    return chain;
 }
 
 template <class L>
 Chain first_chain(const ScanShape& s, void* workspace) {
-    return chain_of(s, 0, L::kSteps, workspace);
+    Chain chain = chain_of(s, 0, L::kSteps, workspace);
+    chain.blocks = L::kChained ? chain.columns * chain.tiles
+                               : static_cast<unsigned>((chain.columns + static_cast<long long>(L::kRows) - 1) / L::kRows);
+    return chain;
+}
+
+dim3 grid_of(const Chain& chain) {
+    constexpr unsigned kMost = 1u << 21;
+    return dim3(std::min(chain.blocks, kMost), (chain.blocks + kMost - 1) / kMost);
 }
 
 long long chain_bytes(const Chain& chain, int channels) {
@@ -108,15 +119,16 @@ long long chain_bytes(const Chain& chain, int channels) {
     return (chain.columns * static_cast<long long>(kCounterBytes) + 8 * words + 15) / 16 * 16;
 }
 
-// Whether a launch has as many workgroups as the chain has tiles.
-bool chain_fits(const Chain& chain) {
-    return static_cast<__int128>(chain.columns) * chain.tiles <= 0x7fffffff;
+// Whether the workgroups of all tiles can be counted.
+bool chain_fits(const ScanShape& s, const Chain& chain) {
+    return static_cast<__int128>(s.batch) * chain.slabs * chain.tiles <= 0x7fffffff;
 }
 
 hipError_t clear(const Chain& chain, int channels, hipStream_t stream) {
     const long long count = chain_bytes(chain, channels) / 16;
     if (count == 0) return hipSuccess;
-    clear_chain<<<static_cast<unsigned>((count + kLanes - 1) / kLanes), kLanes, 0, stream>>>(
+    const long long blocks = std::min((count + kLanes - 1) / kLanes, 1LL << 20);
+    clear_chain<<<static_cast<unsigned>(blocks), kLanes, 0, stream>>>(
         reinterpret_cast<uint4*>(chain.drawn), chain.columns * (kCounterBytes / 16LL), count);
     return hipGetLastError();
 }
@@ -127,7 +139,7 @@ hipError_t launch_last(void (*kernel)(ScanShape, Args, Chain), const ScanShape& 
     const Chain chain = last_chain<L>(s, a.workspace);
     const hipError_t err = clear(chain, L::kChannels, stream);
     if (err != hipSuccess) return err;
-    kernel<<<chain.columns * chain.tiles, L::kLanes, 0, stream>>>(s, a, chain);
+    kernel<<<grid_of(chain), L::kLanes, 0, stream>>>(s, a, chain);
     return hipGetLastError();
 }
 
@@ -137,9 +149,7 @@ hipError_t launch_first(void (*kernel)(ScanShape, Args, Chain), const ScanShape&
     const Chain chain = first_chain<L>(s, a.workspace);
     const hipError_t err = clear(chain, 0, stream);
     if (err != hipSuccess) return err;
-    const unsigned blocks =
-        L::kChained ? chain.columns * chain.tiles : (chain.columns + L::kRows - 1) / L::kRows;
-    kernel<<<blocks, L::kLanes, 0, stream>>>(s, a, chain);
+    kernel<<<grid_of(chain), L::kLanes, 0, stream>>>(s, a, chain);
     return hipGetLastError();
 }
 
@@ -209,8 +219,8 @@ long long scan_workspace_bytes(const ScanShape& s) {
 
 bool scan_fits(const ScanShape& s) {
     if (static_cast<long long>(s.batch) * s.channels > 0x7fffff00LL) return false;
-    if (s.channels_first) return chain_fits(first_chain<LongLine>(s, nullptr));
-    const auto fits = [&](auto tile) { return chain_fits(last_chain<decltype(tile)>(s, nullptr)); };
+    if (s.channels_first) return chain_fits(s, first_chain<LongLine>(s, nullptr));
+    const auto fits = [&](auto tile) { return chain_fits(s, last_chain<decltype(tile)>(s, nullptr)); };
     return with_type(s, [&](auto v) {
         using T = decltype(v);
         return with_tile<T, false>(s, fits) && with_tile<T, true>(s, fits);

@@ -63,7 +63,6 @@ __device__ __forceinline__ Span then(Span first, Span second) {
 __device__ __forceinline__ float after(Span s, float h) { return fmaf(s.a, h, s.b); }
 
 using Word = unsigned long long;
-constexpr Word kEmpty = ~0ull;
 
 __device__ __forceinline__ void publish(Word* to, Span s) {
     // The one NaN that looks empty is replaced by another.
@@ -105,11 +104,14 @@ struct Chain {
     Word* words;
     int slabs, tiles;  // tiles along the channels, along the steps
     unsigned columns;  // batch * slabs
+    unsigned blocks;   // workgroups
     Divider by_columns, by_slabs;
 
+    // A launch has less than 2^32 lanes along x, so many workgroups take rows of a grid.
+    __device__ __forceinline__ unsigned block() const { return blockIdx.y * gridDim.x + blockIdx.x; }
     // The column of a workgroup, and the tile of it that it expects to draw.
-    __device__ __forceinline__ int expected() const { return by_columns.quotient(blockIdx.x); }
-    __device__ __forceinline__ int column() const { return blockIdx.x - expected() * columns; }
+    __device__ __forceinline__ int expected() const { return by_columns.quotient(block()); }
+    __device__ __forceinline__ int column() const { return block() - expected() * columns; }
 };
 constexpr int kCounterBytes = 64;
 

@@ -84,7 +84,8 @@ struct Stretch {
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
         const int rows = s.batch * s.channels;
         const int mine = L::kChained ? chain.column()
-                                     : blockIdx.x * L::kRows + wave / L::WPR * (64 / L::LPR) + lane / L::LPR;
+                                     : static_cast<int>(chain.block()) * L::kRows +
+                                           wave / L::WPR * (64 / L::LPR) + lane / L::LPR;
         active = mine < rows;
         row = min(mine, rows - 1);
         b = chain.by_slabs.quotient(row);
@@ -102,8 +103,10 @@ struct Stretch {
     }
 };
 
+// Nothing is read that is not used, but for what a vector reads of another lane's steps.
 template <class T, class L>
 __device__ __forceinline__ pack<T, L::V> load_line(const T* row, const Stretch<L>& p, int n) {
+    if (p.first >= p.len) return pack<T, L::V>{};
     if (n >= L::V) return load_pack<T, L::V>(row + p.at);
     pack<T, L::V> v = {};
 #pragma unroll
@@ -176,20 +179,21 @@ struct RowLink {
 
 // Joins a workgroup's waves, whose spans are in `waves` in the order of the chain, and the
 // tiles; returns the state before the wave's first step in that order.  `given`: the row's
-// first state, on every lane.  own: the wave's place in its row.
+// first state, on every lane.  own: the wave's place in its row.  Every tile has its place in the
+// chain, also past the sequence's end, so that no wait depends on the lengths.
 template <class L>
 __device__ __forceinline__ float join_tile(const Chain& chain, const Span* waves, float* start, int own,
-                                           int r, bool part, bool later, float given) {
+                                           int r, float given) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     if constexpr (L::WPR == 1) return given;
     if constexpr (L::kChained) {
         if (wave == 0) {
-            RowLink link(chain.words + chain.column(), chain.columns, part ? r : 0);
+            RowLink link(chain.words + chain.column(), chain.columns, r);
             __syncthreads();
             Span all = waves[0];
 #pragma unroll
             for (int w = 1; w < L::W; ++w) all = then(all, waves[w]);
-            const float h = link.join(all, part && later, given);
+            const float h = link.join(all, r + 1 < chain.tiles, given);
             if (threadIdx.x == 0) start[0] = h;
             __syncthreads();
         } else {
@@ -212,12 +216,11 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_forward(ScanShape s, Sca
     __shared__ Span waves[L::W];
     __shared__ float start[L::W];
     __shared__ int drawn;
+    if (chain.block() >= chain.blocks) return;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const Stretch<L> p(s, a.lengths, chain, L::kChained ? draw_tile(chain, &drawn, 0) : 0);
     const int srow = state_row(s, a.slots, p.b);
     const long long state = static_cast<long long>(srow) * s.channels + p.c;
-    // A tile that lies past the sequence's end has zeros to write and no part in the chain.
-    const bool part = p.tile * L::kSteps < p.len || p.tile == 0;
     pack<T, V> g = {}, x = {};
     if (s.n > 0) {
         g = load_line<T, L>(static_cast<const T*>(a.gate) + p.row * s.gate_stride, p, s.n);
@@ -246,8 +249,7 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_forward(ScanShape s, Sca
         // Through LDS, so that it has been read before anyone stores a last state there.
         if (lane == 0 && wave % L::WPR == 0) start[wave / L::WPR] = given;
     }
-    float h = join_tile<L>(chain, waves, start, wave % L::WPR, p.tile, part,
-                           (p.tile + 1) * static_cast<long long>(L::kSteps) < p.len, given);
+    float h = join_tile<L>(chain, waves, start, wave % L::WPR, p.tile, given);
     if (a.saved && p.active && p.first == p.tile * L::kSteps)
         a.saved[static_cast<long long>(p.row) * chain.tiles + p.tile] = h;
     h = after(before, h);
@@ -271,10 +273,10 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_backward(ScanShape s, Sc
     __shared__ Span waves[L::W], back[L::W];
     __shared__ float start[L::W];
     __shared__ int drawn;
+    if (chain.block() >= chain.blocks) return;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const Stretch<L> p(s, a.lengths, chain, L::kChained ? chain.tiles - 1 - draw_tile(chain, &drawn, 0) : 0);
-    const bool part = p.tile * L::kSteps < p.len || p.tile == 0;
-    const int r = max(p.len - 1, 0) / L::kSteps - p.tile;
+    const int r = chain.tiles - 1 - p.tile;
     pack<T, V> g = {}, x = {}, dy = {};
     if (s.n > 0) {
         g = load_line<T, L>(static_cast<const T*>(a.gate) + p.row * s.gate_stride, p, s.n);
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_backward(ScanShape s, Sc
         dy = load_line<T, L>(static_cast<const T*>(a.dy) + p.row * s.y_stride, p, s.n);
     }
     float given = r == 0 && a.dstate_out ? a.dstate_out[p.row] : 0.0f;
-    float h = part && s.n > 0 ? a.saved[static_cast<long long>(p.row) * chain.tiles + p.tile] : 0.0f;
+    float h = s.n > 0 ? a.saved[static_cast<long long>(p.row) * chain.tiles + p.tile] : 0.0f;
     const bool full = p.full();
     float f[V], enter[V], q[V], d[V];
 #pragma unroll
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_backward(ScanShape s, Sc
         if (lane == 0) back[wave - own + L::WPR - 1 - own] = behind;
         if (lane == 0 && own == 0) start[wave / L::WPR] = given;
     }
-    float grad = join_tile<L>(chain, back, start, L::WPR - 1 - own, r, part, p.tile > 0, given);
+    float grad = join_tile<L>(chain, back, start, L::WPR - 1 - own, r, given);
     for (int w = 0; w < own; ++w) h = after(waves[wave - own + w], h);
     h = after(before, h);
 #pragma unroll

@@ -85,7 +85,7 @@ __device__ __forceinline__ void load_steps(pack<T, L::VEC> (&to)[L::S], const T*
     }
 #pragma unroll
     for (int k = 0; k < S; ++k) to[k] = pack<T, VEC>{};
-    if (in.rows <= 0 || in.some <= 0) return;
+    if (in.inside <= 0 || in.some <= 0) return;  // nothing that is used
     const int shift = VEC - in.some;
     const T* p = at + lane;
     if (channels < VEC) {
@@ -143,8 +143,6 @@ struct Place {
         len = length_of(lengths, b, s.n);
     }
     __device__ __forceinline__ int t0() const { return tile * L::kSteps; }
-    // A tile that lies past the sequence's end has zeros to write and no part in the chain.
-    __device__ __forceinline__ bool part() const { return t0() < len || tile == 0; }
     // The lane's, whose first step is `sub` from the tile's.
     __device__ __forceinline__ Inside inside(const ScanShape& s, int wave, int sub) const {
         const int t = t0() + sub;
@@ -174,13 +172,15 @@ __device__ __forceinline__ void run_chain(const ScanShape& s, const int* lengths
     constexpr int N = L::kChannels > 64 * L::C ? L::kChannels / (64 * L::C) : 1;
     const int lane = threadIdx.x - 64 * L::W, c = lane * N;
     const Place<L, Backward> p(ticket, s, lengths, chain);
-    const bool part = p.part() && c < L::kChannels;
+    const bool mine = c < L::kChannels;
+    // Every tile has its place in the chain, also past the sequence's end, where its span changes
+    // nothing: that no wait depends on the lengths is worth more than the shorter chain.
     Link<N> link;
     link.words = chain.words + static_cast<long long>(p.column) * L::kChannels + c;
     link.step = static_cast<long long>(chain.columns) * L::kChannels;
-    link.r = Backward ? max(p.len - 1, 0) / L::kSteps - p.tile : p.tile;
+    link.r = Backward ? chain.tiles - 1 - p.tile : p.tile;
     float given[N] = {};
-    if (part) {
+    if (mine) {
         link.ask();
         const float* from = state(p);
 #pragma unroll
@@ -188,9 +188,7 @@ __device__ __forceinline__ void run_chain(const ScanShape& s, const int* lengths
             if (link.r == 0 && from && p.c0 + c + v < s.channels) given[v] = from[c + v];
     }
     __syncthreads();
-    if (part) {
-        // Whether a tile waits for this one.
-        const bool later = Backward ? p.tile > 0 : p.t0() + L::kSteps < p.len;
+    if (mine) {
         Span all[N];
 #pragma unroll
         for (int v = 0; v < N; ++v) {
@@ -212,7 +210,7 @@ __device__ __forceinline__ void run_chain(const ScanShape& s, const int* lengths
             }
         }
         float h[N];
-        link.join(h, all, later, given);
+        link.join(h, all, link.r + 1 < chain.tiles, given);
 #pragma unroll
         for (int v = 0; v < N; ++v) start[c + v] = h[v];
     }
@@ -227,6 +225,7 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(Sc
     __shared__ Span waves[L::W][L::kChannels];
     __shared__ float start[L::kChannels];
     __shared__ int drawn;
+    if (chain.block() >= chain.blocks) return;
     const bool chained = chain.tiles > 1;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int cl = lane % L::CL * VEC, sub = (wave * TL + lane / L::CL) * S;
@@ -329,6 +328,7 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
     __shared__ Span waves[W][L::kChannels], back[W][L::kChannels];
     __shared__ float start[L::kChannels];
     __shared__ int drawn;
+    if (chain.block() >= chain.blocks) return;
     const bool chained = chain.tiles > 1;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int cl = lane % L::CL * VEC, sub = (wave * TL + lane / L::CL) * S;
