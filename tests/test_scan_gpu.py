@@ -272,6 +272,22 @@ def test_non_finite_values_stay_in_their_sequence(layout, bad):
 
 
 @pytest.mark.parametrize("layout", LAYOUTS)
+def test_infinite_values_stay_infinite(layout):
+    """A state that has overflowed keeps its sign to the end, however many gates, all above zero,
+    have been multiplied since; so does a gradient to the first step."""
+    x, gate, dy, state, _ = values(12, "half", layout, 2, 9000, 6)
+    axis = 1 if layout == "channels_last" else 2
+    first, last = x.narrow(axis, 3, 1), dy.narrow(axis, 8990, 1)
+    first.copy_(torch.where(first > 0, float("inf"), -float("inf")))
+    last.copy_(torch.where(last > 0, float("inf"), -float("inf")))
+    got = run("half", layout, x, gate, dy, state, None, with_state=False)
+    assert torch.equal(got["y"].narrow(axis, 3, 8997), first.expand(x.shape).narrow(axis, 3, 8997))
+    assert torch.isfinite(got["y"].narrow(axis, 0, 3)).all()
+    assert torch.equal(got["dx"].narrow(axis, 0, 8991), last.expand(x.shape).narrow(axis, 0, 8991))
+    assert torch.isfinite(got["dx"].narrow(axis, 8991, 9)).all()
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
 def test_same_bits_each_time(layout):
     """Calls repeat to the bit, whatever the workspace held and whatever runs beside them."""
     x, gate, dy, state, dstate = values(8, "bfloat16", layout, 2, 6000, 130)

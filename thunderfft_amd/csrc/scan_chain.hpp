@@ -56,8 +56,17 @@ struct Span {
     float a, b;
 };
 
+// A product of gates stays above zero, as each gate is: an infinite state stays infinite, and a
+// finite one does not see 2^-149 of itself.  (A NaN is lost from A, and is in B.)
+__device__ __forceinline__ float held(float a) { return fmaxf(a, 0x1p-149f); }
+
 __device__ __forceinline__ Span then(Span first, Span second) {
-    return {first.a * second.a, fmaf(second.a, first.b, second.b)};
+    return {held(first.a * second.a), fmaf(second.a, first.b, second.b)};
+}
+
+// One step more.  A is held when all of a lane's steps are in.
+__device__ __forceinline__ Span then_step(Span first, float f, float u) {
+    return {first.a * f, fmaf(f, first.b, u)};
 }
 
 __device__ __forceinline__ float after(Span s, float h) { return fmaf(s.a, h, s.b); }

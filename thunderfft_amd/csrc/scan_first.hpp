@@ -37,6 +37,7 @@ template <int LPR>
 __device__ __forceinline__ Span join_line(Span& mine) {
     constexpr Span kNone = {1.0f, 0.0f};
     const int lane = threadIdx.x % LPR;
+    mine.a = held(mine.a);
     static_assert(LPR >= 4 && LPR <= 64 && (LPR & (LPR - 1)) == 0, "a power of two");
     if constexpr (LPR < 16) {
         // Groups that a row of 16 lanes has several of.
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_forward(ScanShape s, Sca
             if (!p.in(i)) f[i] = 1.0f, u[i] = 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) mine = then(mine, {f[i], u[i]});
+    for (int i = 0; i < V; ++i) mine = then_step(mine, f[i], u[i]);
     const Span before = join_line<L::LPR>(mine);
     if (L::WPR > 1) {
         if (lane == 63) waves[wave] = mine;
@@ -302,9 +303,9 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_backward(ScanShape s, Sc
     }
     Span mine = {1.0f, 0.0f}, behind = {1.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < V; ++i) mine = then(mine, {f[i], enter[i] * q[i]});
+    for (int i = 0; i < V; ++i) mine = then_step(mine, f[i], enter[i] * q[i]);
 #pragma unroll
-    for (int i = V - 1; i >= 0; --i) behind = then(behind, {f[i], f[i] * d[i]});
+    for (int i = V - 1; i >= 0; --i) behind = then_step(behind, f[i], f[i] * d[i]);
     const Span before = join_line<L::LPR>(mine);
     const Span past = join_line_back<L::LPR>(behind);
     const int own = wave % L::WPR;

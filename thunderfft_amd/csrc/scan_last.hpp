@@ -29,6 +29,7 @@ constexpr int kSaved = 56;
 template <int CL, bool Backward>
 __device__ __forceinline__ Span join_lanes(Span& mine) {
     const int lane = threadIdx.x % 64;
+    mine.a = held(mine.a);
 #pragma unroll
     for (int d = CL; d < 64; d *= 2) {
         const int from = Backward ? lane + d : lane - d;
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_forward(Sc
             const Gate q = gate_of(to_float<T>(g[k][v]));
             f[k][v] = q.keep;
             u[k][v] = q.enter * to_float<T>(x[k][v]);
-            before[v] = then(before[v], {f[k][v], u[k][v]});
+            before[v] = then_step(before[v], f[k][v], u[k][v]);
         }
     }
 #pragma unroll
@@ -386,14 +387,14 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
             f[k][v] = r.keep;
             enter[k][v] = r.enter;
             q[k][v] = to_float<T>(x[k][v]);
-            before[v] = then(before[v], {r.keep, r.enter * q[k][v]});
+            before[v] = then_step(before[v], r.keep, r.enter * q[k][v]);
         }
     }
 #pragma unroll
     for (int k = S - 1; k >= 0; --k)
 #pragma unroll
         for (int v = 0; v < VEC; ++v)
-            past[v] = then(past[v], {f[k][v], f[k][v] * to_float<T>(dy[k][v])});
+            past[v] = then_step(past[v], f[k][v], f[k][v] * to_float<T>(dy[k][v]));
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         Span mine = before[v], behind = past[v];
