@@ -302,3 +302,11 @@ def test_drawn(seed):
         cols = max(8, cols // 8 * 8)
     rows = max(1, min(int(2 ** rng.uniform(0, 13)), (1 << 21) // cols))
     compare(T, *values(seed, T, rows, cols), gap=rng.choice([0, 0, 3, 8]), offset=rng.choice([0, 0, 1, 8]))
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("cols", [33, 60, 2500, 2560, 4104, 5120, 5121, 6001, 9000, 10240, 11001, 12288])
+def test_rows_of_any_number_of_waves(T, cols):
+    """Rows on both sides of what 1, 3, 5, 6, 10 and 12 waves hold, more of them than a pass takes."""
+    for rows in (1, 1301):
+        compare(T, *values(cols + rows, T, rows, cols), gap=cols % 3)

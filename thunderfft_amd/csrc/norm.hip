@@ -392,16 +392,26 @@ __global__ __launch_bounds__(1024) void long_weights(NormBackward a) {
     }
 }
 
-// Calls f with the type of row for `cols` values of T, at most Held of them a lane: as few
-// lanes as hold the row in vectors of 16 bytes; one wave where that will do, so that no barrier
-// is needed, and fewer vectors where its lanes have them to spare.  W: waves of a workgroup
-// unless the row takes more.  False if the row is too long for 16 waves.
-template <class T, int Held, int W, class F>
+// Calls f with the type of row for `cols` values of T: as few lanes as hold the row in vectors of
+// 16 bytes; one wave where that will do, so that no barrier is needed, and fewer vectors where its
+// lanes have them to spare.  False if the row is too long for 16 waves.
+//
+// Forward: up to 32 values a lane, which are all that it keeps.  Backward: 16, next to the
+// weights, two sums each, and the next row (2048 columns by 2 waves take 77 us for 32768 rows of
+// bfloat16; by one wave with 32 values each, which spill, 85 us).
+//
+// Waves of a row are of every number that leaves few of them idle, up to 12, and of a workgroup as
+// many as have registers for it backward, 8 to 12 (half 10000 x 4104, which takes 5 of 8 waves: 71
+// against 90 us; 8000 x 5120: 55 against 67; 4000 x 12288, by 12 waves and not 16, which have none
+// for the next row: 79 against 96.  12 where 8 would do: 12 against 10.3 us at half 2048 x 1024,
+// whose rows then lie on fewer compute units, and 55.6 against 53 at 10000 x 4096).
+template <class T, bool Backward, class F>
 bool with_rows(int cols, F f) {
-    constexpr int V = 16 / sizeof(T), M = Held / V;
+    constexpr int V = 16 / sizeof(T), M = (Backward ? 16 : 32) / V, W = Backward ? 8 : 4;
     const int vectors = (cols + V - 1) / V;
     if (cols < V) f(Rows<T, 1, 2, 4, 1, W>{});
     else if (vectors <= 4) f(Rows<T, V, 1, 4, 1, W>{});
+    else if (vectors <= 8) f(Rows<T, V, 1, 8, 1, W>{});
     else if (vectors <= 16) f(Rows<T, V, 1, 16, 1, W>{});
     else if (vectors <= 32) f(Rows<T, V, 2, 16, 1, W>{});
     else if (vectors <= 64) f(Rows<T, V, 1, 64, 1, W>{});
@@ -409,8 +419,13 @@ bool with_rows(int cols, F f) {
     else if (M > 4 && vectors <= 256) f(Rows<T, V, M / 2, 64, 1, W>{});
     else if (vectors <= 64 * M) f(Rows<T, V, M, 64, 1, W>{});
     else if (vectors <= 128 * M) f(Rows<T, V, M, 64, 2, W>{});
+    else if (vectors <= 192 * M) f(Rows<T, V, M, 64, 3, Backward ? 12 : 3>{});
     else if (vectors <= 256 * M) f(Rows<T, V, M, 64, 4, W>{});
+    else if (vectors <= 320 * M) f(Rows<T, V, M, 64, 5, Backward ? 10 : 5>{});
+    else if (vectors <= 384 * M) f(Rows<T, V, M, 64, 6, Backward ? 12 : 6>{});
     else if (vectors <= 512 * M) f(Rows<T, V, M, 64, 8, 8>{});
+    else if (vectors <= 640 * M) f(Rows<T, V, M, 64, 10, 10>{});
+    else if (vectors <= 768 * M) f(Rows<T, V, M, 64, 12, 12>{});
     else if (vectors <= 1024 * M) f(Rows<T, V, M, 64, 16, 16>{});
     else return false;
     return true;
@@ -429,19 +444,6 @@ unsigned long_blocks(long long count) {
     return static_cast<unsigned>(std::min<long long>(count, 1 << 20));
 }
 
-// Forward: 32 values a lane, which are all that it keeps.  Backward: 16, next to the weights,
-// two sums each, and the next row: 2048 columns by 2 waves take 77 us (32768 rows, bfloat16),
-// by one wave with 32 values each, which spill, 85 us.
-template <class T, class F>
-bool with_forward_rows(int cols, F f) {
-    return with_rows<T, 32, 4>(cols, f);
-}
-
-template <class T, class F>
-bool with_backward_rows(int cols, F f) {
-    return with_rows<T, 16, 8>(cols, f);
-}
-
 template <class R>
 int parts_of(long long rows) {
     return static_cast<int>(std::min<long long>(kMostParts, (rows + R::kRows - 1) / R::kRows));
@@ -450,7 +452,7 @@ int parts_of(long long rows) {
 template <class T>
 hipError_t forward_of(const NormForward& a, hipStream_t stream) {
     hipError_t err = hipSuccess;
-    const bool held = with_forward_rows<T>(a.cols, [&](auto type) {
+    const bool held = with_rows<T, false>(a.cols, [&](auto type) {
         using R = decltype(type);
         // A launch has less than 2^32 lanes.
         constexpr long long kMost = (1LL << 31) / R::kLanes * R::kRows;
@@ -474,7 +476,7 @@ hipError_t forward_of(const NormForward& a, hipStream_t stream) {
 template <class T>
 hipError_t backward_of(const NormBackward& a, hipStream_t stream) {
     const bool weights = a.dweight || a.dbias;
-    const bool held = with_backward_rows<T>(a.cols, [&](auto type) {
+    const bool held = with_rows<T, true>(a.cols, [&](auto type) {
         using R = decltype(type);
         const int parts = parts_of<R>(a.rows);
         if (parts > 0) norm_backward<R><<<parts, R::kLanes, 0, stream>>>(a, parts);
