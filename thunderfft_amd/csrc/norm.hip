@@ -12,6 +12,11 @@
 // The backward pass goes over the rows once as well: a workgroup takes rows in turn, keeps
 // their share of dweight and dbias in registers, and leaves one partial sum a column, which
 // a second kernel adds up.  Every order of summation is fixed.
+//
+// Memory bounds both: bfloat16 32768 x 2048 takes 51 us forward (268 MB, 5.2 TB/s) and 63 us
+// backward (407 MB, 6.5 TB/s, some of it still cached), 5 more for adding the parts up; half
+// 2048 x 8192 15 us, 28 us and 4 us.  Few rows are bound by latency: bfloat16 8 x 1024 2.6 us,
+// float 1001 x 777 4.3 us, 6.8 us and 3.1 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -146,7 +151,9 @@ __global__ __launch_bounds__(R::kLanes) void norm_forward(NormForward a) {
     }
 }
 
-// Workgroups of the backward pass at most, each with a partial sum: one a compute unit.
+// Workgroups of the backward pass at most, each with a partial sum: one a compute unit.  (Twice as
+// many: 81 against 77 us at 32768 x 2048, 49 against 33 at 2048 x 8192, whose sums are then as large
+// as a third of its rows.)
 constexpr int kMostParts = 256;
 
 template <class R>

@@ -15,7 +15,8 @@ namespace {
 constexpr int kLanes = 256;
 
 // Sets the counters of a chain to zero and empties its words.  (A kernel: a captured memset
-// is not replayed reliably.)
+// is not replayed reliably.)  Two to five microseconds of a call, its launch most of them: 1 MB
+// of words takes 2.0 us, 4.9 MB 4 to 5 (as many with 256 or 1024 workgroups that loop).
 __global__ __launch_bounds__(kLanes) void clear_chain(uint4* to, long long counters,
                                                       long long count) {
     for (long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x; i < count;

@@ -2,6 +2,10 @@
 // layout): one pass over the data.  A lane takes 8 or 16 neighbouring steps and composes them; the
 // lanes of a row join theirs in registers, its waves through LDS, and where a row takes several
 // workgroups, they join through the chain.  Short rows lie side by side in a wave.
+//
+// Memory bounds it: half 256 x 64 x 4096 takes 70 us (403 MB, 5.7 TB/s; a row is a workgroup's, so
+// that nothing waits for another).  float 33 x 96 x 512, a wave a row and all of it in the
+// caches: 5.2 us forward and 6.8 backward, the latency of one round of loads, sums and stores.
 #pragma once
 
 #include "scan_chain.hpp"
@@ -73,8 +77,7 @@ __device__ __forceinline__ Span join_line_back(Span& mine) {
 }
 
 // A lane's V steps: those of its own that are `in` the sequence; the first `skip` of the vector
-// it reads are another lane's (the row ends inside its own), the others up to `own` are in the
-// tensor.
+// it reads are another lane's (the row ends inside its own).
 template <class L>
 struct Stretch {
     int row, b, c, tile, len, first, at, skip;
