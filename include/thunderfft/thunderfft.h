@@ -261,7 +261,7 @@ int thff_copy_nt(void* d_dst, const void* d_src, long long bytes, void* stream);
  * halves of one projection's rows.  x_stride and gate_stride hold for the
  * gradients of x and the gate too, y_stride for y and its gradient.  batch, n
  * and channels may be 0, and are at most 2^30, batch * channels at most
- * 2^31 - 256 (THFF_EINVAL too where one launch does not take the shape).
+ * 2^31 - 256 (THFF_EINVAL too where a call has too many steps for its grid).
  * states: rows of the state pool that slots index (unused without slots). */
 typedef struct thff_scan_shape {
     int precision, layout;
@@ -282,8 +282,8 @@ long long thff_gated_scan_workspace_bytes(const thff_scan_shape* shape);
  * one goes to d_state_out; both are fp32 rows of `channels` values, row b for
  * sequence b, or row slots[b] of a pool of shape->states rows.  A slot outside
  * the pool (-1, say) is an empty place: it starts from zero and stores no state.
- * Two places with the same slot race.  d_state_out may be d_state_in (one
- * token after another in place: n = 1); the two must not overlap otherwise.
+ * Two places with the same slot race.  d_state_out may be d_state_in
+ * (states kept in place); the two must not overlap otherwise.
  * lengths[b] is taken into [0, n]; y is 0 from there on, and x and the gate are
  * not used there, whatever they hold.  Null d_state_in: zeros; null
  * d_state_out, d_saved: not stored; null d_slots: row b; null d_lengths: n each.

@@ -499,3 +499,19 @@ def test_long_sequences():
         x, gate, dy, state, dstate = values(14, T, layout, 1, 30011, 6)
         gate += 6
         compare(T, layout, x, gate, dy, state, dstate)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("n", [1, 700, 9000])
+def test_states_in_place(layout, n):
+    """The last state may go where the first one was, also where many workgroups share a row and a
+    sequence ends in the first of them."""
+    x, gate, _, state, _ = values(14, "bfloat16", layout, 4, n, 70)
+    s = shape_of("bfloat16", layout, x, gate)
+    lengths = torch.tensor([n, n // 2, 3, 0], dtype=torch.int32).clamp(max=n).cuda()
+    out, apart, inplace, y = torch.empty_like(state), torch.empty_like(x), state.clone(), torch.empty_like(x)
+    thff.ThunderFFT_gated_scan(s, x, gate, apart, d_state_in=state, d_state_out=out, d_lengths=lengths,
+                               d_workspace=buffers(s)[1])
+    thff.ThunderFFT_gated_scan(s, x, gate, y, d_state_in=inplace, d_state_out=inplace, d_lengths=lengths,
+                               d_workspace=buffers(s)[1])
+    assert torch.equal(inplace, out) and torch.equal(y, apart)
