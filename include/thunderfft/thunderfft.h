@@ -287,8 +287,10 @@ long long thff_gated_scan_workspace_bytes(const thff_scan_shape* shape);
  * lengths[b] is taken into [0, n]; y is 0 from there on, and x and the gate are
  * not used there, whatever they hold.  Null d_state_in: zeros; null
  * d_state_out, d_saved: not stored; null d_slots: row b; null d_lengths: n each.
- * An infinity or NaN in x or the gate makes later outputs of its sequence and
- * channel infinite or NaN, and no others.
+ * An infinity in x, or a NaN in x or the gate, makes later outputs of its
+ * sequence and channel infinite or NaN, and no others.  A gate of infinity keeps
+ * the state, one of minus infinity puts x in its place (a gate below -87.3
+ * keeps 2^-126 of the state).
  * x, gate and y start on a boundary of their element, states, slots and lengths
  * on 4 bytes, d_saved and d_workspace on 16.  y may alias neither x nor gate
  * (disjoint rows interleaved in one buffer are fine).  Empty batches and

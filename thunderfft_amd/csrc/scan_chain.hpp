@@ -216,7 +216,7 @@ __device__ __forceinline__ T open_gate() {
 // Draws the workgroup's tile of its column, by the first lane of wave `drawer`.
 __device__ __forceinline__ int draw_tile(const Chain& chain, int* drawn, int drawer) {
     if (static_cast<int>(threadIdx.x) == 64 * drawer) {
-        unsigned* counter = chain.drawn + chain.column() * (kCounterBytes / 4);
+        unsigned* counter = chain.drawn + chain.column() * (kCounterBytes / 4LL);
         *drawn = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
