@@ -310,3 +310,21 @@ def test_rows_of_any_number_of_waves(T, cols):
     """Rows on both sides of what 1, 3, 5, 6, 10 and 12 waves hold, more of them than a pass takes."""
     for rows in (1, 1301):
         compare(T, *values(cols + rows, T, rows, cols), gap=cols % 3)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64], ids=str)
+def test_tensor_function_whatever_the_default_type(default):
+    """Statistics and weights' gradients are float32 where torch makes other tensors by default."""
+    x, weight, bias, dy = values(15, "bfloat16", 60, 200)
+    leaves = [v.detach().clone().requires_grad_() for v in (x, weight, bias)]
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        y = thff.layer_norm(*leaves)
+        y.backward(dy)
+    finally:
+        torch.set_default_dtype(before)
+    want = oracle.norm("bfloat16", x, weight, bias, EPS, dy)
+    for name, v in (("y", y), ("dx", leaves[0].grad), ("dweight", leaves[1].grad), ("dbias", leaves[2].grad)):
+        assert v.dtype == (torch.float32 if name in ("dweight", "dbias") else torch.bfloat16)
+        oracle.check(name, v, want[name])

@@ -515,3 +515,23 @@ def test_states_in_place(layout, n):
     thff.ThunderFFT_gated_scan(s, x, gate, y, d_state_in=inplace, d_state_out=inplace, d_lengths=lengths,
                                d_workspace=buffers(s)[1])
     assert torch.equal(inplace, out) and torch.equal(y, apart)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64], ids=str)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_tensor_function_whatever_the_default_type(layout, default):
+    """States and their gradients are float32 where torch makes other tensors by default."""
+    x, gate, dy, state, dstate = values(16, "bfloat16", layout, 3, 150, 40)
+    leaves = [v.detach().clone().requires_grad_() for v in (x, gate, state)]
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        y, last = thff.gated_scan(*leaves, layout=layout)
+        torch.autograd.backward([y, last], [dy, dstate])
+    finally:
+        torch.set_default_dtype(before)
+    assert last.dtype == torch.float32 and leaves[2].grad.dtype == torch.float32
+    want = oracle.scan("bfloat16", layout, x, gate, state, None, dy, dstate)
+    for name, v in (("y", y), ("state", last), ("dx", leaves[0].grad), ("dgate", leaves[1].grad),
+                    ("dstate", leaves[2].grad)):
+        oracle.check(name, v, want[name])

@@ -54,13 +54,19 @@ def _bytes(count, device):
     return torch.empty(count, dtype=torch.uint8, device=device)
 
 
+def _floats(*shape, device):
+    """A buffer of states, statistics or weights' gradients: the kernels have them in float32,
+    whatever torch's default type is."""
+    return torch.empty(shape, dtype=torch.float32, device=device)
+
+
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, state, lengths, layout):
         (x, x_stride), (gate, gate_stride) = _rows(x), _rows(gate)
         shape = _shape_of(x, x_stride, gate_stride, layout)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        last = torch.empty(shape.batch, shape.channels, device=x.device)
+        last = _floats(shape.batch, shape.channels, device=x.device)
         train = any(ctx.needs_input_grad[:3])
         with torch.cuda.device(x.device):
             saved = _bytes(shape.saved_bytes(), x.device) if train else None
@@ -83,7 +89,7 @@ class _GatedScan(torch.autograd.Function):
         x, gate = x.contiguous(), gate.contiguous()
         shape = _shape_of(x, None, None, ctx.layout, dy_stride)
         dx, dgate = torch.empty_like(x), torch.empty_like(gate)
-        dstate = torch.empty(shape.batch, shape.channels, device=x.device)
+        dstate = _floats(shape.batch, shape.channels, device=x.device)
         dlast = dlast.contiguous()
         with torch.cuda.device(x.device):
             thff.ThunderFFT_gated_scan_backward_async(
@@ -128,8 +134,8 @@ class _LayerNorm(torch.autograd.Function):
         rows = x.numel() // cols
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         train = any(ctx.needs_input_grad[:3])
-        mean = torch.empty(rows, device=x.device) if train else None
-        rstd = torch.empty(rows, device=x.device) if train else None
+        mean = _floats(rows, device=x.device) if train else None
+        rstd = _floats(rows, device=x.device) if train else None
         with torch.cuda.device(x.device):
             thff.ThunderFFT_layer_norm_async(x.dtype, x, weight, bias, eps, y, rows, cols,
                                              d_mean=mean, d_rstd=rstd, x_stride=x_stride,
@@ -147,8 +153,8 @@ class _LayerNorm(torch.autograd.Function):
         cols = x.shape[-1]
         rows = x.numel() // cols
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dweight = torch.empty(cols, device=x.device) if needs[1] else None
-        dbias = torch.empty(cols, device=x.device) if needs[2] else None
+        dweight = _floats(cols, device=x.device) if needs[1] else None
+        dbias = _floats(cols, device=x.device) if needs[2] else None
         with torch.cuda.device(x.device):
             workspace = (_bytes(thff.layer_norm_workspace_bytes(rows, cols), x.device)
                          if needs[1] or needs[2] else None)
