@@ -535,3 +535,20 @@ def test_tensor_function_whatever_the_default_type(layout, default):
     for name, v in (("y", y), ("state", last), ("dx", leaves[0].grad), ("dgate", leaves[1].grad),
                     ("dstate", leaves[2].grad)):
         oracle.check(name, v, want[name])
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("n", [0, 1, 40, 9000])
+def test_saved_states_stay_in_their_bytes(layout, n):
+    """Buffers cut from one block: nothing is written past saved_bytes(), which are none for n = 0."""
+    batch, channels = 3, 37
+    dims = (batch, n, channels) if layout == "channels_last" else (batch, channels, n)
+    x, gate = torch.randn(dims).half().cuda(), torch.randn(dims).half().cuda()
+    s = thff.ScanShape("half", batch, n, channels, layout=layout)
+    size = s.saved_bytes()
+    assert n > 0 or size == 0
+    block = torch.full((64 + size + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+    workspace, last = buffers(s)[1], torch.empty(batch, channels, device="cuda")
+    thff.ThunderFFT_gated_scan(s, x, gate, torch.empty_like(x), d_state_out=last, d_saved=block[64:],
+                               d_workspace=workspace)
+    assert (block[:64] == 0x5A).all() and (block[64 + size:] == 0x5A).all()

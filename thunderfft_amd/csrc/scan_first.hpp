@@ -254,7 +254,8 @@ __global__ __launch_bounds__(L::kLanes) void scan_first_forward(ScanShape s, Sca
         if (lane == 0 && wave % L::WPR == 0) start[wave / L::WPR] = given;
     }
     float h = join_tile<L>(chain, waves, start, wave % L::WPR, p.tile, given);
-    if (a.saved && p.active && p.first == p.tile * L::kSteps)
+    // (No steps save nothing: d_saved has no bytes then, wherever it points.)
+    if (a.saved && s.n > 0 && p.active && p.first == p.tile * L::kSteps)
         a.saved[static_cast<long long>(p.row) * chain.tiles + p.tile] = h;
     h = after(before, h);
     pack<T, V> out;
