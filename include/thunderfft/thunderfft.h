@@ -338,7 +338,8 @@ int thff_layer_norm_async(int precision, const void* d_x, long long x_stride,
                           long long y_stride, void* d_mean, void* d_rstd, long long rows, int cols,
                           void* stream);
 
-/* Bytes of thff_layer_norm_backward's d_workspace (0: may be null). */
+/* Bytes of thff_layer_norm_backward's d_workspace (0, as for all rows of more than
+ * 16384 columns: may be null). */
 long long thff_layer_norm_workspace_bytes(long long rows, int cols);
 
 /* Gradients of thff_layer_norm from dy, x and the statistics: with

@@ -328,3 +328,26 @@ def test_tensor_function_whatever_the_default_type(default):
     for name, v in (("y", y), ("dx", leaves[0].grad), ("dweight", leaves[1].grad), ("dbias", leaves[2].grad)):
         assert v.dtype == (torch.float32 if name in ("dweight", "dbias") else torch.bfloat16)
         oracle.check(name, v, want[name])
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("cols", [16385, 40000])
+def test_wide_rows_need_no_workspace(T, cols):
+    """All gradients of rows past the widest that registers hold, without scratch memory."""
+    rows = 270
+    x, weight, bias, dy = values(17, T, rows, cols)
+    mean, rstd = (torch.empty(rows, dtype=torch.float32, device="cuda") for _ in range(2))
+    dw, db = (torch.empty(cols, dtype=torch.float32, device="cuda") for _ in range(2))
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    thff.ThunderFFT_layer_norm(T, x, weight, bias, EPS, y, rows, cols, d_mean=mean, d_rstd=rstd)
+    thff.ThunderFFT_layer_norm_backward(T, dy, x, mean, rstd, weight, dx, dw, db, None, rows, cols)
+    want = oracle.norm(T, x, weight, bias, EPS, dy)
+    for name, v in (("y", y), ("dx", dx), ("dweight", dw), ("dbias", db)):
+        oracle.check(name, v, want[name])
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+def test_widest_held_rows(T):
+    """On both sides of the widest row that registers hold, backward (16384) and forward (32768)."""
+    for cols in (16383, 16384, 16385, 32767, 32768, 32769):
+        compare(T, *values(cols, T, 2, cols))

@@ -262,3 +262,11 @@ def test_norm_oracle_gradients():
         up[at], down[at] = ins[at] + eps * v, ins[at] - eps * v
         along = float((got[name][0] * v).sum())
         assert abs((loss(*up) - loss(*down)) / (2 * eps) - along) < 1e-7, name
+
+
+def test_norm_workspace_is_what_a_call_uses():
+    """Partial sums of at most 256 workgroups, and none for rows that are not held in registers."""
+    assert thff.layer_norm_workspace_bytes(300, 16384) == 8 * 256 * 16384
+    assert thff.layer_norm_workspace_bytes(3, 16384) == 8 * 3 * 16384
+    for rows, cols in ((3, 16385), (256, 65536), (256, 1 << 20), (1 << 40, 1 << 30)):
+        assert thff.layer_norm_workspace_bytes(rows, cols) == 0

@@ -399,6 +399,13 @@ __global__ __launch_bounds__(1024) void long_weights(NormBackward a) {
     }
 }
 
+// Values a lane holds at most, and columns of the longest row that 16 waves hold: the same for all
+// types.
+template <bool Backward>
+constexpr int kLaneValues = Backward ? 16 : 32;
+template <bool Backward>
+constexpr int kMostHeld = 1024 * kLaneValues<Backward>;
+
 // Calls f with the type of row for `cols` values of T: as few lanes as hold the row in vectors of
 // 16 bytes; one wave where that will do, so that no barrier is needed, and fewer vectors where its
 // lanes have them to spare.  False if the row is too long for 16 waves.
@@ -414,7 +421,7 @@ __global__ __launch_bounds__(1024) void long_weights(NormBackward a) {
 // whose rows then lie on fewer compute units, and 55.6 against 53 at 10000 x 4096).
 template <class T, bool Backward, class F>
 bool with_rows(int cols, F f) {
-    constexpr int V = 16 / sizeof(T), M = (Backward ? 16 : 32) / V, W = Backward ? 8 : 4;
+    constexpr int V = 16 / sizeof(T), M = kLaneValues<Backward> / V, W = Backward ? 8 : 4;
     const int vectors = (cols + V - 1) / V;
     if (cols < V) f(Rows<T, 1, 2, 4, 1, W>{});
     else if (vectors <= 4) f(Rows<T, V, 1, 4, 1, W>{});
@@ -433,7 +440,7 @@ bool with_rows(int cols, F f) {
     else if (vectors <= 512 * M) f(Rows<T, V, M, 64, 8, 8>{});
     else if (vectors <= 640 * M) f(Rows<T, V, M, 64, 10, 10>{});
     else if (vectors <= 768 * M) f(Rows<T, V, M, 64, 12, 12>{});
-    else if (vectors <= 1024 * M) f(Rows<T, V, M, 64, 16, 16>{});
+    else if (cols <= kMostHeld<Backward>) f(Rows<T, V, M, 64, 16, 16>{});
     else return false;
     return true;
 }
@@ -503,6 +510,8 @@ hipError_t backward_of(const NormBackward& a, hipStream_t stream) {
 long long norm_workspace_bytes(long long rows, int cols) {
     // One size for all types: a type's parts are at most kMostParts, and none takes a workgroup
     // for less than one row.
+    // Rows too long for registers leave no parts.
+    if (cols > kMostHeld<true>) return 0;
     return 8 * std::min<long long>(kMostParts, rows) * cols;
 }
 
