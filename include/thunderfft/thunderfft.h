@@ -290,7 +290,9 @@ long long thff_gated_scan_workspace_bytes(const thff_scan_shape* shape);
  * An infinity in x, or a NaN in x or the gate, makes later outputs of its
  * sequence and channel infinite or NaN, and no others.  A gate of infinity keeps
  * the state, one of minus infinity puts x in its place (a gate below -87.3
- * keeps 2^-126 of the state).
+ * keeps 2^-126 of the state).  Steps are joined by products of their gates,
+ * which are rounded to multiples of 2^-149: what closed gates leave of a state
+ * is off by less than 2^-144 of that state (1.6e-5 for the largest float).
  * x, gate and y start on a boundary of their element, states, slots and lengths
  * on 4 bytes, d_saved and d_workspace on 16.  y may alias neither x nor gate
  * (disjoint rows interleaved in one buffer are fine).  Empty batches and

@@ -552,3 +552,19 @@ def test_saved_states_stay_in_their_bytes(layout, n):
     thff.ThunderFFT_gated_scan(s, x, gate, torch.empty_like(x), d_state_out=last, d_saved=block[64:],
                                d_workspace=workspace)
     assert (block[:64] == 0x5A).all() and (block[64 + size:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("T", ["float", "bfloat16"])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("n", [40, 700, 9000])
+def test_huge_states_are_forgotten(T, layout, n):
+    """States and gradients near the type's ends leave nothing behind closing gates, whose products
+    are below any number: what follows has the size of small inputs.  (Each gate is 2e-9, so that
+    the product of up to 4 is a normal number and that of more than 5 rounds to zero.)"""
+    batch, channels = 2, 37
+    x, gate, dy, state, dstate = values(17, T, layout, batch, n, channels)
+    x, gate, dy = x.mul_(2.0 ** -30), gate.fill_(-20.0), dy.mul_(2.0 ** -30)
+    state, dstate = state.sign() * 1e38, dstate.sign() * 1e38
+    axis = 1 if layout == "channels_last" else 2
+    x.narrow(axis, n // 2, 1).fill_(1e38)
+    compare(T, layout, x, gate, dy, state, dstate)

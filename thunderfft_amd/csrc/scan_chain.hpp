@@ -56,20 +56,23 @@ struct Span {
     float a, b;
 };
 
-// A product of gates stays above zero, as each gate is: an infinite state stays infinite, and a
-// finite one does not see 2^-149 of itself.  (A NaN is lost from A, and is in B.)
-__device__ __forceinline__ float held(float a) { return fmaxf(a, 0x1p-149f); }
-
-__device__ __forceinline__ Span then(Span first, Span second) {
-    return {held(first.a * second.a), fmaf(second.a, first.b, second.b)};
+// An infinite state stays infinite: each gate is above zero, also where their product has been
+// rounded to zero.  A finite state takes the product as it is: below 2^-126 it has fewer bits, and
+// what is left of the state is off by 2^-150 of it for each joining.  (A product held at 2^-149 for
+// all states leaves 1.4e-7 of 1e38 for good.  The choice costs 0.5% of bfloat16 8 x 4096 x 2048
+// forward, 89.9 us with the chain's clearing, and 1.5% of 16 x 64 x 65536, channels first, 87.0 us.)
+__device__ __forceinline__ float after(Span s, float h) {
+    return fmaf(__builtin_isinf(h) ? 1.0f : s.a, h, s.b);
 }
 
-// One step more.  A is held when all of a lane's steps are in.
+__device__ __forceinline__ Span then(Span first, Span second) {
+    return {first.a * second.a, after(second, first.b)};
+}
+
+// One step more.
 __device__ __forceinline__ Span then_step(Span first, float f, float u) {
     return {first.a * f, fmaf(f, first.b, u)};
 }
-
-__device__ __forceinline__ float after(Span s, float h) { return fmaf(s.a, h, s.b); }
 
 using Word = unsigned long long;
 

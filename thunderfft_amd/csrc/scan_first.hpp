@@ -41,7 +41,6 @@ template <int LPR>
 __device__ __forceinline__ Span join_line(Span& mine) {
     constexpr Span kNone = {1.0f, 0.0f};
     const int lane = threadIdx.x % LPR;
-    mine.a = held(mine.a);
     static_assert(LPR >= 4 && LPR <= 64 && (LPR & (LPR - 1)) == 0, "a power of two");
     if constexpr (LPR < 16) {
         // Groups that a row of 16 lanes has several of.

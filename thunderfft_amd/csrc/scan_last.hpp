@@ -44,7 +44,6 @@ constexpr int kSaved = 56;
 template <int CL, bool Backward>
 __device__ __forceinline__ Span join_lanes(Span& mine) {
     const int lane = threadIdx.x % 64;
-    mine.a = held(mine.a);
 #pragma unroll
     for (int d = CL; d < 64; d *= 2) {
         const int from = Backward ? lane + d : lane - d;
@@ -421,9 +420,8 @@ __global__ __launch_bounds__(L::kLanes, L::kOccupancy) void scan_last_backward(S
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        Span ahead = {1.0f, 0.0f};
-        for (int w = 0; w < wave; ++w) ahead = then(ahead, waves[w][cl + v]);
-        h[v] = after(before[v], after(ahead, h[v]));
+        for (int w = 0; w < wave; ++w) h[v] = after(waves[w][cl + v], h[v]);
+        h[v] = after(before[v], h[v]);
     }
     // q becomes what lam is multiplied with for the gate's gradient.
 #pragma unroll
