@@ -83,12 +83,18 @@ class _GatedScan(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
         x, gate, lengths, saved = ctx.saved_tensors
-        dy, dy_stride = _rows(dy)
-        # The gradients are dense; the kernels take one stride for x and its gradient, so x
-        # and the gate are read from dense copies where theirs is another.
-        x, gate = x.contiguous(), gate.contiguous()
-        shape = _shape_of(x, None, None, ctx.layout, dy_stride)
-        dx, dgate = torch.empty_like(x), torch.empty_like(gate)
+        (dy, dy_stride), (x, x_stride), (gate, gate_stride) = _rows(dy), _rows(x), _rows(gate)
+        # The kernels take one stride for x and its gradient, and one for the gate and its own.
+        # Halves of a projection have theirs as halves of one buffer; rows that are further apart
+        # otherwise are read from dense copies, so that the gradients need no such gaps.
+        last = x.shape[-1]
+        if x_stride == gate_stride == 2 * last:
+            both = torch.empty(*x.shape[:-1], 2 * last, dtype=x.dtype, device=x.device)
+            dx, dgate = both[..., :last], both[..., last:]
+        else:
+            x, gate, x_stride, gate_stride = x.contiguous(), gate.contiguous(), None, None
+            dx, dgate = torch.empty_like(x), torch.empty_like(gate)
+        shape = _shape_of(x, x_stride, gate_stride, ctx.layout, dy_stride)
         dstate = _floats(shape.batch, shape.channels, device=x.device)
         dlast = dlast.contiguous()
         with torch.cuda.device(x.device):
@@ -106,7 +112,7 @@ def gated_scan(x, gate, state=None, lengths=None, layout="channels_last"):
 
     x and gate: float32, float16 or bfloat16 of one shape, (batch, n, channels) or, with
     layout "channels_first", (batch, channels, n); halves of one projection are read in
-    place.  state: float32 (batch, channels) before the first step, None for zeros.
+    place, backward too, and have the halves of one buffer as gradients.  state: float32 (batch, channels) before the first step, None for zeros.
     lengths: int32 (batch,), steps from there on are left out and give y = 0.  The last
     states are float32 (batch, channels).  Differentiable (once) by x, gate and state.
     """
