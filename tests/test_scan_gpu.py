@@ -568,3 +568,91 @@ def test_huge_states_are_forgotten(T, layout, n):
     axis = 1 if layout == "channels_last" else 2
     x.narrow(axis, n // 2, 1).fill_(1e38)
     compare(T, layout, x, gate, dy, state, dstate)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_same_bits_whatever_the_workspace_held(layout):
+    """Zeros, the chain's empty words, random words, plausible spans and what another call has left
+    in the workspace change no bit, also while another stream keeps the card busy."""
+    x, gate, dy, state, dstate = values(18, "half", layout, 2, 9000, 70)
+    s = shape_of("half", layout, x, gate)
+    saved, workspace = buffers(s)
+    other = torch.empty_like(workspace)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    words = workspace.numel() // 8
+    spans = torch.stack([torch.rand(words, device="cuda", generator=gen), torch.randn(words, device="cuda", generator=gen)], 1)
+    contents = [torch.zeros_like(workspace), torch.full_like(workspace, 0xFF),
+                torch.randint(0, 256, workspace.shape, dtype=torch.uint8, device="cuda", generator=gen),
+                torch.cat([spans.flatten().view(torch.uint8), workspace.new_zeros(workspace.numel() - 8 * words)])]
+
+    def calls(space, v):
+        x, gate, dy, state, dstate = v
+        y, dx, dg = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+        last, first = torch.empty_like(state), torch.empty_like(state)
+        stream = torch.cuda.current_stream()
+        thff.ThunderFFT_gated_scan_async(s, x, gate, y, d_state_in=state, d_state_out=last, d_saved=saved,
+                                         d_workspace=space, stream=stream)
+        kept = space.clone()
+        thff.ThunderFFT_gated_scan_backward_async(s, dy, x, gate, saved, dx, dg, d_dstate_out=dstate, d_dstate_in=first,
+                                                  d_workspace=space, stream=stream)
+        return (y, last, dx, dg, first), kept
+
+    ours = (x, gate, dy, state, dstate)
+    want, _ = calls(workspace, ours)
+    _, left = calls(other, values(19, "half", layout, 2, 9000, 70))  # another call's chains, complete
+    a = torch.randn(2048, 2048, device="cuda", generator=gen)
+    side = torch.cuda.Stream()
+    for content in (*contents, left, other):
+        for busy in (False, True):
+            workspace.copy_(content)
+            torch.cuda.synchronize()
+            if busy:
+                with torch.cuda.stream(side):
+                    for _ in range(8):
+                        a @ a
+            got, _ = calls(workspace, ours)
+            torch.cuda.synchronize()
+            for v, w in zip(got, want):
+                assert torch.equal(v, w)
+
+
+# Shapes of more workgroups than one row of the grid has (2^21), with and without a chain:
+# layout, batch, n, channels.
+WIDE_GRIDS = [("channels_last", (1 << 21) + 5, 2, 1), ("channels_last", (1 << 20) + 3, 449, 1),
+              ("channels_first", (1 << 20) + 7, 2, 128), ("channels_first", (1 << 13) + 1, 4097, 128)]
+
+
+@pytest.mark.parametrize("shape", WIDE_GRIDS, ids=str)
+def test_more_workgroups_than_a_row_of_the_grid(shape):
+    """Gates of 0 (f = 1/2) and inputs of one value c a sequence: y[t] = c (1 - 2^-(t+1)), and with
+    gradients of one value d, dx[t] = d (1 - 2^-(n-t)).  Sums of halves are exact in float as long as
+    they differ from their limit, so each output is off by its rounding to half at most: 2^-11."""
+    layout, batch, n, channels = shape
+    first = layout == "channels_first"
+    dims = (batch, channels, n) if first else (batch, n, channels)
+    c = (torch.arange(batch, device="cuda") % 7 + 1).half().view(-1, 1, 1)
+    d = (torch.arange(batch, device="cuda") % 5 + 1).half().view(-1, 1, 1)
+    x, dy = c.expand(dims).contiguous(), d.expand(dims).contiguous()
+    gate = torch.zeros_like(x)
+    y, dx, dg = (torch.full_like(x, GUARD) for _ in range(3))
+    last, dfirst = (torch.full((batch, channels), GUARD, device="cuda") for _ in range(2))
+    s = thff.ScanShape("half", batch, n, channels, layout=layout)
+    saved, workspace = buffers(s)
+    print(layout, dims, flush=True)
+    thff.ThunderFFT_gated_scan(s, x, gate, y, d_state_out=last, d_saved=saved, d_workspace=workspace)
+    thff.ThunderFFT_gated_scan_backward(s, dy, x, gate, saved, dx, dg, d_dstate_in=dfirst, d_workspace=workspace)
+    t = torch.arange(n, device="cuda", dtype=torch.float64).view((1, 1, n) if first else (1, n, 1))
+    rising, falling = 1 - 0.5 ** (t + 1), 1 - 0.5 ** (n - t)
+    step = max(1, (1 << 27) // (n * channels))
+    for lo in range(0, batch, step):
+        part = slice(lo, min(lo + step, batch))
+        cs, ds = c[part].double(), d[part].double()
+        for got, want in ((y, cs * rising), (dx, ds * falling)):
+            assert bool(((got[part].double() - want).abs() <= want * 2.0 ** -11).all())
+        # lam = 2 dx, h[t-1] - x = -c 2^-t: its own roundings are those of sums near c, 2^-24 of it.
+        want = -0.5 * ds * falling * cs * 0.5 ** t
+        bound = want.abs() * 2.0 ** -10 + ds * cs * 2.0 ** -23 + 2.0 ** -25
+        assert bool(((dg[part].double() - want).abs() <= bound).all())
+    cs, ds = c.double().view(-1, 1), d.double().view(-1, 1)
+    assert bool(((last.double() - cs * (1 - 0.5 ** n)).abs() <= cs * 2.0 ** -23).all())
+    assert bool(((dfirst.double() - ds * (1 - 0.5 ** n)).abs() <= ds * 2.0 ** -23).all())
