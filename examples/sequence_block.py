@@ -24,6 +24,8 @@ sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."
 import thunderfft_amd as thff  # noqa: E402
 
 FEATURES = 4
+# The operators hold states and weights in float32, whatever torch's default type is; so do the values here.
+FLOAT = dict(device="cuda", dtype=torch.float32)
 
 
 class Model:
@@ -31,12 +33,12 @@ class Model:
         gen = torch.Generator(device="cuda").manual_seed(seed)
 
         def matrix(rows, cols):
-            return (torch.randn(rows, cols, device="cuda", generator=gen) / rows ** 0.5).requires_grad_()
+            return (torch.randn(rows, cols, generator=gen, **FLOAT) / rows ** 0.5).requires_grad_()
 
         self.channels = channels
         self.embed = matrix(FEATURES, channels)
-        self.blocks = [dict(weight=torch.ones(channels, device="cuda", requires_grad=True),
-                            bias=torch.zeros(channels, device="cuda", requires_grad=True),
+        self.blocks = [dict(weight=torch.ones(channels, requires_grad=True, **FLOAT),
+                            bias=torch.zeros(channels, requires_grad=True, **FLOAT),
                             w_in=matrix(channels, 2 * channels), w_out=matrix(channels, channels))
                        for _ in range(layers)]
         self.head = matrix(channels, 1)
@@ -60,10 +62,10 @@ class Server:
 
     def __init__(self, model: Model, slots: int, batch: int):
         self.model, self.batch, c = model, batch, model.channels
-        self.pools = [torch.zeros(slots, c, device="cuda") for _ in model.blocks]
+        self.pools = [torch.zeros(slots, c, **FLOAT) for _ in model.blocks]
         self.shape = thff.ScanShape("float", batch, 1, c, x_stride=2 * c, gate_stride=2 * c, states=slots)
-        self.normed, self.mixed = torch.empty(batch, c, device="cuda"), torch.empty(batch, c, device="cuda")
-        self.inner = torch.empty(batch, 2 * c, device="cuda")
+        self.normed, self.mixed = torch.empty(batch, c, **FLOAT), torch.empty(batch, c, **FLOAT)
+        self.inner = torch.empty(batch, 2 * c, **FLOAT)
 
     def fill(self, slots, states):
         """Puts a prompt's last states into the slots."""
@@ -86,9 +88,9 @@ class Server:
 
 def sample(batch: int, n: int, gen):
     """Features and the memory to learn: it takes up feature 0 where feature 1 is on, and decays."""
-    features = torch.randn(batch, n, FEATURES, device="cuda", generator=gen)
+    features = torch.randn(batch, n, FEATURES, generator=gen, **FLOAT)
     on = (features[..., 1] > 1.0).float()
-    target, memory = torch.empty(batch, n, device="cuda"), torch.zeros(batch, device="cuda")
+    target, memory = torch.empty(batch, n, **FLOAT), torch.zeros(batch, **FLOAT)
     for t in range(n):
         memory = torch.where(on[:, t] > 0, features[:, t, 0], 0.97 * memory)
         target[:, t] = memory
@@ -119,7 +121,7 @@ def serve(model: Model, lengths=(40, 1, 77, 13), tokens: int = 24, seed: int = 2
     """The largest difference between tokens served one by one and whole sequences."""
     gen = torch.Generator(device="cuda").manual_seed(seed)
     batch, most = len(lengths), max(lengths)
-    features = torch.randn(batch, most + tokens, FEATURES, device="cuda", generator=gen)
+    features = torch.randn(batch, most + tokens, FEATURES, generator=gen, **FLOAT)
     ends = torch.tensor(lengths, dtype=torch.int32, device="cuda")
     # Prompts of unlike lengths in one pass; what lies past an end reaches no state.
     _, states = model(features[:, :most].contiguous(), ends)
