@@ -237,8 +237,10 @@ int thff_copy_nt(void* d_dst, const void* d_src, long long bytes, void* stream);
 /* ---- Sequence operators beside the long convolutions (no reference counterpart) ----
  *
  * The gated linear recurrence, the other mixer of a sequence model next to the
- * long convolution, and the layer norm before either.  They need no
- * thff_initialize.  precision: THFF_FLOAT, THFF_HALF or THFF_BFLOAT16, the
+ * long convolution, and layer norm over rows that lie side by side: the
+ * channels where they come last, as before a projection.  (Where the steps come
+ * last, as the convolutions have them, a norm over the channels needs a
+ * transposed copy.)  They need no thff_initialize.  precision: THFF_FLOAT, THFF_HALF or THFF_BFLOAT16, the
  * type of the values (here real ones: float, half, bfloat16); states, weights,
  * biases and their gradients are fp32 for all three.  Sums, states and
  * statistics are held in fp32 and every output is rounded once, to nearest

@@ -13,10 +13,13 @@
 // their share of dweight and dbias in registers, and leaves one partial sum a column, which
 // a second kernel adds up.  Every order of summation is fixed.
 //
-// Memory bounds both: bfloat16 32768 x 2048 takes 51 us forward (268 MB, 5.2 TB/s) and 63 us
+// Memory bounds both: bfloat16 32768 x 2048 takes 52 us forward (268 MB, 5.2 TB/s) and 63 us
 // backward (407 MB, 6.5 TB/s, some of it still cached), 5 more for adding the parts up; half
-// 2048 x 8192 15 us, 28 us and 4 us.  Few rows are bound by latency: bfloat16 8 x 1024 2.6 us,
-// float 1001 x 777 4.3 us, 6.8 us and 3.1 us.
+// 2048 x 8192 14 us, 28 us and 4 us.  Few rows are bound by latency: bfloat16 8 x 1024 2.6 us,
+// float 1001 x 777 4.3 us, 6.7 us and 3.3 us.  These are the kernels' own times, a training step
+// of forward and backward passes in turn; further down "a call" is a backward call among its
+// like, with both its kernels and the time between them (75 us at bfloat16 32768 x 2048, whose
+// dy and x the forward pass has then not just brought into the caches).
 #include <algorithm>
 #include <type_traits>
 
@@ -152,8 +155,8 @@ __global__ __launch_bounds__(R::kLanes) void norm_forward(NormForward a) {
 }
 
 // Workgroups of the backward pass at most, each with a partial sum: one a compute unit.  (Twice as
-// many: 81 against 77 us at 32768 x 2048, 49 against 33 at 2048 x 8192, whose sums are then as large
-// as a third of its rows.)
+// many: 79 against 75 us a call at 32768 x 2048, 48 against 34 at 2048 x 8192, whose parts are
+// then 34 MB, written and read, next to 101 MB of rows.)
 constexpr int kMostParts = 256;
 
 template <class R>
@@ -411,8 +414,8 @@ constexpr int kMostHeld = 1024 * kLaneValues<Backward>;
 // lanes have them to spare.  False if the row is too long for 16 waves.
 //
 // Forward: up to 32 values a lane, which are all that it keeps.  Backward: 16, next to the
-// weights, two sums each, and the next row (2048 columns by 2 waves take 77 us for 32768 rows of
-// bfloat16; by one wave with 32 values each, which spill, 85 us).
+// weights, two sums each, and the next row (2048 columns by 2 waves take 75 us a call for 32768 rows
+// of bfloat16; by one wave with 32 values each, which spill, 84 us).
 //
 // Waves of a row are of every number that leaves few of them idle, up to 12, and of a workgroup as
 // many as have registers for it backward, 8 to 12 (half 10000 x 4104, which takes 5 of 8 waves: 71

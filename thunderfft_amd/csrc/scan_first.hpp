@@ -5,7 +5,7 @@
 //
 // Memory bounds it: half 256 x 64 x 4096 takes 70 us (403 MB, 5.7 TB/s; a row is a workgroup's, so
 // that nothing waits for another).  float 33 x 96 x 512, a wave a row and all of it in the
-// caches: 5.2 us forward and 6.8 backward, the latency of one round of loads, sums and stores.
+// caches: 5.3 us forward and 7.0 backward, the latency of one round of loads, sums and stores.
 #pragma once
 
 #include "scan_chain.hpp"

@@ -4,11 +4,11 @@
 //
 // About 10 operations for 6 bytes forward (2-byte values): memory bounds it, and next to it the
 // time from a tile's loads to its stores, in which its registers serve nobody else.  bfloat16
-// 8 x 4096 x 2048: 85 us forward (403 MB, 4.8 TB/s) and 145 us backward (671 MB, 4.6 TB/s); the
+// 8 x 4096 x 2048: 85 us forward (403 MB, 4.8 TB/s) and 146 us backward (671 MB, 4.6 TB/s); the
 // same tiles copied with no work between take 70 to 75 us forward.  Of the 10.4 us from a
 // workgroup's start to the next one's in its place, 2.7 go to the draw and the first loads, 1.8
 // until the last wave has its own, 1.7 to the chain, 1.4 to arithmetic and 2.8 pass between the
-// two.  1 x 65536 x 1024 takes 106 us for the same bytes: 64 tiles of a column run side by side
+// two.  1 x 65536 x 1024 takes 108 us for the same bytes: 64 tiles of a column run side by side
 // there, and each waits for the slowest of those before it.
 #pragma once
 
@@ -27,7 +27,8 @@ namespace thff {
 // that two workgroups of 16 waves fill a compute unit: one loads while the other waits.  (16 steps
 // at half the occupancy: 114 against 110 us at 1 x 65536 x 1024, 26 against 22.5 at
 // 1 x 10000 x 1024.  Workgroups that go on to a next tile, its loads under way meanwhile: 101
-// to 105 against 97 us at 8 x 4096 x 2048.)
+// to 105 against 97 us at 8 x 4096 x 2048.)  The narrow tile's backward pass of 2-byte values does
+// not quite fit, and has 40 bytes a lane in scratch memory.
 template <int VEC_, int CL_, int S_, int W_, int C_, int Occupancy_>
 struct Tile {
     static constexpr int VEC = VEC_, CL = CL_, S = S_, W = W_, C = C_;

@@ -1,6 +1,6 @@
 // scan_step.hpp -- one step of the gated recurrence (n = 1: a token of each sequence): no
 // tiles, no chain; a lane takes V channels of a sequence.  Latency bounds it: bfloat16 8 x 1024
-// takes 3.1 us, half 256 x 4096 4.8 us (14.7 MB, 3.1 TB/s, most of it from the caches).
+// takes 3.1 us, half 256 x 4096 4.7 us (14.7 MB, 3.1 TB/s, most of it from the caches).
 #pragma once
 
 #include "scan_chain.hpp"
