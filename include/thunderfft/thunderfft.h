@@ -363,6 +363,180 @@ int thff_layer_norm_backward_async(int precision, const void* d_dy, long long dy
                                    long long dx_stride, void* d_dweight, void* d_dbias,
                                    void* d_workspace, long long rows, int cols, void* stream);
 
+/* ---- Operators of a state space block (no reference counterpart) ----
+ *
+ * The mixer beside the gated recurrence that keeps several states a channel, the short
+ * convolution that goes before it, and the norm between blocks.  Types, sums, roundings,
+ * alignment, return codes and synchronisation are those of the sequence operators above.
+ * Values are [batch][n][channels], one row of `channels` values a step; strides are
+ * elements between the starts of consecutive rows, at least a row's length, or 0 for rows
+ * without a gap.  Sequence b's states are row b of their array, or row slots[b] of a pool
+ * of shape->states rows; a slot outside the pool (-1, say) is an empty place, which
+ * starts from zero and stores no state, and two places with the same slot race.
+ * state_out may be state_in (states kept in place); the two must not overlap otherwise.
+ * lengths[b] is taken into [0, n]; outputs and gradients are 0 from there on, and no
+ * input is used there, whatever it holds. */
+
+/* Short causal convolution.  x_stride holds for the gradient of x too, y_stride for y's.
+ * width: 2 to 4 taps.  silu: 1 for the activation, 0 for none.  batch, n, channels at
+ * most 2^30, batch * channels at most 2^31 - 256. */
+typedef struct thff_conv_shape {
+    int precision, silu;
+    int batch, n, channels, width, states;
+    long long x_stride, y_stride;
+} thff_conv_shape;
+
+/* Bytes of thff_short_conv_backward's d_workspace (0: may be null), or THFF_EINVAL. */
+long long thff_short_conv_workspace_bytes(const thff_conv_shape* shape);
+
+/* For every sequence and channel, with xe the width - 1 values of the state and then x:
+ *   p[t] = bias + sum_{k < width} weight[k] * xe[t + k],   y[t] = p / (1 + exp(-p)) or p,
+ * t < lengths[b].  weight is fp32 [channels][width], bias fp32 [channels] (null: zeros).
+ * A state is [width - 1][channels] values of the shape's type, the last before the next
+ * step: state_out is xe's values from lengths[b] on (null: not stored), state_in the
+ * same of the call before (null: zeros).  y may not alias x.  Empty batches and channels
+ * are no-ops; n = 0 copies the states. */
+int thff_short_conv(const thff_conv_shape* shape, const void* d_x, const void* d_weight,
+                    const void* d_bias, void* d_y, const void* d_state_in, void* d_state_out,
+                    const void* d_slots, const void* d_lengths, void* stream);
+int thff_short_conv_async(const thff_conv_shape* shape, const void* d_x, const void* d_weight,
+                          const void* d_bias, void* d_y, const void* d_state_in,
+                          void* d_state_out, const void* d_slots, const void* d_lengths,
+                          void* stream);
+
+/* Gradients of thff_short_conv from dy and that of the last states (d_dstate_out, null:
+ * zeros), with dp = dy * (the activation's slope at p):
+ *   dxe[e] = sum_k weight[k] * dp[e - k]  (+ dstate_out from e = lengths[b] on),
+ *   dweight[k] = sum over all steps of dp[t] * xe[t + k],   dbias = sum of dp,
+ * the first width - 1 of dxe to d_dstate_in (null: not stored), the rest to d_dx.
+ * d_dweight and d_dbias, fp32, are not accumulated (null: not computed).  The states and
+ * their gradients are row b for sequence b, of the shape's type; d_state_in is the
+ * forward call's.  d_dx may alias no input, d_workspace starts on 16 bytes. */
+int thff_short_conv_backward(const thff_conv_shape* shape, const void* d_dy, const void* d_x,
+                             const void* d_weight, const void* d_bias, const void* d_state_in,
+                             const void* d_dstate_out, const void* d_lengths, void* d_dx,
+                             void* d_dweight, void* d_dbias, void* d_dstate_in,
+                             void* d_workspace, void* stream);
+int thff_short_conv_backward_async(const thff_conv_shape* shape, const void* d_dy,
+                                   const void* d_x, const void* d_weight, const void* d_bias,
+                                   const void* d_state_in, const void* d_dstate_out,
+                                   const void* d_lengths, void* d_dx, void* d_dweight,
+                                   void* d_dbias, void* d_dstate_in, void* d_workspace,
+                                   void* stream);
+
+/* State space scan.  order: states of a channel, 1 to 64.  groups divide the channels:
+ * channel c has row c / (channels / groups) of b and c, which are [batch][n][groups][order].
+ * Each stride holds for the gradient of its array too.  Sizes at most 2^30, batch *
+ * channels at most 2^31 - 256 (THFF_EINVAL too where a call has too many workgroups). */
+typedef struct thff_state_shape {
+    int precision;
+    int batch, n, channels, order, groups, states;
+    long long x_stride, delta_stride, gate_stride, b_stride, c_stride, y_stride;
+} thff_state_shape;
+
+/* Bytes of d_saved (what the forward pass keeps for the backward pass) and of d_workspace
+ * (scratch of one call, either way) for a shape; THFF_EINVAL for a bad shape. */
+long long thff_state_scan_saved_bytes(const thff_state_shape* shape);
+long long thff_state_scan_workspace_bytes(const thff_state_shape* shape);
+
+/* For every sequence and channel, over its states s < order:
+ *   dt = log(1 + exp(delta[t] + delta_bias)),
+ *   h[t][s] = exp(dt * a[s]) * h[t-1][s] + dt * x[t] * b[t][s],
+ *   y[t] = (sum_s c[t][s] * h[t][s] + skip * x[t]) * gate[t] / (1 + exp(-gate[t])),
+ * t < lengths[b].  a is fp32 [channels][order]; skip, delta_bias fp32 [channels] (null:
+ * zeros); gate null: y without its last factor.  h before the first step is the state
+ * d_state_in (null: zeros), after the last one it goes to d_state_out (null: not
+ * stored): fp32 rows of [channels][order].  y may alias no input.  Empty batches and
+ * channels are no-ops; n = 0 copies the states.  An infinity or a NaN in an input makes
+ * later outputs that depend on it infinite or NaN, and no others. */
+int thff_state_scan(const thff_state_shape* shape, const void* d_x, const void* d_delta,
+                    const void* d_a, const void* d_b, const void* d_c, const void* d_skip,
+                    const void* d_gate, const void* d_delta_bias, void* d_y,
+                    const void* d_state_in, void* d_state_out, const void* d_slots,
+                    const void* d_lengths, void* d_saved, void* d_workspace, void* stream);
+int thff_state_scan_async(const thff_state_shape* shape, const void* d_x, const void* d_delta,
+                          const void* d_a, const void* d_b, const void* d_c, const void* d_skip,
+                          const void* d_gate, const void* d_delta_bias, void* d_y,
+                          const void* d_state_in, void* d_state_out, const void* d_slots,
+                          const void* d_lengths, void* d_saved, void* d_workspace, void* stream);
+
+/* What thff_state_scan_backward reads, and what it writes: pointers on the device.  saved
+ * is what the forward call of the same shape and inputs wrote.  dstate_out (null: zeros)
+ * and dstate_in (null: not stored) are fp32 [batch][channels][order], row b for sequence
+ * b.  dx, ddelta, db, dc and, with a gate, dgate are of the shape's type; da, dskip and
+ * ddelta_bias fp32, not accumulated (dskip, ddelta_bias null: not computed).  No output
+ * may alias an input or another output. */
+typedef struct thff_state_gradients {
+    const void *dy, *x, *delta, *a, *b, *c, *skip, *gate, *delta_bias, *saved, *dstate_out,
+        *lengths;
+    void *dx, *ddelta, *da, *db, *dc, *dskip, *dgate, *ddelta_bias, *dstate_in;
+} thff_state_gradients;
+
+/* Gradients of thff_state_scan from dy and that of the last states: with dinner the
+ * gradient of the sum before the gate, lam[t] = dinner[t] * c[t] + exp(dt[t+1] * a) * lam[t+1]
+ * (dstate_out behind the last step) and q[t] = lam[t] * exp(dt[t] * a) * h[t-1],
+ *   dx = dt * sum_s lam * b + dinner * skip,   da = sum over all steps of q * dt,
+ *   ddelta = (x * sum_s lam * b + sum_s q * a) / (1 + exp(-(delta + delta_bias))),
+ *   db = sum over a group's channels of lam * dt * x,   dc = the same of dinner * h. */
+int thff_state_scan_backward(const thff_state_shape* shape, const thff_state_gradients* arrays,
+                             void* d_workspace, void* stream);
+int thff_state_scan_backward_async(const thff_state_shape* shape,
+                                   const thff_state_gradients* arrays, void* d_workspace,
+                                   void* stream);
+
+/* Root-mean-square norm of `rows` rows of `cols` values, after a residual's addition:
+ *   s = x + residual, rounded to the type of the values,   y = s * rstd * weight,
+ * rstd = 1 / sqrt(mean(s^2) + eps).  residual null: s = x.  weight fp32 [cols] (null:
+ * ones).  s goes to d_sum (null: not stored), which may be d_residual (the residuals are
+ * kept in place, d_sum_stride equal to theirs) and neither x nor y; rstd to d_rstd,
+ * fp32 [rows] (null: not stored).  cols >= 1, eps >= 0; rows = 0 is a no-op. */
+int thff_rms_norm(int precision, const void* d_x, long long x_stride, const void* d_residual,
+                  long long residual_stride, const void* d_weight, float eps, void* d_y,
+                  long long y_stride, void* d_sum, long long sum_stride, void* d_rstd,
+                  long long rows, int cols, void* stream);
+int thff_rms_norm_async(int precision, const void* d_x, long long x_stride,
+                        const void* d_residual, long long residual_stride, const void* d_weight,
+                        float eps, void* d_y, long long y_stride, void* d_sum,
+                        long long sum_stride, void* d_rstd, long long rows, int cols,
+                        void* stream);
+
+/* The same with an output of 8 bits (e4m3: 4 exponent bits, 3 of mantissa, finite, 448 the
+ * largest): q = y / scale, rounded to nearest even, with a scale for every `block` columns
+ * of a row, the largest |y| of them / 448 (at least 2^-126).  block: 128, or cols for one
+ * scale a row.  y is rounded once, to q.  q_stride in bytes; d_scales is fp32
+ * [rows][ceil(cols / block)].  A NaN in a row makes its q NaN. */
+int thff_rms_norm_8bit(int precision, const void* d_x, long long x_stride,
+                       const void* d_residual, long long residual_stride, const void* d_weight,
+                       float eps, void* d_q, long long q_stride, void* d_scales, int block,
+                       void* d_sum, long long sum_stride, long long rows, int cols,
+                       void* stream);
+int thff_rms_norm_8bit_async(int precision, const void* d_x, long long x_stride,
+                             const void* d_residual, long long residual_stride,
+                             const void* d_weight, float eps, void* d_q, long long q_stride,
+                             void* d_scales, int block, void* d_sum, long long sum_stride,
+                             long long rows, int cols, void* stream);
+
+/* Bytes of thff_rms_norm_backward's d_workspace (0: may be null). */
+long long thff_rms_norm_workspace_bytes(long long rows, int cols);
+
+/* Gradients of thff_rms_norm from dy, the sums s (x itself without a residual) and their
+ * rstd, with xh = s * rstd, g = dy * weight and dsum the gradient that reaches s from
+ * elsewhere (null: zeros):
+ *   dx = rstd * (g - xh * mean(g * xh)) + dsum,   dweight = sum over the rows of dy * xh,
+ * dx for x and the residual alike, dweight fp32 [cols], not accumulated (null: not
+ * computed; zeros where rows = 0).  dx may alias no input. */
+int thff_rms_norm_backward(int precision, const void* d_dy, long long dy_stride,
+                           const void* d_sum, long long sum_stride, const void* d_rstd,
+                           const void* d_weight, const void* d_dsum, long long dsum_stride,
+                           void* d_dx, long long dx_stride, void* d_dweight, void* d_workspace,
+                           long long rows, int cols, void* stream);
+int thff_rms_norm_backward_async(int precision, const void* d_dy, long long dy_stride,
+                                 const void* d_sum, long long sum_stride, const void* d_rstd,
+                                 const void* d_weight, const void* d_dsum,
+                                 long long dsum_stride, void* d_dx, long long dx_stride,
+                                 void* d_dweight, void* d_workspace, long long rows, int cols,
+                                 void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,386 @@
+"""The state space scan on the GPU against its definition in 64 bits: outputs, states and gradients,
+in all types, orders and groups, for one token, for prompts and for long sequences in segments."""
+import pytest
+import torch
+
+import block_oracle as oracle
+import thunderfft_amd as thff
+
+pytestmark = pytest.mark.gpu
+GUARD = -271.0
+SHARED = ("b", "c")
+VALUES = ("x", "delta", "gate")
+
+
+def values(seed, T, batch, n, channels, order, groups=1):
+    """The arguments by name, on the GPU: steps from a thousandth to a tenth, rates from one up."""
+    gen, dt = torch.Generator().manual_seed(seed), oracle.TYPES[T]
+
+    def normal(*s):
+        return torch.randn(*s, generator=gen)
+
+    v = dict(x=normal(batch, n, channels).to(dt), delta=(0.5 * normal(batch, n, channels)).to(dt),
+             a=-(torch.arange(1, order + 1) * (0.2 * normal(channels, order)).exp()), b=normal(batch, n, groups, order).to(dt),
+             c=normal(batch, n, groups, order).to(dt), skip=1 + 0.2 * normal(channels), gate=normal(batch, n, channels).to(dt),
+             delta_bias=torch.linspace(-7, -2, channels), state=normal(batch, channels, order))
+    return {k: t.cuda() for k, t in v.items()} | dict(dy=normal(batch, n, channels).to(dt).cuda(),
+                                                      dstate=normal(batch, channels, order).cuda())
+
+
+def ends(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def placed(v, gap, offset):
+    """A copy of v (batch, n, ...) with rows `gap` more apart than they are long, `offset` elements
+    into its buffer, and whether what is around the rows is as it was."""
+    flat = v.flatten(2)
+    batch, n, row = flat.shape
+    stride = row + gap
+    whole = torch.full((offset + batch * n * stride + 64,), GUARD, dtype=v.dtype, device="cuda")
+    out = whole[offset:offset + batch * n * stride].view(batch, n, stride)[..., :row]
+    out.copy_(flat)
+
+    def intact():
+        around = whole.clone()
+        around[offset:offset + batch * n * stride].view(batch, n, stride)[..., :row] = GUARD
+        return bool((around == GUARD).all())
+
+    return out, intact
+
+
+def run(T, v, lengths=None, gap=0, offset=0):
+    """Outputs and gradients by the calls on device buffers; every buffer is guarded."""
+    batch, n, channels = v["x"].shape
+    groups, order = v["b"].shape[2:]
+    row = groups * order
+    print(f"{T} {batch} x {n} x {channels} order {order} groups {groups} gap {gap} offset {offset} "
+          f"without {[k for k in v if v[k] is None]}", flush=True)
+    stride = channels + gap
+    shape = thff.StateShape(T, batch, n, channels, order, groups, stride, stride, stride, row + gap, row + gap, stride)
+    at = {k: placed(v[k], gap, offset)[0] for k in ("x", "delta", "b", "c", "dy")}
+    gate = None if v["gate"] is None else placed(v["gate"], gap, offset)[0]
+    nan = torch.full_like(v["x"], float("nan"))
+    out = {k: placed(nan, gap, offset) for k in ("y", "dx", "ddelta", "dgate")}
+    out |= {k: placed(torch.full_like(v["b"], float("nan")), gap, offset) for k in ("db", "dc")}
+    sizes = dict(state=batch * channels * order, dstate=batch * channels * order, da=channels * order, dskip=channels,
+                 ddelta_bias=channels)
+    weights = {k: torch.full((size + 4,), GUARD, device="cuda") for k, size in sizes.items()}
+
+    def scratch(count):
+        return torch.full((count + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+
+    saved, workspace = scratch(shape.saved_bytes()), scratch(shape.workspace_bytes())
+    thff.ThunderFFT_state_scan(shape, at["x"], at["delta"], v["a"], at["b"], at["c"], out["y"][0], d_skip=v["skip"], d_gate=gate,
+                               d_delta_bias=v["delta_bias"], d_state_in=v["state"], d_state_out=weights["state"], d_lengths=lengths,
+                               d_saved=saved, d_workspace=workspace)
+    assert (saved[-64:] == 0xFF).all() and (workspace[-64:] == 0xFF).all()
+    workspace = scratch(shape.workspace_bytes())
+    thff.ThunderFFT_state_scan_backward(
+        shape, at["dy"], at["x"], at["delta"], v["a"], at["b"], at["c"], saved, out["dx"][0], out["ddelta"][0], weights["da"],
+        out["db"][0], out["dc"][0], d_skip=v["skip"], d_dskip=weights["dskip"], d_gate=gate,
+        d_dgate=None if gate is None else out["dgate"][0], d_delta_bias=v["delta_bias"], d_ddelta_bias=weights["ddelta_bias"],
+        d_dstate_out=v["dstate"], d_dstate_in=weights["dstate"], d_lengths=lengths, d_workspace=workspace)
+    assert (workspace[-64:] == 0xFF).all()
+    got = {}
+    for k, (t, intact) in out.items():
+        assert intact(), k
+        got[k] = t.reshape(v["b"].shape) if k in ("db", "dc") else t
+    for k, t in weights.items():
+        assert (t[sizes[k]:] == GUARD).all(), k
+        got[k] = t[:sizes[k]].view(channels, order) if k == "da" else t[:sizes[k]].view(
+            (batch, channels, order) if k in ("state", "dstate") else (channels,))
+    if gate is None:
+        del got["dgate"]
+    return got
+
+
+def wanted(T, v, lengths=None):
+    return oracle.state(T, v["x"], v["delta"], v["a"], v["b"], v["c"], v["skip"], v["gate"], v["delta_bias"], v["state"], lengths,
+                        v["dy"], v["dstate"])
+
+
+def compare(T, v, lengths=None, **how):
+    got, want = run(T, v, lengths, **how), wanted(T, v, lengths)
+    assert got.keys() == want.keys()
+    for name in want:
+        oracle.check(name, got[name], want[name])
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("size", [(1, 1, 1, 1), (2, 2, 3, 4), (3, 3, 17, 5), (2, 15, 8, 8), (1, 16, 64, 16), (2, 17, 65, 16),
+                                  (3, 31, 40, 12), (1, 33, 130, 3), (2, 64, 16, 16), (1, 100, 33, 24), (2, 50, 20, 32), (1, 70, 9, 33),
+                                  (2, 40, 12, 64), (40, 5, 48, 16)], ids=str)
+def test_sizes(T, size):
+    compare(T, values(sum(size), T, *size))
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("size", [(2, 40, 12, 7, 12), (1, 20, 96, 16, 2), (3, 9, 300, 16, 3), (2, 35, 8, 40, 4)], ids=str)
+def test_groups(T, size):
+    compare(T, values(1, T, *size))
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("without", [("gate",), ("skip",), ("delta_bias",), ("state",), ("dstate",),
+                                     ("gate", "skip", "delta_bias", "state", "dstate")], ids=str)
+def test_optional_arguments(T, without):
+    v = values(2, T, 3, 37, 24, 16)
+    if "delta_bias" in without:
+        v["delta"] -= 3
+    compare(T, v | {k: None for k in without})
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("how", [dict(gap=1), dict(gap=8), dict(offset=1), dict(offset=4), dict(gap=48, offset=8)], ids=str)
+def test_strides_and_offsets(T, how):
+    for size in ((3, 37, 72, 16, 1), (2, 20, 30, 5, 2)):
+        compare(T, values(3, T, *size), **how)
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("order", [4, 16, 24])
+def test_lengths(T, order):
+    """Sequences that end early, before the first step, and outside [0, n]; junk behind the ends
+    reaches nothing."""
+    n = 75
+    v = values(4, T, 9, n, 24, order)
+    lengths = ends(0, 1, 15, 16, 17, 32, 64, n, 500)
+    compare(T, v, lengths)
+    clean = run(T, v, lengths)
+    dirty = {k: t.clone() for k, t in v.items()}
+    for b, end in enumerate(lengths.tolist()):
+        for name, junk in (("x", "nan"), ("delta", "inf"), ("gate", "-inf"), ("b", "inf"), ("c", "nan"), ("dy", "nan")):
+            dirty[name][b, end:] = float(junk)
+    got = run(T, dirty, lengths)
+    for name in clean:
+        assert torch.equal(clean[name], got[name]), name
+    below = run(T, v, ends(-3, 1, 15, 16, 17, 32, 64, n, 500))
+    for name in clean:
+        assert torch.equal(clean[name], below[name]), name
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("size", [(1, 3000, 20, 16, 1), (2, 1500, 6, 5, 2), (1, 2500, 70, 4, 1), (1, 1100, 9, 40, 1)], ids=str)
+def test_long_sequences(T, size):
+    compare(T, values(5, T, *size))
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+def test_long_sequences_that_end_early(T):
+    v = values(6, T, 4, 2100, 24, 16)
+    compare(T, v, ends(2100, 1000, 5, 0))
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+def test_steps_of_all_sizes(T):
+    """Steps from nothing, which keep the states, to ones that leave nothing of them; rates of zero."""
+    v = values(7, T, 2, 60, 32, 16)
+    v["delta"][0, ::3] = -40
+    v["delta"][0, 1::3] = 40
+    v["delta"][1] = 6
+    v["a"][:, 3] = 0
+    v["a"][5] = -30
+    compare(T, v)
+
+
+def test_growing_states():
+    """Positive rates: the states grow."""
+    v = values(8, "float", 2, 40, 16, 8)
+    v["a"] = -0.3 * v["a"]
+    compare("float", v)
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("size", [(37, 5), (24, 16), (9, 64), (16, 24)], ids=str)
+def test_tokens_follow_prompts_in_a_pool(T, size):
+    """A prompt, a second chunk and single tokens, the states in place in rows of a pool, are as the
+    whole sequence; rows of the pool that are no slot's stay, and empty places store nothing."""
+    channels, order = size
+    batch, n = 5, 60
+    v = values(9, T, batch, n, channels, order)
+    v["state"] = None
+    whole = oracle.state(T, v["x"], v["delta"], v["a"], v["b"], v["c"], v["skip"], v["gate"], v["delta_bias"])
+    pool = torch.full((9, channels, order), GUARD, device="cuda")
+    slots, rows = ends(7, 0, -1, 3, 8), [0, 1, 3, 4]
+    pool[slots[rows].long()] = 0
+    kept = pool.clone()
+    at, y = 0, torch.empty_like(v["x"])
+    for count in (33, 2, 18) + (1,) * 7:
+        part = {k: v[k][:, at:at + count].contiguous() for k in VALUES + SHARED}
+        shape = thff.StateShape(T, batch, count, channels, order, states=9)
+        out = torch.empty_like(part["x"])
+        work = torch.empty(shape.workspace_bytes(), dtype=torch.uint8, device="cuda")
+        thff.ThunderFFT_state_scan(shape, part["x"], part["delta"], v["a"], part["b"], part["c"], out, d_skip=v["skip"],
+                                   d_gate=part["gate"], d_delta_bias=v["delta_bias"], d_state_in=pool, d_state_out=pool,
+                                   d_slots=slots, d_workspace=work)
+        y[:, at:at + count] = out
+        at += count
+    for name, got in (("y", y), ("state", pool[slots.long()])):
+        value, bound = whole[name]
+        oracle.check(name, got[rows], (value[rows], bound[rows]))
+    free = [r for r in range(9) if r not in (7, 0, 3, 8)]
+    assert torch.equal(pool[free], kept[free])
+    # The empty place had no past.
+    last = {k: v[k][2:3, n - 1:] for k in VALUES + SHARED}
+    want = oracle.state(T, last["x"], last["delta"], v["a"], last["b"], last["c"], v["skip"], last["gate"], v["delta_bias"])
+    oracle.check("empty", y[2:3, n - 1:], want["y"])
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("size", [(70, 16, 1, 1), (3, 24, 3, 3), (260, 48, 16, 2), (4, 40, 33, 1), (5, 1000, 16, 1)], ids=str)
+def test_one_token(T, size):
+    """n = 1, with lengths of 0 and 1, a shape of strides, and without each optional argument."""
+    batch, channels, order, groups = size
+    v = values(10, T, batch, 1, channels, order, groups)
+    lengths = (torch.arange(batch, device="cuda") % 3 != 1).to(torch.int32)
+    for without in ((), ("gate",), ("skip", "state"), ("delta_bias",)):
+        w = v | {k: None for k in without}
+        for end in (None, lengths):
+            want = oracle.state(T, w["x"], w["delta"], w["a"], w["b"], w["c"], w["skip"], w["gate"], w["delta_bias"], w["state"], end)
+            at = {k: None if w[k] is None else placed(w[k], 3, 1)[0] for k in VALUES + SHARED}
+            y, intact = placed(torch.full_like(v["x"], float("nan")), 3, 1)
+            row = groups * order + 3
+            shape = thff.StateShape(T, batch, 1, channels, order, groups, *(channels + 3,) * 3, row, row, channels + 3)
+            state = torch.full((batch * channels * order + 4,), GUARD, device="cuda")
+            work = torch.empty(shape.workspace_bytes(), dtype=torch.uint8, device="cuda")
+            thff.ThunderFFT_state_scan(shape, at["x"], at["delta"], w["a"], at["b"], at["c"], y, d_skip=w["skip"], d_gate=at["gate"],
+                                       d_delta_bias=w["delta_bias"], d_state_in=w["state"], d_state_out=state, d_lengths=end,
+                                       d_workspace=work)
+            assert intact() and (state[-4:] == GUARD).all()
+            oracle.check("y", y, want["y"])
+            oracle.check("state", state[:-4].view(batch, channels, order), want["state"])
+
+
+def test_no_steps_and_nothing():
+    """No steps copy the states and their gradients; no sequences leave the weights' gradients zero."""
+    for order in (5, 16):
+        v = values(11, "half", 3, 0, 21, order)
+        got = run("half", v)
+        assert torch.equal(got["state"], v["state"]) and torch.equal(got["dstate"], v["dstate"])
+        assert all((got[k] == 0).all() for k in ("da", "dskip", "ddelta_bias"))
+    shape = thff.StateShape("half", 0, 9, 21, 5)
+    da, dskip, dbias = (torch.full(s, GUARD, device="cuda") for s in ((21, 5), (21,), (21,)))
+    thff.ThunderFFT_state_scan_backward(shape, 0, 0, 0, 0, 0, 0, 0, 0, 0, da, 0, 0, d_dskip=dskip, d_ddelta_bias=dbias)
+    assert all((t == 0).all() for t in (da, dskip, dbias))
+
+
+@pytest.mark.parametrize("name,junk", [("x", "nan"), ("x", "inf"), ("delta", "nan"), ("b", "nan"), ("c", "inf"), ("gate", "nan")])
+def test_non_finite_values_stay_where_they_belong(name, junk):
+    """Outputs that do not depend on a NaN or an infinity are as without it; those of its step that do are not finite."""
+    v = values(12, "half", 2, 700, 24, 16, 2)
+    clean = run("half", v)
+    w = {k: t.clone() for k, t in v.items()}
+    if name in SHARED:
+        w[name][1, 333, 1, 4] = float(junk)
+    else:
+        w[name][1, 333, 17] = float(junk)
+    got = run("half", w)
+    touched = torch.zeros_like(v["x"], dtype=torch.bool)
+    if name in SHARED:
+        touched[1, 333:334 if name == "c" else 700, 12:] = True
+    else:
+        touched[1, 333:334 if name == "gate" else 700, 17] = True
+    assert torch.equal(got["y"][~touched], clean["y"][~touched])
+    assert not torch.isfinite(got["y"][1, 333][touched[1, 333]]).any()
+
+
+@pytest.mark.parametrize("size", [(3, 200, 72, 16), (1, 3000, 24, 16), (2, 100, 20, 40)], ids=str)
+def test_same_bits_each_time(size):
+    v = values(13, "bfloat16", *size)
+    first = run("bfloat16", v)
+    for _ in range(3):
+        again = run("bfloat16", v)
+        for name in first:
+            assert torch.equal(first[name], again[name]), name
+
+
+@pytest.mark.parametrize("size", [(4, 100, 136, 16), (1, 3000, 24, 16)], ids=str)
+def test_streams_and_graph_replays(size):
+    """On a stream of its own, captured, and replayed with new inputs and eager calls between."""
+    v = values(14, "bfloat16", *size)
+    batch, n, channels, order = size
+    shape = thff.StateShape("bfloat16", *size)
+    out = {k: torch.empty_like(v[k[1:]]) for k in ("dx", "ddelta", "dgate", "da", "db", "dc", "dskip", "ddelta_bias", "dstate")}
+    out |= dict(y=torch.empty_like(v["x"]), state=torch.empty_like(v["state"]))
+    saved = torch.empty(shape.saved_bytes(), dtype=torch.uint8, device="cuda")
+    workspace = torch.empty(shape.workspace_bytes(), dtype=torch.uint8, device="cuda")
+
+    def calls(stream):
+        thff.ThunderFFT_state_scan_async(shape, v["x"], v["delta"], v["a"], v["b"], v["c"], out["y"], d_skip=v["skip"],
+                                         d_gate=v["gate"], d_delta_bias=v["delta_bias"], d_state_in=v["state"],
+                                         d_state_out=out["state"], d_saved=saved, d_workspace=workspace, stream=stream)
+        thff.ThunderFFT_state_scan_backward_async(
+            shape, v["dy"], v["x"], v["delta"], v["a"], v["b"], v["c"], saved, out["dx"], out["ddelta"], out["da"], out["db"],
+            out["dc"], d_skip=v["skip"], d_dskip=out["dskip"], d_gate=v["gate"], d_dgate=out["dgate"], d_delta_bias=v["delta_bias"],
+            d_ddelta_bias=out["ddelta_bias"], d_dstate_out=v["dstate"], d_dstate_in=out["dstate"], d_workspace=workspace,
+            stream=stream)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    calls(side)
+    torch.cuda.synchronize()
+    want = run("bfloat16", v)
+    assert all(torch.equal(want[name], t) for name, t in out.items())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(torch.cuda.current_stream())
+    for k in range(4):
+        new = values(50 + k, "bfloat16", *size)
+        for name in v:
+            v[name].copy_(new[name])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run("bfloat16", new)
+        for name, t in out.items():
+            assert torch.equal(want[name], t), (k, name)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_tensor_function(fused):
+    """state_scan's outputs and gradients, from dense arguments and from slices of projections' rows."""
+    v = values(15, "bfloat16", 3, 40, 64, 16, 2)
+    lengths = ends(40, 7, 0)
+    if fused:
+        v["gate"] = torch.cat([torch.full_like(v["x"], float("nan")), v["gate"]], 2)[..., 64:]
+        rows = torch.cat([torch.zeros_like(v["x"][..., :5]), v["b"].flatten(2), v["c"].flatten(2)], 2)
+        v["b"], v["c"] = rows[..., 5:37].unflatten(2, (2, 16)), rows[..., 37:].unflatten(2, (2, 16))
+    names = ("x", "delta", "a", "b", "c", "skip", "gate", "delta_bias", "state")
+    leaves = [v[k].detach().requires_grad_() for k in names]
+    y, last = thff.state_scan(*leaves, lengths)
+    torch.autograd.backward([y, last], [v["dy"], v["dstate"]])
+    want = wanted("bfloat16", v, lengths)
+    got = {"d" + k: t.grad for k, t in zip(names, leaves)} | dict(y=y, state=last)
+    for name in want:
+        oracle.check(name, got[name], want[name])
+    # One group without an axis of its own, no optional arguments, gradients of some alone.
+    w = values(16, "float", 2, 30, 20, 8)
+    x, a = w["x"].requires_grad_(), w["a"].requires_grad_()
+    y, last = thff.state_scan(x, w["delta"], a, w["b"][:, :, 0], w["c"][:, :, 0])
+    last.backward(w["dstate"])
+    w |= dict(skip=None, gate=None, delta_bias=None, state=None, dy=torch.zeros_like(w["dy"]))
+    want = wanted("float", w)
+    for name, t in (("y", y), ("state", last), ("dx", x.grad), ("da", a.grad)):
+        oracle.check(name, t, want[name])
+    with pytest.raises(ValueError, match="groups must divide"):
+        thff.state_scan(w["x"], w["delta"], w["a"], w["b"].expand(-1, -1, 3, -1), w["c"].expand(-1, -1, 3, -1))
+    with pytest.raises(ValueError, match="order 1 to 64"):
+        thff.state_scan(w["x"], w["delta"], torch.zeros(20, 65, device="cuda"), w["b"], w["c"])
+
+
+def test_gradients_against_differences():
+    """Along a random direction of all arguments at once: float32 outputs are off by some 1e-6 of sums
+    of order ten, and a step of 2^-6 of smooth functions by its square."""
+    v = values(17, "float", 2, 23, 12, 6)
+    names = ("x", "delta", "a", "b", "c", "skip", "gate", "delta_bias", "state")
+    gen = torch.Generator().manual_seed(18)
+    way = {k: 0.1 * torch.randn(v[k].shape, generator=gen).cuda() for k in names}
+
+    def outputs(step):
+        y, last = thff.state_scan(*(v[k] + step * way[k] for k in names))
+        return float((y.double() * v["dy"]).sum() + (last.double() * v["dstate"]).sum())
+
+    got = run("float", v)
+    along = sum(float((got["d" + k].double() * way[k].double()).sum()) for k in names)
+    quotient = (outputs(2.0 ** -6) - outputs(-(2.0 ** -6))) * 2 ** 5
+    assert abs(quotient - along) < 2e-3 * max(1.0, abs(along)), (quotient, along)

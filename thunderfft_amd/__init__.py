@@ -30,7 +30,13 @@ __all__ = [
     "ThunderFFT_gated_scan_backward", "ThunderFFT_gated_scan_backward_async",
     "ThunderFFT_layer_norm", "ThunderFFT_layer_norm_async", "ThunderFFT_layer_norm_backward",
     "ThunderFFT_layer_norm_backward_async", "layer_norm_workspace_bytes", "gated_scan",
-    "layer_norm",
+    "layer_norm", "ConvShape", "ThunderFFT_short_conv", "ThunderFFT_short_conv_async",
+    "ThunderFFT_short_conv_backward", "ThunderFFT_short_conv_backward_async", "StateShape",
+    "ThunderFFT_state_scan", "ThunderFFT_state_scan_async", "ThunderFFT_state_scan_backward",
+    "ThunderFFT_state_scan_backward_async", "ThunderFFT_rms_norm", "ThunderFFT_rms_norm_async",
+    "ThunderFFT_rms_norm_8bit", "ThunderFFT_rms_norm_8bit_async", "ThunderFFT_rms_norm_backward",
+    "ThunderFFT_rms_norm_backward_async", "rms_norm_workspace_bytes", "short_conv", "state_scan",
+    "rms_norm", "rms_norm_8bit",
 ]
 
 SUPPORTED_N = (64, 128, 256, 512, 1024, 2048, 4096)
@@ -103,6 +109,25 @@ def lib() -> ctypes.CDLL:
                 i32, vp, i64, vp, vp, f32, vp, i64, vp, vp, i64, i32, vp]
             getattr(L, "thff_layer_norm_backward" + twin).argtypes = [
                 i32, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i32, vp]
+        cp, tp = ctypes.POINTER(ConvShape), ctypes.POINTER(StateShape)
+        for name, p in (("short_conv_workspace", cp), ("state_scan_saved", tp),
+                        ("state_scan_workspace", tp)):
+            fn = getattr(L, f"thff_{name}_bytes")
+            fn.argtypes, fn.restype = [p], i64
+        L.thff_rms_norm_workspace_bytes.argtypes = [i64, i32]
+        L.thff_rms_norm_workspace_bytes.restype = i64
+        for twin in ("", "_async"):
+            getattr(L, "thff_short_conv" + twin).argtypes = [cp] + [vp] * 9
+            getattr(L, "thff_short_conv_backward" + twin).argtypes = [cp] + [vp] * 13
+            getattr(L, "thff_state_scan" + twin).argtypes = [tp] + [vp] * 16
+            getattr(L, "thff_state_scan_backward" + twin).argtypes = [
+                tp, ctypes.POINTER(_StateGradients), vp, vp]
+            getattr(L, "thff_rms_norm" + twin).argtypes = [
+                i32, vp, i64, vp, i64, vp, f32, vp, i64, vp, i64, vp, i64, i32, vp]
+            getattr(L, "thff_rms_norm_8bit" + twin).argtypes = [
+                i32, vp, i64, vp, i64, vp, f32, vp, i64, vp, i32, vp, i64, i64, i32, vp]
+            getattr(L, "thff_rms_norm_backward" + twin).argtypes = [
+                i32, vp, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, i64, i32, vp]
         _lib = L
     return _lib
 
@@ -423,6 +448,290 @@ def ThunderFFT_layer_norm_backward_async(T, d_dy, d_x, d_mean, d_rstd, d_weight,
                          x_stride, dx_stride, stream)
 
 
+def _sizes(**named):
+    """The values as integers; ctypes would wrap larger ones round."""
+    for what, v in named.items():
+        if not -2**31 <= int(v) < 2**31:
+            raise ValueError(f"{what} is out of range")
+    return [int(v) for v in named.values()]
+
+
+class ConvShape(ctypes.Structure):
+    """What a short convolution works on; kept by the caller from call to call.
+
+    T: "float", "half" or "bfloat16" (or the torch dtype), of values [batch][n][channels].
+    width: taps, 2 to 4.  silu: whether the activation follows.  Strides: elements between the
+    starts of consecutive rows, None for rows without a gap; each holds for its array's
+    gradient too.  states: rows of the state pool that slots index (None: batch).
+    """
+
+    _fields_ = [("precision", ctypes.c_int), ("silu", ctypes.c_int), ("batch", ctypes.c_int),
+                ("n", ctypes.c_int), ("channels", ctypes.c_int), ("width", ctypes.c_int),
+                ("states", ctypes.c_int), ("x_stride", ctypes.c_longlong),
+                ("y_stride", ctypes.c_longlong)]
+
+    def __init__(self, T, batch, n, channels, width, silu=True, x_stride=None, y_stride=None,
+                 states=None):
+        sizes = _sizes(batch=batch, n=n, channels=channels, width=width,
+                       states=batch if states is None else states)
+        super().__init__(_value_type(T), int(bool(silu)), *sizes, int(x_stride or 0),
+                         int(y_stride or 0))
+
+    def workspace_bytes(self) -> int:
+        """Bytes of a backward call's scratch memory (d_workspace)."""
+        return _bytes(lib().thff_short_conv_workspace_bytes(ctypes.byref(self)))
+
+
+def _short_conv(call, shape, d_x, d_weight, d_bias, d_y, d_state_in, d_state_out, d_slots, d_lengths,
+                stream):
+    _raise(call(shape, _ptr(d_x), _ptr(d_weight), _ptr(d_bias), _ptr(d_y), _ptr(d_state_in),
+                _ptr(d_state_out), _ptr(d_slots), _ptr(d_lengths), _stream(stream)))
+
+
+def ThunderFFT_short_conv(shape, d_x, d_weight, d_bias, d_y, d_state_in=None, d_state_out=None,
+                          d_slots=None, d_lengths=None, stream=0) -> None:
+    """Short causal convolution y[t] = silu(bias + sum_k weight[k] x[t - width + 1 + k]) of each
+    channel, on values of ``shape`` (a ConvShape); weight float32 [channels][width], bias float32
+    [channels] (None: zeros).  The width - 1 values before the first step (d_state_in) and the last
+    ones (d_state_out, the same buffer if wanted) are rows [width - 1][channels] of the shape's type,
+    row b for sequence b or row d_slots[b] (int32) of a pool; d_lengths (int32) ends each sequence
+    early.  Synchronous."""
+    _short_conv(lib().thff_short_conv, shape, d_x, d_weight, d_bias, d_y, d_state_in, d_state_out,
+                d_slots, d_lengths, stream)
+
+
+def ThunderFFT_short_conv_async(shape, d_x, d_weight, d_bias, d_y, d_state_in=None,
+                                d_state_out=None, d_slots=None, d_lengths=None, stream=0) -> None:
+    """As ThunderFFT_short_conv, but returns once the work is enqueued on ``stream``."""
+    _short_conv(lib().thff_short_conv_async, shape, d_x, d_weight, d_bias, d_y, d_state_in,
+                d_state_out, d_slots, d_lengths, stream)
+
+
+def _short_conv_backward(call, shape, d_dy, d_x, d_weight, d_bias, d_dx, d_dweight, d_dbias,
+                         d_state_in, d_dstate_out, d_dstate_in, d_lengths, d_workspace, stream):
+    _raise(call(shape, _ptr(d_dy), _ptr(d_x), _ptr(d_weight), _ptr(d_bias), _ptr(d_state_in),
+                _ptr(d_dstate_out), _ptr(d_lengths), _ptr(d_dx), _ptr(d_dweight), _ptr(d_dbias),
+                _ptr(d_dstate_in), _ptr(d_workspace), _stream(stream)))
+
+
+def ThunderFFT_short_conv_backward(shape, d_dy, d_x, d_weight, d_bias, d_dx, d_dweight=None,
+                                   d_dbias=None, d_state_in=None, d_dstate_out=None,
+                                   d_dstate_in=None, d_lengths=None, d_workspace=None,
+                                   stream=0) -> None:
+    """Gradients of ThunderFFT_short_conv by x, by the weights and the bias (float32; None: not
+    computed) and by the first state (d_dstate_in), from those by y and by the last states
+    (d_dstate_out, None: zero); states and their gradients are row b for sequence b, of the shape's
+    type.  d_workspace: shape.workspace_bytes().  Synchronous."""
+    _short_conv_backward(lib().thff_short_conv_backward, shape, d_dy, d_x, d_weight, d_bias, d_dx,
+                         d_dweight, d_dbias, d_state_in, d_dstate_out, d_dstate_in, d_lengths,
+                         d_workspace, stream)
+
+
+def ThunderFFT_short_conv_backward_async(shape, d_dy, d_x, d_weight, d_bias, d_dx, d_dweight=None,
+                                         d_dbias=None, d_state_in=None, d_dstate_out=None,
+                                         d_dstate_in=None, d_lengths=None, d_workspace=None,
+                                         stream=0) -> None:
+    """As ThunderFFT_short_conv_backward, but returns once the work is enqueued."""
+    _short_conv_backward(lib().thff_short_conv_backward_async, shape, d_dy, d_x, d_weight, d_bias,
+                         d_dx, d_dweight, d_dbias, d_state_in, d_dstate_out, d_dstate_in,
+                         d_lengths, d_workspace, stream)
+
+
+class StateShape(ctypes.Structure):
+    """What a state space scan works on; kept by the caller from call to call.
+
+    T: "float", "half" or "bfloat16" (or the torch dtype), of x, delta, the gate and y,
+    [batch][n][channels], and of b and c, [batch][n][groups][order].  order: states of a channel, 1
+    to 64.  groups divide the channels.  Strides: elements between the starts of consecutive rows,
+    None for rows without a gap; each holds for its array's gradient too.  states: rows of the state
+    pool that slots index (None: batch).
+    """
+
+    _fields_ = [("precision", ctypes.c_int), ("batch", ctypes.c_int), ("n", ctypes.c_int),
+                ("channels", ctypes.c_int), ("order", ctypes.c_int), ("groups", ctypes.c_int),
+                ("states", ctypes.c_int), ("x_stride", ctypes.c_longlong),
+                ("delta_stride", ctypes.c_longlong), ("gate_stride", ctypes.c_longlong),
+                ("b_stride", ctypes.c_longlong), ("c_stride", ctypes.c_longlong),
+                ("y_stride", ctypes.c_longlong)]
+
+    def __init__(self, T, batch, n, channels, order, groups=1, x_stride=None, delta_stride=None,
+                 gate_stride=None, b_stride=None, c_stride=None, y_stride=None, states=None):
+        sizes = _sizes(batch=batch, n=n, channels=channels, order=order, groups=groups,
+                       states=batch if states is None else states)
+        super().__init__(_value_type(T), *sizes,
+                         *(int(v or 0) for v in (x_stride, delta_stride, gate_stride, b_stride,
+                                                 c_stride, y_stride)))
+
+    def saved_bytes(self) -> int:
+        """Bytes that the forward call keeps for the backward call (d_saved)."""
+        return _bytes(lib().thff_state_scan_saved_bytes(ctypes.byref(self)))
+
+    def workspace_bytes(self) -> int:
+        """Bytes of a call's scratch memory (d_workspace), forward or backward."""
+        return _bytes(lib().thff_state_scan_workspace_bytes(ctypes.byref(self)))
+
+
+def _state_scan(call, shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip, d_gate, d_delta_bias, d_state_in,
+                d_state_out, d_slots, d_lengths, d_saved, d_workspace, stream):
+    _raise(call(shape, _ptr(d_x), _ptr(d_delta), _ptr(d_a), _ptr(d_b), _ptr(d_c), _ptr(d_skip),
+                _ptr(d_gate), _ptr(d_delta_bias), _ptr(d_y), _ptr(d_state_in), _ptr(d_state_out),
+                _ptr(d_slots), _ptr(d_lengths), _ptr(d_saved), _ptr(d_workspace), _stream(stream)))
+
+
+def ThunderFFT_state_scan(shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip=None, d_gate=None,
+                          d_delta_bias=None, d_state_in=None, d_state_out=None, d_slots=None,
+                          d_lengths=None, d_saved=None, d_workspace=None, stream=0) -> None:
+    """State space scan on values of ``shape`` (a StateShape): dt = softplus(delta + delta_bias),
+    h[t] = exp(dt a) h[t-1] + dt x b for each of a channel's states, y = (sum of c h + skip x)
+    silu(gate).  a is float32 [channels][order], skip and delta_bias float32 [channels] (None:
+    zeros); without a gate y is the sum.  The states before the first step (d_state_in) and after
+    the last (d_state_out, the same buffer if wanted) are float32 rows [channels][order], row b for
+    sequence b or row d_slots[b] (int32) of a pool; d_lengths (int32) ends each sequence early.
+    d_saved (shape.saved_bytes()) is kept for the backward call, d_workspace
+    (shape.workspace_bytes()) is scratch.  Synchronous."""
+    _state_scan(lib().thff_state_scan, shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip, d_gate,
+                d_delta_bias, d_state_in, d_state_out, d_slots, d_lengths, d_saved, d_workspace,
+                stream)
+
+
+def ThunderFFT_state_scan_async(shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip=None, d_gate=None,
+                                d_delta_bias=None, d_state_in=None, d_state_out=None, d_slots=None,
+                                d_lengths=None, d_saved=None, d_workspace=None, stream=0) -> None:
+    """As ThunderFFT_state_scan, but returns once the work is enqueued on ``stream``."""
+    _state_scan(lib().thff_state_scan_async, shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip, d_gate,
+                d_delta_bias, d_state_in, d_state_out, d_slots, d_lengths, d_saved, d_workspace,
+                stream)
+
+
+class _StateGradients(ctypes.Structure):
+    """thff_state_gradients: the arrays of a backward call."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "dy", "x", "delta", "a", "b", "c", "skip", "gate", "delta_bias", "saved", "dstate_out",
+        "lengths", "dx", "ddelta", "da", "db", "dc", "dskip", "dgate", "ddelta_bias", "dstate_in")]
+
+
+def _state_scan_backward(call, shape, d_dy, d_x, d_delta, d_a, d_b, d_c, d_saved, d_dx, d_ddelta, d_da,
+                         d_db, d_dc, d_skip, d_dskip, d_gate, d_dgate, d_delta_bias, d_ddelta_bias,
+                         d_dstate_out, d_dstate_in, d_lengths, d_workspace, stream):
+    arrays = _StateGradients(*map(_ptr, (
+        d_dy, d_x, d_delta, d_a, d_b, d_c, d_skip, d_gate, d_delta_bias, d_saved, d_dstate_out,
+        d_lengths, d_dx, d_ddelta, d_da, d_db, d_dc, d_dskip, d_dgate, d_ddelta_bias, d_dstate_in)))
+    _raise(call(shape, arrays, _ptr(d_workspace), _stream(stream)))
+
+
+def ThunderFFT_state_scan_backward(shape, d_dy, d_x, d_delta, d_a, d_b, d_c, d_saved, d_dx, d_ddelta,
+                                   d_da, d_db, d_dc, d_skip=None, d_dskip=None, d_gate=None,
+                                   d_dgate=None, d_delta_bias=None, d_ddelta_bias=None,
+                                   d_dstate_out=None, d_dstate_in=None, d_lengths=None,
+                                   d_workspace=None, stream=0) -> None:
+    """Gradients of ThunderFFT_state_scan from those by y (d_dy) and by the last states
+    (d_dstate_out, None: zero), by x, delta, b, c and the gate (d_dgate, where there is one) in the
+    shape's type, and by a, skip, the bias (the latter two None: not computed) and the first state
+    (None: not stored) in float32.  d_saved is what the forward call of the same shape and inputs
+    wrote.  Synchronous."""
+    _state_scan_backward(lib().thff_state_scan_backward, shape, d_dy, d_x, d_delta, d_a, d_b, d_c,
+                         d_saved, d_dx, d_ddelta, d_da, d_db, d_dc, d_skip, d_dskip, d_gate, d_dgate,
+                         d_delta_bias, d_ddelta_bias, d_dstate_out, d_dstate_in, d_lengths,
+                         d_workspace, stream)
+
+
+def ThunderFFT_state_scan_backward_async(shape, d_dy, d_x, d_delta, d_a, d_b, d_c, d_saved, d_dx,
+                                         d_ddelta, d_da, d_db, d_dc, d_skip=None, d_dskip=None,
+                                         d_gate=None, d_dgate=None, d_delta_bias=None,
+                                         d_ddelta_bias=None, d_dstate_out=None, d_dstate_in=None,
+                                         d_lengths=None, d_workspace=None, stream=0) -> None:
+    """As ThunderFFT_state_scan_backward, but returns once the work is enqueued."""
+    _state_scan_backward(lib().thff_state_scan_backward_async, shape, d_dy, d_x, d_delta, d_a, d_b,
+                         d_c, d_saved, d_dx, d_ddelta, d_da, d_db, d_dc, d_skip, d_dskip, d_gate,
+                         d_dgate, d_delta_bias, d_ddelta_bias, d_dstate_out, d_dstate_in, d_lengths,
+                         d_workspace, stream)
+
+
+def _rms_norm(call, T, d_x, d_weight, eps, d_y, rows, cols, d_residual, d_sum, d_rstd, x_stride,
+              residual_stride, y_stride, sum_stride, stream):
+    _raise(call(_value_type(T), _ptr(d_x), x_stride or 0, _ptr(d_residual), residual_stride or 0,
+                _ptr(d_weight), eps, _ptr(d_y), y_stride or 0, _ptr(d_sum), sum_stride or 0,
+                _ptr(d_rstd), rows, _int(cols), _stream(stream)))
+
+
+def ThunderFFT_rms_norm(T, d_x, d_weight, eps, d_y, rows, cols, d_residual=None, d_sum=None,
+                        d_rstd=None, x_stride=None, residual_stride=None, y_stride=None,
+                        sum_stride=None, stream=0) -> None:
+    """Root-mean-square norm y = s rstd weight of `rows` rows of `cols` values of type T, with
+    s = x + d_residual rounded to T (None: s = x), which goes to d_sum (the residual's own buffer if
+    wanted; None: not stored); weight float32 (None: ones); d_rstd (float32, one a row) keeps the
+    statistics for the backward call.  Synchronous."""
+    _rms_norm(lib().thff_rms_norm, T, d_x, d_weight, eps, d_y, rows, cols, d_residual, d_sum, d_rstd,
+              x_stride, residual_stride, y_stride, sum_stride, stream)
+
+
+def ThunderFFT_rms_norm_async(T, d_x, d_weight, eps, d_y, rows, cols, d_residual=None, d_sum=None,
+                              d_rstd=None, x_stride=None, residual_stride=None, y_stride=None,
+                              sum_stride=None, stream=0) -> None:
+    """As ThunderFFT_rms_norm, but returns once the launch is enqueued on ``stream``."""
+    _rms_norm(lib().thff_rms_norm_async, T, d_x, d_weight, eps, d_y, rows, cols, d_residual, d_sum,
+              d_rstd, x_stride, residual_stride, y_stride, sum_stride, stream)
+
+
+def _rms_norm_8bit(call, T, d_x, d_weight, eps, d_q, d_scales, rows, cols, block, d_residual, d_sum,
+                   x_stride, residual_stride, q_stride, sum_stride, stream):
+    _raise(call(_value_type(T), _ptr(d_x), x_stride or 0, _ptr(d_residual), residual_stride or 0,
+                _ptr(d_weight), eps, _ptr(d_q), q_stride or 0, _ptr(d_scales), _int(block),
+                _ptr(d_sum), sum_stride or 0, rows, _int(cols), _stream(stream)))
+
+
+def ThunderFFT_rms_norm_8bit(T, d_x, d_weight, eps, d_q, d_scales, rows, cols, block=128,
+                             d_residual=None, d_sum=None, x_stride=None, residual_stride=None,
+                             q_stride=None, sum_stride=None, stream=0) -> None:
+    """As ThunderFFT_rms_norm, with an output of 8 bits (e4m3, torch.float8_e4m3fn) and a float32
+    scale for every `block` columns of a row (128, or cols): y is near d_q * scale, the scale the
+    largest |y| of the block / 448.  Synchronous."""
+    _rms_norm_8bit(lib().thff_rms_norm_8bit, T, d_x, d_weight, eps, d_q, d_scales, rows, cols, block,
+                   d_residual, d_sum, x_stride, residual_stride, q_stride, sum_stride, stream)
+
+
+def ThunderFFT_rms_norm_8bit_async(T, d_x, d_weight, eps, d_q, d_scales, rows, cols, block=128,
+                                   d_residual=None, d_sum=None, x_stride=None, residual_stride=None,
+                                   q_stride=None, sum_stride=None, stream=0) -> None:
+    """As ThunderFFT_rms_norm_8bit, but returns once the launch is enqueued on ``stream``."""
+    _rms_norm_8bit(lib().thff_rms_norm_8bit_async, T, d_x, d_weight, eps, d_q, d_scales, rows, cols,
+                   block, d_residual, d_sum, x_stride, residual_stride, q_stride, sum_stride, stream)
+
+
+def rms_norm_workspace_bytes(rows: int, cols: int) -> int:
+    """Bytes of ThunderFFT_rms_norm_backward's d_workspace."""
+    return _bytes(lib().thff_rms_norm_workspace_bytes(int(rows), _int(int(cols))))
+
+
+def _rms_norm_backward(call, T, d_dy, d_sum, d_rstd, d_weight, d_dx, d_dweight, d_workspace, rows, cols,
+                       d_dsum, dy_stride, sum_stride, dsum_stride, dx_stride, stream):
+    _raise(call(_value_type(T), _ptr(d_dy), dy_stride or 0, _ptr(d_sum), sum_stride or 0, _ptr(d_rstd),
+                _ptr(d_weight), _ptr(d_dsum), dsum_stride or 0, _ptr(d_dx), dx_stride or 0,
+                _ptr(d_dweight), _ptr(d_workspace), rows, _int(cols), _stream(stream)))
+
+
+def ThunderFFT_rms_norm_backward(T, d_dy, d_sum, d_rstd, d_weight, d_dx, d_dweight, d_workspace, rows,
+                                 cols, d_dsum=None, dy_stride=None, sum_stride=None, dsum_stride=None,
+                                 dx_stride=None, stream=0) -> None:
+    """Gradients of ThunderFFT_rms_norm by x (the residual's is the same) and, in float32, by the
+    weight (None: not computed), from that by y (d_dy), the one that reaches the sums from elsewhere
+    (d_dsum, None: zero), the sums (x itself without a residual) and the forward call's statistics.
+    Synchronous."""
+    _rms_norm_backward(lib().thff_rms_norm_backward, T, d_dy, d_sum, d_rstd, d_weight, d_dx, d_dweight,
+                       d_workspace, rows, cols, d_dsum, dy_stride, sum_stride, dsum_stride, dx_stride,
+                       stream)
+
+
+def ThunderFFT_rms_norm_backward_async(T, d_dy, d_sum, d_rstd, d_weight, d_dx, d_dweight, d_workspace,
+                                       rows, cols, d_dsum=None, dy_stride=None, sum_stride=None,
+                                       dsum_stride=None, dx_stride=None, stream=0) -> None:
+    """As ThunderFFT_rms_norm_backward, but returns once the work is enqueued."""
+    _rms_norm_backward(lib().thff_rms_norm_backward_async, T, d_dy, d_sum, d_rstd, d_weight, d_dx,
+                       d_dweight, d_workspace, rows, cols, d_dsum, dy_stride, sum_stride, dsum_stride,
+                       dx_stride, stream)
+
+
 def gated_scan(x, gate, state=None, lengths=None, layout="channels_last"):
     """(y, last states) of the gated linear recurrence on CUDA tensors, differentiable by x,
     gate and state: see thunderfft_amd.sequence.gated_scan."""
@@ -437,6 +746,38 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     from . import sequence
 
     return sequence.layer_norm(x, weight, bias, eps)
+
+
+def short_conv(x, weight, bias=None, state=None, lengths=None, silu: bool = True):
+    """(y, last state) of the short causal convolution on CUDA tensors, differentiable by x, weight,
+    bias and state: see thunderfft_amd.block.short_conv."""
+    from . import block
+
+    return block.short_conv(x, weight, bias, state, lengths, silu)
+
+
+def state_scan(x, delta, a, b, c, skip=None, gate=None, delta_bias=None, state=None, lengths=None):
+    """(y, last states) of the state space scan on CUDA tensors, differentiable by all its floating
+    arguments: see thunderfft_amd.block.state_scan."""
+    from . import block
+
+    return block.state_scan(x, delta, a, b, c, skip, gate, delta_bias, state, lengths)
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
+    """Root-mean-square norm of a CUDA tensor's last axis, with a residual (y, x + residual),
+    differentiable by x, weight and residual: see thunderfft_amd.block.rms_norm."""
+    from . import block
+
+    return block.rms_norm(x, weight, residual, eps)
+
+
+def rms_norm_8bit(x, weight=None, residual=None, eps: float = 1e-5, block: int | None = 128):
+    """(q, scales) of the norm in 8 bits, with a residual (q, scales, x + residual): see
+    thunderfft_amd.block.rms_norm_8bit."""
+    from . import block as operators
+
+    return operators.rms_norm_8bit(x, weight, residual, eps, block)
 
 
 def twiddle_info(T) -> tuple[int, int]:

@@ -5,8 +5,8 @@
 Every kernel translation unit is compiled for gfx950 only, with packed FP32
 instructions disabled (-Xclang -target-feature -Xclang -packed-fp32-ops) and
 MFMA results kept in VGPRs (-mllvm -amdgpu-mfma-vgpr-form).  The
-per-length kernel file is compiled once per transform length so the lengths
-build in parallel.  Objects go to thunderfft_amd/_build/, the shared library
+per-length kernel file is compiled once per transform length, and the state
+space scan once per type of values, so that they build in parallel.  Objects go to thunderfft_amd/_build/, the shared library
 to thunderfft_amd/libthunderfft_amd.so (loaded by thunderfft_amd/__init__.py).
 """
 from __future__ import annotations
@@ -50,9 +50,12 @@ def units() -> list[tuple[str, str, list[str]]]:
     for n in LENGTHS:
         out.append((os.path.join(CSRC, "c2c_instance.hip"), os.path.join(BUILD, f"c2c_n{n}.o"),
                     [f"-DTHFF_N={n}"]))
-    for name in ("fill", "scan", "norm"):
+    for name in ("float", "half_t", "bfloat_t"):
+        out.append((os.path.join(CSRC, "state_instance.hip"), os.path.join(BUILD, f"state_{name}.o"),
+                    [f"-DTHFF_STATE_TYPE={name}"]))
+    for name in ("rms_norm", "fill", "scan", "norm", "short_conv", "state_scan"):
         out.append((os.path.join(CSRC, name + ".hip"), os.path.join(BUILD, name + ".o"), []))
-    for name in ("capi", "capi_sequence"):
+    for name in ("capi", "capi_sequence", "capi_block"):
         out.append((os.path.join(CSRC, name + ".cpp"), os.path.join(BUILD, name + ".o"),
                     ["-x", "hip"]))
     return out

@@ -2,34 +2,14 @@
 // include/thunderfft/thunderfft.h: argument checks, all before any HIP call, and dispatch.
 #include <hip/hip_runtime.h>
 
-#include <cstdint>
 #include <string>
 
-#include "errors.hpp"
+#include "capi_checks.hpp"
 #include "sequence.hpp"
-#include "thunderfft/thunderfft.h"
 
 namespace {
 
-using thff::fail;
-using thff::fail_hip;
-using thff::ScanShape;
-
-constexpr int kMostSize = 1 << 30;
-// Elements of a strided buffer: byte offsets stay within 63 bits.
-constexpr __int128 kMostSpan = static_cast<__int128>(1) << 60;
-
-bool value_type(int p) { return p == THFF_FLOAT || p == THFF_HALF || p == THFF_BFLOAT16; }
-
-bool aligned(const void* p, unsigned bytes) {
-    return reinterpret_cast<std::uintptr_t>(p) % bytes == 0;
-}
-
-// Fills a stride of 0 in; false: rows of `length` would overlap, or the offsets overflow.
-bool stride_of(long long given, long long length, long long rows, long long* stride) {
-    *stride = given ? given : length;
-    return *stride >= length && static_cast<__int128>(rows) * *stride <= kMostSpan;
-}
+using namespace thff;
 
 int check_shape(const thff_scan_shape* shape, ScanShape* out) {
     if (!shape) return fail(THFF_EINVAL, "thff_scan_shape is null");
@@ -54,15 +34,6 @@ int check_shape(const thff_scan_shape* shape, ScanShape* out) {
     if (!thff::scan_fits(*out))
         return fail(THFF_EINVAL, "ThunderFFT_gated_scan shape exceeds one launch");
     return THFF_OK;
-}
-
-unsigned element_bytes(int precision) { return precision == THFF_FLOAT ? 4 : 2; }
-
-int finish(hipError_t err, hipStream_t s, bool synchronize, const char* who) {
-    if (err != hipSuccess) return fail_hip(err, who);
-    if (!synchronize) return THFF_OK;
-    err = hipStreamSynchronize(s);
-    return err == hipSuccess ? THFF_OK : fail_hip(err, who);
 }
 
 int scan_impl(const thff_scan_shape* shape, const void* x, const void* gate, void* y,
@@ -243,16 +214,6 @@ int norm_backward_impl(int precision, const void* dy, long long dy_stride, const
     auto st = static_cast<hipStream_t>(stream);
     return finish(thff::launch_layer_norm_backward(a, st), st, synchronize,
                   "ThunderFFT_layer_norm_backward");
-}
-
-// Nothing is thrown through the C ABI (a message's allocation may fail).
-template <class F>
-auto guarded(F f) noexcept -> decltype(f()) {
-    try {
-        return f();
-    } catch (...) {
-        return THFF_EIO;
-    }
 }
 
 }  // namespace

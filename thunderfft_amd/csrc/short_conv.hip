@@ -1,0 +1,396 @@
+// short_conv.hip -- short causal convolution per channel, K = 2 to 4 taps: with xe the K - 1 values
+// of the state and then x,
+//   p[t] = bias + sum_k weight[k] xe[t + k],  y[t] = p silu'd or p,
+// and its gradients: dp[t] = dy[t] slope(p[t]),
+//   dxe[e] = sum_k weight[k] dp[e - k]  (+ dstate_out behind the end),
+//   dweight[k] = sum_t dp[t] xe[t + k],  dbias = sum_t dp[t].
+//
+// A lane takes 16 bytes of channels and some steps one after the other, with the last K - 1 rows
+// in registers.
+#include <algorithm>
+
+#include "block.hpp"
+#include "sequence_io.hpp"
+
+namespace thff {
+namespace {
+
+constexpr int kLanes = 256;
+
+__device__ __forceinline__ int length_of(const int* lengths, int b, int n) {
+    return lengths ? min(max(lengths[b], 0), n) : n;
+}
+
+// 1 / (1 + exp(-v))
+__device__ __forceinline__ float opened(float v) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+}
+
+// Where a lane's V channels are: the last lane of a row takes the last V, `skip` of which are also
+// the lane's before it.
+struct Channels {
+    int at, skip;
+};
+
+template <int V>
+__device__ __forceinline__ Channels channels_of(int vector, int channels) {
+    return {min(vector * V, channels - V), max(0, vector * V + V - channels)};
+}
+
+// Stores values from the skip-th on: where the lane before stores its own, and may have read other
+// values for them (states kept in place).
+template <class T, int V>
+__device__ __forceinline__ void store_own(T* p, pack<T, V> v, int skip) {
+    if (skip == 0) {
+        store_pack<T, V>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i >= skip) p[i] = v[i];
+}
+
+// w[k][i]: tap k of channel i; and the bias.
+template <int V, int K>
+struct Taps {
+    float w[K][V], bias[V];
+
+    __device__ __forceinline__ Taps(const float* weight, const float* b, int at) {
+        const pack<float, V * K> all = load_pack<float, V * K>(weight + static_cast<long long>(at) * K);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[k][i] = all[i * K + k];
+#pragma unroll
+        for (int i = 0; i < V; ++i) bias[i] = b ? b[at + i] : 0.0f;
+    }
+};
+
+// Steps of a lane forward.
+constexpr int kSteps = 16;
+
+template <class T, int V, int K, int TS>
+__global__ __launch_bounds__(kLanes) void conv_forward(ConvShape s, ConvForward a, int vectors, long long tiles) {
+    constexpr int H = K - 1;
+    const long long lanes = s.batch * tiles * vectors;
+    for (long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x; i < lanes;
+         i += static_cast<long long>(gridDim.x) * kLanes) {
+        const long long column = i / vectors;
+        const Channels c = channels_of<V>(static_cast<int>(i - column * vectors), s.channels);
+        const int b = static_cast<int>(column / tiles), t0 = static_cast<int>(column - b * tiles) * TS;
+        const int length = length_of(a.lengths, b, s.n);
+        const T* x = static_cast<const T*>(a.x) + b * static_cast<long long>(s.n) * s.x_stride + c.at;
+        const Taps<V, K> taps(a.weight, a.bias, c.at);
+        pack<T, V> in[TS + H];
+        int slot = b;
+        if (t0 == 0) {
+            if (a.slots) slot = a.slots[b];
+            if (a.slots && (slot < 0 || slot >= s.states)) slot = -1;
+            const T* state = static_cast<const T*>(a.state_in) + static_cast<long long>(slot) * H * s.channels + c.at;
+#pragma unroll
+            for (int k = 0; k < H; ++k) {
+                in[k] = pack<T, V>{};
+                if (a.state_in && slot >= 0) in[k] = load_pack<T, V>(state + static_cast<long long>(k) * s.channels);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < H; ++k) in[k] = load_pack<T, V>(x + (t0 - H + k) * s.x_stride);
+        }
+        if (s.n > 0) {
+#pragma unroll
+            for (int j = 0; j < TS; ++j) in[H + j] = load_pack<T, V>(x + min(t0 + j, s.n - 1) * s.x_stride);
+        }
+        if (t0 == 0 && a.state_out && slot >= 0) {
+            // All of the old state is read before any of it is written.
+            pack<T, V> last[H];
+#pragma unroll
+            for (int k = 0; k < H; ++k) {
+                const int t = length - H + k;
+                if (t >= 0) {
+                    last[k] = load_pack<T, V>(x + t * s.x_stride);
+                } else {
+                    last[k] = in[0];
+#pragma unroll
+                    for (int m = 1; m < H; ++m)
+                        if (length + k == m) last[k] = in[m];
+                }
+            }
+            T* to = static_cast<T*>(a.state_out) + static_cast<long long>(slot) * H * s.channels + c.at;
+#pragma unroll
+            for (int k = 0; k < H; ++k)
+                store_own<T, V>(to + static_cast<long long>(k) * s.channels, last[k], c.skip);
+        }
+        T* y = static_cast<T*>(a.y) + b * static_cast<long long>(s.n) * s.y_stride + c.at;
+#pragma unroll
+        for (int j = 0; j < TS; ++j) {
+            if (t0 + j >= s.n) break;
+            pack<T, V> out;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float p = taps.bias[v];
+#pragma unroll
+                for (int k = 0; k < K; ++k) p = fmaf(taps.w[k][v], to_float<T>(in[j + k][v]), p);
+                if (s.silu) p *= opened(p);
+                out[v] = from_float<T>(t0 + j < length ? p : 0.0f);
+            }
+            store_own<T, V>(y + (t0 + j) * s.y_stride, out, c.skip);
+        }
+    }
+}
+
+// Steps of a lane backward, a multiple of kAhead; lanes of a workgroup along the channels; and the
+// workgroups that share a channel.
+struct ConvParts {
+    int steps, across;
+    int chunks;       // of a sequence, one a lane
+    long long count;  // parts of the weights' gradients
+};
+
+constexpr int kAhead = 8;  // rows loaded at a time
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(kLanes) void conv_backward(ConvShape s, ConvBackward a, int vectors, ConvParts g) {
+    constexpr int H = K - 1;
+    __shared__ float lds[V * (K + 1)][kLanes];
+    const int lane = threadIdx.x % g.across, row = threadIdx.x / g.across, rows = kLanes / g.across;
+    const int slabs = (vectors + g.across - 1) / g.across;
+    const long long part = blockIdx.x / slabs;
+    const int vector = static_cast<int>(blockIdx.x - part * slabs) * g.across + lane;
+    const long long chunk = part * rows + row;  // of all sequences
+    const bool on = vector < vectors && chunk < static_cast<long long>(s.batch) * g.chunks;
+    float dw[K][V] = {}, db[V] = {};
+    const Channels c = channels_of<V>(min(vector, vectors - 1), s.channels);
+    if (on) {
+        const int b = static_cast<int>(chunk / g.chunks), t0 = static_cast<int>(chunk - static_cast<long long>(b) * g.chunks) * g.steps;
+        const int length = length_of(a.lengths, b, s.n), t1 = min(t0 + g.steps, s.n);
+        const long long first = b * static_cast<long long>(s.n);
+        const T* x = static_cast<const T*>(a.x) + first * s.x_stride + c.at;
+        const T* dy = static_cast<const T*>(a.dy) + first * s.y_stride + c.at;
+        T* dx = static_cast<T*>(a.dx) + first * s.x_stride + c.at;
+        const long long state = static_cast<long long>(b) * H * s.channels + c.at;
+        const Taps<V, K> taps(a.weight, a.bias, c.at);
+        // xe[t ... t + K - 1] and dp[t - K + 1 ... t].
+        float xe[K][V] = {}, dp[K][V] = {};
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            pack<T, V> in = {};
+            if (t0 > 0) in = load_pack<T, V>(x + (t0 - H + k) * s.x_stride);
+            else if (a.state_in) in = load_pack<T, V>(static_cast<const T*>(a.state_in) + state + static_cast<long long>(k) * s.channels);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                xe[k + 1][v] = t0 == 0 || t0 - H + k < length ? to_float<T>(in[v]) : 0.0f;
+        }
+        const int end = t1 + H;
+        for (int t = t0; t < end; t += kAhead) {
+            pack<T, V> xs[kAhead], ds[kAhead];
+            if (s.n > 0) {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const long long at = min(t + j, s.n - 1);
+                    xs[j] = load_pack<T, V>(x + at * s.x_stride);
+                    ds[j] = load_pack<T, V>(dy + at * s.y_stride);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int e = t + j;
+                if (e >= end) break;
+                const bool inside = e < length;
+                pack<T, V> out, after = {};
+                const bool behind = a.dstate_out && e >= length && e < length + H;
+                if (behind)
+                    after = load_pack<T, V>(static_cast<const T*>(a.dstate_out) + state + static_cast<long long>(e - length) * s.channels);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+#pragma unroll
+                    for (int k = 0; k < H; ++k) {
+                        xe[k][v] = xe[k + 1][v];
+                        dp[k][v] = dp[k + 1][v];
+                    }
+                    xe[H][v] = inside ? to_float<T>(xs[j][v]) : 0.0f;
+                    float p = taps.bias[v];
+#pragma unroll
+                    for (int k = 0; k < K; ++k) p = fmaf(taps.w[k][v], xe[k][v], p);
+                    float d = to_float<T>(ds[j][v]);
+                    if (s.silu) {
+                        const float f = opened(p);
+                        d *= fmaf(f * (1.0f - f), p, f);
+                    }
+                    d = inside ? d : 0.0f;
+                    dp[H][v] = d;
+                    if (e < t1) {
+#pragma unroll
+                        for (int k = 0; k < K; ++k) dw[k][v] = fmaf(d, xe[k][v], dw[k][v]);
+                        db[v] += d;
+                    }
+                    float sum = to_float<T>(after[v]);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) sum = fmaf(taps.w[k][v], dp[H - k][v], sum);
+                    out[v] = from_float<T>(e - H < length ? sum : 0.0f);
+                }
+                if (e - H >= t0) store_pack<T, V>(dx + (e - H) * s.x_stride, out);
+                else if (t0 == 0 && a.dstate_in) store_pack<T, V>(static_cast<T*>(a.dstate_in) + state + static_cast<long long>(e) * s.channels, out);
+            }
+        }
+    }
+    if (!a.dweight && !a.dbias) return;
+    // The sums of the workgroup's rows, halving their number.
+    for (int half = rows / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (row >= half && row < 2 * half) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) lds[v * (K + 1) + k][threadIdx.x] = dw[k][v];
+                lds[v * (K + 1) + K][threadIdx.x] = db[v];
+            }
+        }
+        __syncthreads();
+        if (row < half) {
+            const int from = threadIdx.x + half * g.across;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) dw[k][v] += lds[v * (K + 1) + k][from];
+                db[v] += lds[v * (K + 1) + K][from];
+            }
+        }
+    }
+    if (row == 0 && vector < vectors) {
+        // workspace[part][tap, the last the bias][channel]
+        float* to = a.workspace + part * (K + 1) * s.channels + c.at;
+#pragma unroll
+        for (int k = 0; k <= K; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v >= c.skip) to[static_cast<long long>(k) * s.channels + v] = k < K ? dw[k < K ? k : 0][v] : db[v];
+    }
+}
+
+// Adds the parts of 32 sums: 32 lanes a sum, each every 32nd part.  Sums lie as [tap][channel].
+__global__ __launch_bounds__(1024) void conv_add_parts(const float* parts, long long count, int channels, int width,
+                                                       float* dweight, float* dbias) {
+    __shared__ float lds[32][33];
+    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+    const long long sums = static_cast<long long>(width + 1) * channels;
+    for (long long first = 32LL * blockIdx.x; first < sums; first += 32LL * gridDim.x) {
+        float sum = 0.0f;
+        if (first + lane < sums)
+            for (long long k = group; k < count; k += 32) sum += parts[k * sums + first + lane];
+        __syncthreads();
+        lds[group][lane] = sum;
+        __syncthreads();
+        sum = lds[lane][group];
+#pragma unroll
+        for (int m = 1; m < 32; m *= 2) sum += __shfl_xor(sum, m);
+        const long long at = first + group;
+        if (lane == 0 && at < sums) {
+            const long long tap = at / channels, c = at - tap * channels;
+            if (tap < width) {
+                if (dweight) dweight[c * width + tap] = sum;
+            } else if (dbias) {
+                dbias[c] = sum;
+            }
+        }
+    }
+}
+
+template <class F>
+auto with_type(int precision, F f) {
+    if (precision == THFF_FLOAT) return f(float{});
+    if (precision == THFF_HALF) return f(half_t{});
+    return f(bfloat_t{});
+}
+
+template <int V_, int K_>
+struct Kind {
+    static constexpr int V = V_, K = K_;
+};
+
+// 16 bytes of channels a lane; fewer channels than that, one.
+template <class T, class F>
+auto with_kind(const ConvShape& s, F f) {
+    constexpr int V = 16 / sizeof(T);
+    if (s.channels < V) {
+        if (s.width == 2) return f(Kind<1, 2>{});
+        if (s.width == 3) return f(Kind<1, 3>{});
+        return f(Kind<1, 4>{});
+    }
+    if (s.width == 2) return f(Kind<V, 2>{});
+    if (s.width == 3) return f(Kind<V, 3>{});
+    return f(Kind<V, 4>{});
+}
+
+int vectors_of(const ConvShape& s, int v) { return (s.channels + v - 1) / v; }
+
+ConvParts parts_of(const ConvShape& s, int v) {
+    constexpr long long kWanted = 1 << 17;  // lanes
+    ConvParts g;
+    const int vectors = vectors_of(s, v);
+    g.across = 1;
+    while (g.across < 64 && g.across < vectors) g.across *= 2;
+    const long long steps = static_cast<long long>(s.batch) * s.n * vectors / kWanted;
+    g.steps = static_cast<int>(std::min<long long>(std::max<long long>(steps, 32), 1 << 20)) / kAhead * kAhead;
+    g.chunks = std::max(1, static_cast<int>((s.n + static_cast<long long>(g.steps) - 1) / g.steps));
+    const int rows = kLanes / g.across;
+    g.count = (static_cast<long long>(s.batch) * g.chunks + rows - 1) / rows;
+    return g;
+}
+
+template <class T, int V, int K, int TS>
+hipError_t launch_forward(const ConvShape& s, const ConvForward& a, hipStream_t stream) {
+    const int vectors = vectors_of(s, V);
+    const long long tiles = std::max<long long>(1, (s.n + TS - 1LL) / TS);
+    const __int128 lanes = static_cast<__int128>(s.batch) * tiles * vectors;
+    const long long blocks = static_cast<long long>(std::min<__int128>((lanes + kLanes - 1) / kLanes, 1 << 23));
+    conv_forward<T, V, K, TS><<<static_cast<unsigned>(blocks), kLanes, 0, stream>>>(s, a, vectors, tiles);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+long long conv_workspace_bytes(const ConvShape& s) {
+    if (s.batch == 0 || s.n == 0 || s.channels == 0) return 0;
+    const long long parts = with_type(s.precision, [&](auto v) {
+        return with_kind<decltype(v)>(s, [&](auto kind) { return parts_of(s, decltype(kind)::V).count; });
+    });
+    return 4 * parts * (s.width + 1) * s.channels;
+}
+
+hipError_t launch_short_conv(const ConvShape& s, const ConvForward& a, hipStream_t stream) {
+    return with_type(s.precision, [&](auto v) {
+        using T = decltype(v);
+        return with_kind<T>(s, [&](auto kind) {
+            using Q = decltype(kind);
+            if (s.n <= 1) return launch_forward<T, Q::V, Q::K, 1>(s, a, stream);
+            return launch_forward<T, Q::V, Q::K, kSteps>(s, a, stream);
+        });
+    });
+}
+
+hipError_t launch_short_conv_backward(const ConvShape& s, const ConvBackward& a, hipStream_t stream) {
+    return with_type(s.precision, [&](auto v) {
+        using T = decltype(v);
+        return with_kind<T>(s, [&](auto kind) {
+            using Q = decltype(kind);
+            const int vectors = vectors_of(s, Q::V);
+            const ConvParts g = parts_of(s, Q::V);
+            const bool none = s.batch == 0 || s.n == 0;
+            ConvBackward call = a;
+            if (none) call.dweight = call.dbias = nullptr;
+            if (s.batch > 0) {
+                const long long slabs = (vectors + g.across - 1) / g.across;
+                conv_backward<T, Q::V, Q::K>
+                    <<<static_cast<unsigned>(g.count * slabs), kLanes, 0, stream>>>(s, call, vectors, g);
+            }
+            if (a.dweight || a.dbias) {
+                const long long sums = static_cast<long long>(s.width + 1) * s.channels;
+                conv_add_parts<<<static_cast<unsigned>(std::min<long long>((sums + 31) / 32, 1 << 20)), 1024, 0, stream>>>(
+                    a.workspace, none ? 0 : g.count, s.channels, s.width, a.dweight, a.dbias);
+            }
+            return hipGetLastError();
+        });
+    });
+}
+
+}  // namespace thff

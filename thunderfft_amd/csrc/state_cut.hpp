@@ -1,0 +1,70 @@
+// state_cut.hpp -- how the state space scan is cut into workgroups, and what its translation units
+// (state_instance.hip, one for each type of values) offer.
+#pragma once
+
+#include "block.hpp"
+
+namespace thff {
+
+constexpr int kStateWaves = 4;
+constexpr int kStateBlock = 32;  // steps whose b and c are in LDS at a time, forward
+constexpr int kStateTile = 16;   // steps between saved states, and of the backward pass at a time
+
+// S states of a channel on each of LPC neighbouring lanes.
+template <int S_, int LPC_>
+struct Lanes {
+    static constexpr int S = S_, LPC = LPC_, P = S * LPC, kWave = 64 / LPC, kSlab = kStateWaves * kWave;
+};
+
+// Calls f with how lanes share a channel of `order` states.
+template <class F>
+auto with_lanes(int order, F f) {
+    if (order <= 4) return f(Lanes<1, 4>{});
+    if (order <= 8) return f(Lanes<2, 4>{});
+    if (order <= 16) return f(Lanes<4, 4>{});
+    if (order <= 32) return f(Lanes<4, 8>{});
+    return f(Lanes<4, 16>{});
+}
+
+// Slabs of the channels of a group, segments of the steps.
+struct Cut {
+    int slabs, segments, steps;  // steps of a segment, a multiple of kStateBlock
+    int padded;                  // states of a channel in saved and workspace
+    long long blocks;
+};
+
+// Workspace of the segments, for each sequence and segment: the end of the segment before it
+// (segment 0: the given state) as padded rows of states a channel, and its own sums of dt; the
+// backward pass has the gradient that leaves the segment instead.
+struct Ends {
+    float *states, *sums;
+    __host__ __device__ Ends(float* workspace, const StateShape& s, const Cut& cut)
+        : states(workspace),
+          sums(workspace + static_cast<long long>(s.batch) * cut.segments * s.channels * cut.padded) {}
+    static __device__ __forceinline__ long long row(const StateShape& s, const Cut& cut, int b, int segment,
+                                                    int channel) {
+        return (static_cast<long long>(b) * cut.segments + segment) * s.channels + channel;
+    }
+};
+
+// Behind those: db and dc of a slab's channels, [slab][b][t][group][b's, c's] in padded rows; da,
+// [b and segment][channel] in padded rows; dskip and ddelta_bias, two values for each b, segment
+// and channel.
+struct Parts {
+    long long shared, da, pairs, count;  // offsets in floats; parts of da
+
+    __host__ __device__ Parts(const StateShape& s, const Cut& cut) {
+        count = static_cast<long long>(s.batch) * cut.segments;
+        shared = cut.segments > 1 ? (count * s.channels * (cut.padded + 1) + 3) / 4 * 4 : 0;
+        da = shared + static_cast<long long>(cut.slabs) * s.batch * s.n * s.groups * 2 * cut.padded;
+        pairs = da + count * s.channels * cut.padded;
+    }
+    long long bytes(const StateShape& s) const { return 4 * (pairs + count * s.channels * 2); }
+};
+
+template <class T>
+hipError_t launch_state_forward(const StateShape& s, const StateForward& a, const Cut& cut, hipStream_t stream);
+template <class T>
+hipError_t launch_state_backward(const StateShape& s, const StateBackward& a, const Cut& cut, hipStream_t stream);
+
+}  // namespace thff

@@ -1,0 +1,80 @@
+// state_instance.hip -- the state space scan for one type of values, THFF_STATE_TYPE.
+#include "state_kernels.hpp"
+
+namespace thff {
+namespace {
+
+dim3 grid_of(long long blocks) {
+    // A launch has less than 2^32 lanes along x, so many workgroups take rows of a grid.
+    constexpr long long kMost = 1LL << 21;
+    return dim3(static_cast<unsigned>(std::min(blocks, kMost)), static_cast<unsigned>((blocks + kMost - 1) / kMost));
+}
+
+// Lanes of a channel for one step.
+template <class F>
+auto with_step_lanes(int order, F f) {
+    if (order <= 4) return f(std::integral_constant<int, 1>{});
+    if (order <= 8) return f(std::integral_constant<int, 2>{});
+    if (order <= 16) return f(std::integral_constant<int, 4>{});
+    if (order <= 32) return f(std::integral_constant<int, 8>{});
+    return f(std::integral_constant<int, 16>{});
+}
+
+}  // namespace
+
+template <class T>
+hipError_t launch_state_forward(const StateShape& s, const StateForward& a, const Cut& cut, hipStream_t stream) {
+    // A single step that saves nothing.
+    if (s.n == 1 && !a.saved)
+        return with_step_lanes(s.order, [&](auto lanes) {
+            constexpr int N = decltype(lanes)::value;
+            const long long count = static_cast<long long>(s.batch) * s.channels * N;
+            state_step<T, N><<<grid_of((count + kLanes - 1) / kLanes), kLanes, 0, stream>>>(s, a);
+            return hipGetLastError();
+        });
+    return with_lanes(s.order, [&](auto lanes) {
+        using L = decltype(lanes);
+        if (cut.segments > 1) {
+            state_forward<T, L, true><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+            const hipError_t err = hipGetLastError();
+            if (err != hipSuccess) return err;
+        }
+        state_forward<T, L, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+        return hipGetLastError();
+    });
+}
+
+template <class T>
+hipError_t launch_state_backward(const StateShape& s, const StateBackward& a, const Cut& cut, hipStream_t stream) {
+    return with_lanes(s.order, [&](auto lanes) {
+        using L = decltype(lanes);
+        if (s.batch > 0) {
+            if (cut.segments > 1) {
+                state_backward<T, L, true><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+                const hipError_t err = hipGetLastError();
+                if (err != hipSuccess) return err;
+            }
+            state_backward<T, L, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+            hipError_t err = hipGetLastError();
+            if (err != hipSuccess) return err;
+            const long long shared = static_cast<long long>(s.batch) * s.n * s.groups * 2 * cut.padded;
+            if (shared > 0) {
+                const long long blocks = std::min((shared + kLanes - 1) / kLanes, 1LL << 20);
+                add_shared<T><<<static_cast<unsigned>(blocks), kLanes, 0, stream>>>(s, a, cut);
+                err = hipGetLastError();
+                if (err != hipSuccess) return err;
+            }
+        }
+        const long long sums = static_cast<long long>(s.channels) * (cut.padded + 2);
+        add_weights<<<static_cast<unsigned>(std::min((sums + 31) / 32, 1LL << 20)), 1024, 0, stream>>>(
+            s, a, cut, static_cast<long long>(s.batch) * cut.segments);
+        return hipGetLastError();
+    });
+}
+
+template hipError_t launch_state_forward<THFF_STATE_TYPE>(const StateShape&, const StateForward&, const Cut&,
+                                                          hipStream_t);
+template hipError_t launch_state_backward<THFF_STATE_TYPE>(const StateShape&, const StateBackward&, const Cut&,
+                                                           hipStream_t);
+
+}  // namespace thff

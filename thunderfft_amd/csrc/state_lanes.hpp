@@ -1,0 +1,157 @@
+// state_lanes.hpp -- how the lanes of a wave share the state space scan: LPC neighbouring lanes
+// have a channel, S states each, and the wave 64 / LPC channels.  A lane also has one of every LPC
+// steps of its channel, whose values it loads and whose sums over the states it ends up with.
+#pragma once
+
+#include "sequence_io.hpp"
+
+namespace thff {
+
+constexpr float kLog2e = 1.44269504f;
+
+template <int Control>
+__device__ __forceinline__ float moved(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), Control, 0xf, 0xf, true));
+}
+
+// The value of the K-th lane of each LPC, on all of them.
+template <int LPC, int K>
+__device__ __forceinline__ float from_lane(float v) {
+    static_assert(LPC == 4 || LPC == 8 || LPC == 16, "4, 8 or 16 lanes a channel");
+    if constexpr (LPC == 4) {
+        return moved<K * 0x55>(v);
+    } else if constexpr (LPC == 8) {
+        const int low = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + K, 0xf, 0xf, true);
+        return __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(v), 0x158 + K, 0xf, 0xc, false));
+    } else {
+        return moved<0x150 + K>(v);
+    }
+}
+
+// The value of the lane mirrored within N lanes.
+template <int N>
+__device__ __forceinline__ float mirrored(float v) {
+    return moved<N == 16 ? 0x140 : N == 8 ? 0x141 : N == 4 ? 0x1b : 0xb1>(v);
+}
+
+// Sums of v[k] over each LPC lanes: that of v[k] on the k-th lane.
+template <int LPC>
+__device__ __forceinline__ float sum_to_lanes(float (&v)[LPC], int lane) {
+    if constexpr (LPC >= 16) {
+        const bool high = lane & 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = (high ? v[k + 8] : v[k]) + mirrored<16>(high ? v[k] : v[k + 8]);
+    }
+    if constexpr (LPC >= 8) {
+        const bool high = lane & 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (high ? v[k + 4] : v[k]) + mirrored<8>(high ? v[k] : v[k + 4]);
+    }
+    const bool two = lane & 2, one = lane & 1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) v[k] = (two ? v[k + 2] : v[k]) + mirrored<4>(two ? v[k] : v[k + 2]);
+    return (one ? v[1] : v[0]) + mirrored<2>(one ? v[0] : v[1]);
+}
+
+// Adds the lanes whose bit `Bit` differs: 2^Bit lanes away.
+template <int Bit>
+__device__ __forceinline__ float sum_across(float v) {
+    if constexpr (Bit == 5) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else if constexpr (Bit == 4) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else if constexpr (Bit == 3) {
+        return v + moved<0x128>(v);
+    } else {
+        // 4 lanes on for the lower half of every 8, 4 back for the upper one.
+        static_assert(Bit == 2, "channels begin at 4 lanes at least");
+        const int up = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x104, 0xf, 0x5, false);
+        return v + __int_as_float(__builtin_amdgcn_update_dpp(up, __float_as_int(v), 0x114, 0xf, 0xa, false));
+    }
+}
+
+// Sums of one and two over the lanes whose bit `Bit` differs: one's where the bit is 0, two's where
+// it is 1.
+template <int Bit>
+__device__ __forceinline__ float sum_apart(float one, float two, int lane) {
+    if constexpr (Bit == 5) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(one), __float_as_uint(two), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else if constexpr (Bit == 4) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(one), __float_as_uint(two), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+        static_assert(Bit == 3, "bits 5, 4 and 3");
+        const bool high = lane & 8;
+        return (high ? two : one) + moved<0x128>(high ? one : two);
+    }
+}
+
+// Sums of v[0 ... N) over the channels of a wave, whose lanes have bits 5 down to log2(LPC).  With
+// each bit the values halve while there are several; v[0 ...) are then those from
+// channel_sum_first(lane) on, the same ones on lanes that differ in the bits left.
+template <int LPC, int N, int Bit = 5>
+__device__ __forceinline__ void channel_sums(float* v, int lane) {
+    if constexpr ((1 << Bit) >= LPC) {
+        if constexpr (N > 1) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) v[i] = sum_apart<Bit>(v[i], v[i + N / 2], lane);
+            channel_sums<LPC, N / 2, Bit - 1>(v, lane);
+        } else {
+            v[0] = sum_across<Bit>(v[0]);
+            channel_sums<LPC, 1, Bit - 1>(v, lane);
+        }
+    }
+}
+
+// What is left of N values a lane, where the first of them belongs, and whether the lane is the one
+// of its likes that stores them.
+template <int LPC, int N>
+struct ChannelSums {
+    static constexpr int kBits = LPC == 4 ? 4 : LPC == 8 ? 3 : 2;
+    static constexpr int log2(int n) { return n == 1 ? 0 : 1 + log2(n / 2); }
+    static constexpr int kApart = log2(N) < kBits ? log2(N) : kBits;  // bits that tell values apart
+    static constexpr int kLeft = N >> kApart;
+
+    static __device__ __forceinline__ int first(int lane) {
+        int at = 0;
+#pragma unroll
+        for (int k = 0; k < kApart; ++k) at += (lane >> (5 - k) & 1) * (N >> (k + 1));
+        return at;
+    }
+    static __device__ __forceinline__ bool stores(int lane) {
+        constexpr int kSame = ((1 << (kBits - kApart)) - 1) * LPC;
+        return (lane & kSame) == 0;
+    }
+};
+
+// log(1 + exp(v)) by exp(-|v|) and log(1 + e) = 2 atanh(s) with s = e / (2 + e) <= 1/3, whose series
+// is cut where it is 2e-9 of the first term; and its slope, 1 / (1 + exp(-v)).
+__device__ __forceinline__ float softplus(float v) {
+    const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(v));
+    const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+    float p = fmaf(q, 1.0f / 15, 1.0f / 13);
+    p = fmaf(q, p, 1.0f / 11);
+    p = fmaf(q, p, 1.0f / 9);
+    p = fmaf(q, p, 1.0f / 7);
+    p = fmaf(q, p, 1.0f / 5);
+    p = fmaf(q, p, 1.0f / 3);
+    p = fmaf(q, p, 1.0f);
+    return __builtin_elementwise_maximum(v, 0.0f) + 2.0f * s * p;
+}
+
+__device__ __forceinline__ float opened(float v) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
+}
+
+template <int N, class F, int K = 0>
+__device__ __forceinline__ void each_step(F f) {
+    if constexpr (K < N) {
+        f(std::integral_constant<int, K>{});
+        each_step<N, F, K + 1>(f);
+    }
+}
+
+}  // namespace thff
