@@ -426,8 +426,9 @@ int thff_short_conv_backward_async(const thff_conv_shape* shape, const void* d_d
 
 /* State space scan.  order: states of a channel, 1 to 64.  groups divide the channels:
  * channel c has row c / (channels / groups) of b and c, which are [batch][n][groups][order].
- * Each stride holds for the gradient of its array too.  Sizes at most 2^30, batch *
- * channels at most 2^31 - 256 (THFF_EINVAL too where a call has too many workgroups). */
+ * Each stride holds for the gradient of its array too, and is at most 2^24.  Sizes at
+ * most 2^30, batch * channels at most 2^31 - 256 (THFF_EINVAL too where a call has too
+ * many workgroups). */
 typedef struct thff_state_shape {
     int precision;
     int batch, n, channels, order, groups, states;
@@ -435,8 +436,10 @@ typedef struct thff_state_shape {
 } thff_state_shape;
 
 /* Bytes of d_saved (what the forward pass keeps for the backward pass) and of d_workspace
- * (scratch of one call, either way) for a shape; THFF_EINVAL for a bad shape. */
+ * (scratch of one call): what a forward call needs (0: may be null), and enough for a call
+ * either way; THFF_EINVAL for a bad shape. */
 long long thff_state_scan_saved_bytes(const thff_state_shape* shape);
+long long thff_state_scan_forward_bytes(const thff_state_shape* shape);
 long long thff_state_scan_workspace_bytes(const thff_state_shape* shape);
 
 /* For every sequence and channel, over its states s < order:

@@ -67,6 +67,10 @@ def test_state_shapes_refused():
                 dict(groups=2, b_stride=31)):
         with pytest.raises(ValueError, match="stride"):
             state_shape(**bad).saved_bytes()
+    for bad in ("x", "delta", "gate", "b", "c", "y"):
+        with pytest.raises(ValueError, match="at most 2\\^24"):
+            state_shape(**{bad + "_stride": (1 << 24) + 1}).saved_bytes()
+        assert state_shape(**{bad + "_stride": 1 << 24}).saved_bytes() > 0
     with pytest.raises(ValueError, match="exceeds one launch"):
         state_shape(batch=1 << 28, n=1 << 30, channels=1, order=4).saved_bytes()
     assert thff.lib().thff_state_scan_saved_bytes(None) == thff.THFF_EINVAL
@@ -79,6 +83,9 @@ def test_sizes():
         s = [state_shape(n=n, order=order).saved_bytes() for n in (0, 1, 300, 3000, 1 << 30)]
         assert s[0] == 0 and s == sorted(s)
         assert all(state_shape(n=n, order=order).workspace_bytes() > 0 for n in (0, 1, 300, 1 << 20))
+        assert state_shape(n=1, order=order).forward_bytes() == 0 and state_shape(n=1 << 16, order=order).forward_bytes() > 0
+    # Many channels leave no segments, and a forward call no scratch.
+    assert state_shape(batch=8, n=4096, channels=2048).forward_bytes() == 0
     assert state_shape(channels=0).workspace_bytes() == 0
     for T in ("float", "half"):
         assert conv_shape(T, n=0).workspace_bytes() == 0 and conv_shape(T, batch=0).workspace_bytes() == 0
@@ -164,6 +171,7 @@ def test_state_refused(call):
     for name in ("d_saved", "d_workspace"):
         with pytest.raises(ValueError, match="16-byte aligned"):
             call(s, **dict(good, **{name: H + 8}))
+    assert s.forward_bytes() > 0
     with pytest.raises(ValueError, match="requires a workspace"):
         call(s, **dict(good, d_workspace=0))
     with pytest.raises(ValueError, match="states must"):

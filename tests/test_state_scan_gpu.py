@@ -70,11 +70,12 @@ def run(T, v, lengths=None, gap=0, offset=0):
     def scratch(count):
         return torch.full((count + 64,), 0xFF, dtype=torch.uint8, device="cuda")
 
-    saved, workspace = scratch(shape.saved_bytes()), scratch(shape.workspace_bytes())
+    saved, workspace = scratch(shape.saved_bytes()), scratch(shape.forward_bytes())
     thff.ThunderFFT_state_scan(shape, at["x"], at["delta"], v["a"], at["b"], at["c"], out["y"][0], d_skip=v["skip"], d_gate=gate,
                                d_delta_bias=v["delta_bias"], d_state_in=v["state"], d_state_out=weights["state"], d_lengths=lengths,
                                d_saved=saved, d_workspace=workspace)
-    assert (saved[-64:] == 0xFF).all() and (workspace[-64:] == 0xFF).all()
+    assert (workspace[-64:] == 0xFF).all()
+    assert (saved[-64:] == 0xFF).all()
     workspace = scratch(shape.workspace_bytes())
     thff.ThunderFFT_state_scan_backward(
         shape, at["dy"], at["x"], at["delta"], v["a"], at["b"], at["c"], saved, out["dx"][0], out["ddelta"][0], weights["da"],
@@ -210,7 +211,7 @@ def test_tokens_follow_prompts_in_a_pool(T, size):
         part = {k: v[k][:, at:at + count].contiguous() for k in VALUES + SHARED}
         shape = thff.StateShape(T, batch, count, channels, order, states=9)
         out = torch.empty_like(part["x"])
-        work = torch.empty(shape.workspace_bytes(), dtype=torch.uint8, device="cuda")
+        work = torch.empty(shape.forward_bytes(), dtype=torch.uint8, device="cuda")
         thff.ThunderFFT_state_scan(shape, part["x"], part["delta"], v["a"], part["b"], part["c"], out, d_skip=v["skip"],
                                    d_gate=part["gate"], d_delta_bias=v["delta_bias"], d_state_in=pool, d_state_out=pool,
                                    d_slots=slots, d_workspace=work)
@@ -243,7 +244,7 @@ def test_one_token(T, size):
             row = groups * order + 3
             shape = thff.StateShape(T, batch, 1, channels, order, groups, *(channels + 3,) * 3, row, row, channels + 3)
             state = torch.full((batch * channels * order + 4,), GUARD, device="cuda")
-            work = torch.empty(shape.workspace_bytes(), dtype=torch.uint8, device="cuda")
+            work = torch.empty(shape.forward_bytes(), dtype=torch.uint8, device="cuda")
             thff.ThunderFFT_state_scan(shape, at["x"], at["delta"], w["a"], at["b"], at["c"], y, d_skip=w["skip"], d_gate=at["gate"],
                                        d_delta_bias=w["delta_bias"], d_state_in=w["state"], d_state_out=state, d_lengths=end,
                                        d_workspace=work)

@@ -111,7 +111,7 @@ def lib() -> ctypes.CDLL:
                 i32, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i32, vp]
         cp, tp = ctypes.POINTER(ConvShape), ctypes.POINTER(StateShape)
         for name, p in (("short_conv_workspace", cp), ("state_scan_saved", tp),
-                        ("state_scan_workspace", tp)):
+                        ("state_scan_forward", tp), ("state_scan_workspace", tp)):
             fn = getattr(L, f"thff_{name}_bytes")
             fn.argtypes, fn.restype = [p], i64
         L.thff_rms_norm_workspace_bytes.argtypes = [i64, i32]
@@ -566,8 +566,12 @@ class StateShape(ctypes.Structure):
         """Bytes that the forward call keeps for the backward call (d_saved)."""
         return _bytes(lib().thff_state_scan_saved_bytes(ctypes.byref(self)))
 
+    def forward_bytes(self) -> int:
+        """Bytes of a forward call's scratch memory alone."""
+        return _bytes(lib().thff_state_scan_forward_bytes(ctypes.byref(self)))
+
     def workspace_bytes(self) -> int:
-        """Bytes of a call's scratch memory (d_workspace), forward or backward."""
+        """Bytes of a call's scratch memory (d_workspace), enough for forward and backward calls."""
         return _bytes(lib().thff_state_scan_workspace_bytes(ctypes.byref(self)))
 
 
@@ -588,7 +592,7 @@ def ThunderFFT_state_scan(shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip=None, 
     the last (d_state_out, the same buffer if wanted) are float32 rows [channels][order], row b for
     sequence b or row d_slots[b] (int32) of a pool; d_lengths (int32) ends each sequence early.
     d_saved (shape.saved_bytes()) is kept for the backward call, d_workspace
-    (shape.workspace_bytes()) is scratch.  Synchronous."""
+    (shape.forward_bytes()) is scratch.  Synchronous."""
     _state_scan(lib().thff_state_scan, shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip, d_gate,
                 d_delta_bias, d_state_in, d_state_out, d_slots, d_lengths, d_saved, d_workspace,
                 stream)

@@ -124,7 +124,7 @@ class _StateScan(torch.autograd.Function):
             thff.ThunderFFT_state_scan_async(
                 shape, x, delta, a, b_rows, c_rows, y, d_skip=skip, d_gate=gate_rows[0], d_delta_bias=delta_bias,
                 d_state_in=state, d_state_out=last, d_lengths=lengths, d_saved=saved,
-                d_workspace=_bytes(shape.workspace_bytes(), x.device), stream=torch.cuda.current_stream())
+                d_workspace=_bytes(shape.forward_bytes(), x.device), stream=torch.cuda.current_stream())
         if train:
             ctx.save_for_backward(x, delta, a, b_rows, c_rows, skip, gate_rows[0], delta_bias, lengths, saved)
             ctx.groups = groups

@@ -98,8 +98,9 @@ struct StateBackward {
     float* workspace;
 };
 
-// Bytes of `saved` and of `workspace` for a shape.
+// Bytes of `saved` and of `workspace` for a shape: of the forward pass, and enough for either.
 long long state_saved_bytes(const StateShape& shape);
+long long state_forward_bytes(const StateShape& shape);
 long long state_workspace_bytes(const StateShape& shape);
 // Whether the shape's grids fit one launch, and its buffers 63 bits.
 bool state_fits(const StateShape& shape);

@@ -7,6 +7,7 @@
 
 #include "block.hpp"
 #include "capi_checks.hpp"
+#include "state_cut.hpp"
 
 namespace {
 
@@ -136,6 +137,8 @@ int check_shape(const thff_state_shape* shape, StateShape* out) {
         !stride_of(shape->b_stride, shared, rows, &out->b_stride) ||
         !stride_of(shape->c_stride, shared, rows, &out->c_stride))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan stride is shorter than a row or too long");
+    for (long long stride : {out->x_stride, out->delta_stride, out->gate_stride, out->y_stride, out->b_stride, out->c_stride})
+        if (stride > kStateStride) return fail(THFF_EINVAL, "ThunderFFT_state_scan stride must be at most 2^24");
     if (!state_fits(*out)) return fail(THFF_EINVAL, "ThunderFFT_state_scan shape exceeds one launch");
     return THFF_OK;
 }
@@ -160,9 +163,9 @@ int state_impl(const thff_state_shape* shape, const StateForward& a, void* strea
         return fail(THFF_EINVAL, "ThunderFFT_state_scan states must be nonnegative");
     if (!all_aligned({a.saved, a.workspace}, 16))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan requires 16-byte aligned saved and workspace");
-    if (!a.workspace && state_workspace_bytes(s) > 0)
+    if (!a.workspace && state_forward_bytes(s) > 0)
         return fail(THFF_EINVAL, "ThunderFFT_state_scan requires a workspace of " +
-                                     std::to_string(state_workspace_bytes(s)) + " bytes");
+                                     std::to_string(state_forward_bytes(s)) + " bytes");
     auto st = static_cast<hipStream_t>(stream);
     return finish(launch_state_scan(s, a, st), st, synchronize, "ThunderFFT_state_scan");
 }
@@ -346,6 +349,14 @@ long long thff_state_scan_saved_bytes(const thff_state_shape* shape) {
         StateShape s;
         const int rc = check_shape(shape, &s);
         return rc == THFF_OK ? state_saved_bytes(s) : rc;
+    });
+}
+
+long long thff_state_scan_forward_bytes(const thff_state_shape* shape) {
+    return guarded([&]() -> long long {
+        StateShape s;
+        const int rc = check_shape(shape, &s);
+        return rc == THFF_OK ? state_forward_bytes(s) : rc;
     });
 }
 

@@ -8,6 +8,7 @@ namespace thff {
 
 constexpr int kStateWaves = 4;
 constexpr int kStateBlock = 32;  // steps whose b and c are in LDS at a time, forward
+constexpr long long kStateStride = 1 << 24;  // the longest: offsets of a lane's rows fit 32 bits
 constexpr int kStateTile = 16;   // steps between saved states, and of the backward pass at a time
 
 // S states of a channel on each of LPC neighbouring lanes.

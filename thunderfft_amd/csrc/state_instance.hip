@@ -35,11 +35,12 @@ hipError_t launch_state_forward(const StateShape& s, const StateForward& a, cons
     return with_lanes(s.order, [&](auto lanes) {
         using L = decltype(lanes);
         if (cut.segments > 1) {
-            state_forward<T, L, true><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+            state_forward<T, L, true, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
             const hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
         }
-        state_forward<T, L, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+        if (a.saved) state_forward<T, L, false, true><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+        else state_forward<T, L, false, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
         return hipGetLastError();
     });
 }

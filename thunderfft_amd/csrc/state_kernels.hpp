@@ -28,7 +28,8 @@ template <class L>
 struct Place {
     int lane, wave, sub;  // sub: of the channel's lanes
     int b, group, slab, segment;
-    int channel;  // the last one again where there is none
+    int base;  // the wave's first channel, or the group's last where the wave has none
+    int in;    // the lane's from there, the group's last one again where it has none
     bool valid;
 
     __device__ __forceinline__ Place(const StateShape& s, const Cut& cut, long long block)
@@ -39,12 +40,20 @@ struct Place {
         block /= s.groups;
         segment = static_cast<int>(block % cut.segments);
         b = static_cast<int>(block / cut.segments);
-        const int each = s.channels / s.groups;
-        const int c = slab * L::kSlab + wave * L::kWave + lane / L::LPC;
-        valid = c < each;
-        channel = group * each + min(c, each - 1);
+        const int each = s.channels / s.groups, c = slab * L::kSlab + wave * L::kWave;
+        valid = c + lane / L::LPC < each;
+        base = group * each + min(c, each - 1);
+        in = min(lane / L::LPC, max(each - 1 - c, 0));
     }
+    __device__ __forceinline__ int channel() const { return base + in; }
 };
+
+// What lies at `at`, the same for all lanes of a wave, plus an offset of the lane's in elements.
+template <class T>
+__device__ __forceinline__ T& lane_at(T* at, unsigned offset) {
+    return *reinterpret_cast<T*>(reinterpret_cast<char*>(const_cast<std::remove_const_t<T>*>(at)) +
+                                 offset * static_cast<unsigned>(sizeof(T)));
+}
 
 __device__ __forceinline__ long long block_index() {
     return static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x;
@@ -82,20 +91,64 @@ __device__ __forceinline__ void store_padded(float* row, const float (&h)[L::S],
     __builtin_nontemporal_store(v, reinterpret_cast<V*>(row + sub * L::S));
 }
 
+// N values of a lane, LPC steps apart, from step t on, where `at` is: past the last step of n, the
+// last one again.  offset: the lane's, of its step and channel.
+template <int N, int LPC, class T>
+__device__ __forceinline__ void load_steps(T (&v)[N], const T* at, unsigned offset, long long stride, int t, int sub, int n) {
+    if (t + N * LPC <= n) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] = lane_at(at, offset);
+            at += LPC * stride;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = (&lane_at(at, offset))[(min(t + j * LPC + sub, n - 1) - sub - t) * stride];
+    }
+}
+
+// Offsets of a lane's first step and channel in rows of each stride, and of its row and state of b's
+// and c's; strides of more than kStateStride are refused.
+template <class L>
+struct Offsets {
+    unsigned x, delta, gate, y, b, c;
+    __device__ __forceinline__ Offsets(const StateShape& s, const Place<L>& p)
+        : x(at(s.x_stride, p)), delta(at(s.delta_stride, p)), gate(at(s.gate_stride, p)), y(at(s.y_stride, p)),
+          b(shared(s.b_stride, s, p)), c(shared(s.c_stride, s, p)) {}
+    static __device__ __forceinline__ unsigned at(long long stride, const Place<L>& p) {
+        return p.sub * static_cast<unsigned>(stride) + p.in;
+    }
+    static __device__ __forceinline__ unsigned shared(long long stride, const StateShape& s, const Place<L>& p) {
+        return threadIdx.x / L::P * static_cast<unsigned>(stride) + min(static_cast<int>(threadIdx.x % L::P), s.order - 1);
+    }
+};
+
 // b and c of N steps: loaded ahead into registers, then to LDS as [step][lane of a channel][b's, c's].
 template <class T, class L, int N>
 struct Shared {
     static constexpr int kEach = (N * L::P + kLanes - 1) / kLanes;
     using Rows = float[L::LPC][2 * L::S];
+    static constexpr int kRows = kLanes / L::P;  // steps loaded at a time
     T b[kEach], c[kEach];
 
-    __device__ __forceinline__ void load(const StateShape& s, const T* bs, const T* cs, int t0) {
+    // Steps from t0 on, where bs and cs are; b_at, c_at: the offsets of the lane's row of them and its state.
+    __device__ __forceinline__ void load(const StateShape& s, const T* bs, const T* cs, unsigned b_at, unsigned c_at, int t0) {
+        if (t0 + kEach * kRows <= s.n) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = e * kLanes + threadIdx.x, st = min(i % L::P, s.order - 1);
-            const long long t = min(t0 + i / L::P, s.n - 1);
-            b[e] = bs[t * s.b_stride + st];
-            c[e] = cs[t * s.c_stride + st];
+            for (int e = 0; e < kEach; ++e) {
+                b[e] = lane_at(bs, b_at);
+                c[e] = lane_at(cs, c_at);
+                bs += kRows * s.b_stride;
+                cs += kRows * s.c_stride;
+            }
+        } else {
+            const int row = threadIdx.x / L::P;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const long long t = min(t0 + e * kRows + row, s.n - 1) - row - t0;
+                b[e] = (&lane_at(bs, b_at))[t * s.b_stride];
+                c[e] = (&lane_at(cs, c_at))[t * s.c_stride];
+            }
         }
     }
     // Zeros from step `end` on and for states that are none.
@@ -122,9 +175,37 @@ __device__ __forceinline__ void load_shared(float (&b)[S], float (&c)[S], const 
     }
 }
 
+// Takes h through the segments from `from` on, `count` of them one after the other, `way` apart: each
+// decays it by its sum of dt and adds its own end.  ends_of, sums_of: rows of the first one.
+template <class L>
+__device__ __forceinline__ void fold(float (&h)[L::S], const float (&decay)[L::S], const float* ends_of, const float* sums_of,
+                                     long long way, int count, int sub) {
+    constexpr int kAtOnce = 8;  // loads under way together
+    for (int k = 0; k < count; k += kAtOnce) {
+        float own[kAtOnce][L::S], dt[kAtOnce];
+#pragma unroll
+        for (int m = 0; m < kAtOnce; ++m) {
+            const long long at = min(k + m, count - 1) * way;
+            load_padded<L>(own[m], ends_of + at * L::P, sub);
+            dt[m] = sums_of[at];
+        }
+#pragma unroll
+        for (int m = 0; m < kAtOnce; ++m) {
+            if (k + m == count) break;
+#pragma unroll
+            for (int i = 0; i < L::S; ++i) h[i] = fmaf(__builtin_amdgcn_exp2f(dt[m] * decay[i]), h[i], own[m][i]);
+        }
+    }
+}
+
 // The segment's end from a state of zero (the first segment: from the given one) where Only is
-// `true`, for the segments but the last; its outputs otherwise.
-template <class T, class L, bool Only>
+// `true`, for the segments but the last; its outputs otherwise.  Save: the states before every
+// kTile-th step are kept.
+//
+// A block of steps that all count has no branches, so that the reads of LDS and the exponentials
+// of one step are under way while those before it are worked on.  Lanes of no channel do as the
+// last channel's, stores included.
+template <class T, class L, bool Only, bool Save>
 __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForward a, Cut cut) {
     constexpr int S = L::S, LPC = L::LPC, J = kBlock / LPC;
     __shared__ alignas(16) float bc[2][kBlock][LPC][2 * S];
@@ -134,19 +215,20 @@ __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForwa
     if (Only && p.segment + 1 == cut.segments) return;
     const int length = length_of(a.lengths, p.b, s.n), t0 = p.segment * cut.steps, t1 = min(t0 + cut.steps, s.n);
     const int end = min(length, t1);
-    const long long first = p.b * static_cast<long long>(s.n);
-    const int shared = p.group * s.order;
-    const T* x = static_cast<const T*>(a.x) + first * s.x_stride + p.channel;
-    const T* delta = static_cast<const T*>(a.delta) + first * s.delta_stride + p.channel;
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + first * s.gate_stride + p.channel : nullptr;
-    const T* bs = static_cast<const T*>(a.b) + first * s.b_stride + shared;
-    const T* cs = static_cast<const T*>(a.c) + first * s.c_stride + shared;
-    T* y = static_cast<T*>(a.y) + first * s.y_stride + p.channel;
+    const long long first = p.b * static_cast<long long>(s.n) + t0;
+    const Offsets<L> lane(s, p);
+    const T* x = static_cast<const T*>(a.x) + first * s.x_stride + p.base;
+    const T* delta = static_cast<const T*>(a.delta) + first * s.delta_stride + p.base;
+    const T* gate = a.gate ? static_cast<const T*>(a.gate) + first * s.gate_stride + p.base : nullptr;
+    const T* bs = static_cast<const T*>(a.b) + first * s.b_stride + p.group * s.order;
+    const T* cs = static_cast<const T*>(a.c) + first * s.c_stride + p.group * s.order;
+    T* y = static_cast<T*>(a.y) + first * s.y_stride + p.base;
+    const int channel = p.channel();
     float decay[S], h[S], sum = 0.0f;
-    load_states<L>(decay, a.a + static_cast<long long>(p.channel) * s.order, p.sub, s.order);
+    load_states<L>(decay, a.a + static_cast<long long>(channel) * s.order, p.sub, s.order);
 #pragma unroll
     for (int i = 0; i < S; ++i) decay[i] *= kLog2e;
-    const float skip = a.skip ? a.skip[p.channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[p.channel] : 0.0f;
+    const float skip = a.skip ? a.skip[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
 
     int slot = p.b;
     if (a.slots) {
@@ -158,95 +240,108 @@ __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForwa
     for (int i = 0; i < S; ++i) h[i] = 0.0f;
     if (Only || cut.segments == 1) {
         if (p.segment == 0 && a.state_in && slot >= 0)
-            load_states<L>(h, a.state_in + (static_cast<long long>(slot) * s.channels + p.channel) * s.order, p.sub, s.order);
-        if (Only && p.segment == 0 && p.valid)
-            store_padded<L>(ends.states + ends.row(s, cut, p.b, 0, p.channel) * L::P, h, p.sub);
+            load_states<L>(h, a.state_in + (static_cast<long long>(slot) * s.channels + channel) * s.order, p.sub, s.order);
+        if (Only && p.segment == 0)
+            store_padded<L>(ends.states + ends.row(s, cut, p.b, 0, channel) * L::P, h, p.sub);
     } else {
-        load_padded<L>(h, ends.states + ends.row(s, cut, p.b, min(p.segment, 1), p.channel) * L::P, p.sub);
-        for (int k = 2; k <= p.segment; ++k) {
-            float own[S];
-            load_padded<L>(own, ends.states + ends.row(s, cut, p.b, k, p.channel) * L::P, p.sub);
-            const float dt = ends.sums[ends.row(s, cut, p.b, k - 1, p.channel)];
-#pragma unroll
-            for (int i = 0; i < S; ++i) h[i] = fmaf(__builtin_amdgcn_exp2f(dt * decay[i]), h[i], own[i]);
-        }
+        load_padded<L>(h, ends.states + ends.row(s, cut, p.b, min(p.segment, 1), channel) * L::P, p.sub);
+        fold<L>(h, decay, ends.states + ends.row(s, cut, p.b, 2, channel) * L::P, ends.sums + ends.row(s, cut, p.b, 1, channel),
+                s.channels, p.segment - 1, p.sub);
     }
+    const long long tiles = (s.n + kTile - 1) / kTile;
+    float* saved = Save ? a.saved + (p.b * tiles * s.channels + channel) * L::P : nullptr;
 
     // The next block's values are under way while a block is worked on.
     Shared<T, L, kBlock> ahead;
     T nx[J], nd[J], nz[J];
     const auto load = [&](int t) {
-        ahead.load(s, bs, cs, t);
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const long long at = min(t + j * LPC + p.sub, s.n - 1);
-            nx[j] = x[at * s.x_stride];
-            nd[j] = delta[at * s.delta_stride];
-            if (!Only && gate) nz[j] = gate[at * s.gate_stride];
-        }
+        ahead.load(s, bs, cs, lane.b, lane.c, t);
+        load_steps<J, LPC>(nx, x, lane.x, s.x_stride, t, p.sub, s.n);
+        load_steps<J, LPC>(nd, delta, lane.delta, s.delta_stride, t, p.sub, s.n);
+        if (!Only && gate) load_steps<J, LPC>(nz, gate, lane.gate, s.gate_stride, t, p.sub, s.n);
+        bs += kBlock * s.b_stride;
+        cs += kBlock * s.c_stride;
+        x += kBlock * s.x_stride;
+        delta += kBlock * s.delta_stride;
+        if (!Only && gate) gate += kBlock * s.gate_stride;
     };
     int which = 0;
-    if (t0 < end) load(t0);
-    int t = t0;
-    for (; t < end; t += kBlock, which ^= 1) {
+    const auto steps = [&](auto whole, int t) {
+        constexpr bool kWhole = decltype(whole)::value;
         ahead.store(s, bc[which], t, end);
-        T xs[J], ds[J], zs[J];
+        float xv[J], dt[J], out[J];
+        T zs[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            xs[j] = nx[j];
-            ds[j] = nd[j];
-            if (!Only && gate) zs[j] = nz[j];
+            const bool on = kWhole || t + j * LPC + p.sub < end;
+            xv[j] = on ? to_float<T>(nx[j]) : 0.0f;
+            dt[j] = softplus(to_float<T>(nd[j]) + bias);
+            dt[j] = on ? dt[j] : 0.0f;
+            zs[j] = nz[j];
+            sum += dt[j];
         }
         __syncthreads();
         load(t + kBlock);
+        // The next LPC steps' b and c are read from LDS while LPC steps are worked on.
+        float b[2][LPC][S], c[2][LPC][S];
+        const auto read = [&](int j) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int now = t + j * LPC + p.sub;
-            const bool on = now < end;
-            const float xv = on ? to_float<T>(xs[j]) : 0.0f;
-            const float dt = on ? softplus(to_float<T>(ds[j]) + bias) : 0.0f, u = dt * xv;
-            if (!Only && j * LPC % kTile == 0 && a.saved && p.valid && t + j * LPC < end) {
-                const long long tile = static_cast<long long>(p.b) * ((s.n + kTile - 1) / kTile) + (t + j * LPC) / kTile;
-                store_padded<L>(a.saved + (tile * s.channels + p.channel) * L::P, h, p.sub);
+            for (int k = 0; k < LPC; ++k) load_shared<S>(b[j & 1][k], c[j & 1][k], bc[which][j * LPC + k][p.sub]);
+        };
+        read(0);
+        each_step<J>([&](auto j) {
+            if constexpr (j + 1 < J) read(j + 1);
+            if constexpr (Save && j * LPC % kTile == 0) {
+                if (kWhole || t + j * LPC < end)
+                    store_padded<L>(saved + static_cast<long long>((t + j * LPC) / kTile) * s.channels * L::P, h, p.sub);
             }
-            sum += dt;
-            float out[LPC];
+            const float u = dt[j] * xv[j];
+            float part[LPC];
             each_step<LPC>([&](auto k) {
-                const float d = from_lane<LPC, k>(dt), v = from_lane<LPC, k>(u);
-                float b[S], c[S];
-                load_shared<S>(b, c, bc[which][j * LPC + k][p.sub]);
-                out[k] = 0.0f;
+                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u);
+                part[k] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
-                    h[i] = fmaf(__builtin_amdgcn_exp2f(d * decay[i]), h[i], v * b[i]);
-                    if (!Only) out[k] = fmaf(c[i], h[i], out[k]);
+                    h[i] = fmaf(__builtin_amdgcn_exp2f(d * decay[i]), h[i], v * b[j & 1][k][i]);
+                    if (!Only) part[k] = fmaf(c[j & 1][k][i], h[i], part[k]);
                 }
             });
-            if constexpr (!Only) {
-                float v = fmaf(skip, xv, sum_to_lanes<LPC>(out, p.lane));
-                if (gate) {
+            if constexpr (!Only) out[j] = fmaf(skip, xv[j], sum_to_lanes<LPC>(part, p.lane));
+        });
+        if constexpr (!Only) {
+            if (gate) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
                     const float z = to_float<T>(zs[j]);
-                    v *= z * opened(z);
+                    out[j] *= z * opened(z);
                 }
-                if (p.valid && now < t1) y[now * s.y_stride] = from_float<T>(on ? v : 0.0f);
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int now = t + j * LPC + p.sub;
+                if (kWhole) lane_at(y, lane.y) = from_float<T>(out[j]);
+                else if (now < t1) lane_at(y, lane.y) = from_float<T>(now < end ? out[j] : 0.0f);
+                y += LPC * s.y_stride;
             }
         }
-    }
+        which ^= 1;
+    };
+    if (t0 < end) load(t0);
+    int t = t0;
+    for (; t + kBlock <= end; t += kBlock) steps(std::true_type{}, t);
+    for (; t < end; t += kBlock) steps(std::false_type{}, t);
     if constexpr (Only) {
-        if (!p.valid) return;
-        store_padded<L>(ends.states + ends.row(s, cut, p.b, p.segment + 1, p.channel) * L::P, h, p.sub);
+        store_padded<L>(ends.states + ends.row(s, cut, p.b, p.segment + 1, channel) * L::P, h, p.sub);
         // The sum of the lanes' steps.
         float all[LPC];
 #pragma unroll
         for (int k = 0; k < LPC; ++k) all[k] = sum;
-        sum = sum_to_lanes<LPC>(all, p.lane);
-        if (p.sub == 0) ends.sums[ends.row(s, cut, p.b, p.segment, p.channel)] = sum;
+        ends.sums[ends.row(s, cut, p.b, p.segment, channel)] = sum_to_lanes<LPC>(all, p.lane);
     } else {
-        if (!p.valid) return;
-        for (; t < t1; t += LPC)
-            if (t + p.sub < t1) y[(t + p.sub) * s.y_stride] = from_float<T>(0.0f);
+        for (; t < t1; t += LPC, y += LPC * s.y_stride)
+            if (t + p.sub < t1) lane_at(y, lane.y) = from_float<T>(0.0f);
         if (a.state_out && slot >= 0 && p.segment + 1 == cut.segments)
-            store_states<L>(a.state_out + (static_cast<long long>(slot) * s.channels + p.channel) * s.order, h, p.sub, s.order);
+            store_states<L>(a.state_out + (static_cast<long long>(slot) * s.channels + channel) * s.order, h, p.sub, s.order);
     }
 }
 
@@ -254,7 +349,10 @@ __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForwa
 
 // The gradient that leaves a segment towards its start, from one of zero behind it (the last
 // segment: from dstate_out), where Only is `true`, for the segments but the first; the gradients
-// otherwise.
+// otherwise.  Tiles go from the last to the first: the states of a tile are worked out again from the
+// saved one and kept in registers with their decays, then the gradients go back over it.
+//
+// A tile whose steps and channels all count has no branches.
 template <class T, class L, bool Only>
 __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateBackward a, Cut cut) {
     constexpr int S = L::S, LPC = L::LPC, P = L::P, J = kTile / LPC;
@@ -267,24 +365,27 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
     if (Only && p.segment == 0) return;
     const int length = length_of(a.lengths, p.b, s.n), t0 = p.segment * cut.steps, t1 = min(t0 + cut.steps, s.n);
     const int end = min(length, t1);
-    const long long first = p.b * static_cast<long long>(s.n);
-    const int shared = p.group * s.order;
-    const T* x = static_cast<const T*>(a.x) + first * s.x_stride + p.channel;
-    const T* delta = static_cast<const T*>(a.delta) + first * s.delta_stride + p.channel;
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + first * s.gate_stride + p.channel : nullptr;
-    const T* dy = static_cast<const T*>(a.dy) + first * s.y_stride + p.channel;
-    const T* bs = static_cast<const T*>(a.b) + first * s.b_stride + shared;
-    const T* cs = static_cast<const T*>(a.c) + first * s.c_stride + shared;
-    T* dx = static_cast<T*>(a.dx) + first * s.x_stride + p.channel;
-    T* ddelta = static_cast<T*>(a.ddelta) + first * s.delta_stride + p.channel;
-    T* dgate = gate ? static_cast<T*>(a.dgate) + first * s.gate_stride + p.channel : nullptr;
-    const long long tiles = (s.n + kTile - 1) / kTile;
-    const float* saved = a.saved + (p.b * tiles * s.channels + p.channel) * P;
+    // The tile of the last step.
+    const int from = end > t0 ? (end - 1 - t0) / kTile * kTile + t0 : t0 - kTile;
+    const long long first = p.b * static_cast<long long>(s.n) + from, tiles = (s.n + kTile - 1) / kTile;
+    const Offsets<L> lane(s, p);
+    const T* x = static_cast<const T*>(a.x) + first * s.x_stride + p.base;
+    const T* delta = static_cast<const T*>(a.delta) + first * s.delta_stride + p.base;
+    const T* gate = a.gate ? static_cast<const T*>(a.gate) + first * s.gate_stride + p.base : nullptr;
+    const T* dy = static_cast<const T*>(a.dy) + first * s.y_stride + p.base;
+    const T* bs = static_cast<const T*>(a.b) + first * s.b_stride + p.group * s.order;
+    const T* cs = static_cast<const T*>(a.c) + first * s.c_stride + p.group * s.order;
+    T* dx = static_cast<T*>(a.dx) + first * s.x_stride + p.base;
+    T* ddelta = static_cast<T*>(a.ddelta) + first * s.delta_stride + p.base;
+    T* dgate = gate ? static_cast<T*>(a.dgate) + first * s.gate_stride + p.base : nullptr;
+    const float* saved = a.saved + ((p.b * tiles + from / kTile) * s.channels + p.base) * P;
+    const unsigned saved_at = p.in * P + p.sub * S;
+    const int channel = p.channel();
     float decay[S], g[S], sum = 0.0f;
-    load_states<L>(decay, a.a + static_cast<long long>(p.channel) * s.order, p.sub, s.order);
+    load_states<L>(decay, a.a + static_cast<long long>(channel) * s.order, p.sub, s.order);
 #pragma unroll
     for (int i = 0; i < S; ++i) decay[i] *= kLog2e;
-    const float skip = a.skip ? a.skip[p.channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[p.channel] : 0.0f;
+    const float skip = a.skip ? a.skip[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
 
     // g: the gradient of the state behind the steps that are done, from the steps behind it.
     const Ends ends(a.workspace, s, cut);
@@ -292,79 +393,89 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
     for (int i = 0; i < S; ++i) g[i] = 0.0f;
     const int last = cut.segments - 1;
     if (p.segment == last) {
-        if (a.dstate_out && p.valid)
-            load_states<L>(g, a.dstate_out + (static_cast<long long>(p.b) * s.channels + p.channel) * s.order, p.sub, s.order);
+        if (a.dstate_out)
+            load_states<L>(g, a.dstate_out + (static_cast<long long>(p.b) * s.channels + channel) * s.order, p.sub, s.order);
     } else if (!Only) {
-        load_padded<L>(g, ends.states + ends.row(s, cut, p.b, last, p.channel) * P, p.sub);
-        for (int k = last - 1; k > p.segment; --k) {
-            float own[S];
-            load_padded<L>(own, ends.states + ends.row(s, cut, p.b, k, p.channel) * P, p.sub);
-            const float dt = ends.sums[ends.row(s, cut, p.b, k, p.channel)];
-#pragma unroll
-            for (int i = 0; i < S; ++i) g[i] = fmaf(__builtin_amdgcn_exp2f(dt * decay[i]), g[i], own[i]);
-        }
-        if (!p.valid) {
-#pragma unroll
-            for (int i = 0; i < S; ++i) g[i] = 0.0f;
-        }
+        load_padded<L>(g, ends.states + ends.row(s, cut, p.b, last, channel) * P, p.sub);
+        fold<L>(g, decay, ends.states + ends.row(s, cut, p.b, last - 1, channel) * P, ends.sums + ends.row(s, cut, p.b, last - 1, channel),
+                -static_cast<long long>(s.channels), last - 1 - p.segment, p.sub);
     }
+    // Lanes of no channel add nothing to the sums over channels.
+#pragma unroll
+    for (int i = 0; i < S; ++i) g[i] = p.valid ? g[i] : 0.0f;
     float da[S] = {}, dskip = 0.0f, dbias = 0.0f;
     const Parts parts(s, cut);
     float* shared_sums = a.workspace + parts.shared +
                          ((static_cast<long long>(p.slab) * s.batch + p.b) * s.n * s.groups + p.group) * 2 * P;
+    const bool all_valid = (p.slab + 1) * static_cast<long long>(L::kSlab) <= s.channels / s.groups;
 
     // The values of the tile before are under way while a tile is worked on.
     Shared<T, L, kTile> ahead;
     T nx[J], nd[J], nz[J], ny[J];
     float nh[S];
     const auto load = [&](int t) {
-        t = max(t, 0);
-        ahead.load(s, bs, cs, t);
-        if (!Only) load_padded<L>(nh, saved + static_cast<long long>(t / kTile) * s.channels * P, p.sub);
+        if (t < t0) return;
+        ahead.load(s, bs, cs, lane.b, lane.c, t);
+        if (!Only) load_padded<L>(nh, &lane_at(saved, saved_at), 0);
+        load_steps<J, LPC>(nx, x, lane.x, s.x_stride, t, p.sub, s.n);
+        load_steps<J, LPC>(nd, delta, lane.delta, s.delta_stride, t, p.sub, s.n);
+        load_steps<J, LPC>(ny, dy, lane.y, s.y_stride, t, p.sub, s.n);
+        if (gate) load_steps<J, LPC>(nz, gate, lane.gate, s.gate_stride, t, p.sub, s.n);
+        bs -= kTile * s.b_stride;
+        cs -= kTile * s.c_stride;
+        saved -= static_cast<long long>(s.channels) * P;
+        x -= kTile * s.x_stride;
+        delta -= kTile * s.delta_stride;
+        dy -= kTile * s.y_stride;
+        if (gate) gate -= kTile * s.gate_stride;
+    };
+    // Stores a value of each of the lane's steps.
+    const auto store = [&](auto whole, T* to, unsigned offset, long long stride, int t, const float (&v)[J]) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const long long at = min(t + j * LPC + p.sub, s.n - 1);
-            nx[j] = x[at * s.x_stride];
-            nd[j] = delta[at * s.delta_stride];
-            ny[j] = dy[at * s.y_stride];
-            if (gate) nz[j] = gate[at * s.gate_stride];
+            if (decltype(whole)::value || (p.valid && t + j * LPC + p.sub < t1)) lane_at(to, offset) = from_float<T>(v[j]);
+            to += LPC * stride;
         }
     };
-    const int from = end > t0 ? (end - 1 - t0) / kTile * kTile + t0 : t0 - kTile;
     int which = 0;
-    if (from >= t0) load(from);
-    for (int t = from; t >= t0; t -= kTile, which ^= 1) {
+    const auto steps = [&](auto whole, int t) {
+        constexpr bool kWhole = decltype(whole)::value;
         ahead.store(s, bc[which], t, end);
         // Of the lane's step of each LPC.
-        float xv[J], dt[J], u[J], along[J], z[J], dyv[J], raw[J];
+        float xv[J], dt[J], along[J], raw[J], dyv[J], h[S];
+        T zs[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const bool on = p.valid && t + j * LPC + p.sub < end;
+            const bool on = kWhole || (p.valid && t + j * LPC + p.sub < end);
             xv[j] = on ? to_float<T>(nx[j]) : 0.0f;
             raw[j] = to_float<T>(nd[j]) + bias;
-            dt[j] = on ? softplus(raw[j]) : 0.0f;
-            u[j] = dt[j] * xv[j];
+            dt[j] = softplus(raw[j]);
+            dt[j] = on ? dt[j] : 0.0f;
             dyv[j] = on ? to_float<T>(ny[j]) : 0.0f;
             along[j] = dyv[j];
-            if (gate) {
-                z[j] = to_float<T>(nz[j]);
-                along[j] = on ? dyv[j] * z[j] * opened(z[j]) : 0.0f;
-            }
+            zs[j] = nz[j];
             sum += dt[j];
         }
-        float h[S];
+        if (gate) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) h[i] = Only ? 0.0f : nh[i];
+            for (int j = 0; j < J; ++j) {
+                const float z = to_float<T>(zs[j]);
+                const bool on = kWhole || (p.valid && t + j * LPC + p.sub < end);
+                along[j] = on ? dyv[j] * z * opened(z) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < S; ++i) h[i] = nh[i];
         __syncthreads();
         load(t - kTile);
-        float inner[J];
-        float keep[kTile][S], before[Only ? 1 : kTile][S];
+        float keep[kTile][S], before[Only ? 1 : kTile][S], inner[J];
         // Forward again from the saved state.
         each_step<J>([&](auto j) {
+            const float u = dt[j] * xv[j];
             float out[LPC];
             each_step<LPC>([&](auto k) {
                 constexpr int m = j * LPC + k;
-                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u[j]);
+                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u);
                 float b[S], c[S];
                 load_shared<S>(b, c, bc[which][m][p.sub]);
                 out[k] = 0.0f;
@@ -378,16 +489,28 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
                     }
                 }
             });
-            if constexpr (!Only) {
-                if (gate) inner[j] = fmaf(skip, xv[j], sum_to_lanes<LPC>(out, p.lane));
-            }
+            if constexpr (!Only) inner[j] = fmaf(skip, xv[j], sum_to_lanes<LPC>(out, p.lane));
         });
+        if constexpr (!Only) {
+            if (gate) {
+                float dz[J];
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const float z = to_float<T>(zs[j]), f = opened(z);
+                    const bool on = kWhole || t + j * LPC + p.sub < end;
+                    dz[j] = on ? dyv[j] * inner[j] * fmaf(z * f, 1.0f - f, f) : 0.0f;
+                }
+                store(whole, dgate, lane.gate, s.gate_stride, t, dz);
+            }
+        }
+        float ex[J], ed[J];
         each_step<J>([&](auto back) {
             constexpr int j = J - 1 - back;
+            const float u = dt[j] * xv[j];
             float du[LPC], de[LPC];
             each_step<LPC>([&](auto behind) {
                 constexpr int k = LPC - 1 - behind, m = j * LPC + k;
-                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u[j]), dn = from_lane<LPC, k>(along[j]);
+                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u), dn = from_lane<LPC, k>(along[j]);
                 float b[S], c[S], both[2 * S];
                 load_shared<S>(b, c, bc[which][m][p.sub]);
                 du[k] = de[k] = 0.0f;
@@ -406,35 +529,32 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
                     }
                 }
                 if constexpr (!Only) {
+                    // Lanes with the same sums store them all.
                     channel_sums<LPC, 2 * S>(both, p.lane);
-                    if (Sums::stores(p.lane)) {
 #pragma unroll
-                        for (int l = 0; l < Sums::kLeft; ++l) {
-                            const int at = Sums::first(p.lane) + l;
-                            sums[p.wave][m][at / S * P + p.sub * S + at % S] = both[l];
-                        }
+                    for (int l = 0; l < Sums::kLeft; ++l) {
+                        const int at = Sums::first(p.lane) + l;
+                        sums[p.wave][m][at / S * P + p.sub * S + at % S] = both[l];
                     }
                 }
             });
             if constexpr (!Only) {
-                const int now = t + j * LPC + p.sub;
-                const bool on = now < end;
+                const bool on = kWhole || t + j * LPC + p.sub < end;
                 const float su = sum_to_lanes<LPC>(du, p.lane), se = sum_to_lanes<LPC>(de, p.lane) * (1.0f / kLog2e);
-                const float dr = on ? fmaf(su, xv[j], se) * opened(raw[j]) : 0.0f;
+                ed[j] = fmaf(su, xv[j], se) * opened(raw[j]);
+                ed[j] = on ? ed[j] : 0.0f;
+                ex[j] = fmaf(su, dt[j], along[j] * skip);
+                ex[j] = on ? ex[j] : 0.0f;
                 dskip = fmaf(along[j], xv[j], dskip);
-                dbias += dr;
-                if (p.valid && now < t1) {
-                    dx[now * s.x_stride] = from_float<T>(on ? fmaf(su, dt[j], along[j] * skip) : 0.0f);
-                    ddelta[now * s.delta_stride] = from_float<T>(dr);
-                    if (gate) {
-                        const float f = opened(z[j]);
-                        dgate[now * s.gate_stride] =
-                            from_float<T>(on ? dyv[j] * inner[j] * fmaf(z[j] * f, 1.0f - f, f) : 0.0f);
-                    }
-                }
+                dbias += ed[j];
             }
         });
         if constexpr (!Only) {
+            store(whole, dx, lane.x, s.x_stride, t, ex);
+            store(whole, ddelta, lane.delta, s.delta_stride, t, ed);
+            dx -= kTile * s.x_stride;
+            ddelta -= kTile * s.delta_stride;
+            if (gate) dgate -= kTile * s.gate_stride;
             // The sums of the waves' channels.
             __syncthreads();
             for (int e = threadIdx.x; e < kTile * 2 * P; e += kLanes) {
@@ -442,10 +562,15 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
                 float v = sums[0][m][at];
 #pragma unroll
                 for (int w = 1; w < kWaves; ++w) v += sums[w][m][at];
-                if (t + m < end) shared_sums[static_cast<long long>(t + m) * s.groups * 2 * P + at] = v;
+                if (kWhole || t + m < end) shared_sums[static_cast<long long>(t + m) * s.groups * 2 * P + at] = v;
             }
         }
-    }
+        which ^= 1;
+    };
+    load(from);
+    int t = from;
+    for (; t >= t0 && (t + kTile > end || !all_valid); t -= kTile) steps(std::false_type{}, t);
+    for (; t >= t0; t -= kTile) steps(std::true_type{}, t);
     if (!p.valid) return;
     float all[LPC];
     const auto over_lanes = [&](float v) {
@@ -453,25 +578,27 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
         for (int k = 0; k < LPC; ++k) all[k] = v;
         return sum_to_lanes<LPC>(all, p.lane);
     };
-    const long long row = ends.row(s, cut, p.b, p.segment, p.channel);
+    const long long part = ends.row(s, cut, p.b, p.segment, channel);
     if constexpr (Only) {
-        store_padded<L>(ends.states + row * P, g, p.sub);
+        store_padded<L>(ends.states + part * P, g, p.sub);
         sum = over_lanes(sum);
-        if (p.sub == 0) ends.sums[row] = sum;
+        if (p.sub == 0) ends.sums[part] = sum;
     } else {
-        for (int t = max(from + kTile, t0) + p.sub; t < t1; t += LPC) {
-            dx[t * s.x_stride] = from_float<T>(0.0f);
-            ddelta[t * s.delta_stride] = from_float<T>(0.0f);
-            if (gate) dgate[t * s.gate_stride] = from_float<T>(0.0f);
+        // The pointers are a tile before the segment's first step.
+        for (int t = max(from + kTile, t0); t + p.sub < t1; t += LPC) {
+            const long long behind = t - t0 + kTile;
+            lane_at(dx + behind * s.x_stride, lane.x) = from_float<T>(0.0f);
+            lane_at(ddelta + behind * s.delta_stride, lane.delta) = from_float<T>(0.0f);
+            if (gate) lane_at(dgate + behind * s.gate_stride, lane.gate) = from_float<T>(0.0f);
         }
         if (a.dstate_in && p.segment == 0)
-            store_states<L>(a.dstate_in + (static_cast<long long>(p.b) * s.channels + p.channel) * s.order, g, p.sub, s.order);
-        store_padded<L>(a.workspace + parts.da + row * P, da, p.sub);
+            store_states<L>(a.dstate_in + (static_cast<long long>(p.b) * s.channels + channel) * s.order, g, p.sub, s.order);
+        store_padded<L>(a.workspace + parts.da + part * P, da, p.sub);
         dskip = over_lanes(dskip);
         dbias = over_lanes(dbias);
         if (p.sub == 0) {
-            a.workspace[parts.pairs + 2 * row] = dskip;
-            a.workspace[parts.pairs + 2 * row + 1] = dbias;
+            a.workspace[parts.pairs + 2 * part] = dskip;
+            a.workspace[parts.pairs + 2 * part + 1] = dbias;
         }
     }
 }

@@ -10,16 +10,31 @@
 namespace thff {
 namespace {
 
-Cut cut_of(const StateShape& s) {
+// Segments of the steps.  They cost a kernel over the steps that only finds the segments' ends, 0.4
+// (forward) and 0.2 (backward) of the time of the steps themselves, and where there is one wave a
+// SIMD (1024 in all) the steps take 0.8 of it with two and more.  bfloat16, order 16, us a call by
+// one segment against these: forward 7 x 1000 x 2048 (896 waves) 94 and 8 x 4096 x 2048 (1024)
+// 444 against 82 and 533, 1 x 65536 x 1024 (64) 6775 against 560; backward 8 x 4096 x 2048 1210
+// against 1105, float 33 x 512 x 96 in two groups (264) 181 against 82.
+int segments_of(long long waves, int n, bool backward) {
+    const long long few = backward ? 1024 : 832, wanted = backward ? 8192 : 4096;
+    if (waves == 0 || waves > few || n < (backward ? 128 : 256)) return 1;
+    return static_cast<int>(std::min<long long>((wanted + waves - 1) / waves, n / 64));
+}
+
+Cut cut_of(const StateShape& s, bool backward) {
     return with_lanes(s.order, [&](auto lanes) {
         using L = decltype(lanes);
         Cut cut;
         const int each = s.channels / s.groups;
         cut.padded = L::P;
         cut.slabs = (each + L::kSlab - 1) / L::kSlab;
-        cut.segments = 1;
-        cut.steps = (s.n + kStateBlock - 1) / kStateBlock * kStateBlock;
-        cut.blocks = static_cast<long long>(s.batch) * s.groups * cut.slabs * cut.segments;
+        const long long columns = static_cast<long long>(s.batch) * s.groups * cut.slabs;
+        const int blocks = (s.n + kStateBlock - 1) / kStateBlock;
+        const int want = segments_of(columns * kStateWaves, s.n, backward);
+        cut.steps = (blocks + want - 1) / want * kStateBlock;
+        cut.segments = s.n > 0 ? (s.n + cut.steps - 1) / cut.steps : 1;
+        cut.blocks = columns * cut.segments;
         return cut;
     });
 }
@@ -35,30 +50,33 @@ auto with_type(int precision, F f) {
 
 long long state_saved_bytes(const StateShape& s) {
     const long long tiles = (s.n + kStateTile - 1) / kStateTile;
-    return 4 * s.batch * tiles * s.channels * cut_of(s).padded;
+    return 4 * s.batch * tiles * s.channels * cut_of(s, false).padded;
+}
+
+long long state_forward_bytes(const StateShape& s) {
+    return s.channels == 0 ? 0 : 4 * Parts(s, cut_of(s, false)).shared;
 }
 
 long long state_workspace_bytes(const StateShape& s) {
-    if (s.channels == 0) return 0;
-    return Parts(s, cut_of(s)).bytes(s);
+    return s.channels == 0 ? 0 : std::max(state_forward_bytes(s), Parts(s, cut_of(s, true)).bytes(s));
 }
 
 bool state_fits(const StateShape& s) {
-    const Cut cut = cut_of(s);
     // Sizes of the buffers in bytes, from above.
+    const Cut cut = cut_of(s, true);
     const __int128 rows = static_cast<__int128>(s.batch) * s.n;
     const __int128 shared = rows * s.groups * cut.slabs * 2 * cut.padded;
-    const __int128 states = (static_cast<__int128>(s.batch) * cut.segments + rows / kStateTile + s.batch) * s.channels * (cut.padded + 4);
+    const __int128 states = (static_cast<__int128>(s.batch) * (cut.segments + 1) + rows / kStateTile) * s.channels * (cut.padded + 4);
     return 4 * (shared + 2 * states) < static_cast<__int128>(1) << 62 && cut.blocks <= 1LL << 36;
 }
 
 hipError_t launch_state_scan(const StateShape& s, const StateForward& a, hipStream_t stream) {
-    const Cut cut = cut_of(s);
+    const Cut cut = cut_of(s, false);
     return with_type(s.precision, [&](auto v) { return launch_state_forward<decltype(v)>(s, a, cut, stream); });
 }
 
 hipError_t launch_state_scan_backward(const StateShape& s, const StateBackward& a, hipStream_t stream) {
-    const Cut cut = cut_of(s);
+    const Cut cut = cut_of(s, true);
     return with_type(s.precision, [&](auto v) { return launch_state_backward<decltype(v)>(s, a, cut, stream); });
 }
 
