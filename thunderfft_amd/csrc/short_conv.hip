@@ -8,6 +8,7 @@
 // A lane takes 16 bytes of channels and some steps one after the other, with the last K - 1 rows
 // in registers.
 #include <algorithm>
+#include <type_traits>
 
 #include "block.hpp"
 #include "sequence_io.hpp"
@@ -69,7 +70,7 @@ struct Taps {
 // Steps of a lane forward.
 constexpr int kSteps = 16;
 
-template <class T, int V, int K, int TS>
+template <class T, int V, int K, bool Silu, int TS>
 __global__ __launch_bounds__(kLanes) void conv_forward(ConvShape s, ConvForward a, int vectors, long long tiles) {
     constexpr int H = K - 1;
     const long long lanes = s.batch * tiles * vectors;
@@ -80,6 +81,11 @@ __global__ __launch_bounds__(kLanes) void conv_forward(ConvShape s, ConvForward 
         const int b = static_cast<int>(column / tiles), t0 = static_cast<int>(column - b * tiles) * TS;
         const int length = length_of(a.lengths, b, s.n);
         const T* x = static_cast<const T*>(a.x) + b * static_cast<long long>(s.n) * s.x_stride + c.at;
+        if (t0 > 0 && t0 >= length) {
+            T* y = static_cast<T*>(a.y) + (b * static_cast<long long>(s.n) + t0) * s.y_stride + c.at;
+            for (int j = 0; j < TS && t0 + j < s.n; ++j) store_pack<T, V>(y + j * s.y_stride, pack<T, V>{});
+            continue;
+        }
         const Taps<V, K> taps(a.weight, a.bias, c.at);
         pack<T, V> in[TS + H];
         int slot = b;
@@ -96,7 +102,13 @@ __global__ __launch_bounds__(kLanes) void conv_forward(ConvShape s, ConvForward 
 #pragma unroll
             for (int k = 0; k < H; ++k) in[k] = load_pack<T, V>(x + (t0 - H + k) * s.x_stride);
         }
-        if (s.n > 0) {
+        T* y = static_cast<T*>(a.y) + b * static_cast<long long>(s.n) * s.y_stride + c.at + t0 * s.y_stride;
+        const bool whole = t0 + TS <= s.n;
+        if (whole) {
+            const T* from = x + t0 * s.x_stride;
+#pragma unroll
+            for (int j = 0; j < TS; ++j) in[H + j] = load_pack<T, V>(from + j * s.x_stride);
+        } else if (s.n > 0) {
 #pragma unroll
             for (int j = 0; j < TS; ++j) in[H + j] = load_pack<T, V>(x + min(t0 + j, s.n - 1) * s.x_stride);
         }
@@ -120,21 +132,26 @@ __global__ __launch_bounds__(kLanes) void conv_forward(ConvShape s, ConvForward 
             for (int k = 0; k < H; ++k)
                 store_own<T, V>(to + static_cast<long long>(k) * s.channels, last[k], c.skip);
         }
-        T* y = static_cast<T*>(a.y) + b * static_cast<long long>(s.n) * s.y_stride + c.at;
+        const auto outputs = [&](auto all) {
 #pragma unroll
-        for (int j = 0; j < TS; ++j) {
-            if (t0 + j >= s.n) break;
-            pack<T, V> out;
+            for (int j = 0; j < TS; ++j) {
+                if (!decltype(all)::value && t0 + j >= s.n) break;
+                pack<T, V> out;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float p = taps.bias[v];
+                for (int v = 0; v < V; ++v) {
+                    float p = taps.bias[v];
 #pragma unroll
-                for (int k = 0; k < K; ++k) p = fmaf(taps.w[k][v], to_float<T>(in[j + k][v]), p);
-                if (s.silu) p *= opened(p);
-                out[v] = from_float<T>(t0 + j < length ? p : 0.0f);
+                    for (int k = 0; k < K; ++k) p = fmaf(taps.w[k][v], to_float<T>(in[j + k][v]), p);
+                    if constexpr (Silu) p *= opened(p);
+                    out[v] = from_float<T>(decltype(all)::value || t0 + j < length ? p : 0.0f);
+                }
+                if (decltype(all)::value) store_pack<T, V>(y + j * s.y_stride, out);
+                else store_own<T, V>(y + j * s.y_stride, out, c.skip);
             }
-            store_own<T, V>(y + (t0 + j) * s.y_stride, out, c.skip);
-        }
+        };
+        // The first tile's values may depend on states that another lane is replacing.
+        if (whole && t0 + TS <= length && (c.skip == 0 || t0 > 0)) outputs(std::true_type{});
+        else outputs(std::false_type{});
     }
 }
 
@@ -146,9 +163,12 @@ struct ConvParts {
     long long count;  // parts of the weights' gradients
 };
 
-constexpr int kAhead = 8;  // rows loaded at a time
+constexpr int kAhead = 4;  // rows loaded at a time
 
-template <class T, int V, int K>
+// A lane takes a chunk of steps in blocks of kAhead rows, the next block's loads under way.  dxe of a
+// step needs dp of the width - 1 steps behind it, so dx comes that many steps late, and a lane goes so
+// many steps into the next chunk.  Blocks with all their steps in the chunk have no branches.
+template <class T, int V, int K, bool Silu>
 __global__ __launch_bounds__(kLanes) void conv_backward(ConvShape s, ConvBackward a, int vectors, ConvParts g) {
     constexpr int H = K - 1;
     __shared__ float lds[V * (K + 1)][kLanes];
@@ -169,68 +189,103 @@ __global__ __launch_bounds__(kLanes) void conv_backward(ConvShape s, ConvBackwar
         T* dx = static_cast<T*>(a.dx) + first * s.x_stride + c.at;
         const long long state = static_cast<long long>(b) * H * s.channels + c.at;
         const Taps<V, K> taps(a.weight, a.bias, c.at);
-        // xe[t ... t + K - 1] and dp[t - K + 1 ... t].
-        float xe[K][V] = {}, dp[K][V] = {};
+        // xe[j] and dp[j]: of the step H before the block's j-th.
+        float xe[kAhead + H][V], dp[kAhead + H][V];
 #pragma unroll
         for (int k = 0; k < H; ++k) {
             pack<T, V> in = {};
             if (t0 > 0) in = load_pack<T, V>(x + (t0 - H + k) * s.x_stride);
             else if (a.state_in) in = load_pack<T, V>(static_cast<const T*>(a.state_in) + state + static_cast<long long>(k) * s.channels);
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                xe[k + 1][v] = t0 == 0 || t0 - H + k < length ? to_float<T>(in[v]) : 0.0f;
+            for (int v = 0; v < V; ++v) {
+                xe[kAhead + k][v] = t0 == 0 || t0 - H + k < length ? to_float<T>(in[v]) : 0.0f;
+                dp[kAhead + k][v] = 0.0f;
+            }
         }
         const int end = t1 + H;
-        for (int t = t0; t < end; t += kAhead) {
-            pack<T, V> xs[kAhead], ds[kAhead];
-            if (s.n > 0) {
+        pack<T, V> nx[kAhead], ny[kAhead];
+        const auto load = [&](int t) {
+            if (t + kAhead <= s.n) {
+                const T *from_x = x + t * s.x_stride, *from_y = dy + t * s.y_stride;
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    nx[j] = load_pack<T, V>(from_x + j * s.x_stride);
+                    ny[j] = load_pack<T, V>(from_y + j * s.y_stride);
+                }
+            } else if (s.n > 0) {
 #pragma unroll
                 for (int j = 0; j < kAhead; ++j) {
                     const long long at = min(t + j, s.n - 1);
-                    xs[j] = load_pack<T, V>(x + at * s.x_stride);
-                    ds[j] = load_pack<T, V>(dy + at * s.y_stride);
+                    nx[j] = load_pack<T, V>(x + at * s.x_stride);
+                    ny[j] = load_pack<T, V>(dy + at * s.y_stride);
                 }
             }
+        };
+        // Whole: every step counts, and so does each dx.
+        const auto block = [&](auto whole, int t) {
+            constexpr bool kWhole = decltype(whole)::value;
+            pack<T, V> ys[kAhead];
+#pragma unroll
+            for (int k = 0; k < H; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    xe[k][v] = xe[kAhead + k][v];
+                    dp[k][v] = dp[kAhead + k][v];
+                }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                ys[j] = ny[j];
+#pragma unroll
+                for (int v = 0; v < V; ++v) xe[H + j][v] = kWhole || t + j < length ? to_float<T>(nx[j][v]) : 0.0f;
+            }
+            if (t + kAhead < end) load(t + kAhead);
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 const int e = t + j;
-                if (e >= end) break;
-                const bool inside = e < length;
-                pack<T, V> out, after = {};
-                const bool behind = a.dstate_out && e >= length && e < length + H;
-                if (behind)
-                    after = load_pack<T, V>(static_cast<const T*>(a.dstate_out) + state + static_cast<long long>(e - length) * s.channels);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-#pragma unroll
-                    for (int k = 0; k < H; ++k) {
-                        xe[k][v] = xe[k + 1][v];
-                        dp[k][v] = dp[k + 1][v];
-                    }
-                    xe[H][v] = inside ? to_float<T>(xs[j][v]) : 0.0f;
                     float p = taps.bias[v];
 #pragma unroll
-                    for (int k = 0; k < K; ++k) p = fmaf(taps.w[k][v], xe[k][v], p);
-                    float d = to_float<T>(ds[j][v]);
-                    if (s.silu) {
+                    for (int k = 0; k < K; ++k) p = fmaf(taps.w[k][v], xe[j + k][v], p);
+                    float d = to_float<T>(ys[j][v]);
+                    if constexpr (Silu) {
                         const float f = opened(p);
                         d *= fmaf(f * (1.0f - f), p, f);
                     }
-                    d = inside ? d : 0.0f;
-                    dp[H][v] = d;
-                    if (e < t1) {
+                    d = kWhole || e < length ? d : 0.0f;
+                    dp[H + j][v] = d;
+                    if (kWhole || e < t1) {
 #pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][v] = fmaf(d, xe[k][v], dw[k][v]);
+                        for (int k = 0; k < K; ++k) dw[k][v] = fmaf(d, xe[j + k][v], dw[k][v]);
                         db[v] += d;
                     }
-                    float sum = to_float<T>(after[v]);
-#pragma unroll
-                    for (int k = 0; k < K; ++k) sum = fmaf(taps.w[k][v], dp[H - k][v], sum);
-                    out[v] = from_float<T>(e - H < length ? sum : 0.0f);
                 }
-                if (e - H >= t0) store_pack<T, V>(dx + (e - H) * s.x_stride, out);
-                else if (t0 == 0 && a.dstate_in) store_pack<T, V>(static_cast<T*>(a.dstate_in) + state + static_cast<long long>(e) * s.channels, out);
             }
+            T* to = dx + (t - H) * s.x_stride;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int e = t + j;
+                if (!kWhole && e >= end) break;
+                pack<T, V> out, after = {};
+                if (!kWhole && a.dstate_out && e >= length && e < length + H)
+                    after = load_pack<T, V>(static_cast<const T*>(a.dstate_out) + state + static_cast<long long>(e - length) * s.channels);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float sum = kWhole ? 0.0f : to_float<T>(after[v]);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) sum = fmaf(taps.w[k][v], dp[H + j - k][v], sum);
+                    out[v] = from_float<T>(kWhole || e - H < length ? sum : 0.0f);
+                }
+                if (kWhole || e - H >= t0)
+                    store_pack<T, V>(to + j * s.x_stride, out);
+                else if (t0 == 0 && a.dstate_in)
+                    store_pack<T, V>(static_cast<T*>(a.dstate_in) + state + static_cast<long long>(e) * s.channels, out);
+            }
+        };
+        load(t0);
+        for (int t = t0; t < end; t += kAhead) {
+            if (t > t0 && t + kAhead <= t1 && t + kAhead <= length) block(std::true_type{}, t);
+            else block(std::false_type{}, t);
         }
     }
     if (!a.dweight && !a.dbias) return;
@@ -307,10 +362,10 @@ struct Kind {
     static constexpr int V = V_, K = K_;
 };
 
-// 16 bytes of channels a lane; fewer channels than that, one.
-template <class T, class F>
+// Bytes bytes of channels a lane; fewer channels than that, one.
+template <class T, int Bytes, class F>
 auto with_kind(const ConvShape& s, F f) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = Bytes / sizeof(T);
     if (s.channels < V) {
         if (s.width == 2) return f(Kind<1, 2>{});
         if (s.width == 3) return f(Kind<1, 3>{});
@@ -320,6 +375,9 @@ auto with_kind(const ConvShape& s, F f) {
     if (s.width == 3) return f(Kind<V, 3>{});
     return f(Kind<V, 4>{});
 }
+
+// Backward, where a channel takes four times the registers.
+constexpr int kBackwardBytes = 8;
 
 int vectors_of(const ConvShape& s, int v) { return (s.channels + v - 1) / v; }
 
@@ -337,13 +395,13 @@ ConvParts parts_of(const ConvShape& s, int v) {
     return g;
 }
 
-template <class T, int V, int K, int TS>
+template <class T, int V, int K, bool Silu, int TS>
 hipError_t launch_forward(const ConvShape& s, const ConvForward& a, hipStream_t stream) {
     const int vectors = vectors_of(s, V);
     const long long tiles = std::max<long long>(1, (s.n + TS - 1LL) / TS);
     const __int128 lanes = static_cast<__int128>(s.batch) * tiles * vectors;
     const long long blocks = static_cast<long long>(std::min<__int128>((lanes + kLanes - 1) / kLanes, 1 << 23));
-    conv_forward<T, V, K, TS><<<static_cast<unsigned>(blocks), kLanes, 0, stream>>>(s, a, vectors, tiles);
+    conv_forward<T, V, K, Silu, TS><<<static_cast<unsigned>(blocks), kLanes, 0, stream>>>(s, a, vectors, tiles);
     return hipGetLastError();
 }
 
@@ -352,7 +410,7 @@ hipError_t launch_forward(const ConvShape& s, const ConvForward& a, hipStream_t 
 long long conv_workspace_bytes(const ConvShape& s) {
     if (s.batch == 0 || s.n == 0 || s.channels == 0) return 0;
     const long long parts = with_type(s.precision, [&](auto v) {
-        return with_kind<decltype(v)>(s, [&](auto kind) { return parts_of(s, decltype(kind)::V).count; });
+        return with_kind<decltype(v), kBackwardBytes>(s, [&](auto kind) { return parts_of(s, decltype(kind)::V).count; });
     });
     return 4 * parts * (s.width + 1) * s.channels;
 }
@@ -360,10 +418,13 @@ long long conv_workspace_bytes(const ConvShape& s) {
 hipError_t launch_short_conv(const ConvShape& s, const ConvForward& a, hipStream_t stream) {
     return with_type(s.precision, [&](auto v) {
         using T = decltype(v);
-        return with_kind<T>(s, [&](auto kind) {
+        return with_kind<T, 16>(s, [&](auto kind) {
             using Q = decltype(kind);
-            if (s.n <= 1) return launch_forward<T, Q::V, Q::K, 1>(s, a, stream);
-            return launch_forward<T, Q::V, Q::K, kSteps>(s, a, stream);
+            if (s.n <= 1)
+                return s.silu ? launch_forward<T, Q::V, Q::K, true, 1>(s, a, stream)
+                              : launch_forward<T, Q::V, Q::K, false, 1>(s, a, stream);
+            return s.silu ? launch_forward<T, Q::V, Q::K, true, kSteps>(s, a, stream)
+                          : launch_forward<T, Q::V, Q::K, false, kSteps>(s, a, stream);
         });
     });
 }
@@ -371,7 +432,7 @@ hipError_t launch_short_conv(const ConvShape& s, const ConvForward& a, hipStream
 hipError_t launch_short_conv_backward(const ConvShape& s, const ConvBackward& a, hipStream_t stream) {
     return with_type(s.precision, [&](auto v) {
         using T = decltype(v);
-        return with_kind<T>(s, [&](auto kind) {
+        return with_kind<T, kBackwardBytes>(s, [&](auto kind) {
             using Q = decltype(kind);
             const int vectors = vectors_of(s, Q::V);
             const ConvParts g = parts_of(s, Q::V);
@@ -380,8 +441,8 @@ hipError_t launch_short_conv_backward(const ConvShape& s, const ConvBackward& a,
             if (none) call.dweight = call.dbias = nullptr;
             if (s.batch > 0) {
                 const long long slabs = (vectors + g.across - 1) / g.across;
-                conv_backward<T, Q::V, Q::K>
-                    <<<static_cast<unsigned>(g.count * slabs), kLanes, 0, stream>>>(s, call, vectors, g);
+                const auto kernel = s.silu ? conv_backward<T, Q::V, Q::K, true> : conv_backward<T, Q::V, Q::K, false>;
+                kernel<<<static_cast<unsigned>(g.count * slabs), kLanes, 0, stream>>>(s, call, vectors, g);
             }
             if (a.dweight || a.dbias) {
                 const long long sums = static_cast<long long>(s.width + 1) * s.channels;

@@ -10,6 +10,9 @@ dim3 grid_of(long long blocks) {
     return dim3(static_cast<unsigned>(std::min(blocks, kMost)), static_cast<unsigned>((blocks + kMost - 1) / kMost));
 }
 
+// From so many lanes on a lane of a single step takes two sequences.
+constexpr long long kManyLanes = 1 << 20;
+
 // Lanes of a channel for one step.
 template <class F>
 auto with_step_lanes(int order, F f) {
@@ -28,9 +31,13 @@ hipError_t launch_state_forward(const StateShape& s, const StateForward& a, cons
     if (s.n == 1 && !a.saved)
         return with_step_lanes(s.order, [&](auto lanes) {
             constexpr int N = decltype(lanes)::value;
-            const long long count = static_cast<long long>(s.batch) * s.channels * N;
-            state_step<T, N><<<grid_of((count + kLanes - 1) / kLanes), kLanes, 0, stream>>>(s, a);
-            return hipGetLastError();
+            const auto launch = [&](auto kernel, int rows) {
+                const long long count = static_cast<long long>((s.batch + rows - 1) / rows) * s.channels * N;
+                kernel<<<grid_of((count + kLanes - 1) / kLanes), kLanes, 0, stream>>>(s, a);
+                return hipGetLastError();
+            };
+            return static_cast<long long>(s.batch) * s.channels * N < kManyLanes ? launch(state_step<T, N, 1>, 1)
+                                                                                : launch(state_step<T, N, 2>, 2);
         });
     return with_lanes(s.order, [&](auto lanes) {
         using L = decltype(lanes);

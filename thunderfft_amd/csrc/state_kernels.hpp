@@ -656,65 +656,89 @@ __global__ __launch_bounds__(1024) void add_weights(StateShape s, StateBackward 
     }
 }
 
-// One step (n = 1: a token of each sequence): 4 states a lane, Lanes of them a channel.
-template <class T, int Lanes>
-__global__ __launch_bounds__(kLanes) void state_step(StateShape s, StateForward a) {
-    const long long i = (block_index() * kLanes + threadIdx.x) / Lanes;
-    const int b = static_cast<int>(i / s.channels), channel = static_cast<int>(i - static_cast<long long>(b) * s.channels);
-    if (b >= s.batch) return;
-    const int sub = threadIdx.x % Lanes, at = sub * 4, some = min(4, s.order - at);
-    int slot = b;
-    if (a.slots) {
-        slot = a.slots[b];
-        if (slot < 0 || slot >= s.states) slot = -1;
-    }
-    const bool on = length_of(a.lengths, b, 1) > 0;
-    const long long state = (static_cast<long long>(slot) * s.channels + channel) * s.order + at;
+// One step (n = 1: a token of each sequence): 4 states a lane, Each lanes of them a channel, and Rows
+// sequences one after the other, whose loads are all under way together and share a's.
+template <class T, int Each, int Rows>
+__global__ __launch_bounds__(kLanes, 6) void state_step(StateShape s, StateForward a) {
+    const long long i = (block_index() * kLanes + threadIdx.x) / Each;
+    const int b0 = static_cast<int>(i / s.channels), channel = static_cast<int>(i - static_cast<long long>(b0) * s.channels);
+    if (b0 >= (s.batch + Rows - 1) / Rows) return;
+    const int sub = threadIdx.x % Each, at = sub * 4, some = min(4, s.order - at);
     const int shared = channel / (s.channels / s.groups) * s.order + at;
-    const float* decay = a.a + static_cast<long long>(channel) * s.order + at;
-    const T* bs = static_cast<const T*>(a.b) + b * s.b_stride + shared;
-    const T* cs = static_cast<const T*>(a.c) + b * s.c_stride + shared;
-    pack<float, 4> h = {}, rate = {};
-    pack<T, 4> bv = {}, cv = {};
-    const bool stored = a.state_in && slot >= 0;
-    if (some == 4) {
-        if (stored) h = load_pack<float, 4>(a.state_in + state);
-        rate = load_pack<float, 4>(decay);
-        bv = load_pack<T, 4>(bs);
-        cv = load_pack<T, 4>(cs);
-    } else {
+    // Values of one lane's states, 0 where it has none.
+    const auto load = [&](const auto* from) {
+        using U = std::remove_const_t<std::remove_pointer_t<decltype(from)>>;
+        pack<U, 4> v = {};
+        if (some == 4) {
+            v = load_pack<U, 4>(from);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < some) {
-                if (stored) h[k] = a.state_in[state + k];
-                rate[k] = decay[k];
-                bv[k] = bs[k];
-                cv[k] = cs[k];
+            for (int k = 0; k < 4; ++k)
+                if (k < some) v[k] = from[k];
+        }
+        return v;
+    };
+    pack<float, 4> h[Rows];
+    pack<T, 4> bv[Rows], cv[Rows];
+    T x[Rows], delta[Rows], gate[Rows];
+    long long state[Rows];
+    int slot[Rows];
+    bool on[Rows];
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        // Sequences behind the last are the last, and not stored.
+        const int b = min(b0 * Rows + r, s.batch - 1);
+        slot[r] = a.slots ? a.slots[b] : b;
+        if (a.slots && (slot[r] < 0 || slot[r] >= s.states)) slot[r] = -1;
+        on[r] = length_of(a.lengths, b, 1) > 0;
+        state[r] = (static_cast<long long>(slot[r]) * s.channels + channel) * s.order + at;
+        x[r] = static_cast<const T*>(a.x)[b * s.x_stride + channel];
+        delta[r] = static_cast<const T*>(a.delta)[b * s.delta_stride + channel];
+        if (a.gate) gate[r] = static_cast<const T*>(a.gate)[b * s.gate_stride + channel];
+        bv[r] = load(static_cast<const T*>(a.b) + b * s.b_stride + shared);
+        cv[r] = load(static_cast<const T*>(a.c) + b * s.c_stride + shared);
+    }
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        h[r] = pack<float, 4>{};
+        if (a.state_in && slot[r] >= 0) h[r] = load(a.state_in + state[r]);
+    }
+    const pack<float, 4> rate = load(a.a + static_cast<long long>(channel) * s.order + at);
+    const float bias = a.delta_bias ? a.delta_bias[channel] : 0.0f, skip = a.skip ? a.skip[channel] : 0.0f;
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        const int b = b0 * Rows + r;
+        const float xv = to_float<T>(x[r]), dt = softplus(to_float<T>(delta[r]) + bias), u = dt * xv;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float next = fmaf(__builtin_amdgcn_exp2f(dt * (rate[k] * kLog2e)), h[r][k], u * to_float<T>(bv[r][k]));
+            if (on[r]) h[r][k] = next;
+            if (k < some) sum = fmaf(to_float<T>(cv[r][k]), next, sum);
+        }
+        if constexpr (Each >= 2) sum += mirrored<2>(sum);
+        if constexpr (Each >= 4) sum += mirrored<4>(sum);
+        if constexpr (Each >= 8) sum += mirrored<8>(sum);
+        if constexpr (Each >= 16) sum += mirrored<16>(sum);
+        sum = fmaf(skip, xv, sum);
+        if (a.gate) {
+            const float z = to_float<T>(gate[r]);
+            sum *= z * opened(z);
+        }
+        if (b >= s.batch) continue;
+        if (sub == 0) static_cast<T*>(a.y)[b * s.y_stride + channel] = from_float<T>(on[r] ? sum : 0.0f);
+        if (a.state_out && slot[r] >= 0) {
+            // Few states through the caches, as the next token reads them soon; many past them.
+            if (some == 4 && Rows > 1) {
+                store_pack<float, 4>(a.state_out + state[r], h[r]);
+            } else if (some == 4) {
+                *reinterpret_cast<pack<float, 4>*>(a.state_out + state[r]) = h[r];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k < some) a.state_out[state[r] + k] = h[r][k];
             }
-    }
-    const float x = to_float<T>(static_cast<const T*>(a.x)[b * s.x_stride + channel]);
-    const float raw = to_float<T>(static_cast<const T*>(a.delta)[b * s.delta_stride + channel]);
-    const float z = a.gate ? to_float<T>(static_cast<const T*>(a.gate)[b * s.gate_stride + channel]) : 0.0f;
-    const float dt = softplus(raw + (a.delta_bias ? a.delta_bias[channel] : 0.0f)), u = dt * x;
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float next = fmaf(__builtin_amdgcn_exp2f(dt * (rate[k] * kLog2e)), h[k], u * to_float<T>(bv[k]));
-        if (on) h[k] = next;
-        if (k < some) sum = fmaf(to_float<T>(cv[k]), next, sum);
-    }
-    if constexpr (Lanes >= 2) sum += mirrored<2>(sum);
-    if constexpr (Lanes >= 4) sum += mirrored<4>(sum);
-    if constexpr (Lanes >= 8) sum += mirrored<8>(sum);
-    if constexpr (Lanes >= 16) sum += mirrored<16>(sum);
-    if (a.skip) sum = fmaf(a.skip[channel], x, sum);
-    if (a.gate) sum *= z * opened(z);
-    if (sub == 0) static_cast<T*>(a.y)[b * s.y_stride + channel] = from_float<T>(on ? sum : 0.0f);
-    if (a.state_out && slot >= 0) {
-        // Through the caches: the next token reads it soon.
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < some) a.state_out[state + k] = h[k];
+        }
     }
 }
 
