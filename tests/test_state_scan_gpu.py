@@ -111,7 +111,8 @@ def compare(T, v, lengths=None, **how):
 @pytest.mark.parametrize("T", list(oracle.TYPES))
 @pytest.mark.parametrize("size", [(1, 1, 1, 1), (2, 2, 3, 4), (3, 3, 17, 5), (2, 15, 8, 8), (1, 16, 64, 16), (2, 17, 65, 16),
                                   (3, 31, 40, 12), (1, 33, 130, 3), (2, 64, 16, 16), (1, 100, 33, 24), (2, 50, 20, 32), (1, 70, 9, 33),
-                                  (2, 40, 12, 64), (40, 5, 48, 16)], ids=str)
+                                  (2, 40, 12, 64), (40, 5, 48, 16), (130, 45, 24, 16), (140, 70, 9, 12),
+                                  (300, 20, 17, 16)], ids=str)
 def test_sizes(T, size):
     compare(T, values(sum(size), T, *size))
 
@@ -171,6 +172,12 @@ def test_long_sequences(T, size):
 def test_long_sequences_that_end_early(T):
     v = values(6, T, 4, 2100, 24, 16)
     compare(T, v, ends(2100, 1000, 5, 0))
+
+
+def test_many_sequences_that_end_early():
+    """As many waves as have 8 lanes a channel."""
+    v = values(19, "half", 150, 100, 40, 16)
+    compare("half", v, (torch.arange(150, device="cuda") * 37 % 101).to(torch.int32))
 
 
 @pytest.mark.parametrize("T", list(oracle.TYPES))

@@ -39,16 +39,18 @@ hipError_t launch_state_forward(const StateShape& s, const StateForward& a, cons
             return static_cast<long long>(s.batch) * s.channels * N < kManyLanes ? launch(state_step<T, N, 1>, 1)
                                                                                 : launch(state_step<T, N, 2>, 2);
         });
-    return with_lanes(s.order, [&](auto lanes) {
+    return with_forward_lanes(s, [&](auto lanes) {
         using L = decltype(lanes);
+        const auto launch = [&](auto kernel) {
+            kernel<<<grid_of(cut.blocks), L::kLanes, 0, stream>>>(s, a, cut);
+            return hipGetLastError();
+        };
         if (cut.segments > 1) {
-            state_forward<T, L, true, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
-            const hipError_t err = hipGetLastError();
+            const hipError_t err = launch(state_forward<T, L, true, false, false>);
             if (err != hipSuccess) return err;
         }
-        if (a.saved) state_forward<T, L, false, true><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
-        else state_forward<T, L, false, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
-        return hipGetLastError();
+        if (a.saved) return a.gate ? launch(state_forward<T, L, false, true, true>) : launch(state_forward<T, L, false, true, false>);
+        return a.gate ? launch(state_forward<T, L, false, false, true>) : launch(state_forward<T, L, false, false, false>);
     });
 }
 
@@ -58,14 +60,14 @@ hipError_t launch_state_backward(const StateShape& s, const StateBackward& a, co
         using L = decltype(lanes);
         if (s.batch > 0) {
             if (cut.segments > 1) {
-                state_backward<T, L, true><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+                state_backward<T, L, true><<<grid_of(cut.blocks), L::kLanes, 0, stream>>>(s, a, cut);
                 const hipError_t err = hipGetLastError();
                 if (err != hipSuccess) return err;
             }
-            state_backward<T, L, false><<<grid_of(cut.blocks), kLanes, 0, stream>>>(s, a, cut);
+            state_backward<T, L, false><<<grid_of(cut.blocks), L::kLanes, 0, stream>>>(s, a, cut);
             hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
-            const long long shared = static_cast<long long>(s.batch) * s.n * s.groups * 2 * cut.padded;
+            const long long shared = static_cast<long long>(s.batch) * s.n * s.groups * 2 * cut.padded / 4;
             if (shared > 0) {
                 const long long blocks = std::min((shared + kLanes - 1) / kLanes, 1LL << 20);
                 add_shared<T><<<static_cast<unsigned>(blocks), kLanes, 0, stream>>>(s, a, cut);

@@ -18,7 +18,7 @@
 namespace thff {
 namespace {
 
-constexpr int kWaves = kStateWaves, kLanes = 64 * kWaves, kBlock = kStateBlock, kTile = kStateTile;
+constexpr int kLanes = 256, kBlock = kStateBlock, kTile = kStateTile;
 
 __device__ __forceinline__ int length_of(const int* lengths, int b, int n) {
     return lengths ? min(max(lengths[b], 0), n) : n;
@@ -126,14 +126,15 @@ struct Offsets {
 // b and c of N steps: loaded ahead into registers, then to LDS as [step][lane of a channel][b's, c's].
 template <class T, class L, int N>
 struct Shared {
-    static constexpr int kEach = (N * L::P + kLanes - 1) / kLanes;
+    static constexpr int kEach = (N * L::P + L::kLanes - 1) / L::kLanes;
     using Rows = float[L::LPC][2 * L::S];
-    static constexpr int kRows = kLanes / L::P;  // steps loaded at a time
+    static constexpr int kRows = L::kLanes / L::P;  // steps loaded at a time
     T b[kEach], c[kEach];
 
     // Steps from t0 on, where bs and cs are; b_at, c_at: the offsets of the lane's row of them and its state.
+    template <bool Whole = false>
     __device__ __forceinline__ void load(const StateShape& s, const T* bs, const T* cs, unsigned b_at, unsigned c_at, int t0) {
-        if (t0 + kEach * kRows <= s.n) {
+        if (Whole || t0 + kEach * kRows <= s.n) {
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 b[e] = lane_at(bs, b_at);
@@ -155,8 +156,8 @@ struct Shared {
     __device__ __forceinline__ void store(const StateShape& s, Rows* to, int t0, int end) const {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int i = e * kLanes + threadIdx.x, st = i % L::P, t = i / L::P;
-            if (N * L::P % kLanes != 0 && t >= N) break;
+            const int i = e * L::kLanes + threadIdx.x, st = i % L::P, t = i / L::P;
+            if (N * L::P % L::kLanes != 0 && t >= N) break;
             const bool on = t0 + t < end && st < s.order;
             to[t][st / L::S][st % L::S] = on ? to_float<T>(b[e]) : 0.0f;
             to[t][st / L::S][L::S + st % L::S] = on ? to_float<T>(c[e]) : 0.0f;
@@ -166,12 +167,12 @@ struct Shared {
 
 template <int S>
 __device__ __forceinline__ void load_shared(float (&b)[S], float (&c)[S], const float* row) {
-    using V = float __attribute__((ext_vector_type(S)));
-    const V vb = *reinterpret_cast<const V*>(row), vc = *reinterpret_cast<const V*>(row + S);
+    using V = float __attribute__((ext_vector_type(2 * S)));
+    const V v = *reinterpret_cast<const V*>(row);
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        b[i] = vb[i];
-        c[i] = vc[i];
+        b[i] = v[i];
+        c[i] = v[S + i];
     }
 }
 
@@ -205,10 +206,10 @@ __device__ __forceinline__ void fold(float (&h)[L::S], const float (&decay)[L::S
 // A block of steps that all count has no branches, so that the reads of LDS and the exponentials
 // of one step are under way while those before it are worked on.  Lanes of no channel do as the
 // last channel's, stores included.
-template <class T, class L, bool Only, bool Save>
-__global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForward a, Cut cut) {
+template <class T, class L, bool Only, bool Save, bool Gate>
+__global__ __launch_bounds__(L::kLanes) void state_forward(StateShape s, StateForward a, Cut cut) {
     constexpr int S = L::S, LPC = L::LPC, J = kBlock / LPC;
-    __shared__ alignas(16) float bc[2][kBlock][LPC][2 * S];
+    __shared__ alignas(32) float bc[2][kBlock][LPC][2 * S];
     const long long block = block_index();
     if (block >= cut.blocks) return;
     const Place<L> p(s, cut, block);
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForwa
     const Offsets<L> lane(s, p);
     const T* x = static_cast<const T*>(a.x) + first * s.x_stride + p.base;
     const T* delta = static_cast<const T*>(a.delta) + first * s.delta_stride + p.base;
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + first * s.gate_stride + p.base : nullptr;
+    const T* gate = static_cast<const T*>(a.gate) + first * s.gate_stride + p.base;
     const T* bs = static_cast<const T*>(a.b) + first * s.b_stride + p.group * s.order;
     const T* cs = static_cast<const T*>(a.c) + first * s.c_stride + p.group * s.order;
     T* y = static_cast<T*>(a.y) + first * s.y_stride + p.base;
@@ -251,54 +252,79 @@ __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForwa
     const long long tiles = (s.n + kTile - 1) / kTile;
     float* saved = Save ? a.saved + (p.b * tiles * s.channels + channel) * L::P : nullptr;
 
-    // The next block's values are under way while a block is worked on.
+    // Blocks of steps, LPC of them at a time, each lane with one.  Everything is under way early: what
+    // the LPC steps have loaded is replaced by the next block's once it is used, dt and the gate of
+    // the next LPC steps are worked out next to these steps' states, their b and c read from LDS, and
+    // the next block's b and c go to LDS before this one ends.
     Shared<T, L, kBlock> ahead;
     T nx[J], nd[J], nz[J];
-    const auto load = [&](int t) {
-        ahead.load(s, bs, cs, lane.b, lane.c, t);
-        load_steps<J, LPC>(nx, x, lane.x, s.x_stride, t, p.sub, s.n);
-        load_steps<J, LPC>(nd, delta, lane.delta, s.delta_stride, t, p.sub, s.n);
-        if (!Only && gate) load_steps<J, LPC>(nz, gate, lane.gate, s.gate_stride, t, p.sub, s.n);
-        bs += kBlock * s.b_stride;
-        cs += kBlock * s.c_stride;
-        x += kBlock * s.x_stride;
-        delta += kBlock * s.delta_stride;
-        if (!Only && gate) gate += kBlock * s.gate_stride;
+    struct Own {
+        float x, dt, z;
     };
+    const auto own_of = [&](int j, bool on) {
+        Own o;
+        o.x = on ? to_float<T>(nx[j]) : 0.0f;
+        o.dt = softplus(to_float<T>(nd[j]) + bias);
+        o.dt = on ? o.dt : 0.0f;
+        o.z = 1.0f;
+        if constexpr (Gate) {
+            o.z = to_float<T>(nz[j]);
+            o.z *= opened(o.z);
+        }
+        return o;
+    };
+    Own next = {};
+    float b[2][LPC][S], c[2][LPC][S];
     int which = 0;
+    const auto read = [&](int buffer, int j) {
+#pragma unroll
+        for (int k = 0; k < LPC; ++k) load_shared<S>(b[j & 1][k], c[j & 1][k], bc[buffer][j * LPC + k][p.sub]);
+    };
+    if (t0 < end) {
+        ahead.load(s, bs, cs, lane.b, lane.c, t0);
+        load_steps<J, LPC>(nx, x, lane.x, s.x_stride, t0, p.sub, s.n);
+        load_steps<J, LPC>(nd, delta, lane.delta, s.delta_stride, t0, p.sub, s.n);
+        if (Gate) load_steps<J, LPC>(nz, gate, lane.gate, s.gate_stride, t0, p.sub, s.n);
+        ahead.store(s, bc[0], t0, end);
+        next = own_of(0, t0 + p.sub < end);
+    }
+    // Whole: the block's steps and the next one's all count, and the loads' rows are all there.
     const auto steps = [&](auto whole, int t) {
         constexpr bool kWhole = decltype(whole)::value;
-        ahead.store(s, bc[which], t, end);
-        float xv[J], dt[J], out[J];
-        T zs[J];
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const bool on = kWhole || t + j * LPC + p.sub < end;
-            xv[j] = on ? to_float<T>(nx[j]) : 0.0f;
-            dt[j] = softplus(to_float<T>(nd[j]) + bias);
-            dt[j] = on ? dt[j] : 0.0f;
-            zs[j] = nz[j];
-            sum += dt[j];
-        }
+        static_assert(J % 2 == 0, "the buffers of b and c go on from block to block");
         __syncthreads();
-        load(t + kBlock);
-        // The next LPC steps' b and c are read from LDS while LPC steps are worked on.
-        float b[2][LPC][S], c[2][LPC][S];
-        const auto read = [&](int j) {
-#pragma unroll
-            for (int k = 0; k < LPC; ++k) load_shared<S>(b[j & 1][k], c[j & 1][k], bc[which][j * LPC + k][p.sub]);
-        };
-        read(0);
+        read(which, 0);
         each_step<J>([&](auto j) {
-            if constexpr (j + 1 < J) read(j + 1);
+            if constexpr (j + 1 < J) read(which, j + 1);
+            // The scheduler is kept to this order: left free it gathers the loads and the reads of LDS.
+            __builtin_amdgcn_sched_barrier(0);
+            const int now = t + j * LPC + p.sub;
+            const Own own = next;
+            sum += own.dt;
+            if constexpr (j == 0) {
+                bs += kBlock * s.b_stride;
+                cs += kBlock * s.c_stride;
+                if (kWhole) ahead.template load<true>(s, bs, cs, lane.b, lane.c, t + kBlock);
+                else ahead.load(s, bs, cs, lane.b, lane.c, t + kBlock);
+            }
+            // The step a block on; past the last step, the last one again.
+            const int skipped = kWhole ? kBlock : min(now + kBlock, s.n - 1) - now;
+            nx[j] = lane_at(x + skipped * s.x_stride, lane.x);
+            nd[j] = lane_at(delta + skipped * s.delta_stride, lane.delta);
+            if (Gate) nz[j] = lane_at(gate + skipped * s.gate_stride, lane.gate);
+            x += LPC * s.x_stride;
+            delta += LPC * s.delta_stride;
+            if (Gate) gate += LPC * s.gate_stride;
+            next = own_of((j + 1) % J, kWhole || now + LPC < end);
+            if constexpr (j == J - 1) ahead.store(s, bc[which ^ 1], t + kBlock, end);
             if constexpr (Save && j * LPC % kTile == 0) {
                 if (kWhole || t + j * LPC < end)
                     store_padded<L>(saved + static_cast<long long>((t + j * LPC) / kTile) * s.channels * L::P, h, p.sub);
             }
-            const float u = dt[j] * xv[j];
+            const Spread<LPC> dts(own.dt), us(own.dt * own.x);
             float part[LPC];
             each_step<LPC>([&](auto k) {
-                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u);
+                const float d = dts.template of<k>(), v = us.template of<k>();
                 part[k] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
@@ -306,29 +332,18 @@ __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForwa
                     if (!Only) part[k] = fmaf(c[j & 1][k][i], h[i], part[k]);
                 }
             });
-            if constexpr (!Only) out[j] = fmaf(skip, xv[j], sum_to_lanes<LPC>(part, p.lane));
-        });
-        if constexpr (!Only) {
-            if (gate) {
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const float z = to_float<T>(zs[j]);
-                    out[j] *= z * opened(z);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int now = t + j * LPC + p.sub;
-                if (kWhole) lane_at(y, lane.y) = from_float<T>(out[j]);
-                else if (now < t1) lane_at(y, lane.y) = from_float<T>(now < end ? out[j] : 0.0f);
+            if constexpr (!Only) {
+                const float v = fmaf(skip, own.x, sum_to_lanes<LPC>(part, p.lane)) * own.z;
+                if (kWhole) lane_at(y, lane.y) = from_float<T>(v);
+                else if (now < t1) lane_at(y, lane.y) = from_float<T>(now < end ? v : 0.0f);
                 y += LPC * s.y_stride;
             }
-        }
+        });
         which ^= 1;
     };
-    if (t0 < end) load(t0);
     int t = t0;
-    for (; t + kBlock <= end; t += kBlock) steps(std::true_type{}, t);
+    constexpr int kAhead = std::max(kBlock, Shared<T, L, kBlock>::kEach * Shared<T, L, kBlock>::kRows);  // rows that a load may touch
+    for (; t + 2 * kBlock <= end && t + kBlock + kAhead <= s.n; t += kBlock) steps(std::true_type{}, t);
     for (; t < end; t += kBlock) steps(std::false_type{}, t);
     if constexpr (Only) {
         store_padded<L>(ends.states + ends.row(s, cut, p.b, p.segment + 1, channel) * L::P, h, p.sub);
@@ -354,11 +369,11 @@ __global__ __launch_bounds__(kLanes) void state_forward(StateShape s, StateForwa
 //
 // A tile whose steps and channels all count has no branches.
 template <class T, class L, bool Only>
-__global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateBackward a, Cut cut) {
+__global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, StateBackward a, Cut cut) {
     constexpr int S = L::S, LPC = L::LPC, P = L::P, J = kTile / LPC;
     using Sums = ChannelSums<LPC, 2 * S>;
-    __shared__ alignas(16) float bc[2][kTile][LPC][2 * S];
-    __shared__ float sums[Only ? 1 : kWaves][kTile][2 * P];
+    __shared__ alignas(32) float bc[2][kTile][LPC][2 * S];
+    __shared__ float sums[Only ? 1 : L::W][kTile][2 * P];
     const long long block = block_index();
     if (block >= cut.blocks) return;
     const Place<L> p(s, cut, block);
@@ -471,11 +486,11 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
         float keep[kTile][S], before[Only ? 1 : kTile][S], inner[J];
         // Forward again from the saved state.
         each_step<J>([&](auto j) {
-            const float u = dt[j] * xv[j];
+            const Spread<LPC> dts(dt[j]), us(dt[j] * xv[j]);
             float out[LPC];
             each_step<LPC>([&](auto k) {
                 constexpr int m = j * LPC + k;
-                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u);
+                const float d = dts.template of<k>(), v = us.template of<k>();
                 float b[S], c[S];
                 load_shared<S>(b, c, bc[which][m][p.sub]);
                 out[k] = 0.0f;
@@ -506,11 +521,11 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
         float ex[J], ed[J];
         each_step<J>([&](auto back) {
             constexpr int j = J - 1 - back;
-            const float u = dt[j] * xv[j];
+            const Spread<LPC> dts(dt[j]), us(dt[j] * xv[j]), alongs(along[j]);
             float du[LPC], de[LPC];
             each_step<LPC>([&](auto behind) {
                 constexpr int k = LPC - 1 - behind, m = j * LPC + k;
-                const float d = from_lane<LPC, k>(dt[j]), v = from_lane<LPC, k>(u), dn = from_lane<LPC, k>(along[j]);
+                const float d = dts.template of<k>(), v = us.template of<k>(), dn = alongs.template of<k>();
                 float b[S], c[S], both[2 * S];
                 load_shared<S>(b, c, bc[which][m][p.sub]);
                 du[k] = de[k] = 0.0f;
@@ -557,11 +572,11 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
             if (gate) dgate -= kTile * s.gate_stride;
             // The sums of the waves' channels.
             __syncthreads();
-            for (int e = threadIdx.x; e < kTile * 2 * P; e += kLanes) {
+            for (int e = threadIdx.x; e < kTile * 2 * P; e += L::kLanes) {
                 const int m = e / (2 * P), at = e % (2 * P);
                 float v = sums[0][m][at];
 #pragma unroll
-                for (int w = 1; w < kWaves; ++w) v += sums[w][m][at];
+                for (int w = 1; w < L::W; ++w) v += sums[w][m][at];
                 if (kWhole || t + m < end) shared_sums[static_cast<long long>(t + m) * s.groups * 2 * P + at] = v;
             }
         }
@@ -603,23 +618,35 @@ __global__ __launch_bounds__(kLanes, 2) void state_backward(StateShape s, StateB
     }
 }
 
-// db and dc: the slabs' sums, in order; 0 behind a sequence's end.
+// db and dc: the slabs' sums, in order; 0 behind a sequence's end.  Four states a lane.
 template <class T>
 __global__ __launch_bounds__(kLanes) void add_shared(StateShape s, StateBackward a, Cut cut) {
+    using V = float __attribute__((ext_vector_type(4)));
     const Parts parts(s, cut);
-    const long long row = 2LL * cut.padded, count = static_cast<long long>(s.batch) * s.n * s.groups * row;
+    const int row = 2 * cut.padded / 4;
+    const long long count = static_cast<long long>(s.batch) * s.n * s.groups * row;
+    const V* from = reinterpret_cast<const V*>(a.workspace + parts.shared);
     for (long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x; i < count;
          i += static_cast<long long>(gridDim.x) * kLanes) {
         const long long at = i / row, step = at / s.groups;
-        const int group = static_cast<int>(at - step * s.groups), st = static_cast<int>(i - at * row);
+        const int group = static_cast<int>(at - step * s.groups), st = 4 * static_cast<int>(i - at * row);
         const int state = st % cut.padded, b = static_cast<int>(step / s.n);
-        if (state >= s.order) continue;
-        float sum = 0.0f;
-        if (step - static_cast<long long>(b) * s.n < length_of(a.lengths, b, s.n))
-            for (int k = 0; k < cut.slabs; ++k) sum += a.workspace[parts.shared + k * count + i];
-        const int column = group * s.order + state;
-        if (st < cut.padded) static_cast<T*>(a.db)[step * s.b_stride + column] = from_float<T>(sum);
-        else static_cast<T*>(a.dc)[step * s.c_stride + column] = from_float<T>(sum);
+        V sum = {};
+        if (step - static_cast<long long>(b) * s.n < length_of(a.lengths, b, s.n)) {
+            constexpr int kAtOnce = 8;
+            for (int k = 0; k < cut.slabs; k += kAtOnce) {
+                V part[kAtOnce];
+#pragma unroll
+                for (int m = 0; m < kAtOnce; ++m) part[m] = from[min(k + m, cut.slabs - 1) * count + i];
+#pragma unroll
+                for (int m = 0; m < kAtOnce; ++m)
+                    if (k + m < cut.slabs) sum += part[m];
+            }
+        }
+        T* to = st < cut.padded ? static_cast<T*>(a.db) + step * s.b_stride : static_cast<T*>(a.dc) + step * s.c_stride;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+            if (state + m < s.order) to[group * s.order + state + m] = from_float<T>(sum[m]);
     }
 }
 

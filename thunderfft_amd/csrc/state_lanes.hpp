@@ -14,19 +14,27 @@ __device__ __forceinline__ float moved(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), Control, 0xf, 0xf, true));
 }
 
-// The value of the K-th lane of each LPC, on all of them.
-template <int LPC, int K>
-__device__ __forceinline__ float from_lane(float v) {
+// Values of the LPC lanes of a channel, to be had on all of them: of<K>() is the K-th lane's.  Among
+// 4 lanes that is a modifier of the instruction that uses it; of 8, each half has a copy of the other.
+template <int LPC>
+struct Spread {
     static_assert(LPC == 4 || LPC == 8 || LPC == 16, "4, 8 or 16 lanes a channel");
-    if constexpr (LPC == 4) {
-        return moved<K * 0x55>(v);
-    } else if constexpr (LPC == 8) {
-        const int low = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + K, 0xf, 0xf, true);
-        return __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(v), 0x158 + K, 0xf, 0xc, false));
-    } else {
-        return moved<0x150 + K>(v);
+    float low, high;
+
+    __device__ __forceinline__ explicit Spread(float v) : low(v), high(v) {
+        if constexpr (LPC == 8) {
+            // 4 lanes back into the upper half of every 8, 4 on into the lower one.
+            const int bits = __float_as_int(v);
+            low = __int_as_float(__builtin_amdgcn_update_dpp(bits, bits, 0x114, 0xf, 0xa, false));
+            high = __int_as_float(__builtin_amdgcn_update_dpp(bits, bits, 0x104, 0xf, 0x5, false));
+        }
     }
-}
+    template <int K>
+    __device__ __forceinline__ float of() const {
+        if constexpr (LPC == 16) return moved<0x150 + K>(low);
+        else return moved<K % 4 * 0x55>(K < 4 ? low : high);
+    }
+};
 
 // The value of the lane mirrored within N lanes.
 template <int N>

@@ -22,21 +22,22 @@ int segments_of(long long waves, int n, bool backward) {
     return static_cast<int>(std::min<long long>((wanted + waves - 1) / waves, n / 64));
 }
 
+template <class L>
+Cut cut_with(const StateShape& s, bool backward) {
+    Cut cut;
+    cut.padded = L::P;
+    cut.slabs = slabs_of<L>(s);
+    const int blocks = (s.n + kStateBlock - 1) / kStateBlock;
+    const int want = segments_of(waves_of<L>(s), s.n, backward);
+    cut.steps = (blocks + want - 1) / want * kStateBlock;
+    cut.segments = s.n > 0 ? (s.n + cut.steps - 1) / cut.steps : 1;
+    cut.blocks = static_cast<long long>(s.batch) * s.groups * cut.slabs * cut.segments;
+    return cut;
+}
+
 Cut cut_of(const StateShape& s, bool backward) {
-    return with_lanes(s.order, [&](auto lanes) {
-        using L = decltype(lanes);
-        Cut cut;
-        const int each = s.channels / s.groups;
-        cut.padded = L::P;
-        cut.slabs = (each + L::kSlab - 1) / L::kSlab;
-        const long long columns = static_cast<long long>(s.batch) * s.groups * cut.slabs;
-        const int blocks = (s.n + kStateBlock - 1) / kStateBlock;
-        const int want = segments_of(columns * kStateWaves, s.n, backward);
-        cut.steps = (blocks + want - 1) / want * kStateBlock;
-        cut.segments = s.n > 0 ? (s.n + cut.steps - 1) / cut.steps : 1;
-        cut.blocks = columns * cut.segments;
-        return cut;
-    });
+    const auto cut = [&](auto lanes) { return cut_with<decltype(lanes)>(s, backward); };
+    return backward ? with_lanes(s.order, cut) : with_forward_lanes(s, cut);
 }
 
 template <class F>
