@@ -261,4 +261,154 @@ inline void ThunderFFT_layer_norm_backward(const T* d_dy, const T* d_x, const fl
                                            static_cast<void*>(stream)));
 }
 
+// ---- Operators of a state space block (contracts at the C ABI's entry points). ----
+
+// Shape of [batch][n][channels] values, rows without gaps; set the strides and the pool's rows
+// (states) in it where they differ.
+template <typename T>
+inline thff_conv_shape ThunderFFT_conv_shape(int batch, int n, int channels, int width,
+                                             bool silu = true) {
+    return {detail::value_code<T>(), silu ? 1 : 0, batch, n, channels, width, batch, 0, 0};
+}
+
+inline size_t ThunderFFT_short_conv_workspace_bytes(const thff_conv_shape& shape) {
+    return detail::check_bytes(thff_short_conv_workspace_bytes(&shape));
+}
+
+// Short causal convolution y[t] = silu(bias + sum_k weight[k] x[t - width + 1 + k]) per channel.
+// Synchronises `stream` before returning, as the other calls here.
+template <typename T>
+inline void ThunderFFT_short_conv(const thff_conv_shape& shape, const T* d_x,
+                                  const float* d_weight, const float* d_bias, T* d_y,
+                                  const T* d_state_in, T* d_state_out, const int* d_slots,
+                                  const int* d_lengths, hipStream_t stream = 0) {
+    if (shape.precision != detail::value_code<T>())
+        throw std::invalid_argument("ThunderFFT_short_conv: the shape is of another type");
+    detail::check(thff_short_conv(&shape, d_x, d_weight, d_bias, d_y, d_state_in, d_state_out,
+                                  d_slots, d_lengths, static_cast<void*>(stream)));
+}
+
+template <typename T>
+inline void ThunderFFT_short_conv_backward(const thff_conv_shape& shape, const T* d_dy,
+                                           const T* d_x, const float* d_weight,
+                                           const float* d_bias, const T* d_state_in,
+                                           const T* d_dstate_out, const int* d_lengths, T* d_dx,
+                                           float* d_dweight, float* d_dbias, T* d_dstate_in,
+                                           void* d_workspace, hipStream_t stream = 0) {
+    if (shape.precision != detail::value_code<T>())
+        throw std::invalid_argument("ThunderFFT_short_conv_backward: the shape is of another type");
+    detail::check(thff_short_conv_backward(&shape, d_dy, d_x, d_weight, d_bias, d_state_in,
+                                           d_dstate_out, d_lengths, d_dx, d_dweight, d_dbias,
+                                           d_dstate_in, d_workspace, static_cast<void*>(stream)));
+}
+
+template <typename T>
+inline thff_state_shape ThunderFFT_state_shape(int batch, int n, int channels, int order,
+                                               int groups = 1) {
+    return {detail::value_code<T>(), batch, n, channels, order, groups, batch, 0, 0, 0, 0, 0, 0};
+}
+
+inline size_t ThunderFFT_state_scan_saved_bytes(const thff_state_shape& shape) {
+    return detail::check_bytes(thff_state_scan_saved_bytes(&shape));
+}
+
+inline size_t ThunderFFT_state_scan_forward_bytes(const thff_state_shape& shape) {
+    return detail::check_bytes(thff_state_scan_forward_bytes(&shape));
+}
+
+inline size_t ThunderFFT_state_scan_workspace_bytes(const thff_state_shape& shape) {
+    return detail::check_bytes(thff_state_scan_workspace_bytes(&shape));
+}
+
+// State space scan: dt = softplus(delta + delta_bias), h[t] = exp(dt a) h[t-1] + dt x b for each
+// state of a channel, y = (sum of c h + skip x) silu(gate).
+template <typename T>
+inline void ThunderFFT_state_scan(const thff_state_shape& shape, const T* d_x, const T* d_delta,
+                                  const float* d_a, const T* d_b, const T* d_c,
+                                  const float* d_skip, const T* d_gate, const float* d_delta_bias,
+                                  T* d_y, const float* d_state_in, float* d_state_out,
+                                  const int* d_slots, const int* d_lengths, void* d_saved,
+                                  void* d_workspace, hipStream_t stream = 0) {
+    if (shape.precision != detail::value_code<T>())
+        throw std::invalid_argument("ThunderFFT_state_scan: the shape is of another type");
+    detail::check(thff_state_scan(&shape, d_x, d_delta, d_a, d_b, d_c, d_skip, d_gate, d_delta_bias,
+                                  d_y, d_state_in, d_state_out, d_slots, d_lengths, d_saved,
+                                  d_workspace, static_cast<void*>(stream)));
+}
+
+// The arrays of ThunderFFT_state_scan_backward by name; T is checked against the shape's.
+template <typename T>
+struct ThunderFFT_state_gradients {
+    const T *dy, *x, *delta;
+    const float* a;
+    const T *b, *c;
+    const float* skip;
+    const T* gate;
+    const float* delta_bias;
+    const void* saved;
+    const float* dstate_out;
+    const int* lengths;
+    T *dx, *ddelta;
+    float* da;
+    T *db, *dc;
+    float* dskip;
+    T* dgate;
+    float *ddelta_bias, *dstate_in;
+};
+
+template <typename T>
+inline void ThunderFFT_state_scan_backward(const thff_state_shape& shape,
+                                           const ThunderFFT_state_gradients<T>& g,
+                                           void* d_workspace, hipStream_t stream = 0) {
+    if (shape.precision != detail::value_code<T>())
+        throw std::invalid_argument("ThunderFFT_state_scan_backward: the shape is of another type");
+    const thff_state_gradients arrays = {
+        g.dy, g.x, g.delta, g.a, g.b, g.c, g.skip, g.gate, g.delta_bias, g.saved, g.dstate_out,
+        g.lengths, g.dx, g.ddelta, g.da, g.db, g.dc, g.dskip, g.dgate, g.ddelta_bias, g.dstate_in};
+    detail::check(thff_state_scan_backward(&shape, &arrays, d_workspace, static_cast<void*>(stream)));
+}
+
+// Root-mean-square norm of s = x + residual (d_residual null: x), s to d_sum where given; strides
+// of 0: rows without gaps.
+template <typename T>
+inline void ThunderFFT_rms_norm(const T* d_x, const T* d_residual, const float* d_weight,
+                                float eps, T* d_y, T* d_sum, long long rows, int cols,
+                                float* d_rstd = nullptr, long long x_stride = 0,
+                                long long residual_stride = 0, long long y_stride = 0,
+                                long long sum_stride = 0, hipStream_t stream = 0) {
+    detail::check(thff_rms_norm(detail::value_code<T>(), d_x, x_stride, d_residual,
+                                residual_stride, d_weight, eps, d_y, y_stride, d_sum, sum_stride,
+                                d_rstd, rows, cols, static_cast<void*>(stream)));
+}
+
+// The same with q of 8 bits (e4m3) and a scale for every `block` columns, 128 or cols.
+template <typename T>
+inline void ThunderFFT_rms_norm_8bit(const T* d_x, const T* d_residual, const float* d_weight,
+                                     float eps, unsigned char* d_q, float* d_scales, int block,
+                                     T* d_sum, long long rows, int cols, long long x_stride = 0,
+                                     long long residual_stride = 0, long long q_stride = 0,
+                                     long long sum_stride = 0, hipStream_t stream = 0) {
+    detail::check(thff_rms_norm_8bit(detail::value_code<T>(), d_x, x_stride, d_residual,
+                                     residual_stride, d_weight, eps, d_q, q_stride, d_scales,
+                                     block, d_sum, sum_stride, rows, cols,
+                                     static_cast<void*>(stream)));
+}
+
+inline size_t ThunderFFT_rms_norm_workspace_bytes(long long rows, int cols) {
+    return detail::check_bytes(thff_rms_norm_workspace_bytes(rows, cols));
+}
+
+template <typename T>
+inline void ThunderFFT_rms_norm_backward(const T* d_dy, const T* d_sum, const float* d_rstd,
+                                         const float* d_weight, const T* d_dsum, T* d_dx,
+                                         float* d_dweight, void* d_workspace, long long rows,
+                                         int cols, long long dy_stride = 0,
+                                         long long sum_stride = 0, long long dsum_stride = 0,
+                                         long long dx_stride = 0, hipStream_t stream = 0) {
+    detail::check(thff_rms_norm_backward(detail::value_code<T>(), d_dy, dy_stride, d_sum,
+                                         sum_stride, d_rstd, d_weight, d_dsum, dsum_stride, d_dx,
+                                         dx_stride, d_dweight, d_workspace, rows, cols,
+                                         static_cast<void*>(stream)));
+}
+
 }  // namespace thunderfft

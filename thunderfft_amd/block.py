@@ -46,6 +46,11 @@ def _like(t, stride):
     return torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
 
 
+def _trained(*tensors):
+    """Whether a backward pass may follow."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _ShortConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, silu):
@@ -108,7 +113,7 @@ def short_conv(x, weight, bias=None, state=None, lengths=None, silu=True):
 
 class _StateScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, delta, a, b, c, skip, gate, delta_bias, state, lengths):
+    def forward(ctx, x, delta, a, b, c, skip, gate, delta_bias, state, lengths, train):
         ctx.set_materialize_grads(False)
         values = [x, delta, gate, b.flatten(2), c.flatten(2)]
         (x, xs), (delta, ds), gate_rows, (b_rows, bs), (c_rows, cs) = (
@@ -118,7 +123,6 @@ class _StateScan(torch.autograd.Function):
         shape = thff.StateShape(x.dtype, batch, n, channels, order, groups, xs, ds, gate_rows[1], bs, cs)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         last = _floats(batch, channels, order, device=x.device)
-        train = any(ctx.needs_input_grad)
         with torch.cuda.device(x.device):
             saved = _bytes(shape.saved_bytes(), x.device) if train else None
             thff.ThunderFFT_state_scan_async(
@@ -156,7 +160,7 @@ class _StateScan(torch.autograd.Function):
                 d_lengths=lengths, d_workspace=_bytes(shape.workspace_bytes(), device),
                 stream=torch.cuda.current_stream())
         shared = (batch, n, ctx.groups, order)
-        got = (dx, ddelta, da, db.unflatten(2, shared[2:]), dc.unflatten(2, shared[2:]), dskip, dgate, dbias, dstate, None)
+        got = (dx, ddelta, da, db.unflatten(2, shared[2:]), dc.unflatten(2, shared[2:]), dskip, dgate, dbias, dstate, None, None)
         return tuple(g if need else None for g, need in zip(got, needs))
 
 
@@ -191,23 +195,23 @@ def state_scan(x, delta, a, b, c, skip=None, gate=None, delta_bias=None, state=N
     _device_tensor("c", c, x.dtype, (batch, n, groups, order), x.device)
     if gate is not None:
         _device_tensor("gate", gate, x.dtype, x.shape, x.device)
-    return _StateScan.apply(x, delta, a.contiguous(), b, c,
-                            _optional("skip", skip, torch.float32, (channels,), x.device), gate,
-                            _optional("delta_bias", delta_bias, torch.float32, (channels,), x.device),
-                            _optional("state", state, torch.float32, (batch, channels, order), x.device),
-                            _optional("lengths", lengths, torch.int32, (batch,), x.device))
+    skip, delta_bias = (_optional(name, t, torch.float32, (channels,), x.device)
+                        for name, t in (("skip", skip), ("delta_bias", delta_bias)))
+    state = _optional("state", state, torch.float32, (batch, channels, order), x.device)
+    lengths = _optional("lengths", lengths, torch.int32, (batch,), x.device)
+    train = _trained(x, delta, a, b, c, skip, gate, delta_bias, state)
+    return _StateScan.apply(x, delta, a.contiguous(), b, c, skip, gate, delta_bias, state, lengths, train)
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps):
+    def forward(ctx, x, weight, residual, eps, train):
         ctx.set_materialize_grads(False)
         (x, x_stride), (residual, residual_stride) = _rows(x), _rows(residual) if residual is not None else (None, None)
         cols = x.shape[-1]
         rows = x.numel() // cols
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-        train = any(ctx.needs_input_grad[:3])
         rstd = _floats(rows, device=x.device) if train else None
         with torch.cuda.device(x.device):
             thff.ThunderFFT_rms_norm_async(x.dtype, x, weight, eps, y, rows, cols, d_residual=residual, d_sum=total,
@@ -235,7 +239,7 @@ class _RmsNorm(torch.autograd.Function):
             thff.ThunderFFT_rms_norm_backward_async(
                 total.dtype, dy, total, rstd, weight, dx, dweight, workspace, rows, cols, d_dsum=dsum, dy_stride=dy_stride,
                 sum_stride=sum_stride, dsum_stride=dsum_stride, stream=torch.cuda.current_stream())
-        return dx if needs[0] else None, dweight, dx if needs[2] else None, None
+        return dx if needs[0] else None, dweight, dx if needs[2] else None, None, None
 
 
 def _norm_arguments(x, weight, residual, eps):
@@ -257,7 +261,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-5):
     ones.  Differentiable (once) by x, weight and residual.
     """
     weight = _norm_arguments(x, weight, residual, eps)
-    return _RmsNorm.apply(x, weight, residual, float(eps))
+    return _RmsNorm.apply(x, weight, residual, float(eps), _trained(x, weight, residual))
 
 
 @torch.no_grad()
