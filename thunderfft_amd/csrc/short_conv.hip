@@ -330,8 +330,10 @@ __global__ __launch_bounds__(1024) void conv_add_parts(const float* parts, long 
     const long long sums = static_cast<long long>(width + 1) * channels;
     for (long long first = 32LL * blockIdx.x; first < sums; first += 32LL * gridDim.x) {
         float sum = 0.0f;
-        if (first + lane < sums)
+        if (first + lane < sums) {
+#pragma unroll 4
             for (long long k = group; k < count; k += 32) sum += parts[k * sums + first + lane];
+        }
         __syncthreads();
         lds[group][lane] = sum;
         __syncthreads();

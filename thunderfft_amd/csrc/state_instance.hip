@@ -65,19 +65,14 @@ hipError_t launch_state_backward(const StateShape& s, const StateBackward& a, co
                 if (err != hipSuccess) return err;
             }
             state_backward<T, L, false><<<grid_of(cut.blocks), L::kLanes, 0, stream>>>(s, a, cut);
-            hipError_t err = hipGetLastError();
+            const hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
-            const long long shared = static_cast<long long>(s.batch) * s.n * s.groups * 2 * cut.padded / 4;
-            if (shared > 0) {
-                const long long blocks = std::min((shared + kLanes - 1) / kLanes, 1LL << 20);
-                add_shared<T><<<static_cast<unsigned>(blocks), kLanes, 0, stream>>>(s, a, cut);
-                err = hipGetLastError();
-                if (err != hipSuccess) return err;
-            }
         }
         const long long sums = static_cast<long long>(s.channels) * (cut.padded + 2);
-        add_weights<<<static_cast<unsigned>(std::min((sums + 31) / 32, 1LL << 20)), 1024, 0, stream>>>(
-            s, a, cut, static_cast<long long>(s.batch) * cut.segments);
+        const long long shared = static_cast<long long>(s.batch) * s.n * s.groups * 2 * cut.padded / 4;
+        const int few = static_cast<int>(std::min((sums + 31) / 32, 1LL << 20));
+        const long long many = std::min((shared + kLanes - 1) / kLanes, 1LL << 20);
+        add_state_parts<T><<<static_cast<unsigned>(few + many), kLanes, 0, stream>>>(s, a, cut, few);
         return hipGetLastError();
     });
 }

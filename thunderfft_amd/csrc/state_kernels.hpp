@@ -620,20 +620,19 @@ __global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, Sta
 
 // db and dc: the slabs' sums, in order; 0 behind a sequence's end.  Four states a lane.
 template <class T>
-__global__ __launch_bounds__(kLanes) void add_shared(StateShape s, StateBackward a, Cut cut) {
+__device__ __forceinline__ void add_shared(const StateShape& s, const StateBackward& a, const Cut& cut, const Parts& parts,
+                                           long long block, long long blocks) {
     using V = float __attribute__((ext_vector_type(4)));
-    const Parts parts(s, cut);
     const int row = 2 * cut.padded / 4;
     const long long count = static_cast<long long>(s.batch) * s.n * s.groups * row;
     const V* from = reinterpret_cast<const V*>(a.workspace + parts.shared);
-    for (long long i = static_cast<long long>(blockIdx.x) * kLanes + threadIdx.x; i < count;
-         i += static_cast<long long>(gridDim.x) * kLanes) {
+    for (long long i = block * kLanes + threadIdx.x; i < count; i += blocks * kLanes) {
         const long long at = i / row, step = at / s.groups;
         const int group = static_cast<int>(at - step * s.groups), st = 4 * static_cast<int>(i - at * row);
         const int state = st % cut.padded, b = static_cast<int>(step / s.n);
         V sum = {};
         if (step - static_cast<long long>(b) * s.n < length_of(a.lengths, b, s.n)) {
-            constexpr int kAtOnce = 8;
+            constexpr int kAtOnce = 8;  // loads under way together
             for (int k = 0; k < cut.slabs; k += kAtOnce) {
                 V part[kAtOnce];
 #pragma unroll
@@ -650,29 +649,30 @@ __global__ __launch_bounds__(kLanes) void add_shared(StateShape s, StateBackward
     }
 }
 
-// da, dskip and ddelta_bias: 32 sums a workgroup, 32 lanes a sum, each every 32nd part.
-__global__ __launch_bounds__(1024) void add_weights(StateShape s, StateBackward a, Cut cut, long long count) {
-    __shared__ float lds[32][33];
-    const Parts parts(s, cut);
+// da, dskip and ddelta_bias: 32 sums a workgroup, 8 lanes a sum, each every 8th part.
+__device__ __forceinline__ void add_weights(const StateShape& s, const StateBackward& a, const Cut& cut, const Parts& parts,
+                                            long long block, long long blocks) {
+    constexpr int kGroups = kLanes / 32;
+    __shared__ float lds[kGroups][32];
     const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
     const long long states = static_cast<long long>(s.channels) * cut.padded, sums = states + 2LL * s.channels;
-    for (long long first = 32LL * blockIdx.x; first < sums; first += 32LL * gridDim.x) {
-        const auto value = [&](long long i, long long part) {
-            return i < states ? a.workspace[parts.da + part * states + i]
-                              : a.workspace[parts.pairs + part * 2 * s.channels + (i - states)];
-        };
+    for (long long first = 32 * block; first < sums; first += 32 * blocks) {
+        const long long i = first + lane;
+        const bool pair = i >= states;
+        const float* from = a.workspace + (pair ? parts.pairs + (i - states) : parts.da + i);
+        const long long way = pair ? 2LL * s.channels : states;
         float sum = 0.0f;
-        if (first + lane < sums)
-            for (long long k = group; k < count; k += 32) sum += value(first + lane, k);
+        if (i < sums) {
+#pragma unroll 8
+            for (long long k = group; k < parts.count; k += kGroups) sum += from[k * way];
+        }
         __syncthreads();
         lds[group][lane] = sum;
         __syncthreads();
-        sum = lds[lane][group];
+        if (group != 0 || i >= sums) continue;
 #pragma unroll
-        for (int m = 1; m < 32; m *= 2) sum += __shfl_xor(sum, m);
-        const long long i = first + group;
-        if (lane != 0 || i >= sums) continue;
-        if (i < states) {
+        for (int g = 1; g < kGroups; ++g) sum += lds[g][lane];
+        if (!pair) {
             const long long c = i / cut.padded, state = i - c * cut.padded;
             if (state < s.order) a.da[c * s.order + state] = sum;
         } else {
@@ -681,6 +681,14 @@ __global__ __launch_bounds__(1024) void add_weights(StateShape s, StateBackward 
             if (to) to[c] = sum;
         }
     }
+}
+
+// What the backward pass's workgroups have left: the first `few` workgroups take the weights' sums.
+template <class T>
+__global__ __launch_bounds__(kLanes) void add_state_parts(StateShape s, StateBackward a, Cut cut, int few) {
+    const Parts parts(s, cut);
+    if (static_cast<int>(blockIdx.x) < few) add_weights(s, a, cut, parts, blockIdx.x, few);
+    else add_shared<T>(s, a, cut, parts, blockIdx.x - few, gridDim.x - few);
 }
 
 // One step (n = 1: a token of each sequence): 4 states a lane, Each lanes of them a channel, and Rows
