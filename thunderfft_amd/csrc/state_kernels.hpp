@@ -373,7 +373,7 @@ __global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, Sta
     constexpr int S = L::S, LPC = L::LPC, P = L::P, J = kTile / LPC;
     using Sums = ChannelSums<LPC, 2 * S>;
     __shared__ alignas(32) float bc[2][kTile][LPC][2 * S];
-    __shared__ float sums[Only ? 1 : L::W][kTile][2 * P];
+    __shared__ float sums[Only ? 1 : L::W * Sums::kParts][kTile][2 * P];
     const long long block = block_index();
     if (block >= cut.blocks) return;
     const Place<L> p(s, cut, block);
@@ -544,12 +544,11 @@ __global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, Sta
                     }
                 }
                 if constexpr (!Only) {
-                    // Lanes with the same sums store them all.
                     channel_sums<LPC, 2 * S>(both, p.lane);
 #pragma unroll
                     for (int l = 0; l < Sums::kLeft; ++l) {
                         const int at = Sums::first(p.lane) + l;
-                        sums[p.wave][m][at / S * P + p.sub * S + at % S] = both[l];
+                        sums[p.wave * Sums::kParts + Sums::part(p.lane)][m][at / S * P + p.sub * S + at % S] = both[l];
                     }
                 }
             });
@@ -570,13 +569,13 @@ __global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, Sta
             dx -= kTile * s.x_stride;
             ddelta -= kTile * s.delta_stride;
             if (gate) dgate -= kTile * s.gate_stride;
-            // The sums of the waves' channels.
+            // The sums of all the waves' channels.
             __syncthreads();
             for (int e = threadIdx.x; e < kTile * 2 * P; e += L::kLanes) {
                 const int m = e / (2 * P), at = e % (2 * P);
                 float v = sums[0][m][at];
 #pragma unroll
-                for (int w = 1; w < L::W; ++w) v += sums[w][m][at];
+                for (int w = 1; w < L::W * Sums::kParts; ++w) v += sums[w][m][at];
                 if (kWhole || t + m < end) shared_sums[static_cast<long long>(t + m) * s.groups * 2 * P + at] = v;
             }
         }

@@ -61,25 +61,6 @@ __device__ __forceinline__ float sum_to_lanes(float (&v)[LPC], int lane) {
     return (one ? v[1] : v[0]) + mirrored<2>(one ? v[0] : v[1]);
 }
 
-// Adds the lanes whose bit `Bit` differs: 2^Bit lanes away.
-template <int Bit>
-__device__ __forceinline__ float sum_across(float v) {
-    if constexpr (Bit == 5) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    } else if constexpr (Bit == 4) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    } else if constexpr (Bit == 3) {
-        return v + moved<0x128>(v);
-    } else {
-        // 4 lanes on for the lower half of every 8, 4 back for the upper one.
-        static_assert(Bit == 2, "channels begin at 4 lanes at least");
-        const int up = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x104, 0xf, 0x5, false);
-        return v + __int_as_float(__builtin_amdgcn_update_dpp(up, __float_as_int(v), 0x114, 0xf, 0xa, false));
-    }
-}
-
 // Sums of one and two over the lanes whose bit `Bit` differs: one's where the bit is 0, two's where
 // it is 1.
 template <int Bit>
@@ -97,31 +78,26 @@ __device__ __forceinline__ float sum_apart(float one, float two, int lane) {
     }
 }
 
-// Sums of v[0 ... N) over the channels of a wave, whose lanes have bits 5 down to log2(LPC).  With
-// each bit the values halve while there are several; v[0 ...) are then those from
-// channel_sum_first(lane) on, the same ones on lanes that differ in the bits left.
+// Sums of v[0 ... N) over the channels of a wave, whose lanes have bits 5 down to log2(LPC): with each
+// bit the values halve, until one is left or the bits are used up.  v[0 ...) are then those from
+// ChannelSums::first(lane) on; lanes that differ in bits left have parts of the same ones.
 template <int LPC, int N, int Bit = 5>
 __device__ __forceinline__ void channel_sums(float* v, int lane) {
-    if constexpr ((1 << Bit) >= LPC) {
-        if constexpr (N > 1) {
+    if constexpr ((1 << Bit) >= LPC && N > 1) {
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) v[i] = sum_apart<Bit>(v[i], v[i + N / 2], lane);
-            channel_sums<LPC, N / 2, Bit - 1>(v, lane);
-        } else {
-            v[0] = sum_across<Bit>(v[0]);
-            channel_sums<LPC, 1, Bit - 1>(v, lane);
-        }
+        for (int i = 0; i < N / 2; ++i) v[i] = sum_apart<Bit>(v[i], v[i + N / 2], lane);
+        channel_sums<LPC, N / 2, Bit - 1>(v, lane);
     }
 }
 
-// What is left of N values a lane, where the first of them belongs, and whether the lane is the one
-// of its likes that stores them.
+// What is left of N values a lane, where the first of them belongs, how many lanes have parts of the
+// same ones, and which of them the lane is.
 template <int LPC, int N>
 struct ChannelSums {
     static constexpr int kBits = LPC == 4 ? 4 : LPC == 8 ? 3 : 2;
     static constexpr int log2(int n) { return n == 1 ? 0 : 1 + log2(n / 2); }
     static constexpr int kApart = log2(N) < kBits ? log2(N) : kBits;  // bits that tell values apart
-    static constexpr int kLeft = N >> kApart;
+    static constexpr int kLeft = N >> kApart, kParts = 1 << (kBits - kApart);
 
     static __device__ __forceinline__ int first(int lane) {
         int at = 0;
@@ -129,10 +105,7 @@ struct ChannelSums {
         for (int k = 0; k < kApart; ++k) at += (lane >> (5 - k) & 1) * (N >> (k + 1));
         return at;
     }
-    static __device__ __forceinline__ bool stores(int lane) {
-        constexpr int kSame = ((1 << (kBits - kApart)) - 1) * LPC;
-        return (lane & kSame) == 0;
-    }
+    static __device__ __forceinline__ int part(int lane) { return lane / LPC % kParts; }
 };
 
 // log(1 + exp(v)) by e = exp(-|v|) and log(1 + e): u = 1 + e is rounded, and what is lost, e - (u - 1),
