@@ -519,6 +519,8 @@ __global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, Sta
             }
         }
         float ex[J], ed[J];
+        // Left free, the scheduler begins with the way back early, for which there are no registers.
+        __builtin_amdgcn_sched_barrier(0);
         each_step<J>([&](auto back) {
             constexpr int j = J - 1 - back;
             const Spread<LPC> dts(dt[j]), us(dt[j] * xv[j]), alongs(along[j]);
