@@ -162,6 +162,14 @@ def test_lengths(T, order):
         assert torch.equal(clean[name], below[name]), name
 
 
+@pytest.mark.parametrize("n", [1, 2, 5, 15, 34])
+@pytest.mark.parametrize("channels,order", [(64, 16), (70, 3), (40, 40)])
+def test_a_few_steps_of_all_lengths(n, channels, order):
+    """Sequences of 0 to n steps: what lies behind each length is 0, wherever it falls in a block."""
+    v = values(27 + n, "half", n + 1, n, channels, order)
+    compare("half", v, ends(*range(n, -1, -1)))
+
+
 @pytest.mark.parametrize("T", list(oracle.TYPES))
 @pytest.mark.parametrize("size", [(1, 3000, 20, 16, 1), (2, 1500, 6, 5, 2), (1, 2500, 70, 4, 1), (1, 1100, 9, 40, 1)], ids=str)
 def test_long_sequences(T, size):
