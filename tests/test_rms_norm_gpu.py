@@ -164,6 +164,20 @@ def test_outputs_wanted_singly(cols):
     assert torch.equal(dx, whole["dx"])
 
 
+@pytest.mark.parametrize("size", [(700, 64), (90, 777), (64, 2048), (7, 20011), (5, 40001)], ids=str)
+def test_8bit_is_the_rounded_quotient(size):
+    """Each bit of it: the scale is the block's largest over 448, q the value over the scale, rounded once."""
+    x, residual, weight, *_ = values(14, "float", *size)
+    rows, cols = size
+    y = run("float", x, residual, weight, x, None)["y"].cpu()
+    for block in (128, cols):
+        q, scales, _ = run8("float", x, residual, weight, block)
+        padded = torch.nn.functional.pad(y, (0, -cols % block)).view(rows, -1, block)
+        assert torch.equal(scales.cpu(), padded.abs().amax(2) / 448)
+        want = (y / scales.cpu().repeat_interleave(block, 1)[:, :cols]).to(torch.float8_e4m3fn)
+        assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8))
+
+
 @pytest.mark.parametrize("cols", [64, 130, 777, 20011, 40001])
 def test_zero_rows(cols):
     """Rows of zeros: y is 0, q is 0 with the least scale; with eps = 0 they are NaN, and no others."""

@@ -24,25 +24,34 @@ __device__ __forceinline__ float lane_max(float v) {
     return v;
 }
 
-__device__ __forceinline__ float scale_of(float largest) {
-    return fmaxf(largest * (1.0f / kLargest8), kLeastScale);
-}
+// What takes a block's largest value to the largest of e4m3, and its reciprocal.
+struct Scale {
+    float scale, inverse;
+    __device__ __forceinline__ explicit Scale(float largest)
+        : scale(fmaxf(largest / kLargest8, kLeastScale)), inverse(1.0f / scale) {}
+    // v / scale to the last bit: v times the reciprocal is off by an ulp or so, which moves values that lie
+    // between two of e4m3's; what is left of v corrects it (float16 4099 x 2048: 11.0 us against 10.4).
+    __device__ __forceinline__ float of(float v) const {
+        const float q = v * inverse;
+        return fmaf(fmaf(-q, scale, v), inverse, q);
+    }
+};
 
 // Two values in e4m3, to nearest even.
 __device__ __forceinline__ unsigned bits8(float a, float b) {
     return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false)) & 0xffffu;
 }
 
-// Stores V values times `by` in 8 bits, from the skip-th on.
+// Stores V values in 8 bits, from the skip-th on.
 template <int V>
-__device__ __forceinline__ void store_8bit(unsigned char* p, const float (&v)[V], float by, int skip) {
+__device__ __forceinline__ void store_8bit(unsigned char* p, const float (&v)[V], const Scale& by, int skip) {
     if constexpr (V == 1) {
-        if (skip == 0) *p = static_cast<unsigned char>(bits8(v[0] * by, 0.0f));
+        if (skip == 0) *p = static_cast<unsigned char>(bits8(by.of(v[0]), 0.0f));
     } else {
         pack<unsigned char, V> out;
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
-            const unsigned two = bits8(v[i] * by, v[i + 1] * by);
+            const unsigned two = bits8(by.of(v[i]), by.of(v[i + 1]));
             out[i] = static_cast<unsigned char>(two);
             out[i + 1] = static_cast<unsigned char>(two >> 8);
         }
@@ -145,10 +154,10 @@ __global__ __launch_bounds__(R::kLanes) void rms_forward(RmsForward a) {
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             const int skip = p.skip(j, a.cols);
-            const float scale = scale_of(largest[kOne ? 0 : j]);
-            if (skip < V) store_8bit<V>(q + p.at(j, a.cols), v[j], 1.0f / scale, skip);
+            const Scale by(largest[kOne ? 0 : j]);
+            if (skip < V) store_8bit<V>(q + p.at(j, a.cols), v[j], by, skip);
             if (kOne ? j == 0 && p.lane == 0 : p.lane % kLanesOfBlock == 0 && p.column(j) < a.cols)
-                scales[kOne ? 0 : p.column(j) / 128] = scale;
+                scales[kOne ? 0 : p.column(j) / 128] = by.scale;
         }
     }
 }
@@ -333,17 +342,17 @@ __global__ __launch_bounds__(kLongLanes) void long_rms_forward(RmsForward a) {
                 if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = whole;
                 __syncthreads();
                 for (int w = 0; w < kLongLanes / 64; ++w) whole = fmaxf(whole, lds[w]);
-                if (threadIdx.x == 0) a.scales[row] = scale_of(whole);
+                if (threadIdx.x == 0) a.scales[row] = Scale(whole).scale;
             }
             each_column(a.cols, [&](long long c, bool one, bool two) {
                 const float u = one ? normed(c) : 0.0f, v = two ? normed(c + 1) : 0.0f;
                 float largest = whole;
                 if (blocks > 1) {
                     largest = lane_max<64>(fmaxf(fabsf(u), fabsf(v)));
-                    if (threadIdx.x % 64 == 0) a.scales[row * blocks + c / 128] = scale_of(largest);
+                    if (threadIdx.x % 64 == 0) a.scales[row * blocks + c / 128] = Scale(largest).scale;
                 }
-                const float by = 1.0f / scale_of(largest);
-                const unsigned both = bits8(u * by, v * by);
+                const Scale by(largest);
+                const unsigned both = bits8(by.of(u), by.of(v));
                 if (one) q[c] = static_cast<unsigned char>(both);
                 if (two) q[c + 1] = static_cast<unsigned char>(both >> 8);
             });
