@@ -87,6 +87,9 @@ def test_sizes():
     # Many channels leave no segments, and a forward call no scratch.
     assert state_shape(batch=8, n=4096, channels=2048).forward_bytes() == 0
     assert state_shape(channels=0).workspace_bytes() == 0
+    # Past 32 bits: 2^30 sequences of a step.
+    assert state_shape(batch=1 << 30, n=1, channels=1, order=16).saved_bytes() == 1 << 36
+    assert state_shape(batch=1 << 30, n=1, channels=1, order=16).workspace_bytes() > 1 << 36
     for T in ("float", "half"):
         assert conv_shape(T, n=0).workspace_bytes() == 0 and conv_shape(T, batch=0).workspace_bytes() == 0
         assert conv_shape(T, n=1).workspace_bytes() > 0 and conv_shape(T, n=1, channels=1).workspace_bytes() > 0
@@ -116,6 +119,8 @@ def test_conv_refused(call):
             call(s, **args)
     with pytest.raises(ValueError, match="states"):
         call(conv_shape(states=-1), A, B, C, D, d_slots=E)
+    with pytest.raises(ValueError, match="non-null"):
+        call(conv_shape(n=0), 0, 0, 0, 0, d_state_in=E, d_state_out=E)
     # A shape with nothing to do is done, whatever the pointers.
     call(conv_shape(batch=0), 0, 0, 0, 0)
     call(conv_shape(channels=0), 0, 0, 0, 0)
@@ -146,6 +151,8 @@ def test_conv_backward_refused(call):
             call(s, **dict(good, **{name: (10 << 16) + 2}))
     with pytest.raises(ValueError, match="16-byte"):
         call(s, **dict(good, d_workspace=H + 8))
+    with pytest.raises(ValueError, match="non-null"):
+        call(conv_shape(n=0), 0, 0, 0, 0, 0, d_dstate_in=A, d_dstate_out=B)
     call(conv_shape(channels=0), 0, 0, 0, 0, 0)
 
 
@@ -176,6 +183,8 @@ def test_state_refused(call):
         call(s, **dict(good, d_workspace=0))
     with pytest.raises(ValueError, match="states must"):
         call(state_shape(states=-1), **dict(good, d_slots=H))
+    with pytest.raises(ValueError, match="non-null"):
+        call(state_shape(n=0), 0, 0, 0, 0, 0, 0, d_state_in=A, d_state_out=A)
     call(state_shape(batch=0), 0, 0, 0, 0, 0, 0)
     call(state_shape(channels=0, groups=1), 0, 0, 0, 0, 0, 0)
 

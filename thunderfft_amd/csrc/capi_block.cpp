@@ -74,9 +74,9 @@ int conv_impl(const thff_conv_shape* shape, const ConvForward& a, void* stream, 
     if (rc != THFF_OK) return rc;
     if (s.batch == 0 || s.channels == 0) return THFF_OK;
     const unsigned e = element_bytes(s.precision);
+    if (!a.weight || (s.n > 0 && any_null({a.x, a.y})))
+        return fail(THFF_EINVAL, "ThunderFFT_short_conv requires non-null x, weight and y");
     if (s.n > 0) {
-        if (any_null({a.x, a.weight, a.y}))
-            return fail(THFF_EINVAL, "ThunderFFT_short_conv requires non-null x, weight and y");
         if (any_alias({a.y}, {a.x, a.weight, a.bias, a.state_in, a.state_out}))
             return fail(THFF_EINVAL, "ThunderFFT_short_conv output must not alias another array");
     }
@@ -97,9 +97,9 @@ int conv_backward_impl(const thff_conv_shape* shape, const ConvBackward& a, void
     if (rc != THFF_OK) return rc;
     if (s.channels == 0) return THFF_OK;
     const unsigned e = element_bytes(s.precision);
+    if (s.batch > 0 && (!a.weight || (s.n > 0 && any_null({a.dy, a.x, a.dx}))))
+        return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward requires non-null dy, x, weight and dx");
     if (s.batch > 0 && s.n > 0) {
-        if (any_null({a.dy, a.x, a.weight, a.dx}))
-            return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward requires non-null dy, x, weight and dx");
         if (!a.workspace && (a.dweight || a.dbias) && conv_workspace_bytes(s) > 0)
             return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward requires a workspace of " +
                                          std::to_string(conv_workspace_bytes(s)) + " bytes");
@@ -148,9 +148,9 @@ int state_impl(const thff_state_shape* shape, const StateForward& a, void* strea
     const int rc = check_shape(shape, &s);
     if (rc != THFF_OK) return rc;
     if (s.batch == 0 || s.channels == 0) return THFF_OK;
+    if (!a.a || (s.n > 0 && any_null({a.x, a.delta, a.b, a.c, a.y})))
+        return fail(THFF_EINVAL, "ThunderFFT_state_scan requires non-null x, delta, a, b, c and y");
     if (s.n > 0) {
-        if (any_null({a.x, a.delta, a.a, a.b, a.c, a.y}))
-            return fail(THFF_EINVAL, "ThunderFFT_state_scan requires non-null x, delta, a, b, c and y");
         if (any_alias({a.y}, {a.x, a.delta, a.a, a.b, a.c, a.skip, a.gate, a.delta_bias, a.state_in, a.state_out}))
             return fail(THFF_EINVAL, "ThunderFFT_state_scan output must not alias another array");
     }
@@ -178,10 +178,10 @@ int state_backward_impl(const thff_state_shape* shape, const thff_state_gradient
     if (!g) return fail(THFF_EINVAL, "thff_state_gradients is null");
     if (s.channels == 0) return THFF_OK;
     if (!g->da) return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward requires non-null da");
+    if (s.batch > 0 && (!g->a || (s.n > 0 && any_null({g->dy, g->x, g->delta, g->b, g->c, g->dx, g->ddelta, g->db, g->dc}))))
+        return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward requires non-null dy, x, delta, a, b, c, dx, "
+                                 "ddelta, db and dc");
     if (s.batch > 0 && s.n > 0) {
-        if (any_null({g->dy, g->x, g->delta, g->a, g->b, g->c, g->dx, g->ddelta, g->db, g->dc}))
-            return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward requires non-null dy, x, delta, a, b, c, dx, "
-                                     "ddelta, db and dc");
         if (g->gate && !g->dgate)
             return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward requires dgate where there is a gate");
         if (!g->saved)

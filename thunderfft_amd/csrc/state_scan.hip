@@ -51,7 +51,7 @@ auto with_type(int precision, F f) {
 
 long long state_saved_bytes(const StateShape& s) {
     const long long tiles = (s.n + kStateTile - 1) / kStateTile;
-    return 4 * s.batch * tiles * s.channels * cut_of(s, false).padded;
+    return 4LL * s.batch * tiles * s.channels * cut_of(s, false).padded;
 }
 
 long long state_forward_bytes(const StateShape& s) {
