@@ -207,6 +207,27 @@ def test_growing_states():
     compare("float", v)
 
 
+@pytest.mark.parametrize("order", [4, 16, 40])
+def test_states_of_zero_do_not_grow(order):
+    """A positive rate and long steps: the factor of some hundred steps is out of range, the states that it
+    would take there are zero.  Only the last steps have an x, only the first ones a dy."""
+    n, few = 2000, 5
+    v = values(17, "float", 1, n, 24, order)
+    v["a"] = v["a"].abs() * 0.0 + 0.5
+    v["delta"][:] = 6
+    v["state"] = v["dstate"] = None
+    v["x"][:, :-few] = 0
+    v["dy"][:, few:] = 0
+    got = run("float", v)
+    last = run("float", dict(v, **{k: v[k][:, -few:].contiguous() for k in ("x", "delta", "b", "c", "gate", "dy")}))
+    first = run("float", dict(v, **{k: v[k][:, :few].contiguous() for k in ("x", "delta", "b", "c", "gate", "dy")}))
+    assert (got["y"][:, :-few] == 0).all() and (got["dx"][:, few:] == 0).all()
+    for name, want in (("y", last["y"]), ("state", last["state"])):
+        # The same steps in fp32, whose dt and factors the two runs round alike.
+        assert torch.allclose(got[name][:, -few:] if name == "y" else got[name], want, rtol=2.0 ** -20, atol=0), name
+    assert torch.allclose(got["dx"][:, :few], first["dx"], rtol=2.0 ** -18, atol=2.0 ** -18 * first["dx"].abs().max().item())
+
+
 @pytest.mark.parametrize("T", list(oracle.TYPES))
 @pytest.mark.parametrize("size", [(37, 5), (24, 16), (9, 64), (16, 24)], ids=str)
 def test_tokens_follow_prompts_in_a_pool(T, size):

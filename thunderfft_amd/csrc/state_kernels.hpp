@@ -177,7 +177,9 @@ __device__ __forceinline__ void load_shared(float (&b)[S], float (&c)[S], const 
 }
 
 // Takes h through the segments from `from` on, `count` of them one after the other, `way` apart: each
-// decays it by its sum of dt and adds its own end.  ends_of, sums_of: rows of the first one.
+// decays it by its sum of dt and adds its own end.  ends_of, sums_of: rows of the first one.  Where a is
+// positive a segment's factor may be out of range though its product with h, or an h of zero, is not:
+// its root is taken twice.
 template <class L>
 __device__ __forceinline__ void fold(float (&h)[L::S], const float (&decay)[L::S], const float* ends_of, const float* sums_of,
                                      long long way, int count, int sub) {
@@ -194,7 +196,10 @@ __device__ __forceinline__ void fold(float (&h)[L::S], const float (&decay)[L::S
         for (int m = 0; m < kAtOnce; ++m) {
             if (k + m == count) break;
 #pragma unroll
-            for (int i = 0; i < L::S; ++i) h[i] = fmaf(__builtin_amdgcn_exp2f(dt[m] * decay[i]), h[i], own[m][i]);
+            for (int i = 0; i < L::S; ++i) {
+                const float root = __builtin_amdgcn_exp2f(0.5f * dt[m] * decay[i]);
+                h[i] = h[i] == 0.0f ? own[m][i] : fmaf(root, root * h[i], own[m][i]);
+            }
         }
     }
 }
@@ -359,6 +364,9 @@ __global__ __launch_bounds__(L::kLanes) void state_forward(StateShape s, StateFo
     } else {
         for (; t < t1; t += LPC, y += LPC * s.y_stride)
             if (t + p.sub < t1) lane_at(y, lane.y) = from_float<T>(0.0f);
+        // Lanes of no channel, in other waves perhaps, have read the last channel's state too, which may be
+        // replaced in place: after the barrier none still waits for it.
+        if (a.state_out) __syncthreads();
         if (a.state_out && slot >= 0 && p.segment + 1 == cut.segments)
             store_states<L>(a.state_out + (static_cast<long long>(slot) * s.channels + channel) * s.order, h, p.sub, s.order);
     }
