@@ -7,6 +7,10 @@
 //
 // s is what the next block's residual is, so the norm is that of the rounded s, and the backward
 // pass reads s alone.  Rows are held as in norm.hip, and the weights' gradients summed alike.
+//
+// Memory bounds both: bfloat16 32768 x 2048 takes 91 us forward (537 MB, 5.9 TB/s) and 94 us backward
+// (540 MB, 5.7 TB/s), 5 more for adding the parts up; with 8 bits half 4099 x 2048 11 us (59 MB, one
+// round of rows).  8 rows of 1024 take 2.8 us, their latency.
 #include "block.hpp"
 #include "norm_rows.hpp"
 

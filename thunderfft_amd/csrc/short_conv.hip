@@ -5,8 +5,13 @@
 //   dxe[e] = sum_k weight[k] dp[e - k]  (+ dstate_out behind the end),
 //   dweight[k] = sum_t dp[t] xe[t + k],  dbias = sum_t dp[t].
 //
-// A lane takes 16 bytes of channels and some steps one after the other, with the last K - 1 rows
-// in registers.
+// A lane takes 16 bytes of channels (backward 8) and some steps one after the other, with the last
+// K - 1 rows in registers, so that a row is read once but for those before a lane's first step.
+//
+// Memory bounds it: bfloat16 8 x 4096 x 2048, 4 taps, 49 us forward (294 MB, 6.0 TB/s) and 75 us
+// backward (417 MB, 5.5 TB/s; the VALU issues in 90% of the cycles too), 5 more for the weights'
+// sums.  A token of 8 sequences 5 us, half 7 x 1000 x 2048 of unlike lengths 12 us: a round of
+// loads and one of stores.
 #include <algorithm>
 #include <type_traits>
 
@@ -67,7 +72,8 @@ struct Taps {
     }
 };
 
-// Steps of a lane forward.
+// Steps of a lane forward: bfloat16 8 x 4096 x 2048 47 us, 52 by 8, 63 by 32 (registers); 1 x 65536 x
+// 1024 49, 55 and 46; half 7 x 1000 x 2048 of unlike lengths 12.1, 11.7 and 14.3.
 constexpr int kSteps = 16;
 
 template <class T, int V, int K, bool Silu, int TS>
@@ -378,7 +384,8 @@ auto with_kind(const ConvShape& s, F f) {
     return f(Kind<V, 4>{});
 }
 
-// Backward, where a channel takes four times the registers.
+// Backward, where a channel takes four times the registers: bfloat16 8 x 4096 x 2048 75 us, 143 by 16
+// bytes a lane.
 constexpr int kBackwardBytes = 8;
 
 int vectors_of(const ConvShape& s, int v) { return (s.channels + v - 1) / v; }

@@ -10,7 +10,9 @@ constexpr int kStateBlock = 32;  // steps whose b and c are in LDS at a time, fo
 constexpr long long kStateStride = 1 << 24;  // the longest: offsets of a lane's rows fit 32 bits
 constexpr int kStateTile = 16;   // steps between saved states, and of the backward pass at a time
 
-// S states of a channel on each of LPC neighbouring lanes, in workgroups of W waves.
+// S states of a channel on each of LPC neighbouring lanes, in workgroups of W waves.  4 lanes a channel
+// are as few as let each load whole sectors and share the work that is once a step; 8 waves a
+// workgroup leave half of the compute units without one where channels are few.
 template <int S_, int LPC_, int W_>
 struct Lanes {
     static constexpr int S = S_, LPC = LPC_, W = W_, P = S * LPC, kLanes = 64 * W, kWave = 64 / LPC, kSlab = W * kWave;
@@ -39,8 +41,9 @@ long long waves_of(const StateShape& s) {
 }
 
 // The forward pass's.  With half of a wave for each SIMD (1024 of them), and not quite one, 8 lanes a
-// channel are as many waves again: bfloat16 7 x 1000 x 2048, ragged (896 waves of 4 lanes) 61 us
-// against 78 by segments; 8 x 4096 x 2048 (1024) 427 against 375.
+// channel are as many waves again, in place of segments: bfloat16 7 x 1000 x 2048, ragged (896 waves
+// of 4 lanes) 56 us against 79 by 4 lanes, 4 x 4096 x 2048 (512) 229 against 241, 6 x 4096 x 2048
+// (768) 354 against 365; 8 x 4096 x 2048 (1024) 427 against 366.
 template <class F>
 auto with_forward_lanes(const StateShape& s, F f) {
     if (s.order > 8 && s.order <= 16) {

@@ -7,6 +7,14 @@
 // Where there are too few channels to fill the card, the steps are split into segments.  A first
 // kernel takes each segment from a state of zero; as the decay of a segment is exp(a sum of dt),
 // the states that the segments start from follow from those ends, in order.
+//
+// Instructions bound it: a state of a step takes 5 at least forward (dt a, its power, dt x b, and the
+// sums of h and y) and 15 backward (those again and the gradients'), and takes 7.6 and 23.8 with what
+// is once a step and channel, the addresses, LDS and the sums over channels.  bfloat16 8 x 4096 x 2048
+// of 16 states (134 MB a tensor): forward 376 us, at a wave a SIMD, the VALU issuing in 67% of the
+// cycles; backward 216 + 897 + 33 us by 8 segments, 87%.  1 x 65536 x 1024, forward: 222 + 323 us by
+// 64 segments, 92% and 90%; all steps by one wave a channel 5.3 ms.  More waves a SIMD would need a
+// backward tile in fewer than 256 registers.
 #pragma once
 
 #include <algorithm>
@@ -709,7 +717,8 @@ __global__ __launch_bounds__(kLanes) void add_state_parts(StateShape s, StateBac
     else add_shared<T>(s, a, cut, parts, blockIdx.x - few, gridDim.x - few);
 }
 
-// One step (n = 1: a token of each sequence): 4 states a lane, Each lanes of them a channel, and Rows
+// One step (n = 1: a token of each sequence): the states read and written once bound it, half 256 x
+// 4096 of 16 states 22.3 us (126 MB, 5.6 TB/s), bfloat16 8 x 1024 3.6 us.  4 states a lane, Each lanes of them a channel, and Rows
 // sequences one after the other, whose loads are all under way together and share a's.
 template <class T, int Each, int Rows>
 __global__ __launch_bounds__(kLanes, 6) void state_step(StateShape s, StateForward a) {

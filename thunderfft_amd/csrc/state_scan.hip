@@ -10,12 +10,13 @@
 namespace thff {
 namespace {
 
-// Segments of the steps.  They cost a kernel over the steps that only finds the segments' ends, 0.4
-// (forward) and 0.2 (backward) of the time of the steps themselves, and where there is one wave a
-// SIMD (1024 in all) the steps take 0.8 of it with two and more.  bfloat16, order 16, us a call by
-// one segment against these: forward 7 x 1000 x 2048 (896 waves) 94 and 8 x 4096 x 2048 (1024)
-// 444 against 82 and 533, 1 x 65536 x 1024 (64) 6775 against 560; backward 8 x 4096 x 2048 1210
-// against 1105, float 33 x 512 x 96 in two groups (264) 181 against 82.
+// Segments of the steps.  They cost a kernel over the steps that only finds the segments' ends, 0.7
+// (forward) and 0.24 (backward) of the time of the steps themselves, and where there is one wave a
+// SIMD (1024 in all) the steps take 0.8 of it with two and more.  Order 16, us a call by one segment
+// against many: forward bfloat16 6 x 4096 x 2048 (1536 waves of 8 lanes) 367 against 410, 8 x 4096 x
+// 2048 (1024 of 4) 390 against 490, 1 x 256 x 2048 (128) 27 against 20, 1 x 65536 x 1024 (64) 5316
+// against 510; backward 8 x 4096 x 2048 1224 against 1106, float 33 x 512 x 96 in two groups (264)
+// 174 against 67.
 int segments_of(long long waves, int n, bool backward) {
     const long long few = backward ? 1024 : 832, wanted = backward ? 8192 : 4096;
     if (waves == 0 || waves > few || n < (backward ? 128 : 256)) return 1;
