@@ -9,10 +9,10 @@
 // the states that the segments start from follow from those ends, in order.
 //
 // Instructions bound it: a state of a step takes 5 at least forward (dt a, its power, dt x b, and the
-// sums of h and y) and 15 backward (those again and the gradients'), and takes 7.6 and 23.8 with what
+// sums of h and y) and 15 backward (those again and the gradients'), and takes 7.6 and 23.7 with what
 // is once a step and channel, the addresses, LDS and the sums over channels.  bfloat16 8 x 4096 x 2048
 // of 16 states (134 MB a tensor): forward 376 us, at a wave a SIMD, the VALU issuing in 67% of the
-// cycles; backward 216 + 897 + 33 us by 8 segments, 87%.  1 x 65536 x 1024, forward: 222 + 323 us by
+// cycles; backward 193 + 910 + 33 us by 4 segments, 84%.  1 x 65536 x 1024, forward: 222 + 323 us by
 // 64 segments, 92% and 90%; all steps by one wave a channel 5.3 ms.  More waves a SIMD would need a
 // backward tile in fewer than 256 registers.
 #pragma once
