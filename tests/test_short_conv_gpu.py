@@ -279,6 +279,21 @@ def test_tensor_function(fused):
         thff.short_conv(x, torch.zeros(64, 5, device="cuda"))
 
 
+@pytest.mark.parametrize("T,width", [("half", 2), ("bfloat16", 3), ("float", 4)])
+def test_many_values(T, width):
+    """Past 2^25 values a lane has other channels: a few of them, the first and the last, against the
+    formulas in 64 bits, as no channel depends on another."""
+    v = values(11, T, 3, 5600, 2051, width)
+    lengths = ends(5600, 17, 5589)
+    got = run(T, *v, lengths=lengths, gap=5)
+    few = torch.tensor([0, 1, 2, 3, 1023, 2044, 2047, 2048, 2049, 2050], device="cuda")
+    x, weight, bias, state, dy, dstate = (t.index_select(0 if t.dim() < 3 else 2, few) for t in v)
+    want = oracle.conv(T, x, weight, bias, state, lengths, True, dy, dstate)
+    for name in want:
+        part = got[name].index_select(0 if name in ("dweight", "dbias") else 2, few)
+        oracle.check(name, part, want[name])
+
+
 def test_offsets_past_32_bits():
     """Rows further than 2^32 bytes into the buffer: the last channels of a long sequence of one
     width as those of a short one."""

@@ -5,7 +5,7 @@
 //   dxe[e] = sum_k weight[k] dp[e - k]  (+ dstate_out behind the end),
 //   dweight[k] = sum_t dp[t] xe[t + k],  dbias = sum_t dp[t].
 //
-// A lane takes 16 bytes of channels (backward 8) and some steps one after the other, with the last
+// A lane takes 16 bytes of channels (backward 2 or 4 of them) and some steps one after the other, with the last
 // K - 1 rows in registers, so that a row is read once but for those before a lane's first step.
 //
 // Memory bounds it: bfloat16 8 x 4096 x 2048, 4 taps, 49 us forward (294 MB, 6.0 TB/s) and 75 us
@@ -370,10 +370,9 @@ struct Kind {
     static constexpr int V = V_, K = K_;
 };
 
-// Bytes bytes of channels a lane; fewer channels than that, one.
-template <class T, int Bytes, class F>
+// V channels a lane; fewer channels than that, one.
+template <int V, class F>
 auto with_kind(const ConvShape& s, F f) {
-    constexpr int V = Bytes / sizeof(T);
     if (s.channels < V) {
         if (s.width == 2) return f(Kind<1, 2>{});
         if (s.width == 3) return f(Kind<1, 3>{});
@@ -384,20 +383,30 @@ auto with_kind(const ConvShape& s, F f) {
     return f(Kind<V, 4>{});
 }
 
-// Backward, where a channel takes four times the registers: bfloat16 8 x 4096 x 2048 75 us, 143 by 16
-// bytes a lane.
-constexpr int kBackwardBytes = 8;
+// Backward, where a channel takes four times the registers: 4 channels a lane from 2^25 values on, for
+// whole sectors of rows that lie apart, and 2 of fewer, for more lanes.  us of both passes by 4 and 2,
+// bfloat16: 8 x 4096 x 2048 in a projection's rows 124 and 139 (8, backward alone: 143 for 75), 1 x
+// 65536 x 1024 137 and 141; 16 x 2048 x 768 63.5 and 61.2, 2 x 2048 x 1024 23.2 and 21.6; float 8 x
+// 4096 x 2048 in a projection's rows 230 and 251, 4 x 2048 x 1024 45 and 35.
+template <class F>
+auto with_backward_kind(const ConvShape& s, F f) {
+    const __int128 values = static_cast<__int128>(s.batch) * s.n * s.channels;
+    return values < 1 << 25 ? with_kind<2>(s, f) : with_kind<4>(s, f);
+}
 
 int vectors_of(const ConvShape& s, int v) { return (s.channels + v - 1) / v; }
 
 ConvParts parts_of(const ConvShape& s, int v) {
-    constexpr long long kWanted = 1 << 17;  // lanes
+    // Lanes, and the least steps of one, which goes width - 1 steps on into the next's: twice the lanes
+    // take 128 us for 124 at bfloat16 8 x 4096 x 2048, at 2 x 2048 x 1024 32 steps 22.7 and 8 steps 21.7
+    // for 21.6.
+    constexpr long long kWanted = 1 << 17, kLeast = 16;
     ConvParts g;
     const int vectors = vectors_of(s, v);
     g.across = 1;
     while (g.across < 64 && g.across < vectors) g.across *= 2;
     const long long steps = static_cast<long long>(s.batch) * s.n * vectors / kWanted;
-    g.steps = static_cast<int>(std::min<long long>(std::max<long long>(steps, 32), 1 << 20)) / kAhead * kAhead;
+    g.steps = static_cast<int>(std::min<long long>(std::max(steps, kLeast), 1 << 20)) / kAhead * kAhead;
     g.chunks = std::max(1, static_cast<int>((s.n + static_cast<long long>(g.steps) - 1) / g.steps));
     const int rows = kLanes / g.across;
     g.count = (static_cast<long long>(s.batch) * g.chunks + rows - 1) / rows;
@@ -419,7 +428,7 @@ hipError_t launch_forward(const ConvShape& s, const ConvForward& a, hipStream_t 
 long long conv_workspace_bytes(const ConvShape& s) {
     if (s.batch == 0 || s.n == 0 || s.channels == 0) return 0;
     const long long parts = with_type(s.precision, [&](auto v) {
-        return with_kind<decltype(v), kBackwardBytes>(s, [&](auto kind) { return parts_of(s, decltype(kind)::V).count; });
+        return with_backward_kind(s, [&](auto kind) { return parts_of(s, decltype(kind)::V).count; });
     });
     return 4 * parts * (s.width + 1) * s.channels;
 }
@@ -427,7 +436,7 @@ long long conv_workspace_bytes(const ConvShape& s) {
 hipError_t launch_short_conv(const ConvShape& s, const ConvForward& a, hipStream_t stream) {
     return with_type(s.precision, [&](auto v) {
         using T = decltype(v);
-        return with_kind<T, 16>(s, [&](auto kind) {
+        return with_kind<16 / sizeof(T)>(s, [&](auto kind) {
             using Q = decltype(kind);
             if (s.n <= 1)
                 return s.silu ? launch_forward<T, Q::V, Q::K, true, 1>(s, a, stream)
@@ -441,7 +450,7 @@ hipError_t launch_short_conv(const ConvShape& s, const ConvForward& a, hipStream
 hipError_t launch_short_conv_backward(const ConvShape& s, const ConvBackward& a, hipStream_t stream) {
     return with_type(s.precision, [&](auto v) {
         using T = decltype(v);
-        return with_kind<T, kBackwardBytes>(s, [&](auto kind) {
+        return with_backward_kind(s, [&](auto kind) {
             using Q = decltype(kind);
             const int vectors = vectors_of(s, Q::V);
             const ConvParts g = parts_of(s, Q::V);
