@@ -421,3 +421,43 @@ def test_gradients_against_differences():
     along = sum(float((got["d" + k].double() * way[k].double()).sum()) for k in names)
     quotient = (outputs(2.0 ** -6) - outputs(-(2.0 ** -6))) * 2 ** 5
     assert abs(quotient - along) < 2e-3 * max(1.0, abs(along)), (quotient, along)
+
+
+@pytest.mark.parametrize("n", [300, 1])
+def test_offsets_past_32_bits(n):
+    """Rows 2^22 apart, the last ones more than 2^32 bytes into their buffers: the same bits as of dense rows."""
+    rows, stride, channels, order = 600, 1 << 22, 40, 16
+    v = values(31, "half", rows // n, n, channels, order)
+    names = dict(x=0, delta=64, gate=128, b=192, c=256, dy=320)
+    far = torch.empty(rows, stride, dtype=torch.float16, device="cuda")
+    out = torch.empty_like(far)
+    for name, at in names.items():
+        part = v[name].reshape(rows, -1)
+        far[:, at:at + part.shape[1]] = part
+    shape = thff.StateShape("half", rows // n, n, channels, order, 1, stride, stride, stride, stride, stride, stride)
+    wide = {name: far[:, at:] for name, at in names.items()}
+    got = {name: out[:, 64 * k:] for k, name in enumerate(("y", "dx", "ddelta", "dgate", "db", "dc"))}
+    state, da = torch.empty_like(v["state"]), torch.empty_like(v["a"])
+    saved = torch.empty(shape.saved_bytes(), dtype=torch.uint8, device="cuda")
+    workspace = torch.empty(shape.workspace_bytes(), dtype=torch.uint8, device="cuda")
+    more = dict(d_skip=v["skip"], d_gate=wide["gate"], d_delta_bias=v["delta_bias"])
+    calls = [(wide["x"], wide["delta"], v["a"], wide["b"], wide["c"], got["y"])]
+    want = run("half", v)
+    for d_saved in (None, saved):
+        # A single step that saves nothing has a kernel of its own.
+        thff.ThunderFFT_state_scan(shape, *calls[0], d_state_in=v["state"], d_state_out=state, d_saved=d_saved,
+                                   d_workspace=workspace, **more)
+        y = got["y"][:, :channels].reshape(want["y"].shape)
+        if n > 1 or d_saved is not None:
+            assert torch.equal(y, want["y"]) and torch.equal(state, want["state"])
+        else:
+            # The sum over the states in another order: two roundings of y's type and 16 of fp32's.
+            bound = 2.0 ** -10 * want["y"].float().abs() + 2.0 ** -18 * want["y"].float().abs().max()
+            assert ((y.float() - want["y"].float()).abs() <= bound).all()
+    thff.ThunderFFT_state_scan_backward(
+        shape, wide["dy"], wide["x"], wide["delta"], v["a"], wide["b"], wide["c"], saved, got["dx"], got["ddelta"], da, got["db"],
+        got["dc"], d_dgate=got["dgate"], d_dstate_out=v["dstate"], d_workspace=workspace, **more)
+    for name in ("dx", "ddelta", "dgate", "db", "dc"):
+        part = want[name].reshape(rows, -1)
+        assert torch.equal(got[name][:, :part.shape[1]], part), name
+    assert torch.equal(da, want["da"])
