@@ -507,7 +507,8 @@ int thff_rms_norm_async(int precision, const void* d_x, long long x_stride,
  * largest): q = y / scale, rounded to nearest even, with a scale for every `block` columns
  * of a row, the largest |y| of them / 448 (at least 2^-126).  block: 128, or cols for one
  * scale a row.  y is rounded once, to q.  q_stride in bytes; d_scales is fp32
- * [rows][ceil(cols / block)].  A NaN in a row makes its q NaN. */
+ * [rows][ceil(cols / block)].  A NaN in a row makes its q NaN; an infinite y makes its own q
+ * NaN, its block's scale infinite and the block's finite values 0. */
 int thff_rms_norm_8bit(int precision, const void* d_x, long long x_stride,
                        const void* d_residual, long long residual_stride, const void* d_weight,
                        float eps, void* d_q, long long q_stride, void* d_scales, int block,

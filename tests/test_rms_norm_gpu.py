@@ -220,6 +220,31 @@ def test_non_finite_rows_stay_alone(cols, junk):
     assert p[7].float().isnan().any() and (junk != junk) == bool(p[7].float().isnan().all())
 
 
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("cols", [5, 64, 130, 777, 2048, 20011, 40001])
+@pytest.mark.parametrize("large", [float("inf"), 3.0e38])
+def test_8bit_infinite_scales(T, cols, large):
+    """An infinite weight, or one whose product is out of range, makes its block's scale infinite: the finite
+    values over it are 0, the infinite one a NaN, and other blocks are as without it."""
+    x, residual, weight, *_ = values(23, T, 9, cols)
+    at = cols // 2
+    x[:, at], residual[:, at] = 64, 32
+    for block in (128, cols):
+        clean, fine, _ = run8(T, x, residual, weight, block)
+        wild = weight.clone()
+        wild[at] = large
+        q, scales, _ = run8(T, x, residual, wild, block)
+        hit = at // block
+        assert (scales[:, hit] == float("inf")).all()
+        inside = torch.arange(cols, device="cuda") // block == hit
+        inside[at] = False
+        assert (q.float()[:, inside] == 0).all() and q[:, at].float().isnan().all()
+        outside = torch.arange(cols, device="cuda") // block != hit
+        assert torch.equal(q.view(torch.uint8)[:, outside], clean.view(torch.uint8)[:, outside])
+        rest = [b for b in range(scales.shape[1]) if b != hit]
+        assert torch.equal(scales[:, rest], fine[:, rest])
+
+
 def test_no_rows():
     """No rows: the weight's gradient is zeros, whatever the workspace."""
     dw = torch.full((40,), GUARD, device="cuda")

@@ -30,14 +30,16 @@ __device__ __forceinline__ float lane_max(float v) {
 
 // What takes a block's largest value to the largest of e4m3, and its reciprocal.
 struct Scale {
-    float scale, inverse;
+    float scale, inverse, back;
     __device__ __forceinline__ explicit Scale(float largest)
-        : scale(fmaxf(largest / kLargest8, kLeastScale)), inverse(1.0f / scale) {}
+        : scale(fmaxf(largest / kLargest8, kLeastScale)), inverse(1.0f / scale), back(inverse == 0.0f ? 0.0f : scale) {}
     // v / scale to the last bit: v times the reciprocal is off by an ulp or so, which moves values that lie
-    // between two of e4m3's; what is left of v corrects it (float16 4099 x 2048: 11.0 us against 10.4).
+    // between two of e4m3's; what is left of v corrects it (float16 4099 x 2048: 11.0 us against 10.4).  Of an
+    // infinite scale (an infinite weight, or a product out of range) nothing is taken back, as 0 times it is a
+    // NaN: finite values over it are 0.
     __device__ __forceinline__ float of(float v) const {
         const float q = v * inverse;
-        return fmaf(fmaf(-q, scale, v), inverse, q);
+        return fmaf(fmaf(-q, back, v), inverse, q);
     }
 };
 
