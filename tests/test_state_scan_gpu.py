@@ -1,5 +1,7 @@
 """The state space scan on the GPU against its definition in 64 bits: outputs, states and gradients,
 in all types, orders and groups, for one token, for prompts and for long sequences in segments."""
+import math
+
 import pytest
 import torch
 
@@ -226,6 +228,34 @@ def test_states_of_zero_do_not_grow(order):
         # The same steps in fp32, whose dt and factors the two runs round alike.
         assert torch.allclose(got[name][:, -few:] if name == "y" else got[name], want, rtol=2.0 ** -20, atol=0), name
     assert torch.allclose(got["dx"][:, :few], first["dx"], rtol=2.0 ** -18, atol=2.0 ** -18 * first["dx"].abs().max().item())
+
+
+@pytest.mark.parametrize("order", [4, 16, 40])
+@pytest.mark.parametrize("power", [250, 257, 260])
+def test_small_states_that_grow(order, power):
+    """A state of 2^-140 that 96 steps in the middle take up by 2^power: the factor alone is out of range,
+    its product with the state is not.  The steps beside them have a dt of 0; the gradient of the state goes
+    back alike.  (dt a) is off by 2^-20 of `power` at most, the state at first by 2^-150 of 2^-140 a step, which
+    a step's growth by 2^2.6 and more makes 2^-9.6 of it in all: 2^-8."""
+    n, at, few = 2000, 960, 96
+    v = values(25, "float", 1, n, 24, order)
+    v["a"] = torch.full_like(v["a"], 0.5)
+    dt = power * math.log(2.0) / few / 0.5
+    v["delta"][:] = -200
+    v["delta"][:, at:at + few] = math.log(math.expm1(dt))
+    v |= dict(delta_bias=None, gate=None, skip=None)
+    for name in ("x", "dy"):
+        v[name][:] = 0
+    small, nothing = torch.full_like(v["state"], 2.0 ** -140), torch.zeros_like(v["state"])
+    # delta is rounded to fp32, with dt = softplus(delta) by the slope of it, 1 at most.
+    slack = few * 0.5 * 4 * 2.0 ** -24 / math.log(2.0)
+    assert slack < 2.0 ** -10
+    for given, name in ((dict(state=small, dstate=nothing), "state"), (dict(state=nothing, dstate=small), "dstate")):
+        got = run("float", v | given)
+        end = got[name].double() / 2.0 ** (power - 140)
+        assert ((end - 1).abs() < 2.0 ** -8).all(), (name, end.min().item(), end.max().item())
+        if name == "state":
+            assert torch.isfinite(got["y"]).all()
 
 
 @pytest.mark.parametrize("T", list(oracle.TYPES))

@@ -186,8 +186,8 @@ __device__ __forceinline__ void load_shared(float (&b)[S], float (&c)[S], const 
 
 // Takes h through the segments from `from` on, `count` of them one after the other, `way` apart: each
 // decays it by its sum of dt and adds its own end.  ends_of, sums_of: rows of the first one.  Where a is
-// positive a segment's factor may be out of range though its product with h, or an h of zero, is not:
-// its root is taken twice.
+// positive a segment's factor may be out of range though its product with h, or an h of zero, is not: its
+// whole powers of two go to h's exponent (those past 300 take any h out of range, or to 0, by themselves).
 template <class L>
 __device__ __forceinline__ void fold(float (&h)[L::S], const float (&decay)[L::S], const float* ends_of, const float* sums_of,
                                      long long way, int count, int sub) {
@@ -205,8 +205,9 @@ __device__ __forceinline__ void fold(float (&h)[L::S], const float (&decay)[L::S
             if (k + m == count) break;
 #pragma unroll
             for (int i = 0; i < L::S; ++i) {
-                const float root = __builtin_amdgcn_exp2f(0.5f * dt[m] * decay[i]);
-                h[i] = h[i] == 0.0f ? own[m][i] : fmaf(root, root * h[i], own[m][i]);
+                const float power = dt[m] * decay[i], whole = fminf(fmaxf(rintf(power), -300.0f), 300.0f);
+                const float grown = __builtin_amdgcn_exp2f(power - whole) * h[i];
+                h[i] = h[i] == 0.0f ? own[m][i] : __builtin_amdgcn_ldexpf(grown, static_cast<int>(whole)) + own[m][i];
             }
         }
     }
