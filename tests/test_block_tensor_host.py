@@ -131,3 +131,24 @@ def test_gradients_of_one_output(calls):
     y.sum().backward()
     args, named = calls["rms_norm_backward"]
     assert named["d_dsum"] is None and args[6] is None and args[7] is None
+
+
+def test_rows_too_far_apart_for_the_scan_are_copied(calls):
+    """The last steps of long sequences: rows more than 2^24 elements apart, which the kernels refuse, forward and
+    as the gradient that comes back."""
+    far = (1 << 25, 6, 1)
+    x, delta, gate = (torch.empty_strided((2, 1, 6), far).requires_grad_() for _ in range(3))
+    b, c = (torch.empty_strided((2, 1, 1, 5), (1 << 25, 6, 6, 1)).requires_grad_() for _ in range(2))
+    y, last = thff.state_scan(x, delta, leaf(6, 5), b, c, gate=gate)
+    (shape, *args), named = calls["state_scan"]
+    assert [shape.x_stride, shape.delta_stride, shape.gate_stride, shape.b_stride, shape.c_stride] == [6, 6, 6, 5, 5]
+    assert args[0].is_contiguous() and named["d_gate"].is_contiguous() and args[3].is_contiguous()
+    y.backward(torch.empty_strided((2, 1, 6), far))
+    (shape, *args), named = calls["state_scan_backward"]
+    assert [shape.x_stride, shape.delta_stride, shape.gate_stride, shape.b_stride, shape.c_stride, shape.y_stride] == [6, 6, 6, 5, 5, 6]
+    assert args[0].is_contiguous() and args[7].is_contiguous() and args[10].is_contiguous()
+    assert all(t.grad.shape == t.shape for t in (x, delta, gate, b, c))
+    # Rows as far apart as the kernels take are read in place.
+    near = torch.empty_strided((2, 1, 6), (1 << 24, 6, 1))
+    thff.state_scan(near, near, leaf(6, 5).detach(), near[..., :5], near[..., 1:])
+    assert calls["state_scan"][0][0].x_stride == calls["state_scan"][0][0].b_stride == 1 << 24

@@ -491,3 +491,26 @@ def test_offsets_past_32_bits(n):
         part = want[name].reshape(rows, -1)
         assert torch.equal(got[name][:, :part.shape[1]], part), name
     assert torch.equal(da, want["da"])
+
+
+def test_last_steps_of_far_sequences():
+    """The tensor function on steps more than 2^24 elements apart, and their gradients, are as on dense ones."""
+    v = values(32, "half", 3, 1, 40, 16)
+    far = torch.empty(3, 1 << 25, dtype=torch.float16, device="cuda")
+    names = ("x", "delta", "a", "b", "c", "skip", "gate", "delta_bias", "state")
+    at, leaves = 0, []
+    for name in names:
+        t = v[name]
+        if t.dtype == torch.float16:
+            row = t.flatten(1).shape[1]
+            part = far[:, at:at + row].unflatten(1, t.shape[1:])
+            part.copy_(t)
+            t, at = part, at + row
+        leaves.append(t.detach().requires_grad_())
+    dense = [v[name].clone().requires_grad_() for name in names]
+    dy = torch.empty(3, 1 << 25, dtype=torch.float16, device="cuda")[:, :40].unflatten(1, (1, 40))
+    dy.copy_(v["dy"])
+    for given, grad in ((leaves, dy), (dense, v["dy"])):
+        torch.autograd.backward(thff.state_scan(*given), [grad, v["dstate"]])
+    for name, one, other in zip(names, leaves, dense):
+        assert torch.equal(one.grad, other.grad), name

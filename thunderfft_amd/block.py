@@ -34,6 +34,17 @@ def _optional(name, t, dtype, shape, device):
     return t.contiguous()
 
 
+# Elements between rows that the scan takes at most.
+_FARTHEST = 1 << 24
+
+
+def _near_rows(t):
+    """As _rows, with a dense copy of rows further apart than the scan takes (the last steps of long
+    sequences, say)."""
+    t, stride = _rows(t)
+    return (t, stride) if stride is None or stride <= _FARTHEST else (t.contiguous(), t.shape[-1])
+
+
 def _like(t, stride):
     """A gradient's buffer for rows `stride` apart (None: no rows): the same distance, as the kernels
     take one for both, without memory for what lies between the last row and the next."""
@@ -117,7 +128,7 @@ class _StateScan(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         values = [x, delta, gate, b.flatten(2), c.flatten(2)]
         (x, xs), (delta, ds), gate_rows, (b_rows, bs), (c_rows, cs) = (
-            _rows(t) if t is not None else (None, None) for t in values)
+            _near_rows(t) if t is not None else (None, None) for t in values)
         batch, n, channels = x.shape
         order, groups = b.shape[3], b.shape[2]
         shape = thff.StateShape(x.dtype, batch, n, channels, order, groups, xs, ds, gate_rows[1], bs, cs)
@@ -142,7 +153,7 @@ class _StateScan(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else dy
         values = [dy, x, delta, gate, b, c]
         (dy, dys), (x, xs), (delta, ds), (gate, gs), (b, bs), (c, cs) = (
-            _rows(t) if t is not None else (None, None) for t in values)
+            _near_rows(t) if t is not None else (None, None) for t in values)
         batch, n, channels = x.shape
         order = a.shape[1]
         shape = thff.StateShape(x.dtype, batch, n, channels, order, ctx.groups, xs, ds, gs, bs, cs, dys)
@@ -172,7 +183,7 @@ def state_scan(x, delta, a, b, c, skip=None, gate=None, delta_bias=None, state=N
     x, delta and gate: float32, float16 or bfloat16 (batch, n, channels); without a gate y is the
     sum.  a: float32 (channels, order), order 1 to 64.  b and c: of x's type, (batch, n, order), or
     (batch, n, groups, order), where the channels fall into that many groups side by side.  Slices of
-    a projection's rows are read in place.  skip and delta_bias: float32 (channels,), None for zeros.
+    a projection's rows are read in place (rows more than 2^24 elements apart are copied).  skip and delta_bias: float32 (channels,), None for zeros.
     state: float32 (batch, channels, order) before the first step, None for zeros; the last states
     are alike.  lengths: int32 (batch,), steps from there on are left out and give y = 0.
     Differentiable (once) by all but lengths.
