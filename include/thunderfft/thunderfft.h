@@ -374,6 +374,8 @@ int thff_layer_norm_backward_async(int precision, const void* d_dy, long long dy
  * of shape->states rows; a slot outside the pool (-1, say) is an empty place, which
  * starts from zero and stores no state, and two places with the same slot race.
  * state_out may be state_in (states kept in place); the two must not overlap otherwise.
+ * Nothing else that a call writes, scratch memory included, may be another of its arrays,
+ * but for the norm's sums in their residuals' place.
  * lengths[b] is taken into [0, n]; outputs and gradients are 0 from there on, and no
  * input is used there, whatever it holds. */
 

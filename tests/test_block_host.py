@@ -374,3 +374,49 @@ def test_rms_oracle_gradients():
         return float((r["y"][0] * dy).sum() + (r["sum"][0] * dsum).sum())
 
     against_differences(values, outputs, got, ("dx", "dweight"))
+
+
+@pytest.mark.parametrize("twin", ["", "_async"])
+def test_outputs_in_another_arrays_place(twin):
+    """States, statistics and scratch memory that a call writes are no other array's: kept in place are only
+    states (state_out = state_in) and residuals."""
+    def refused(call, **arrays):
+        with pytest.raises(ValueError, match="alias"):
+            call(**arrays)
+
+    conv, scan, norm, bits8 = (getattr(thff, f"ThunderFFT_{name}{twin}") for name in ("short_conv", "state_scan", "rms_norm", "rms_norm_8bit"))
+    good = dict(shape=conv_shape(), d_x=A, d_weight=B, d_bias=C, d_y=D, d_slots=E, d_lengths=F)
+    for name in ("d_x", "d_weight", "d_bias", "d_y", "d_slots", "d_lengths"):
+        refused(conv, **good, d_state_out=good[name])
+    for name in ("d_slots", "d_lengths"):
+        refused(conv, **dict(good, d_y=good[name]))
+    refused(conv, **dict(good, shape=conv_shape(n=0), d_state_out=B))
+    more = 9 << 16
+    good = dict(shape=state_shape(), d_x=A, d_delta=B, d_a=C, d_b=D, d_c=E, d_y=F, d_skip=G, d_gate=H, d_delta_bias=more,
+                d_state_in=more << 1, d_slots=more << 2, d_lengths=more << 3, d_saved=more << 4, d_workspace=more << 5)
+    for name in good:
+        if name not in ("shape", "d_state_in"):
+            refused(scan, **good, d_state_out=good[name])
+        if name not in ("shape", "d_saved", "d_workspace"):
+            refused(scan, **dict(good, d_saved=good[name]))
+            refused(scan, **dict(good, d_workspace=good[name]))
+    refused(scan, **dict(good, d_saved=more << 5))
+    refused(norm, T="half", d_x=A, d_weight=B, eps=1e-5, d_y=C, rows=4, cols=8, d_residual=E, d_rstd=E)
+    refused(bits8, T="half", d_x=A, d_weight=B, eps=1e-5, d_q=C, d_scales=E, rows=4, cols=256, d_residual=E)
+
+    back = getattr(thff, "ThunderFFT_short_conv_backward" + twin)
+    good = dict(shape=conv_shape(), d_dy=A, d_x=B, d_weight=C, d_bias=D, d_dx=E, d_dweight=F, d_dbias=G, d_lengths=more, d_workspace=H)
+    for name in good:
+        if name not in ("shape", "d_workspace"):
+            refused(back, **dict(good, d_workspace=good[name]))
+    refused(back, **dict(good, d_dweight=more))
+    back = getattr(thff, "ThunderFFT_state_scan_backward" + twin)
+    names = ("d_dy", "d_x", "d_delta", "d_a", "d_b", "d_c", "d_saved", "d_dx", "d_ddelta", "d_da", "d_db", "d_dc", "d_lengths")
+    good = dict({name: (k + 1) << 16 for k, name in enumerate(names)}, shape=state_shape())
+    for name in names:
+        refused(back, **good, d_workspace=good[name])
+    refused(back, **dict(good, d_da=good["d_lengths"], d_workspace=more << 8))
+    back = getattr(thff, "ThunderFFT_rms_norm_backward" + twin)
+    good = dict(T="half", d_dy=A, d_sum=B, d_rstd=C, d_weight=D, d_dx=E, d_dweight=F, d_dsum=G, rows=4, cols=8)
+    for name in ("d_dy", "d_sum", "d_rstd", "d_weight", "d_dx", "d_dweight", "d_dsum"):
+        refused(back, **good, d_workspace=good[name])

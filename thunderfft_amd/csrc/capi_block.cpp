@@ -76,10 +76,9 @@ int conv_impl(const thff_conv_shape* shape, const ConvForward& a, void* stream, 
     const unsigned e = element_bytes(s.precision);
     if (!a.weight || (s.n > 0 && any_null({a.x, a.y})))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv requires non-null x, weight and y");
-    if (s.n > 0) {
-        if (any_alias({a.y}, {a.x, a.weight, a.bias, a.state_in, a.state_out}))
-            return fail(THFF_EINVAL, "ThunderFFT_short_conv output must not alias another array");
-    }
+    if ((s.n > 0 && any_alias({a.y}, {a.x, a.weight, a.bias, a.state_in, a.state_out, a.slots, a.lengths})) ||
+        any_alias({a.state_out}, {a.x, a.weight, a.bias, a.slots, a.lengths}))
+        return fail(THFF_EINVAL, "ThunderFFT_short_conv output must not alias another array");
     if (!all_aligned({a.x, a.y, a.state_in, a.state_out}, e))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv requires element-aligned values and states");
     if (!all_aligned({a.weight, a.bias, a.slots, a.lengths}, 4))
@@ -104,8 +103,8 @@ int conv_backward_impl(const thff_conv_shape* shape, const ConvBackward& a, void
             return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward requires a workspace of " +
                                          std::to_string(conv_workspace_bytes(s)) + " bytes");
     }
-    if (any_alias({a.dx, a.dweight, a.dbias, a.dstate_in},
-                  {a.dy, a.x, a.weight, a.bias, a.state_in, a.dstate_out}))
+    if (any_alias({a.dx, a.dweight, a.dbias, a.dstate_in, a.workspace},
+                  {a.dy, a.x, a.weight, a.bias, a.state_in, a.dstate_out, a.lengths}))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward outputs must not alias other arrays");
     if (!all_aligned({a.dy, a.x, a.dx, a.state_in, a.dstate_out, a.dstate_in}, e))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward requires element-aligned values and states");
@@ -150,10 +149,10 @@ int state_impl(const thff_state_shape* shape, const StateForward& a, void* strea
     if (s.batch == 0 || s.channels == 0) return THFF_OK;
     if (!a.a || (s.n > 0 && any_null({a.x, a.delta, a.b, a.c, a.y})))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan requires non-null x, delta, a, b, c and y");
-    if (s.n > 0) {
-        if (any_alias({a.y}, {a.x, a.delta, a.a, a.b, a.c, a.skip, a.gate, a.delta_bias, a.state_in, a.state_out}))
-            return fail(THFF_EINVAL, "ThunderFFT_state_scan output must not alias another array");
-    }
+    if (any_alias({s.n > 0 ? a.y : nullptr, a.saved, a.workspace},
+                  {a.x, a.delta, a.a, a.b, a.c, a.skip, a.gate, a.delta_bias, a.state_in, a.state_out, a.slots, a.lengths}) ||
+        any_alias({a.state_out}, {a.x, a.delta, a.a, a.b, a.c, a.skip, a.gate, a.delta_bias, a.slots, a.lengths}))
+        return fail(THFF_EINVAL, "ThunderFFT_state_scan output must not alias another array");
     if (!all_aligned({a.x, a.delta, a.b, a.c, a.gate, a.y}, element_bytes(s.precision)))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan requires element-aligned buffers");
     if (!all_aligned({a.a, a.skip, a.delta_bias, a.state_in, a.state_out, a.slots, a.lengths}, 4))
@@ -190,8 +189,9 @@ int state_backward_impl(const thff_state_shape* shape, const thff_state_gradient
     if (s.batch > 0 && !workspace && state_workspace_bytes(s) > 0)
         return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward requires a workspace of " +
                                      std::to_string(state_workspace_bytes(s)) + " bytes");
-    if (any_alias({g->dx, g->ddelta, g->da, g->db, g->dc, g->dskip, g->dgate, g->ddelta_bias, g->dstate_in},
-                  {g->dy, g->x, g->delta, g->a, g->b, g->c, g->skip, g->gate, g->delta_bias, g->saved, g->dstate_out}))
+    if (any_alias({g->dx, g->ddelta, g->da, g->db, g->dc, g->dskip, g->dgate, g->ddelta_bias, g->dstate_in, workspace},
+                  {g->dy, g->x, g->delta, g->a, g->b, g->c, g->skip, g->gate, g->delta_bias, g->saved, g->dstate_out,
+                   g->lengths}))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward outputs must not alias other arrays");
     if (!all_aligned({g->dy, g->x, g->delta, g->b, g->c, g->gate, g->dx, g->ddelta, g->db, g->dc, g->dgate},
                      element_bytes(s.precision)))
@@ -253,7 +253,7 @@ int rms_impl(RmsForward a, void* stream, bool synchronize) {
     if (a.rows == 0) return THFF_OK;
     if (!a.x || !a.y) return fail(THFF_EINVAL, "ThunderFFT_rms_norm requires non-null x and output");
     if (bits8 && !a.scales) return fail(THFF_EINVAL, "ThunderFFT_rms_norm_8bit requires non-null scales");
-    if (any_alias({a.y, a.sum, a.scales, a.rstd}, {a.x, a.weight}) || (a.residual && a.y == a.residual))
+    if (any_alias({a.y, a.sum, a.scales, a.rstd}, {a.x, a.weight}) || any_alias({a.y, a.scales, a.rstd}, {a.residual}))
         return fail(THFF_EINVAL, "ThunderFFT_rms_norm outputs must not alias its inputs");
     if (a.sum && a.sum == a.residual && a.sum_stride != a.residual_stride)
         return fail(THFF_EINVAL, "ThunderFFT_rms_norm sums in the residual's place need its stride");
@@ -278,7 +278,7 @@ int rms_backward_impl(RmsBackward a, void* stream, bool synchronize) {
     if (a.rows > 0) {
         if (any_null({a.dy, a.sum, a.rstd, a.dx}))
             return fail(THFF_EINVAL, "ThunderFFT_rms_norm_backward requires non-null dy, sum, rstd and dx");
-        if (any_alias({a.dx, a.dweight}, {a.dy, a.sum, a.rstd, a.weight, a.dsum}))
+        if (any_alias({a.dx, a.dweight, a.workspace}, {a.dy, a.sum, a.rstd, a.weight, a.dsum}))
             return fail(THFF_EINVAL, "ThunderFFT_rms_norm_backward outputs must not alias its inputs");
         if (!all_aligned({a.dy, a.sum, a.dsum, a.dx}, element_bytes(a.precision)))
             return fail(THFF_EINVAL, "ThunderFFT_rms_norm_backward requires element-aligned buffers");
