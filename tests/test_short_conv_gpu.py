@@ -311,3 +311,30 @@ def test_offsets_past_32_bits():
     thff.ThunderFFT_short_conv_backward(shape, y, x, weight, None, dx)
     thff.ThunderFFT_short_conv_backward(thff.ConvShape("half", 1, 100, channels, 4), z, tail, weight, None, dz, d_state_in=state)
     assert torch.equal(dx[:, -100:], dz)
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("silu", [True, False])
+def test_same_bits_however_a_sequence_is_cut(T, silu):
+    """A sequence in one call, and in calls of other lengths that hand the state on, fall otherwise into the
+    kernels' tiles: outputs, states and gradients of values have the same bits."""
+    n, channels, width = 1500, 1024, 4
+    x, weight, bias, _, dy, _ = values(41, T, 1, n, channels, width)
+    whole = thff.ConvShape(T, 1, n, channels, width, silu)
+    y, dx, last = torch.empty_like(x), torch.empty_like(x), x.new_empty(1, width - 1, channels)
+    thff.ThunderFFT_short_conv(whole, x, weight, bias, y, d_state_out=last)
+    thff.ThunderFFT_short_conv_backward(whole, dy, x, weight, bias, dx)
+    for count in (1, 7, 24, 401):
+        state, z = torch.zeros_like(last), torch.empty_like(x)
+        for at in range(0, n, count):
+            now = min(count, n - at)
+            part = thff.ConvShape(T, 1, now, channels, width, silu)
+            thff.ThunderFFT_short_conv_async(part, x[:, at:], weight, bias, z[:, at:], d_state_in=state, d_state_out=state)
+        torch.cuda.synchronize()
+        assert torch.equal(y, z) and torch.equal(last, state), count
+    # The gradients of all but the last steps of a call, which others behind it reach too.
+    for at in range(1, 40, 3):
+        part, dz = thff.ConvShape(T, 1, n - at, channels, width, silu), torch.empty_like(x[:, at:])
+        thff.ThunderFFT_short_conv_backward(part, dy[:, at:], x[:, at:], weight, bias, dz, d_state_in=x[:, at - 3:at].contiguous()
+                                            if at >= 3 else torch.cat([torch.zeros_like(x[:, at:3]), x[:, :at]], 1))
+        assert torch.equal(dz, dx[:, at:]), at

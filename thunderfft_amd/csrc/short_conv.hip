@@ -32,6 +32,15 @@ __device__ __forceinline__ float opened(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
 }
 
+// v rounded to T.  (half)(a * b) may become one instruction that rounds the exact product once, or two with
+// one to fp32 between; which, differs from step to step of a tile, and one in 2^14 values with it.  Held in a
+// register v is fp32 everywhere, so that a sequence has the same bits however it is cut into calls.
+template <class T>
+__device__ __forceinline__ T rounded(float v) {
+    if constexpr (std::is_same_v<T, half_t>) asm("" : "+v"(v));
+    return from_float<T>(v);
+}
+
 // Where a lane's V channels are: the last lane of a row takes the last V, `skip` of which are also
 // the lane's before it.
 struct Channels {
@@ -149,7 +158,7 @@ __global__ __launch_bounds__(kLanes) void conv_forward(ConvShape s, ConvForward 
 #pragma unroll
                     for (int k = 0; k < K; ++k) p = fmaf(taps.w[k][v], to_float<T>(in[j + k][v]), p);
                     if constexpr (Silu) p *= opened(p);
-                    out[v] = from_float<T>(decltype(all)::value || t0 + j < length ? p : 0.0f);
+                    out[v] = rounded<T>(decltype(all)::value || t0 + j < length ? p : 0.0f);
                 }
                 if (decltype(all)::value) store_pack<T, V>(y + j * s.y_stride, out);
                 else store_own<T, V>(y + j * s.y_stride, out, c.skip);
@@ -280,7 +289,7 @@ __global__ __launch_bounds__(kLanes) void conv_backward(ConvShape s, ConvBackwar
                     float sum = kWhole ? 0.0f : to_float<T>(after[v]);
 #pragma unroll
                     for (int k = 0; k < K; ++k) sum = fmaf(taps.w[k][v], dp[H + j - k][v], sum);
-                    out[v] = from_float<T>(kWhole || e - H < length ? sum : 0.0f);
+                    out[v] = rounded<T>(kWhole || e - H < length ? sum : 0.0f);
                 }
                 if (kWhole || e - H >= t0)
                     store_pack<T, V>(to + j * s.x_stride, out);
