@@ -420,3 +420,40 @@ def test_outputs_in_another_arrays_place(twin):
     good = dict(T="half", d_dy=A, d_sum=B, d_rstd=C, d_weight=D, d_dx=E, d_dweight=F, d_dsum=G, rows=4, cols=8)
     for name in ("d_dy", "d_sum", "d_rstd", "d_weight", "d_dx", "d_dweight", "d_dsum"):
         refused(back, **good, d_workspace=good[name])
+
+
+class OnDevice:
+    """Stands for a tensor on the device at `at`."""
+
+    def __init__(self, t, at):
+        self.dtype, self.is_cuda, self.is_contiguous, self.stride, self.at = t.dtype, True, t.is_contiguous, t.stride, at
+
+    def data_ptr(self):
+        return self.at
+
+
+def test_slots_and_lengths_refused(monkeypatch):
+    """Tensors in host memory, of another type or with gaps: kernels would index by what they read there."""
+    given = []
+    monkeypatch.setattr(thff, "_raise", lambda rc: given.append(rc))
+    good = torch.zeros(8, dtype=torch.int32)
+    wrong = ((good, "device memory"), (OnDevice(good.long(), G), "int32"), (OnDevice(good.float(), G), "int32"),
+             (OnDevice(good[::2], G), "gaps"), (OnDevice(good.view(4, 2)[:, 0], G), "gaps"))
+    scan = thff.ScanShape("half", 2, 300, 70)
+    args = dict.fromkeys(("d_dy", "d_x", "d_delta", "d_a", "d_b", "d_c", "d_saved", "d_dx", "d_ddelta", "d_da", "d_db", "d_dc"), 0)
+    both = (("d_slots", "d_lengths"), lambda **more: thff.ThunderFFT_short_conv_async(conv_shape(), 0, B, C, D, **more)), (
+        ("d_slots", "d_lengths"), lambda **more: thff.ThunderFFT_state_scan_async(state_shape(), 0, B, C, D, E, F, **more)), (
+        ("d_slots", "d_lengths"), lambda **more: thff.ThunderFFT_gated_scan_async(scan, 0, B, C, **more)), (
+        ("d_lengths",), lambda **more: thff.ThunderFFT_short_conv_backward_async(conv_shape(), 0, B, C, D, E, F, G, **more)), (
+        ("d_lengths",), lambda **more: thff.ThunderFFT_state_scan_backward_async(state_shape(), **args, **more)), (
+        ("d_lengths",), lambda **more: thff.ThunderFFT_gated_scan_backward_async(scan, 0, B, C, D, E, F, **more))
+    for names, call in both:
+        for name in names:
+            for t, what in wrong:
+                with pytest.raises(ValueError, match=what):
+                    call(**{name: t})
+            given.clear()
+            # These reach the library, which refuses the null pointers beside them.
+            for t in (None, G, OnDevice(good, G), OnDevice(good.view(8, 1)[:, 0], G)):
+                call(**{name: t})
+            assert given == [thff.THFF_EINVAL] * 4

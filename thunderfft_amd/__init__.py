@@ -48,11 +48,12 @@ THFF_OK, THFF_EINVAL, THFF_EIO = 0, -22, -5
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libthunderfft_amd.so")
 
 _lib = None
+_int32 = None  # torch's, once it is loaded
 
 
 def lib() -> ctypes.CDLL:
     """Load libthunderfft_amd.so (raises if it has not been built)."""
-    global _lib
+    global _lib, _int32
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise ImportError(
@@ -62,7 +63,9 @@ def lib() -> ctypes.CDLL:
         # be a second runtime in the process, and this library's would find no
         # device; loaded first, this library binds to torch's (same soname).
         try:
-            import torch  # noqa: F401
+            import torch
+
+            _int32 = torch.int32
         except ImportError:
             pass
         L = ctypes.CDLL(LIB_PATH)
@@ -155,15 +158,32 @@ def _ptr(x) -> int:
     raise TypeError(f"expected a device pointer or tensor, got {type(x).__name__}")
 
 
+def _ints(x) -> int:
+    """_ptr of slots or lengths, which kernels index by: a tensor of them is int32 without gaps, in memory
+    that the device reads."""
+    if x is None or isinstance(x, int):
+        return x or 0
+    dtype = getattr(x, "dtype", None)
+    if dtype is None:
+        return _ptr(x)
+    if dtype is not _int32 and str(dtype) != "torch.int32" or not x.is_contiguous():
+        raise ValueError(f"slots and lengths must be int32 without gaps (got {dtype}, strides {tuple(x.stride())})")
+    if not x.is_cuda and not x.is_pinned():
+        raise ValueError("slots and lengths must be in device memory")
+    return x.data_ptr()
+
+
 def _stream(s) -> int:
-    if s is None or s == 0:
+    if s is None:
         return 0
     if isinstance(s, int):
         return s
     handle = getattr(s, "cuda_stream", None)
-    if handle is None:
-        raise TypeError("stream must be an integer hipStream_t or a torch.cuda.Stream")
-    return int(handle)
+    if handle is not None:
+        return int(handle)
+    if s == 0:
+        return 0
+    raise TypeError("stream must be an integer hipStream_t or a torch.cuda.Stream")
 
 
 def _raise(rc: int) -> None:
@@ -338,7 +358,7 @@ def _bytes(rc: int) -> int:
 def _gated_scan(call, shape, d_x, d_gate, d_y, d_state_in, d_state_out, d_slots, d_lengths,
                 d_saved, d_workspace, stream):
     _raise(call(shape, _ptr(d_x), _ptr(d_gate), _ptr(d_y), _ptr(d_state_in), _ptr(d_state_out),
-                _ptr(d_slots), _ptr(d_lengths), _ptr(d_saved), _ptr(d_workspace), _stream(stream)))
+                _ints(d_slots), _ints(d_lengths), _ptr(d_saved), _ptr(d_workspace), _stream(stream)))
 
 
 def ThunderFFT_gated_scan(shape, d_x, d_gate, d_y, d_state_in=None, d_state_out=None, d_slots=None,
@@ -364,7 +384,7 @@ def ThunderFFT_gated_scan_async(shape, d_x, d_gate, d_y, d_state_in=None, d_stat
 def _gated_scan_backward(call, shape, d_dy, d_x, d_gate, d_saved, d_dx, d_dgate, d_dstate_out,
                          d_dstate_in, d_lengths, d_workspace, stream):
     _raise(call(shape, _ptr(d_dy), _ptr(d_x), _ptr(d_gate), _ptr(d_saved), _ptr(d_dstate_out),
-                _ptr(d_lengths), _ptr(d_dx), _ptr(d_dgate), _ptr(d_dstate_in), _ptr(d_workspace),
+                _ints(d_lengths), _ptr(d_dx), _ptr(d_dgate), _ptr(d_dstate_in), _ptr(d_workspace),
                 _stream(stream)))
 
 
@@ -485,7 +505,7 @@ class ConvShape(ctypes.Structure):
 def _short_conv(call, shape, d_x, d_weight, d_bias, d_y, d_state_in, d_state_out, d_slots, d_lengths,
                 stream):
     _raise(call(shape, _ptr(d_x), _ptr(d_weight), _ptr(d_bias), _ptr(d_y), _ptr(d_state_in),
-                _ptr(d_state_out), _ptr(d_slots), _ptr(d_lengths), _stream(stream)))
+                _ptr(d_state_out), _ints(d_slots), _ints(d_lengths), _stream(stream)))
 
 
 def ThunderFFT_short_conv(shape, d_x, d_weight, d_bias, d_y, d_state_in=None, d_state_out=None,
@@ -510,7 +530,7 @@ def ThunderFFT_short_conv_async(shape, d_x, d_weight, d_bias, d_y, d_state_in=No
 def _short_conv_backward(call, shape, d_dy, d_x, d_weight, d_bias, d_dx, d_dweight, d_dbias,
                          d_state_in, d_dstate_out, d_dstate_in, d_lengths, d_workspace, stream):
     _raise(call(shape, _ptr(d_dy), _ptr(d_x), _ptr(d_weight), _ptr(d_bias), _ptr(d_state_in),
-                _ptr(d_dstate_out), _ptr(d_lengths), _ptr(d_dx), _ptr(d_dweight), _ptr(d_dbias),
+                _ptr(d_dstate_out), _ints(d_lengths), _ptr(d_dx), _ptr(d_dweight), _ptr(d_dbias),
                 _ptr(d_dstate_in), _ptr(d_workspace), _stream(stream)))
 
 
@@ -579,7 +599,7 @@ def _state_scan(call, shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip, d_gate, d
                 d_state_out, d_slots, d_lengths, d_saved, d_workspace, stream):
     _raise(call(shape, _ptr(d_x), _ptr(d_delta), _ptr(d_a), _ptr(d_b), _ptr(d_c), _ptr(d_skip),
                 _ptr(d_gate), _ptr(d_delta_bias), _ptr(d_y), _ptr(d_state_in), _ptr(d_state_out),
-                _ptr(d_slots), _ptr(d_lengths), _ptr(d_saved), _ptr(d_workspace), _stream(stream)))
+                _ints(d_slots), _ints(d_lengths), _ptr(d_saved), _ptr(d_workspace), _stream(stream)))
 
 
 def ThunderFFT_state_scan(shape, d_x, d_delta, d_a, d_b, d_c, d_y, d_skip=None, d_gate=None,
@@ -620,7 +640,7 @@ def _state_scan_backward(call, shape, d_dy, d_x, d_delta, d_a, d_b, d_c, d_saved
                          d_dstate_out, d_dstate_in, d_lengths, d_workspace, stream):
     arrays = _StateGradients(*map(_ptr, (
         d_dy, d_x, d_delta, d_a, d_b, d_c, d_skip, d_gate, d_delta_bias, d_saved, d_dstate_out,
-        d_lengths, d_dx, d_ddelta, d_da, d_db, d_dc, d_dskip, d_dgate, d_ddelta_bias, d_dstate_in)))
+        _ints(d_lengths), d_dx, d_ddelta, d_da, d_db, d_dc, d_dskip, d_dgate, d_ddelta_bias, d_dstate_in)))
     _raise(call(shape, arrays, _ptr(d_workspace), _stream(stream)))
 
 
