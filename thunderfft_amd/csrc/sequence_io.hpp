@@ -22,7 +22,13 @@ __device__ __forceinline__ T from_float(float v) {
 // V values in one access that needs no more than the element's alignment (the hardware takes
 // unaligned vectors; rows of an odd length start on any element).
 template <class T, int V>
-using pack = T __attribute__((ext_vector_type(V), aligned(alignof(T))));
+struct Packed {
+    typedef T Vector __attribute__((ext_vector_type(V)));
+    typedef Vector Type __attribute__((aligned(alignof(T))));
+};
+template <class T, int V>
+using pack = typename Packed<T, V>::Type;
+static_assert(alignof(pack<half_t, 8>) == alignof(half_t));
 
 template <class T, int V>
 __device__ __forceinline__ pack<T, V> load_pack(const T* p) {
