@@ -514,3 +514,46 @@ def test_last_steps_of_far_sequences():
         torch.autograd.backward(thff.state_scan(*given), [grad, v["dstate"]])
     for name, one, other in zip(names, leaves, dense):
         assert torch.equal(one.grad, other.grad), name
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("size", [(1025, 1030, 3, 1), (513, 1030, 7, 2), (257, 1030, 16, 1), (263, 1030, 13, 2), (131, 1030, 24, 1),
+                                  (65, 1030, 50, 1)], ids=str)
+def test_one_token_of_many_sequences(T, size):
+    """From 2^20 lanes on a lane has two sequences: an odd batch, strides, lengths of 0 and 1, and states in
+    place in a larger pool, with slots that are none beside ones that are.  Some channels of each group against
+    the formulas, as no channel depends on another."""
+    batch, channels, order, groups = size
+    v = values(33, T, batch, 1, channels, order, groups)
+    gen = torch.Generator().manual_seed(34)
+    states, all_of = batch + 37, torch.arange(batch)
+    slots = torch.randperm(states, generator=gen)[:batch].to(torch.int32)
+    slots[all_of % 5 == 3], slots[all_of % 11 == 7], slots[:2] = -1, states, -1
+    some = (slots >= 0) & (slots < states)
+    assert some[batch - 1] and (some[:-1:2] != some[1::2]).any()
+    pool = torch.randn(states, channels, order, generator=gen).cuda()
+    first = torch.where(some.view(-1, 1, 1).cuda(), pool[slots.clamp(0, states - 1).long().cuda()], 0.0)
+    at = {k: placed(v[k], 3, 1)[0] for k in VALUES + SHARED}
+    row = groups * order + 3
+    shape = thff.StateShape(T, batch, 1, channels, order, groups, *(channels + 3,) * 3, row, row, channels + 3, states=states)
+    few = torch.tensor([0, 1, 513, 514, 515, 516, 1028, 1029], device="cuda")
+    for end in (None, (torch.arange(batch, device="cuda") % 3 != 1).to(torch.int32)):
+        y, intact = placed(torch.full_like(v["x"], float("nan")), 3, 1)
+        kept = torch.cat([pool, torch.full_like(pool[:1], GUARD)])
+        print(f"{T} {size} lengths {end is not None}", flush=True)
+        thff.ThunderFFT_state_scan(shape, at["x"], at["delta"], v["a"], at["b"], at["c"], y, d_skip=v["skip"], d_gate=at["gate"],
+                                   d_delta_bias=v["delta_bias"], d_state_in=kept, d_state_out=kept, d_slots=slots.cuda(),
+                                   d_lengths=end)
+        assert intact() and torch.isfinite(y).all() and (kept[-1] == GUARD).all()
+        free = torch.ones(states, dtype=torch.bool)
+        free[slots[some].long()] = False
+        assert torch.equal(kept[:-1][free.cuda()], pool[free.cuda()])
+        mine = kept[slots[some].long().cuda()]
+        if end is not None:
+            assert torch.equal(mine[(end == 0)[some]], first[some.cuda()][(end == 0)[some]])
+        for g in range(groups):
+            c = few[few // (channels // groups) == g]
+            want = oracle.state(T, v["x"][..., c], v["delta"][..., c], v["a"][c], v["b"][:, :, g:g + 1], v["c"][:, :, g:g + 1],
+                                v["skip"][c], v["gate"][..., c], v["delta_bias"][c], first[:, c], end)
+            oracle.check("y", y[..., c], want["y"])
+            oracle.check("state", mine[:, c], tuple(t[some] for t in want["state"]))
