@@ -557,3 +557,35 @@ def test_one_token_of_many_sequences(T, size):
                                 v["skip"][c], v["gate"][..., c], v["delta_bias"][c], first[:, c], end)
             oracle.check("y", y[..., c], want["y"])
             oracle.check("state", mine[:, c], tuple(t[some] for t in want["state"]))
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("order", [4, 16, 40])
+def test_segments_with_states_in_a_pool(T, order):
+    """Prompts long enough for segments, in two calls, the states in place in rows of a pool: as each whole
+    sequence, with a place that is none and lengths that end in any segment; other rows of the pool stay."""
+    batch, n, channels = 5, 900, 24
+    v = values(35, T, batch, n, channels, order)
+    slots, rows = ends(6, 2, -1, 0, 5), [0, 1, 3, 4]
+    pool = torch.full((8, channels, order), GUARD, device="cuda")
+    pool[slots[rows].long()] = v["state"][rows]
+    kept = pool.clone()
+    lengths, at, y = torch.tensor([900, 700, 900, 30, 533]), 0, torch.empty_like(v["x"])
+    for count in (500, 400):
+        part = {k: v[k][:, at:at + count].contiguous() for k in VALUES + SHARED}
+        shape = thff.StateShape(T, batch, count, channels, order, states=8)
+        out = torch.empty_like(part["x"])
+        assert shape.forward_bytes() > 0
+        work = torch.full((shape.forward_bytes(),), 0xFF, dtype=torch.uint8, device="cuda")
+        end = (lengths - at).clamp(0, count).to(torch.int32).cuda()
+        thff.ThunderFFT_state_scan(shape, part["x"], part["delta"], v["a"], part["b"], part["c"], out, d_skip=v["skip"],
+                                   d_gate=part["gate"], d_delta_bias=v["delta_bias"], d_state_in=pool, d_state_out=pool,
+                                   d_slots=slots, d_lengths=end, d_workspace=work)
+        y[:, at:at + count] = out
+        at += count
+    whole = oracle.state(T, v["x"], v["delta"], v["a"], v["b"], v["c"], v["skip"], v["gate"], v["delta_bias"], v["state"], lengths)
+    for name, got in (("y", y), ("state", pool[slots.long()])):
+        value, bound = whole[name]
+        oracle.check(name, got[rows], (value[rows], bound[rows]))
+    free = [r for r in range(8) if r not in (6, 2, 0, 5)]
+    assert torch.equal(pool[free], kept[free])
