@@ -5,8 +5,10 @@ Values come with bounds, which follow the roundings of the formulas with u = 2^-
 reciprocal and the square root are off by 2 u, and what is below 2^-126 may be lost:
   exp(v)     through exp2: the exponent is off by 2 u of its size more (constant and product).
   sigmoid    (2 |v| + 8) u of itself: exp, a sum, a reciprocal.
-  softplus   of v = delta + bias, off by u |v|: the slope carries that; exp(-|v|), a quotient, nine
-             terms of a series and a sum: (2 |v| + 16) u of itself.
+  softplus   of v = delta + bias, off by u |v|: the slope carries that; exp(-|v|), the logarithm of
+             the rounded 1 + exp(-|v|), what that rounding lost, and a sum: (1.25 |v| + 11) u of
+             log(1 + exp(-|v|)) and u of itself (the test of step sizes has the terms and holds the
+             kernels to them), taken as (2 |v| + 16) u of itself.
   conv       width products, added one after the other: (width + 1) u of the sum of sizes.
   scan       a step multiplies by exp(dt a) and adds dt x b; M is the recurrence of the sizes.
              Segments join by exp(a sum of dt), whose sum is off by no more than the steps' roundings

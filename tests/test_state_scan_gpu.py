@@ -589,3 +589,34 @@ def test_segments_with_states_in_a_pool(T, order):
         oracle.check(name, got[rows], (value[rows], bound[rows]))
     free = [r for r in range(8) if r not in (6, 2, 0, 5)]
     assert torch.equal(pool[free], kept[free])
+
+
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("low,high", [(-80.0, -20.0), (-20.0, -8.0), (-8.0, 0.0), (0.0, 20.0)])
+def test_step_sizes(n, low, high):
+    """dt alone: y is dt where the state is from zero, a = 0 and x = b = c = 1.  With u = 2^-24 and v = delta +
+    delta_bias as fp32 has it: e = exp(-|v|) is off by 1.22 u |v| (the product and log2(e) as fp32 has it) and 2 u
+    (exp2), relative to it and so to log(1 + e) at most; the logarithm of 1 + e rounded by 4 u, its product with
+    log(2) and the sum with what the rounding lost by 1.1 u; what was lost, times 1 - e / 2 for 1 / (1 + e), by
+    2.5 u: in all (1.25 |v| + 11) u of log(1 + e); and the sum with max(v, 0) by u of itself."""
+    gen, u, channels = torch.Generator().manual_seed(36), 2.0 ** -24, 1 << 15
+    delta = low + (high - low) * torch.rand(1, n, channels, generator=gen)
+    bias = torch.randn(channels, generator=gen)
+    shape = thff.StateShape("float", 1, n, channels, 1)
+    for b in (None, bias):
+        v = delta if b is None else (delta - b) + b
+        given = (delta if b is None else delta - b).cuda()
+        one, y = torch.ones_like(given), torch.empty_like(given)
+        # Each step alone: b and c of the others are 0.
+        for t in range(n):
+            on = torch.zeros(1, n, 1, 1, device="cuda")
+            on[:, t] = 1
+            thff.ThunderFFT_state_scan(shape, one, given, torch.zeros(channels, 1, device="cuda"), on, on, y,
+                                       d_delta_bias=None if b is None else b.cuda())
+            got, w = y[:, t].cpu().double(), v[:, t].double()
+            e = torch.log1p(torch.exp(-w.abs()))
+            want = w.clamp(min=0) + e
+            bound = (1.25 * w.abs() + 11) * u * e + u * want + 2.0 ** -126
+            off = (got - want).abs() / bound
+            print(f"n {n} step {t} {low} to {high}: {off.max().item():.3f} of the bound", flush=True)
+            assert (off <= 1).all()
