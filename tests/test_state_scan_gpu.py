@@ -620,3 +620,33 @@ def test_step_sizes(n, low, high):
             off = (got - want).abs() / bound
             print(f"n {n} step {t} {low} to {high}: {off.max().item():.3f} of the bound", flush=True)
             assert (off <= 1).all()
+
+
+@pytest.mark.parametrize("T", list(oracle.TYPES))
+@pytest.mark.parametrize("size", [(3, 1, 24, 5), (3, 18, 70, 16), (2, 45, 9, 40), (2, 700, 24, 4), (1, 1500, 12, 24)], ids=str)
+def test_rates_of_the_lowest_value(T, size):
+    """Rates that leave nothing of a state, at fp32's lowest value and at minus infinity: steps of 0 among the
+    others and behind the ends keep the states, and gradients are finite."""
+    v = values(37, T, *size)
+    batch, n, channels, order = size
+    v["a"][::2, ::2] = torch.finfo(torch.float32).min
+    v["a"][1::3, 1] = torch.finfo(torch.float32).min
+    # dt is exactly 0 where exp(delta + delta_bias) is; a small one is not.
+    v["delta"][:, 3::7], v["delta"][:, 5::11] = -200, -300
+    for lengths in (None, ends(*(n - 1 - n // 3 * b for b in range(batch)))):
+        compare(T, v, lengths)
+        got = run(T, v, lengths)
+        below = dict(v, a=torch.where(v["a"] == torch.finfo(torch.float32).min, -float("inf"), v["a"]))
+        other = run(T, below, lengths)
+        for name in got:
+            assert torch.equal(got[name], other[name]), name
+    # The kernel of single steps.
+    if n == 1:
+        for a in (v["a"], below["a"]):
+            for lengths in (None, ends(1, 0, 1)):
+                delta = v["delta"].clone()
+                delta[0, 0, ::2] = -200
+                want = oracle.state(T, v["x"], delta, v["a"], v["b"], v["c"], v["skip"], v["gate"], v["delta_bias"], v["state"], lengths)
+                y, state = thff.state_scan(v["x"], delta, a, v["b"], v["c"], v["skip"], v["gate"], v["delta_bias"], v["state"], lengths)
+                oracle.check("y", y, want["y"])
+                oracle.check("state", state, want["state"])

@@ -242,7 +242,7 @@ __global__ __launch_bounds__(L::kLanes) void state_forward(StateShape s, StateFo
     float decay[S], h[S], sum = 0.0f;
     load_states<L>(decay, a.a + static_cast<long long>(channel) * s.order, p.sub, s.order);
 #pragma unroll
-    for (int i = 0; i < S; ++i) decay[i] *= kLog2e;
+    for (int i = 0; i < S; ++i) decay[i] = rate_of(decay[i]);
     const float skip = a.skip ? a.skip[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
 
     int slot = p.b;
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, Sta
     float decay[S], g[S], sum = 0.0f;
     load_states<L>(decay, a.a + static_cast<long long>(channel) * s.order, p.sub, s.order);
 #pragma unroll
-    for (int i = 0; i < S; ++i) decay[i] *= kLog2e;
+    for (int i = 0; i < S; ++i) decay[i] = rate_of(decay[i]);
     const float skip = a.skip ? a.skip[channel] : 0.0f, bias = a.delta_bias ? a.delta_bias[channel] : 0.0f;
 
     // g: the gradient of the state behind the steps that are done, from the steps behind it.
@@ -583,7 +583,9 @@ __global__ __launch_bounds__(L::kLanes, 2) void state_backward(StateShape s, Sta
             if constexpr (!Only) {
                 const bool on = kWhole || t + j * LPC + p.sub < end;
                 const float su = sum_to_lanes<LPC>(du, p.lane), se = sum_to_lanes<LPC>(de, p.lane) * (1.0f / kLog2e);
-                ed[j] = fmaf(su, xv[j], se) * opened(raw[j]);
+                // A dt of 0 keeps a state whatever the rate: the sum of q a may then be out of range, the slope is 0.
+                const float slope = opened(raw[j]);
+                ed[j] = fmaf(su, xv[j], slope == 0.0f ? 0.0f : se) * slope;
                 ed[j] = on ? ed[j] : 0.0f;
                 ex[j] = fmaf(su, dt[j], along[j] * skip);
                 ex[j] = on ? ex[j] : 0.0f;
@@ -766,7 +768,9 @@ __global__ __launch_bounds__(kLanes, 6) void state_step(StateShape s, StateForwa
         h[r] = pack<float, 4>{};
         if (a.state_in && slot[r] >= 0) h[r] = load(a.state_in + state[r]);
     }
-    const pack<float, 4> rate = load(a.a + static_cast<long long>(channel) * s.order + at);
+    pack<float, 4> rate = load(a.a + static_cast<long long>(channel) * s.order + at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) rate[k] = rate_of(rate[k]);
     const float bias = a.delta_bias ? a.delta_bias[channel] : 0.0f, skip = a.skip ? a.skip[channel] : 0.0f;
 #pragma unroll
     for (int r = 0; r < Rows; ++r) {
@@ -775,7 +779,7 @@ __global__ __launch_bounds__(kLanes, 6) void state_step(StateShape s, StateForwa
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float next = fmaf(__builtin_amdgcn_exp2f(dt * (rate[k] * kLog2e)), h[r][k], u * to_float<T>(bv[r][k]));
+            const float next = fmaf(__builtin_amdgcn_exp2f(dt * rate[k]), h[r][k], u * to_float<T>(bv[r][k]));
             if (on[r]) h[r][k] = next;
             if (k < some) sum = fmaf(to_float<T>(cv[r][k]), next, sum);
         }

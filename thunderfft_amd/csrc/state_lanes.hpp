@@ -122,6 +122,14 @@ __device__ __forceinline__ float opened(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
 }
 
+// a log2(e), whose product with a dt is the power of two that a state keeps.  The lowest and highest values
+// and infinities are taken as fp32's largest of their sign, so that a dt of 0 (a step behind the end, say)
+// keeps the state, and what is 0 of a state that leaves nothing stays 0 times that; a NaN stays one.
+__device__ __forceinline__ float rate_of(float a) {
+    constexpr float kMost = 3.40282347e38f;
+    return __builtin_elementwise_minimum(__builtin_elementwise_maximum(a * kLog2e, -kMost), kMost);
+}
+
 template <int N, class F, int K = 0>
 __device__ __forceinline__ void each_step(F f) {
     if constexpr (K < N) {
