@@ -8,7 +8,7 @@
 // A lane takes 16 bytes of channels (backward 2 or 4 of them) and some steps one after the other, with the last
 // K - 1 rows in registers, so that a row is read once but for those before a lane's first step.
 //
-// Memory bounds it: bfloat16 8 x 4096 x 2048, 4 taps, 49 us forward (294 MB, 6.0 TB/s) and 75 us
+// Memory bounds it: bfloat16 8 x 4096 x 2048, 4 taps, 46 us forward (294 MB, 6.4 TB/s) and 76 us
 // backward (417 MB, 5.5 TB/s; the VALU issues in 90% of the cycles too), 5 more for the weights'
 // sums.  A token of 8 sequences 5 us, half 7 x 1000 x 2048 of unlike lengths 12 us: a round of
 // loads and one of stores.

@@ -43,7 +43,8 @@ long long waves_of(const StateShape& s) {
 // The forward pass's.  With half of a wave for each SIMD (1024 of them), and not quite one, 8 lanes a
 // channel are as many waves again, in place of segments: bfloat16 7 x 1000 x 2048, ragged (896 waves
 // of 4 lanes) 56 us against 79 by 4 lanes, 4 x 4096 x 2048 (512) 229 against 241, 6 x 4096 x 2048
-// (768) 354 against 365; 8 x 4096 x 2048 (1024) 427 against 366.
+// (768) 354 against 365; 8 x 4096 x 2048 (1024) 427 against 366.  Orders 9 to 16 alone: it was not measured
+// at others.
 template <class F>
 auto with_forward_lanes(const StateShape& s, F f) {
     if (s.order > 8 && s.order <= 16) {

@@ -11,8 +11,8 @@
 // Instructions bound it: a state of a step takes 5 at least forward (dt a, its power, dt x b, and the
 // sums of h and y) and 15 backward (those again and the gradients'), and takes 7.6 and 23.7 with what
 // is once a step and channel, the addresses, LDS and the sums over channels.  bfloat16 8 x 4096 x 2048
-// of 16 states (134 MB a tensor): forward 376 us, at a wave a SIMD, the VALU issuing in 67% of the
-// cycles; backward 193 + 910 + 33 us by 4 segments, 84%.  1 x 65536 x 1024, forward: 222 + 323 us by
+// of 16 states (134 MB a tensor): forward 348 us, at a wave a SIMD, the VALU issuing in 67% of the
+// cycles; backward 187 + 883 + 32 us by 4 segments, 84%.  1 x 65536 x 1024, forward: 202 + 288 us by
 // 64 segments, 92% and 90%; all steps by one wave a channel 5.3 ms.  More waves a SIMD would need a
 // backward tile in fewer than 256 registers.
 #pragma once
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(kLanes) void add_state_parts(StateShape s, StateBac
 }
 
 // One step (n = 1: a token of each sequence): the states read and written once bound it, half 256 x
-// 4096 of 16 states 22.3 us (126 MB, 5.6 TB/s), bfloat16 8 x 1024 3.6 us.  4 states a lane, Each lanes of them a channel, and Rows
+// 4096 of 16 states 22.2 us (126 MB, 5.7 TB/s), bfloat16 8 x 1024 3.5 us.  4 states a lane, Each lanes of them a channel, and Rows
 // sequences one after the other, whose loads are all under way together and share a's.
 template <class T, int Each, int Rows>
 __global__ __launch_bounds__(kLanes, 6) void state_step(StateShape s, StateForward a) {

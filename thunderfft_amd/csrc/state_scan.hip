@@ -15,7 +15,7 @@ namespace {
 // SIMD (1024 in all) the steps take 0.8 of it with two and more.  Order 16, us a call by one segment
 // against many: forward bfloat16 6 x 4096 x 2048 (1536 waves of 8 lanes) 367 against 410, 8 x 4096 x
 // 2048 (1024 of 4) 390 against 490, 1 x 256 x 2048 (128) 27 against 20, 1 x 65536 x 1024 (64) 5316
-// against 510; backward 8 x 4096 x 2048 1224 against 1106, float 33 x 512 x 96 in two groups (264)
+// against 469; backward 8 x 4096 x 2048 1224 against 1106, float 33 x 512 x 96 in two groups (264)
 // 174 against 67.
 //
 // A segment goes through the ends of all before it, so that their number should be small against
@@ -24,6 +24,9 @@ namespace {
 // (256 segments for 1024) 145 + 249 us against 490 + 549, 1 x 16384 x 512 (64 for 128) 99 + 177
 // against 126 + 213, 4 x 1024 x 1024 (8 for 16) 48 + 92 against 56 + 101.  8 waves a SIMD are no
 // faster backward: 8 x 4096 x 2048 1103 us against 1085, 2 x 4096 x 1024 210 against 167.
+//
+// All of it at order 16, 4 states a lane.  Waves of lower orders have less work a step, and the thresholds,
+// which count waves, have not been measured there.
 int segments_of(long long waves, int n, bool backward) {
     if (waves == 0 || waves > (backward ? 1024 : 832) || n < (backward ? 128 : 256)) return 1;
     int segments = 1;
