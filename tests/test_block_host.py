@@ -457,3 +457,29 @@ def test_slots_and_lengths_refused(monkeypatch):
             for t in (None, G, OnDevice(good, G), OnDevice(good.view(8, 1)[:, 0], G)):
                 call(**{name: t})
             assert given == [thff.THFF_EINVAL] * 4
+
+
+def test_arrays_of_no_bytes_lie_anywhere(monkeypatch):
+    """Scratch memory that a call does not use, and arrays of no steps, may have the address of what follows them."""
+    monkeypatch.setattr(thff, "_raise", lambda rc: given.append(rc))
+    given = []
+    one = state_shape(n=1)
+    assert one.forward_bytes() == 0 and thff.rms_norm_workspace_bytes(4, 20000) == 0
+    # The last argument is off its alignment, which is looked at after the addresses.
+    for call, args in (
+            (thff.ThunderFFT_state_scan, dict(shape=one, d_x=A, d_delta=B, d_a=C, d_b=D, d_c=E, d_y=F, d_workspace=F, d_skip=G + 2)),
+            (thff.ThunderFFT_state_scan, dict(shape=state_shape(n=0), d_x=A, d_delta=A, d_a=C, d_b=A, d_c=A, d_y=A, d_state_out=A,
+                                              d_workspace=A, d_skip=G + 2)),
+            (thff.ThunderFFT_short_conv, dict(shape=conv_shape(n=0), d_x=A, d_weight=C, d_bias=D + 2, d_y=A, d_state_out=A)),
+            (thff.ThunderFFT_short_conv_backward, dict(shape=conv_shape(), d_dy=A, d_x=B, d_weight=C, d_bias=D + 2, d_dx=E,
+                                                       d_workspace=E)),
+            (thff.ThunderFFT_short_conv_backward, dict(shape=conv_shape(n=0), d_dy=A, d_x=A, d_weight=C, d_bias=D + 2, d_dx=A,
+                                                       d_dweight=A, d_dstate_in=E)),
+            (thff.ThunderFFT_state_scan_backward, dict(shape=state_shape(n=0), d_dy=A, d_x=A, d_delta=A, d_a=C, d_b=A, d_c=A,
+                                                       d_saved=A, d_dx=A, d_ddelta=A, d_da=A, d_db=A, d_dc=A, d_skip=G + 2,
+                                                       d_workspace=B)),
+            (thff.ThunderFFT_rms_norm_backward, dict(T="half", d_dy=A, d_sum=B, d_rstd=C, d_weight=D + 2, d_dx=E, d_dweight=F,
+                                                     d_workspace=A, rows=4, cols=20000))):
+        given.clear()
+        call(**args)
+        assert given == [thff.THFF_EINVAL] and b"4-byte aligned" in thff.lib().thff_last_error(), (call.__name__, thff.lib().thff_last_error())

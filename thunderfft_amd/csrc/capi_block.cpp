@@ -27,7 +27,8 @@ bool any_null(std::initializer_list<const void*> pointers) {
     return false;
 }
 
-// Whether an output is an input or another output (null pointers are none).
+// Whether an output is an input or another output (null pointers are none).  Arrays of no bytes are given
+// as null: they may lie where another begins.
 bool any_alias(std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs) {
     for (const void* const* o = outputs.begin(); o != outputs.end(); ++o) {
         if (!*o) continue;
@@ -76,8 +77,9 @@ int conv_impl(const thff_conv_shape* shape, const ConvForward& a, void* stream, 
     const unsigned e = element_bytes(s.precision);
     if (!a.weight || (s.n > 0 && any_null({a.x, a.y})))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv requires non-null x, weight and y");
-    if ((s.n > 0 && any_alias({a.y}, {a.x, a.weight, a.bias, a.state_in, a.state_out, a.slots, a.lengths})) ||
-        any_alias({a.state_out}, {a.x, a.weight, a.bias, a.slots, a.lengths}))
+    const bool steps = s.n > 0;
+    if ((steps && any_alias({a.y}, {a.x, a.weight, a.bias, a.state_in, a.state_out, a.slots, a.lengths})) ||
+        any_alias({a.state_out}, {steps ? a.x : nullptr, a.weight, a.bias, a.slots, a.lengths}))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv output must not alias another array");
     if (!all_aligned({a.x, a.y, a.state_in, a.state_out}, e))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv requires element-aligned values and states");
@@ -103,8 +105,10 @@ int conv_backward_impl(const thff_conv_shape* shape, const ConvBackward& a, void
             return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward requires a workspace of " +
                                          std::to_string(conv_workspace_bytes(s)) + " bytes");
     }
-    if (any_alias({a.dx, a.dweight, a.dbias, a.dstate_in, a.workspace},
-                  {a.dy, a.x, a.weight, a.bias, a.state_in, a.dstate_out, a.lengths}))
+    const bool scratch = (a.dweight || a.dbias) && conv_workspace_bytes(s) > 0;
+    const bool steps = s.batch > 0 && s.n > 0;
+    if (any_alias({steps ? a.dx : nullptr, a.dweight, a.dbias, a.dstate_in, scratch ? a.workspace : nullptr},
+                  {steps ? a.dy : nullptr, steps ? a.x : nullptr, a.weight, a.bias, a.state_in, a.dstate_out, a.lengths}))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward outputs must not alias other arrays");
     if (!all_aligned({a.dy, a.x, a.dx, a.state_in, a.dstate_out, a.dstate_in}, e))
         return fail(THFF_EINVAL, "ThunderFFT_short_conv_backward requires element-aligned values and states");
@@ -149,9 +153,12 @@ int state_impl(const thff_state_shape* shape, const StateForward& a, void* strea
     if (s.batch == 0 || s.channels == 0) return THFF_OK;
     if (!a.a || (s.n > 0 && any_null({a.x, a.delta, a.b, a.c, a.y})))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan requires non-null x, delta, a, b, c and y");
-    if (any_alias({s.n > 0 ? a.y : nullptr, a.saved, a.workspace},
-                  {a.x, a.delta, a.a, a.b, a.c, a.skip, a.gate, a.delta_bias, a.state_in, a.state_out, a.slots, a.lengths}) ||
-        any_alias({a.state_out}, {a.x, a.delta, a.a, a.b, a.c, a.skip, a.gate, a.delta_bias, a.slots, a.lengths}))
+    const bool steps = s.n > 0;
+    if ((steps && any_alias({a.y, a.saved, state_forward_bytes(s) > 0 ? a.workspace : nullptr},
+                            {a.x, a.delta, a.a, a.b, a.c, a.skip, a.gate, a.delta_bias, a.state_in, a.state_out, a.slots,
+                             a.lengths})) ||
+        (steps && any_alias({a.state_out}, {a.x, a.delta, a.b, a.c, a.gate})) ||
+        any_alias({a.state_out}, {a.a, a.skip, a.delta_bias, a.slots, a.lengths}))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan output must not alias another array");
     if (!all_aligned({a.x, a.delta, a.b, a.c, a.gate, a.y}, element_bytes(s.precision)))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan requires element-aligned buffers");
@@ -189,9 +196,15 @@ int state_backward_impl(const thff_state_shape* shape, const thff_state_gradient
     if (s.batch > 0 && !workspace && state_workspace_bytes(s) > 0)
         return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward requires a workspace of " +
                                      std::to_string(state_workspace_bytes(s)) + " bytes");
-    if (any_alias({g->dx, g->ddelta, g->da, g->db, g->dc, g->dskip, g->dgate, g->ddelta_bias, g->dstate_in, workspace},
-                  {g->dy, g->x, g->delta, g->a, g->b, g->c, g->skip, g->gate, g->delta_bias, g->saved, g->dstate_out,
-                   g->lengths}))
+    const void* scratch = state_workspace_bytes(s) > 0 ? workspace : nullptr;
+    const bool steps = s.batch > 0 && s.n > 0;
+    if ((steps && any_alias({g->dx, g->ddelta, g->db, g->dc, g->dgate},
+                            {g->dy, g->x, g->delta, g->a, g->b, g->c, g->skip, g->gate, g->delta_bias, g->saved, g->dstate_out,
+                             g->lengths, g->da, g->dskip, g->ddelta_bias, g->dstate_in, scratch})) ||
+        (steps && any_alias({g->da, g->dskip, g->ddelta_bias, g->dstate_in, scratch},
+                            {g->dy, g->x, g->delta, g->b, g->c, g->gate, g->saved})) ||
+        any_alias({g->da, g->dskip, g->ddelta_bias, g->dstate_in, scratch},
+                  {g->a, g->skip, g->delta_bias, g->dstate_out, g->lengths}))
         return fail(THFF_EINVAL, "ThunderFFT_state_scan_backward outputs must not alias other arrays");
     if (!all_aligned({g->dy, g->x, g->delta, g->b, g->c, g->gate, g->dx, g->ddelta, g->db, g->dc, g->dgate},
                      element_bytes(s.precision)))
@@ -278,7 +291,8 @@ int rms_backward_impl(RmsBackward a, void* stream, bool synchronize) {
     if (a.rows > 0) {
         if (any_null({a.dy, a.sum, a.rstd, a.dx}))
             return fail(THFF_EINVAL, "ThunderFFT_rms_norm_backward requires non-null dy, sum, rstd and dx");
-        if (any_alias({a.dx, a.dweight, a.workspace}, {a.dy, a.sum, a.rstd, a.weight, a.dsum}))
+        const bool scratch = a.dweight && rms_workspace_bytes(a.rows, a.cols) > 0;
+        if (any_alias({a.dx, a.dweight, scratch ? a.workspace : nullptr}, {a.dy, a.sum, a.rstd, a.weight, a.dsum}))
             return fail(THFF_EINVAL, "ThunderFFT_rms_norm_backward outputs must not alias its inputs");
         if (!all_aligned({a.dy, a.sum, a.dsum, a.dx}, element_bytes(a.precision)))
             return fail(THFF_EINVAL, "ThunderFFT_rms_norm_backward requires element-aligned buffers");
