@@ -448,17 +448,18 @@ long long thff_state_scan_workspace_bytes(const thff_state_shape* shape);
  *   dt = log(1 + exp(delta[t] + delta_bias)),
  *   h[t][s] = exp(dt * a[s]) * h[t-1][s] + dt * x[t] * b[t][s],
  *   y[t] = (sum_s c[t][s] * h[t][s] + skip * x[t]) * gate[t] / (1 + exp(-gate[t])),
- * t < lengths[b].  a is fp32 [channels][order]; skip, delta_bias fp32 [channels] (null:
+ * t < lengths[b].  a is fp32 [channels][order], infinite ones count as fp32's largest of
+ * their sign (a dt of 0 keeps the state); skip, delta_bias fp32 [channels] (null:
  * zeros); gate null: y without its last factor.  h before the first step is the state
  * d_state_in (null: zeros), after the last one it goes to d_state_out (null: not
  * stored): fp32 rows of [channels][order].  y may alias no input.  Empty batches and
  * channels are no-ops; n = 0 copies the states.  An infinity or a NaN in an input makes
  * later outputs that depend on it infinite or NaN, and no others.  Long sequences may be
- * worked on in segments, each from a state of zero, whose ends are joined: results are as
- * exact as the recurrence of the sizes |state| and |dt * x * b| allows, not that of the
- * states.  The two differ by much only where a is positive and terms that have grown
- * cancel; where the sizes leave fp32's range there, results may be infinite or NaN though
- * the states would not be.  That holds for the gradients too. */
+ * worked on in segments, each from a state of zero, whose ends are joined: results are
+ * as exact as the recurrence of the sizes |state| and |dt * x * b| allows, not that of
+ * the states.  The two differ by much only where a is positive and terms that have grown
+ * cancel; where the sizes leave fp32's range there, results may be infinite or NaN
+ * though the states would not be.  That holds for the gradients too. */
 int thff_state_scan(const thff_state_shape* shape, const void* d_x, const void* d_delta,
                     const void* d_a, const void* d_b, const void* d_c, const void* d_skip,
                     const void* d_gate, const void* d_delta_bias, void* d_y,

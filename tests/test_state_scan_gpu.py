@@ -650,3 +650,23 @@ def test_rates_of_the_lowest_value(T, size):
                 y, state = thff.state_scan(v["x"], delta, a, v["b"], v["c"], v["skip"], v["gate"], v["delta_bias"], v["state"], lengths)
                 oracle.check("y", y, want["y"])
                 oracle.check("state", state, want["state"])
+
+
+@pytest.mark.parametrize("n", [1, 45, 700])
+def test_a_rate_that_is_none(n):
+    """A NaN among the rates makes its channel's outputs, state and gradients NaN, and no other channel's."""
+    v = values(38, "half", 2, n, 24, 16)
+    clean = run("half", v)
+    v["a"][5, 3] = float("nan")
+    got = run("half", v)
+    rest = torch.arange(24, device="cuda") != 5
+    for name in ("y", "dx", "ddelta", "dgate"):
+        assert torch.equal(got[name][..., rest], clean[name][..., rest]), name
+    assert got["y"][..., 5].isnan().all() and got["dgate"][..., 5].isnan().all() and got["ddelta"][..., 5].isnan().all()
+    assert torch.equal(got["state"][:, rest], clean["state"][:, rest]) and got["state"][:, 5, 3].isnan().all()
+    assert torch.equal(got["da"][rest], clean["da"][rest]) and got["da"][5, 3].isnan()
+    if n == 1:
+        names = ("x", "delta", "a", "b", "c", "skip", "gate", "delta_bias", "state")
+        y, state = thff.state_scan(*(v[k] for k in names))
+        assert y[..., 5].isnan().all() and state[:, 5, 3].isnan().all()
+        assert torch.isfinite(y[..., rest]).all() and torch.isfinite(state[:, rest]).all()
